@@ -412,6 +412,79 @@ int m5k_shift_split_condition(const void* gamma, const void* scale, int param_dt
                               const void* shift, const void* w, int operand_dtype, int64_t p_rows,
                               int64_t k, int64_t n, float* combined, float* bias, void* stream);
 
+/*
+ * Attention behind the Q/K/V projections.  out[token, head * head_dim] = softmax over the visible keys of
+ * scale * q . k (FP32 statistics, probabilities rounded to `dtype` for the second product) times v; query
+ * head h reads key head h / (heads / kv_heads).  dtype M5K_BF16 or M5K_F16, head_dim 64 or 128.  q
+ * [heads, tokens, head_dim] and k, v [kv_heads, keys, head_dim] by strides in elements (multiples of 8, rows
+ * contiguous, bases 16-byte aligned); out [tokens, heads * head_dim] contiguous.
+ *   Row i stands at key position p = i + keys - tokens.  Scores: softcap > 0 replaces s by
+ *   softcap * tanh(s / softcap); slopes (float32 [heads]) then adds -slopes[h] * |p - j|.
+ *   Mask: causal keeps j <= p (and j below the document's first key + prefix_lengths[document]); window > 0
+ *   keeps p - j < window, and j - p < window without causal; document_starts (int32 [documents + 1],
+ *   nondecreasing from 0; needs keys == tokens) keeps the row's own document.  A row that sees no key is 0;
+ *   so is a row behind the last document.  What a masked key or value holds does not matter, NaN included.
+ *   prefix_lengths: int32 [documents], or [1] without document_starts; only with causal, not with window.
+ *   splits: key ranges joined by a second launch (m5k_attention_splits gives the number that pays); above 1
+ *   workspace holds splits * tokens * heads * (head_dim + 2) floats that the call may overwrite.
+ */
+int m5k_attention(const void* q, int dtype, int64_t tokens, int64_t heads, int head_dim, int64_t q_head,
+                  int64_t q_token, const void* k, int64_t k_head, int64_t k_key, const void* v, int64_t v_head,
+                  int64_t v_key, int64_t keys, int64_t kv_heads, float scale, int causal, int64_t window,
+                  float softcap, const float* slopes, const int32_t* document_starts, int64_t documents,
+                  const int32_t* prefix_lengths, void* out, int splits, float* workspace, int64_t workspace_elems,
+                  void* stream);
+
+/* Key splits of m5k_attention (paged 0) or m5k_paged_attention (paged 1, keys = table_width * page_size) that
+ * fill `cus` compute units (host only; cus <= 0: 256). */
+int m5k_attention_splits(int paged, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t sequences, int64_t keys,
+                         int cus, int* splits);
+
+/*
+ * Attention of new tokens over a paged cache: k_cache, v_cache [pages, kv_heads, page_size, head_dim] by
+ * strides; page_table int32 [sequences, table_width].  Sequence b's new tokens are rows
+ * [query_starts[b], query_starts[b + 1]) of q and out (query_starts int32 [sequences + 1], nondecreasing from 0)
+ * and the last of the context_lengths[b] keys of its cache (int32 [sequences], new tokens included, at most
+ * table_width * page_size): the mask is causal on those positions, the other arguments are m5k_attention's, with
+ * prefix_lengths int32 [sequences].  Rows behind the last sequence, and of a sequence whose context is empty,
+ * are 0.  A table entry outside [0, pages) names no page; its keys are left out.  page_size is any number.
+ */
+int m5k_paged_attention(const void* q, int dtype, int64_t tokens, int64_t heads, int head_dim, int64_t q_head,
+                        int64_t q_token, const void* k_cache, int64_t k_page, int64_t k_head, int64_t k_slot,
+                        const void* v_cache, int64_t v_page, int64_t v_head, int64_t v_slot, int64_t pages,
+                        int64_t page_size, int64_t kv_heads, const int32_t* page_table, int64_t table_width,
+                        int64_t sequences, const int32_t* query_starts, const int32_t* context_lengths, float scale,
+                        int64_t window, float softcap, const float* slopes, const int32_t* prefix_lengths, void* out,
+                        int splits, float* workspace, int64_t workspace_elems, void* stream);
+
+/*
+ * Rotary positions: y = x with channel pairs of the first 2 * pairs channels turned by
+ * a = positions[token] * frequencies[j] (float64 radians a position; the angle is reduced in 64 bits) and
+ * scaled by `magnitude`: (x1 c - x2 s, x2 c + x1 s), pair j being channels (j, j + pairs), or
+ * (2j, 2j + 1) with interleaved != 0; the other channels are copied.  x [heads, tokens, head_dim] of F32, F16 or
+ * BF16 by strides in elements (channels contiguous), y [heads, tokens, head_dim] contiguous; positions int32.
+ */
+int m5k_rope(const void* x, int dtype, int64_t tokens, int64_t heads, int64_t head_dim, int64_t x_head,
+             int64_t x_token, const int32_t* positions, const double* frequencies, int64_t pairs, int interleaved,
+             float magnitude, void* y, void* stream);
+
+/*
+ * Append keys and values of new tokens to a paged cache (layout, page_table, query_starts and context_lengths as in
+ * m5k_paged_attention): token i of sequence b goes to position context_lengths[b] - n + i, keys turned as in
+ * m5k_rope when pairs > 0.  k, v [kv_heads, tokens, head_dim] and the caches by strides, dtype F16, BF16 or F32.
+ * q (or NULL) [heads, tokens, head_dim] is turned too, into q_out [heads, tokens, head_dim] contiguous, whose rows
+ * behind the last sequence become 0.  A token whose position is negative or lies behind the table, or whose table
+ * entry is outside [0, pages), is not stored; nothing else in the cache is written.
+ */
+int m5k_paged_append(const void* k, int64_t k_head, int64_t k_token, const void* v, int64_t v_head, int64_t v_token,
+                     int dtype, int64_t tokens, int64_t kv_heads, int64_t head_dim, void* k_cache, int64_t kc_page,
+                     int64_t kc_head, int64_t kc_slot, void* v_cache, int64_t vc_page, int64_t vc_head,
+                     int64_t vc_slot, int64_t pages, int64_t page_size, const int32_t* page_table,
+                     int64_t table_width, int64_t sequences, const int32_t* query_starts,
+                     const int32_t* context_lengths, const void* q, int64_t heads, int64_t q_head, int64_t q_token,
+                     void* q_out, const double* frequencies, int64_t pairs, int interleaved, float magnitude,
+                     void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,639 @@
+// Attention for gfx950: out = softmax(scores(Q K^T) + mask) V with one pass over the keys, K and V dense or in
+// the pages of a cache.
+//
+// Rows.  The query heads that share a key head are packed: packed row r of a sequence is token r / G, query head
+// kvh * G + r % G (G = heads / kv_heads), so one K/V tile serves all of them and a single token still fills G rows.
+// A workgroup has 4 waves of 32 rows; a wave keeps its Q in registers.
+//
+// Masks.  Every mask of these operators (causal, window, document, prefix, length) leaves a row one interval
+// [lo, hi) of keys.  Key tiles outside the union of a wave's intervals are skipped, tiles inside all of them need
+// no comparison, the others compare the key index.
+//
+// Products.  v_mfma_f32_32x32x16 on S^T = K Q^T and O^T = V^T P^T.  With S transposed a lane holds scores of one
+// query (lane & 31) only: 16 of the 32 keys of a block, the other 16 in lane ^ 32, so that a row's maximum is a
+// chain of v_max in registers and one exchange, and row statistics are per-lane scalars.  The accumulator's key
+// order (8 (r >> 2) + 4 (lane >> 5) + (r & 3)) is used unchanged as the K order of the second product: register
+// octet s of P is its operand for keys 16 s .. 16 s + 15, and V^T is read in the same order, two groups of 4 keys,
+// by ds_read_b64_tr_b16 (the transpose of a 4 x 16 block on the way out of LDS).  P never leaves registers.
+//
+// Softmax.  Running maximum and sum in FP32 in base 2: p = exp2(t - m), t = scale * log2(e) * score.  The maximum
+// is raised, and O and the sum rescaled, only where a row's tile maximum exceeds it by more than 8: p stays below 2^8,
+// the quotient of O and the sum does not depend on m, and most tiles skip the rescale.  P is rounded to the inputs'
+// type for the matrix cores (as the second product's operand has to be); the sum takes the unrounded p.
+//
+// NaN and infinities.  A masked key's score is replaced, whatever it was, but its value row still meets the product
+// as 0 * v.  A wave whose sums end non-finite makes its workgroup run again in careful mode: non-finite values
+// enter as 0, and their effect on the rows that do see them is found by a second product of indicators.  Key rows
+// behind the length and rows of pages that the cache lacks are read from a block of zeros instead.
+#pragma once
+
+#include "gemm_core.h"
+#include "m5k_common.h"
+
+namespace m5k {
+namespace attn {
+
+using gemm::v16f;
+using gemm::v4i;
+
+constexpr int WAVES = 4, THREADS = 64 * WAVES;
+constexpr float M_FLOOR = -1e30f;  // running maximum before any key: finite, so that no difference is NaN
+constexpr float LAZY = 8.0f;       // log2 of how far a tile maximum may pass the running one unadopted
+constexpr float LOG2E = 1.44269504088896340736f;
+
+struct Args {
+  const uint16_t *q, *k, *v;
+  int64_t q_head, q_token, k_page, k_head, k_row, v_page, v_head, v_row;  // strides in elements
+  const int32_t *table, *starts, *context, *prefix;
+  int64_t table_width;
+  const float* slopes;
+  uint16_t* out;
+  float *part_o, *part_ml;
+  int tokens, keys, heads, kv_heads, group, sequences, pages, page_size, window, causal, splits, slots;
+  uint32_t page_magic, page_shift, group_magic, group_shift;
+  float scale, softcap;
+};
+
+// n / d of 0 <= n < 2^31 by one multiplication: magic = ceil(2^(31 + shift) / d), shift = ceil(log2 d).  The excess
+// magic * d - 2^(31 + shift) is below d <= 2^shift, so n times it stays below 2^(31 + shift) and the quotient is exact.
+__device__ __forceinline__ uint32_t fast_div(uint32_t n, uint32_t magic, uint32_t shift) {
+  return __umulhi(2 * n, magic) >> shift;
+}
+
+template <int DT>
+__device__ __forceinline__ v16f mfma32(v4i a, v4i b, v16f c) {
+  if constexpr (DT == M5K_BF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(gemm::bf16x8, a),
+                                                   __builtin_bit_cast(gemm::bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(gemm::f16x8, a),
+                                                  __builtin_bit_cast(gemm::f16x8, b), c, 0, 0, 0);
+}
+
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (DT == M5K_BF16) return f32x2_to_bf16x2(lo, hi);
+  else return f32_to_f16_bits(lo) | (f32_to_f16_bits(hi) << 16);
+}
+
+// The other half-wave's value of the same row.
+__device__ __forceinline__ float other_half(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+__device__ __forceinline__ float max_halves(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4s* lds_v4s;
+
+// 16 bytes a lane from a 64-bit address straight into LDS at lds_base + 16 lane.  Inline asm for the reason given at
+// gemm::dma16; it has no register outputs, and every reader waits for vmcnt and a barrier.
+__device__ __forceinline__ void dma16_flat(uint32_t lds_base, const void* p) {
+  __asm__ volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, off"
+      :
+      : "s"(__builtin_amdgcn_readfirstlane(lds_base)), "v"(p)
+      : "memory", "m0");
+}
+
+static __device__ const uint4 kZeros[1] = {};
+
+// Key tile in LDS: rows of D * 2 bytes, 16-byte chunk c of row r at chunk c ^ swizzle(r).  The 16 consecutive rows of a
+// ds_read_b128 phase (K) then fall on 16 different bank groups, and so do the 4 rows x 64 bytes that half a wave's
+// transposed read covers (V): rows r and r + 1 (two of them share 256 bytes at D = 64) differ in the 64-byte block.
+template <int D>
+__device__ __forceinline__ int swizzle(int row) {
+  if constexpr (D == 64) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+  else return ((row & 3) << 2) | ((row >> 2) & 3);
+}
+
+struct RowRange {
+  int lo, hi;  // visible keys; lo > hi where there are none
+  int pos;     // position on the key axis, for the distance bias
+};
+
+// The interval of a row at position p of a span [s, e) of keys.
+__device__ __forceinline__ RowRange row_range(int s, int e, int p, int prefix, int causal, int window) {
+  int lo = s, hi = e;
+  if (causal) hi = min(e, max(p + 1, s + prefix));
+  if (window) {
+    lo = max(lo, p - window + 1);
+    if (!causal) hi = min(hi, p + window);
+  }
+  if (hi <= lo) { lo = 0x3FFFFFFF; hi = 0; }
+  return RowRange{lo, hi, p};
+}
+
+// The last b in [0, n) with starts[b] + pad * b ... <= x, by binary search over a nondecreasing key(b); 0 if none.
+template <class Key>
+__device__ __forceinline__ int last_not_above(int n, int x, Key key) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (key(mid) <= x) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ int wave_min_i(int v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = min(v, __shfl_xor(v, o));
+  return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ __forceinline__ int wave_max_i(int v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = max(v, __shfl_xor(v, o));
+  return __builtin_amdgcn_readfirstlane(v);
+}
+
+// tanh in FP32 to a few units of its last place: the series below 1/4 (first term left out 9e-3 y^11), elsewhere
+// 1 - 2 / (e^(2y) + 1), whose absolute error is 1e-7.
+__device__ __forceinline__ float tanh_f32(float y) {
+  const float z = y * y;
+  float s = __builtin_fmaf(z, 62.0f / 2835.0f, -17.0f / 315.0f);
+  s = __builtin_fmaf(z, s, 2.0f / 15.0f);
+  s = __builtin_fmaf(z, s, -1.0f / 3.0f);
+  s = __builtin_fmaf(y * z, s, y);
+  const float e = __builtin_amdgcn_exp2f(y * (2.0f * LOG2E));
+  const float f = __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f);
+  return z < 0.0625f ? s : f;
+}
+
+// Scores in base 2 of one accumulator value.
+template <bool MODS>
+__device__ __forceinline__ float score(float x, const Args& a, float scale2, float slope2, int pos, int key) {
+  if constexpr (!MODS) {
+    return x;
+  } else {
+    float t;
+    if (a.softcap > 0.0f) t = tanh_f32(x * (a.scale / a.softcap)) * (a.softcap * LOG2E);
+    else t = x * scale2;
+    return __builtin_fmaf(-slope2, fabsf(static_cast<float>(pos - key)), t);
+  }
+}
+
+// Non-finite 16-bit values of a fragment: zero in `clean`; `mark` holds 1 for +inf, 128 for -inf, 16384 for NaN.
+template <int DT>
+__device__ __forceinline__ void split_nonfinite(v4i f, v4i& clean, v4i& mark) {
+  constexpr uint32_t EXP = DT == M5K_BF16 ? 0x7F80u : 0x7C00u;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    uint32_t c = 0, m = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t x = (static_cast<uint32_t>(f[w]) >> (16 * h)) & 0xFFFFu;
+      const bool bad = (x & EXP) == EXP;
+      const float code = (x & 0x7FFFu) != EXP ? 16384.0f : (x & 0x8000u) ? 128.0f : 1.0f;
+      const uint32_t bits = DT == M5K_BF16 ? f32_to_bf16_bits(code) : f32_to_f16_bits(code);
+      c |= (bad ? 0u : x) << (16 * h);
+      m |= (bad ? bits : 0u) << (16 * h);
+    }
+    clean[w] = static_cast<int>(c);
+    mark[w] = static_cast<int>(m);
+  }
+}
+
+// What a row gets from the non-finite values that it sees: 0, an infinity or NaN, from the sum of their marks.  A tile
+// has 64 keys, so that the counts of +inf (below 128) and -inf (64 * 128 < 16384) keep apart.
+__device__ __forceinline__ float nonfinite_sum(float marks) {
+  const uint32_t u = static_cast<uint32_t>(marks), plus = u & 127u, minus = u & (127u << 7);
+  const uint32_t inf = plus ? 0x7F800000u : 0xFF800000u;
+  const uint32_t bits = (u >> 14) | (plus & -static_cast<uint32_t>(minus != 0)) ? 0x7FC00000u : inf;
+  return __uint_as_float(u ? bits : 0u);
+}
+
+// One workgroup's place: packed rows [row0, row0 + rows) of a sequence whose first token is `token0`.
+struct Place {
+  int seq, kvh, split, tile, token0, rows;  // rows: packed rows of the whole sequence
+  int span, shift;                          // keys; position of token i is i + shift
+};
+
+template <bool PAGED>
+__device__ __forceinline__ Place place(const Args& a, int rows_per_tile) {
+  int item = gemm::xcd_logical(blockIdx.x, gridDim.x);
+  Place p;
+  p.split = item % a.splits;
+  item /= a.splits;
+  p.kvh = item / a.slots;
+  // Later tiles see more keys under a causal mask: they go first.
+  const int slot = a.slots - 1 - item % a.slots;
+  if constexpr (!PAGED) {
+    p.seq = 0;
+    p.tile = slot;
+    p.token0 = 0;
+    p.rows = a.tokens * a.group;
+    p.span = a.keys;
+    p.shift = a.keys - a.tokens;
+  } else {
+    // Sequence b owns the slots from (starts[b] * G / R) + b on: at least as many as it has tiles, and the first of
+    // them is known without the lengths of the sequences before it.  The tokens behind the last sequence are
+    // sequence number `sequences`, which sees nothing.
+    const int T = a.tokens, B = a.sequences;
+    auto start = [&](int b) { return b == 0 ? 0 : min(max(a.starts[b], 0), T); };
+    auto first = [&](int b) { return static_cast<int>(int64_t{start(b)} * a.group / rows_per_tile) + b; };
+    p.seq = last_not_above(B + 1, slot, first);
+    p.token0 = start(p.seq);
+    p.tile = slot - first(p.seq);
+    const int end = p.seq == B ? T : start(p.seq + 1);
+    const int n = max(0, end - p.token0);
+    p.rows = n * a.group;
+    const int ctx = p.seq == B ? 0 : a.context[p.seq];
+    p.span = min(max(ctx, 0), a.keys);
+    p.shift = ctx - n;
+  }
+  return p;
+}
+
+// The row range, and the token and query head of packed row r (r < p.rows).
+template <bool PAGED>
+__device__ __forceinline__ RowRange range_of(const Args& a, const Place& p, int r, int& token, int& head) {
+  const int i = a.group == 1 ? r : static_cast<int>(fast_div(r, a.group_magic, a.group_shift));
+  head = p.kvh * a.group + r - i * a.group;
+  token = p.token0 + i;
+  int s = 0, e = p.span, prefix = 0;
+  if (!PAGED && a.starts) {
+    const int d = last_not_above(a.sequences, i, [&](int b) { return a.starts[b]; });
+    s = max(a.starts[d], 0);
+    e = min(a.starts[d + 1], a.keys);
+    if (i < s || i >= e) e = s = 0;
+    if (a.prefix) prefix = a.prefix[d];
+  } else if (a.prefix && (!PAGED || p.seq < a.sequences)) {
+    prefix = a.prefix[p.seq];
+  }
+  prefix = min(max(prefix, 0), 0x3FFFFFFF);
+  return row_range(s, e, i + p.shift, prefix, a.causal, a.window);
+}
+
+template <int DT, int D, bool PAGED, bool MODS>
+__global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
+  constexpr int KT = 64, NB = KT / 32;   // keys of a tile, 32-key blocks
+  constexpr int CH = D / 8;              // 16-byte chunks of a row
+  constexpr int RPI = 64 / CH;           // rows of one load instruction
+  constexpr int NI = CH / WAVES;         // load instructions of a wave, each of K and V
+  constexpr int QS = D / 16, OB = D / 32;
+  constexpr uint32_t TILE = KT * D * 2, ROWB = D * 2;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[4 * TILE];  // K, V of stage 0, K, V of stage 1
+  __shared__ int bounds[2 * WAVES];
+
+  const Place p = place<PAGED>(a, 32 * WAVES);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+  const int row0 = p.tile * 32 * WAVES;
+  if (row0 >= p.rows) return;
+  const int row = row0 + 32 * wave + (lane & 31);
+  const bool live = row < p.rows;
+  int token, head;
+  const RowRange rr = range_of<PAGED>(a, p, min(row, p.rows - 1), token, head);
+
+  // Key ranges: of the wave (any row, every row), and of the workgroup.
+  const bool idle = row0 + 32 * wave >= p.rows;
+  const int any_lo = idle ? 0x3FFFFFFF : wave_min_i(rr.lo), any_hi = idle ? 0 : wave_max_i(rr.hi);
+  const int all_lo = wave_max_i(rr.lo), all_hi = wave_min_i(rr.hi);
+  if (lane == 0) {
+    bounds[wave] = any_lo;
+    bounds[WAVES + wave] = any_hi;
+  }
+  __syncthreads();
+  int lo = bounds[0], hi = bounds[WAVES];
+#pragma unroll
+  for (int w = 1; w < WAVES; ++w) {
+    lo = min(lo, bounds[w]);
+    hi = max(hi, bounds[WAVES + w]);
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  hi = __builtin_amdgcn_readfirstlane(hi);
+  int t_begin = 0, t_end = 0;
+  if (lo < hi) {
+    t_begin = lo / KT;
+    t_end = (hi + KT - 1) / KT;
+    if (a.splits > 1) {
+      // At least 4 tiles a split: below, the partial sums cost more than the keys.
+      const int per = max((t_end - t_begin + a.splits - 1) / a.splits, 4);
+      t_begin = min(t_begin + p.split * per, t_end);
+      t_end = min(t_begin + per, t_end);
+    }
+  }
+
+  v4i qf[QS];
+  {
+    const uint16_t* qp = a.q + int64_t{head} * a.q_head + int64_t{token} * a.q_token + 8 * half;
+#pragma unroll
+    for (int s = 0; s < QS; ++s) qf[s] = *reinterpret_cast<const v4i*>(qp + 16 * s);
+  }
+  const float scale2 = a.scale * LOG2E;
+  const float unit = MODS ? 1.0f : scale2;  // what turns score() into base 2
+  const float slope2 = MODS && a.slopes ? a.slopes[head] * LOG2E : 0.0f;
+
+  // Loads: this wave's rows of a tile, and what a lane adds to a row's address.
+  const int ld_row = wave * NI * RPI + lane / CH, ld_chunk = lane % CH;
+  const uint16_t* kbase = a.k + int64_t{p.kvh} * a.k_head;
+  const uint16_t* vbase = a.v + int64_t{p.kvh} * a.v_head;
+  const int32_t* table = PAGED && p.seq < a.sequences ? a.table + int64_t{p.seq} * a.table_width : nullptr;
+  const uint32_t lds0 = gemm::lds_addr(lds);
+  int ids[NI];
+  bool lacking = false;
+
+  auto load_ids = [&](int t) {
+    if constexpr (PAGED) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int key = t * KT + ld_row + i * RPI;
+        ids[i] = key < p.span ? table[fast_div(key, a.page_magic, a.page_shift)] : 0;
+      }
+    }
+  };
+  auto load_tile = [&](int t, int stage) {
+    const uint32_t dst = lds0 + stage * 2 * TILE + wave * NI * 1024;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int r = ld_row + i * RPI, key = t * KT + r;
+      const int chunk = (ld_chunk ^ swizzle<D>(r)) * 8;
+      bool in = key < p.span;
+      int64_t ko, vo;
+      if constexpr (PAGED) {
+        const int page = ids[i];
+        if (in && static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.pages)) {
+          in = false;
+          lacking = true;
+        }
+        const int slot = key - static_cast<int>(fast_div(key, a.page_magic, a.page_shift)) * a.page_size;
+        ko = page * a.k_page + slot * a.k_row;
+        vo = page * a.v_page + slot * a.v_row;
+      } else {
+        ko = key * a.k_row;
+        vo = key * a.v_row;
+      }
+      const void* kp = in ? static_cast<const void*>(kbase + ko + chunk) : kZeros;
+      const void* vp = in ? static_cast<const void*>(vbase + vo + chunk) : kZeros;
+      dma16_flat(dst + i * 1024, kp);
+      dma16_flat(dst + TILE + i * 1024, vp);
+    }
+  };
+
+  // Fragment addresses.
+  const int krow = lane & 31;
+  const uint32_t kread = lds0 + krow * ROWB;
+  const int ksw = swizzle<D>(krow);
+  const int g = lane >> 4, gi = lane & 15;
+  const int vrow = 4 * half + (gi >> 2);
+  const int vchunk = 2 * (g & 1) + ((gi & 3) >> 1);
+  const uint32_t vread = lds0 + TILE + vrow * ROWB + (gi & 1) * 8;
+
+  v16f o[OB];
+  float m, l;
+  // One pass over the keys; true where it has to be made again with care.
+  auto pass = [&](auto with_care) -> bool {
+    constexpr bool careful = decltype(with_care)::value;
+    m = M_FLOOR;
+    l = 0.0f;
+#pragma unroll
+    for (int b = 0; b < OB; ++b) o[b] = v16f{};
+    if (t_begin < t_end) {
+      load_ids(t_begin);
+      load_tile(t_begin, 0);
+      if (t_begin + 1 < t_end) load_ids(t_begin + 1);
+    }
+    for (int t = t_begin; t < t_end; ++t) {
+      const int stage = (t - t_begin) & 1;
+      // This wave's part of tile t is in LDS, its reads of the other stage are done; then everybody's.
+      __asm__ volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      gemm::stage_barrier();
+      if (t + 1 < t_end) {
+        load_tile(t + 1, stage ^ 1);
+        if (t + 2 < t_end) load_ids(t + 2);
+      }
+      const int key0 = t * KT;
+      if (key0 + KT <= any_lo || key0 >= any_hi) continue;  // the same for the whole wave
+      const uint32_t kst = kread + stage * 2 * TILE, vst = vread + stage * 2 * TILE;
+
+      v16f s[NB];
+#pragma unroll
+      for (int b = 0; b < NB; ++b) s[b] = v16f{};
+#pragma unroll
+      for (int c = 0; c < QS; ++c) {
+        const uint32_t at = kst + (((2 * c + half) ^ ksw) << 4);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          const v4i kf = *reinterpret_cast<const __attribute__((address_space(3))) v4i*>(at + b * 32 * ROWB);
+          s[b] = mfma32<DT>(kf, qf[c], s[b]);
+        }
+      }
+
+      uint32_t seen = 0;  // careful mode: the keys of this lane's registers that the row sees
+      const int kofs = key0 + 4 * half;
+      if constexpr (MODS) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            s[b][r] = score<MODS>(s[b][r], a, scale2, slope2, rr.pos, kofs + 32 * b + 8 * (r >> 2) + (r & 3));
+      }
+      if (careful || key0 < all_lo || key0 + KT > all_hi) {
+        const uint32_t width = static_cast<uint32_t>(max(rr.hi - rr.lo, 0));
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int key = kofs + 32 * b + 8 * (r >> 2) + (r & 3);
+            bool sees = static_cast<uint32_t>(key - rr.lo) < width;
+            if constexpr (PAGED && careful) {
+              if (sees)
+                sees = static_cast<uint32_t>(table[fast_div(key, a.page_magic, a.page_shift)]) <
+                       static_cast<uint32_t>(a.pages);
+            }
+            if constexpr (careful) seen |= static_cast<uint32_t>(sees) << (16 * b + r);
+            s[b][r] = sees ? s[b][r] : -__builtin_inff();
+          }
+      }
+
+      float top = s[0][0];
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
+      top = max_halves(top) * unit;
+      if (__builtin_amdgcn_ballot_w64(top > m + LAZY)) {
+        const float next = fmaxf(m, top);
+        const float f = __builtin_amdgcn_exp2f(m - next);
+        m = next;
+        l *= f;
+#pragma unroll
+        for (int b = 0; b < OB; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[b][r] *= f;
+      }
+      v4i pf[2 * NB];
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], unit, -m));
+          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r + 1], unit, -m));
+          sum += p0;
+          sum += p1;
+          pf[2 * b + (r >> 3)][(r & 7) >> 1] = static_cast<int>(pack2<DT>(p0, p1));
+        }
+        l += sum;
+      }
+
+#pragma unroll
+      for (int b = 0; b < OB; ++b) {
+        v16f marks = {};
+#pragma unroll
+        for (int c = 0; c < 2 * NB; ++c) {
+          v4i vf;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            // Row 16 c + 8 h + vrow: its swizzle's low bits are (2 h + half) & 3 at D = 128, and rows 8 apart are
+            // alike at D = 64 but for the same two bits.
+            const int sw = swizzle<D>(8 * h + vrow);
+            const uint32_t at = vst + (16 * c + 8 * h) * ROWB + (((4 * b + vchunk) ^ sw) << 4);
+            const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_v4s>(at));
+            const auto y = __builtin_bit_cast(uint2, x);
+            vf[2 * h] = static_cast<int>(y.x);
+            vf[2 * h + 1] = static_cast<int>(y.y);
+          }
+          if constexpr (careful) {
+            v4i clean, mark, see;
+            split_nonfinite<DT>(vf, clean, mark);
+            const uint32_t one = pack2<DT>(1.0f, 1.0f);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const uint32_t bits = seen >> (8 * c + 2 * w);
+              see[w] = static_cast<int>(((bits & 1u) ? one & 0xFFFFu : 0u) | ((bits & 2u) ? one & 0xFFFF0000u : 0u));
+            }
+            marks = mfma32<DT>(mark, see, marks);
+            vf = clean;
+            __builtin_amdgcn_sched_barrier(0);  // rare: few registers rather than overlap
+          }
+          o[b] = mfma32<DT>(vf, pf[c], o[b]);
+        }
+        if constexpr (careful) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[b][r] += nonfinite_sum(marks[r]);
+        }
+      }
+    }
+    float check = 0.0f;
+#pragma unroll
+    for (int b = 0; b < OB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) check = __builtin_fmaf(o[b][r], 0.0f, check);
+    return __syncthreads_or(lacking || check != 0.0f) != 0;
+  };
+  if (pass(std::false_type{})) pass(std::true_type{});
+
+  l += other_half(l);
+  if (!live) return;
+  if (a.splits > 1) {
+    const int64_t at = (int64_t{p.split} * a.tokens + token) * a.heads + head;
+    if (half == 0) {
+      a.part_ml[2 * at] = m;
+      a.part_ml[2 * at + 1] = l;
+    }
+    if (l == 0.0f) return;  // nothing seen here: the sums are not read
+#pragma unroll
+    for (int b = 0; b < OB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        *reinterpret_cast<float4*>(a.part_o + at * D + 32 * b + 2 * r + 4 * half) =
+            make_float4(o[b][r], o[b][r + 1], o[b][r + 2], o[b][r + 3]);
+    return;
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  uint16_t* op = a.out + (int64_t{token} * a.heads + head) * D + 4 * half;
+#pragma unroll
+  for (int b = 0; b < OB; ++b)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const uint2 w = l == 0.0f ? make_uint2(0u, 0u)
+                                : make_uint2(pack2<DT>(o[b][r] * inv, o[b][r + 1] * inv),
+                                             pack2<DT>(o[b][r + 2] * inv, o[b][r + 3] * inv));
+      *reinterpret_cast<uint2*>(op + 32 * b + 2 * r) = w;
+    }
+}
+
+// Joins the key splits: one wave a (token, head), each split's sum weighted by 2^(m - max m), in split order.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void attention_join(const Args a) {
+  const int64_t rows = int64_t{a.tokens} * a.heads;
+  const int64_t at = int64_t{blockIdx.x} * 4 + (threadIdx.x >> 6);
+  if (at >= rows) return;
+  const int lane = threadIdx.x & 63;
+  constexpr int E = D / 64;
+  float top = M_FLOOR;
+  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_ml[2 * (s * rows + at)]);
+  float sum = 0.0f, acc[E] = {};
+  for (int s = 0; s < a.splits; ++s) {
+    const float l = a.part_ml[2 * (s * rows + at) + 1];
+    if (l == 0.0f) continue;
+    const float w = __builtin_amdgcn_exp2f(a.part_ml[2 * (s * rows + at)] - top);
+    sum = __builtin_fmaf(l, w, sum);
+    const float* src = a.part_o + (s * rows + at) * D + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = __builtin_fmaf(src[e], w, acc[e]);
+  }
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  uint16_t* dst = a.out + at * D + lane * E;
+  if constexpr (E == 2) {
+    *reinterpret_cast<uint32_t*>(dst) = sum == 0.0f ? 0u : pack2<DT>(acc[0] * inv, acc[1] * inv);
+  } else {
+    *dst = static_cast<uint16_t>(sum == 0.0f ? 0u : pack2<DT>(acc[0] * inv, 0.0f) & 0xFFFFu);
+  }
+}
+
+template <int DT, int D, bool PAGED>
+int launch(const Args& a, hipStream_t st) {
+  const bool mods = a.softcap > 0.0f || a.slopes;
+  const int64_t blocks = int64_t{a.slots} * a.kv_heads * a.splits;
+  if (blocks > 0x7FFFFFFF) {
+    set_error("attention: too many tiles for one launch");
+    return M5K_EINVAL;
+  }
+  launch_kernel(mods ? attention_tile<DT, D, PAGED, true> : attention_tile<DT, D, PAGED, false>,
+                dim3(static_cast<uint32_t>(blocks)), dim3(THREADS), st, a);
+  int rc = launch_status("attention");
+  if (rc != M5K_OK || a.splits == 1) return rc;
+  const int64_t rows = int64_t{a.tokens} * a.heads;
+  launch_kernel(attention_join<DT, D>, dim3(static_cast<uint32_t>((rows + 3) / 4)), dim3(256), st, a);
+  return launch_status("attention join");
+}
+
+template <bool PAGED>
+int launch_typed(const Args& a, int dtype, int head_dim, hipStream_t st) {
+  if (dtype == M5K_BF16)
+    return head_dim == 64 ? launch<M5K_BF16, 64, PAGED>(a, st) : launch<M5K_BF16, 128, PAGED>(a, st);
+  return head_dim == 64 ? launch<M5K_F16, 64, PAGED>(a, st) : launch<M5K_F16, 128, PAGED>(a, st);
+}
+
+// Packed rows per workgroup and the key splits of a launch: as many as bring the workgroups to two a compute unit
+// (what its LDS holds), each over at least 256 keys of the longest span.
+inline int plan_slots(bool paged, int64_t tokens, int group, int64_t sequences) {
+  const int64_t r = 32 * WAVES;
+  return static_cast<int>(paged ? tokens * group / r + sequences + 1 : (tokens * group + r - 1) / r);
+}
+inline int plan_splits(bool paged, int64_t tokens, int group, int kv_heads, int64_t sequences, int64_t keys, int cus) {
+  // Tiles that have rows: a paged launch has a spare slot a sequence.
+  const int64_t r = 32 * WAVES, whole = tokens * group / r, at_least = tokens < sequences ? tokens : sequences;
+  const int64_t tiles = paged ? (whole > at_least ? whole : at_least) : (tokens * group + r - 1) / r;
+  const int64_t busy = (tiles > 0 ? tiles : 1) * kv_heads;
+  int64_t n = 2 * int64_t{cus} / busy;
+  const int64_t most = keys / 256;
+  n = n < most ? n : most;
+  return static_cast<int>(n < 1 ? 1 : n > 64 ? 64 : n);
+}
+
+inline void magic_of(uint32_t d, uint32_t& magic, uint32_t& shift) {
+  shift = 0;
+  while ((uint64_t{1} << shift) < d) ++shift;
+  magic = static_cast<uint32_t>(((uint64_t{1} << (31 + shift)) + d - 1) / d);
+}
+
+}  // namespace attn
+}  // namespace m5k

@@ -9,6 +9,7 @@ from .hip import gemm, gemm_i8_accumulators, quantize
 from .qk_rope import projection_qk_rope, projection_qkv_rope, qk_norm_rope
 from .hadamard import SUPPORTED_BLOCK_SIZES, rotate, rotate_quantize
 from .rms_quant import rms_quantize
+from .attention_ops import attention, paged_append, paged_attention, rope, rope_frequencies
 from .chains import gate_chain, norm_shift_split_gemm, shift_split_condition
 from .norm_hadamard import (
     fused_gated_residual_norm_hadamard_quantize,
@@ -35,4 +36,9 @@ __all__ = [
     "gate_chain",
     "shift_split_condition",
     "norm_shift_split_gemm",
+    "rope_frequencies",
+    "rope",
+    "paged_append",
+    "paged_attention",
+    "attention",
 ]

@@ -43,6 +43,7 @@ _p = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int
 _f32 = ctypes.c_float
+_rows3 = [_p, _i64, _i64, _i64]  # a cache: base and three strides
 
 # name -> argtypes (restype is int status unless noted)
 SIGNATURES = {
@@ -76,6 +77,20 @@ SIGNATURES = {
     "m5k_projection_qk_rope": [_p, _p, _i32, _i64, _i64, _i64, _p, _p, _p, _p, _p, _i32, _f32, _p, _p],
     "m5k_qk_norm_rope": [_p, _i64, _i64, _p, _p, _p, _i32, _f32, _p, _p],
     "m5k_qkv_norm_rope": [_p, _i64, _i64, _p, _p, _p, _p, _i32, _f32, _p, _p, _p, _p],
+    "m5k_attention_splits": [_i32, _i64, _i64, _i64, _i64, _i64, _i32, _p],
+    "m5k_attention": [
+        _p, _i32, _i64, _i64, _i32, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _f32, _i32, _i64, _f32, _p,
+        _p, _i64, _p, _p, _i32, _p, _i64, _p,
+    ],
+    "m5k_paged_attention": [
+        _p, _i32, _i64, _i64, _i32, _i64, _i64, *_rows3, *_rows3, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _f32, _i64,
+        _f32, _p, _p, _p, _i32, _p, _i64, _p,
+    ],
+    "m5k_rope": [_p, _i32, _i64, _i64, _i64, _i64, _i64, _p, _p, _i64, _i32, _f32, _p, _p],
+    "m5k_paged_append": [
+        _p, _i64, _i64, _p, _i64, _i64, _i32, _i64, _i64, _i64, *_rows3, *_rows3, _i64, _i64, _p, _i64, _i64, _p, _p,
+        _p, _i64, _i64, _i64, _p, _p, _i64, _i32, _f32, _p,
+    ],
 }
 
 _LIB = None
