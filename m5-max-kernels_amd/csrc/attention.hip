@@ -74,21 +74,24 @@ extern "C" int m5k_attention(const void* q, int dtype, int64_t tokens, int64_t h
   M5K_REQUIRE(m5k::aligned16(k) && m5k::aligned16(v) && k_head % 8 == 0 && k_key % 8 == 0 && v_head % 8 == 0 &&
                   v_key % 8 == 0,
               "attention: k and v rows must be 16-byte aligned");
+  constexpr int64_t kRowMax = 1 << 23;
+  M5K_REQUIRE(keys <= 1 || (k_key >= head_dim && v_key >= head_dim && k_key <= kRowMax && v_key <= kRowMax),
+              "attention: rows of k and v must be head_dim to 2^23 elements apart");
   M5K_REQUIRE(!document_starts || (documents > 0 && documents <= (1 << 24) && tokens == keys),
               "attention: documents need as many keys as tokens");
   M5K_REQUIRE(!prefix_lengths || causal, "attention: a prefix needs a causal mask");
   a.k = static_cast<const uint16_t*>(k);
   a.v = static_cast<const uint16_t*>(v);
   a.k_head = k_head;
-  a.k_row = k_key;
+  a.k_row = keys == 1 ? head_dim : k_key;
   a.v_head = v_head;
-  a.v_row = v_key;
+  a.v_row = keys == 1 ? head_dim : v_key;
   a.keys = static_cast<int>(keys);
   a.causal = causal != 0;
   a.starts = document_starts;
   a.sequences = static_cast<int>(documents);
   a.slots = m5k::attn::plan_slots(false, tokens, a.group, 0);
-  return m5k::attn::launch_typed<false>(a, dtype, head_dim, m5k::as_stream(stream));
+  return m5k::attn::launch_typed<m5k::attn::DENSE>(a, dtype, head_dim, m5k::as_stream(stream));
 }
 
 extern "C" int m5k_paged_attention(const void* q, int dtype, int64_t tokens, int64_t heads, int head_dim,
@@ -131,5 +134,8 @@ extern "C" int m5k_paged_attention(const void* q, int dtype, int64_t tokens, int
   a.causal = 1;
   m5k::attn::magic_of(static_cast<uint32_t>(page_size), a.page_magic, a.page_shift);
   a.slots = m5k::attn::plan_slots(true, tokens, a.group, sequences);
-  return m5k::attn::launch_typed<true>(a, dtype, head_dim, m5k::as_stream(stream));
+  const bool whole = page_size % 16 == 0 && k_slot >= head_dim && v_slot >= head_dim && k_slot <= (1 << 23) &&
+                     v_slot <= (1 << 23);
+  const auto run = whole ? m5k::attn::launch_typed<m5k::attn::PAGES16> : m5k::attn::launch_typed<m5k::attn::PAGES>;
+  return run(a, dtype, head_dim, m5k::as_stream(stream));
 }

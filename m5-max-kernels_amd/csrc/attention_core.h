@@ -103,6 +103,14 @@ __device__ __forceinline__ void dma16_flat(uint32_t lds_base, const void* p) {
 
 static __device__ const uint4 kZeros[1] = {};
 
+// vmcnt(0) lgkmcnt(0), as the builtin: the compiler counts it, and does not wait again for the loads before the loop
+// (Q) among those in flight.
+__device__ __forceinline__ void wait_all() {
+  __asm__ volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070);
+  __asm__ volatile("" ::: "memory");
+}
+
 // Key tile in LDS: rows of D * 2 bytes, 16-byte chunk c of row r at chunk c ^ swizzle(r).  The 16 consecutive rows of a
 // ds_read_b128 phase (K) then fall on 16 different bank groups, and so do the 4 rows x 64 bytes that half a wave's
 // transposed read covers (V): rows r and r + 1 (two of them share 256 bytes at D = 64) differ in the 64-byte block.
@@ -110,6 +118,25 @@ template <int D>
 __device__ __forceinline__ int swizzle(int row) {
   if constexpr (D == 64) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
   else return ((row & 3) << 2) | ((row >> 2) & 3);
+}
+
+// Where keys and values lie.  PAGES16: pages of a multiple of 16 keys, so that the 16 rows of a tile that one wave loads
+// lie in one page and take one address; PAGES: any page size, an address a lane.
+enum Keys { DENSE = 0, PAGES16 = 1, PAGES = 2 };
+
+// Page id at a position of the table, loaded per lane although it is the same for all: a scalar load would share
+// lgkmcnt with the LDS reads, out of order, and so make each of them wait.
+__device__ __forceinline__ int table_entry(const int32_t* table, uint32_t at) {
+  __asm__("" : "+v"(at));
+  return table[at];
+}
+
+// Buffer window of up to `rows` rows of `stride` elements from `p`, reading 0 behind them: rows are at least D apart, so a
+// row behind the last begins behind the window's end.
+template <int D>
+__device__ __forceinline__ v4i rows_rsrc(const uint16_t* p, int rows, int64_t stride) {
+  const int64_t n = rows > 0 ? ((rows - 1) * stride + D) * 2 : 0;
+  return gemm::buffer_rsrc(p, static_cast<uint32_t>(n));
 }
 
 struct RowRange {
@@ -214,7 +241,7 @@ struct Place {
   int span, shift;                          // keys; position of token i is i + shift
 };
 
-template <bool PAGED>
+template <int KEYS>
 __device__ __forceinline__ Place place(const Args& a, int rows_per_tile) {
   int item = gemm::xcd_logical(blockIdx.x, gridDim.x);
   Place p;
@@ -223,7 +250,7 @@ __device__ __forceinline__ Place place(const Args& a, int rows_per_tile) {
   p.kvh = item / a.slots;
   // Later tiles see more keys under a causal mask: they go first.
   const int slot = a.slots - 1 - item % a.slots;
-  if constexpr (!PAGED) {
+  if constexpr (KEYS == DENSE) {
     p.seq = 0;
     p.tile = slot;
     p.token0 = 0;
@@ -251,26 +278,26 @@ __device__ __forceinline__ Place place(const Args& a, int rows_per_tile) {
 }
 
 // The row range, and the token and query head of packed row r (r < p.rows).
-template <bool PAGED>
+template <int KEYS>
 __device__ __forceinline__ RowRange range_of(const Args& a, const Place& p, int r, int& token, int& head) {
   const int i = a.group == 1 ? r : static_cast<int>(fast_div(r, a.group_magic, a.group_shift));
   head = p.kvh * a.group + r - i * a.group;
   token = p.token0 + i;
   int s = 0, e = p.span, prefix = 0;
-  if (!PAGED && a.starts) {
+  if (KEYS == DENSE && a.starts) {
     const int d = last_not_above(a.sequences, i, [&](int b) { return a.starts[b]; });
     s = max(a.starts[d], 0);
     e = min(a.starts[d + 1], a.keys);
     if (i < s || i >= e) e = s = 0;
     if (a.prefix) prefix = a.prefix[d];
-  } else if (a.prefix && (!PAGED || p.seq < a.sequences)) {
+  } else if (a.prefix && (KEYS == DENSE || p.seq < a.sequences)) {
     prefix = a.prefix[p.seq];
   }
   prefix = min(max(prefix, 0), 0x3FFFFFFF);
   return row_range(s, e, i + p.shift, prefix, a.causal, a.window);
 }
 
-template <int DT, int D, bool PAGED, bool MODS>
+template <int DT, int D, int KEYS, bool MODS>
 __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   constexpr int KT = 64, NB = KT / 32;   // keys of a tile, 32-key blocks
   constexpr int CH = D / 8;              // 16-byte chunks of a row
@@ -281,14 +308,14 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   __shared__ __attribute__((aligned(16))) uint8_t lds[4 * TILE];  // K, V of stage 0, K, V of stage 1
   __shared__ int bounds[2 * WAVES];
 
-  const Place p = place<PAGED>(a, 32 * WAVES);
+  const Place p = place<KEYS>(a, 32 * WAVES);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
   const int row0 = p.tile * 32 * WAVES;
   if (row0 >= p.rows) return;
   const int row = row0 + 32 * wave + (lane & 31);
   const bool live = row < p.rows;
   int token, head;
-  const RowRange rr = range_of<PAGED>(a, p, min(row, p.rows - 1), token, head);
+  const RowRange rr = range_of<KEYS>(a, p, min(row, p.rows - 1), token, head);
 
   // Key ranges: of the wave (any row, every row), and of the workgroup.
   const bool idle = row0 + 32 * wave >= p.rows;
@@ -329,49 +356,85 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   const float unit = MODS ? 1.0f : scale2;  // what turns score() into base 2
   const float slope2 = MODS && a.slopes ? a.slopes[head] * LOG2E : 0.0f;
 
-  // Loads: this wave's rows of a tile, and what a lane adds to a row's address.
+  // Loads: instruction i of a wave brings rows wave * 16 + i * RPI + lane / CH of K and of V.
+  const int wave_s = __builtin_amdgcn_readfirstlane(wave);
   const int ld_row = wave * NI * RPI + lane / CH, ld_chunk = lane % CH;
   const uint16_t* kbase = a.k + int64_t{p.kvh} * a.k_head;
   const uint16_t* vbase = a.v + int64_t{p.kvh} * a.v_head;
-  const int32_t* table = PAGED && p.seq < a.sequences ? a.table + int64_t{p.seq} * a.table_width : nullptr;
+  const int32_t* table = KEYS != DENSE && p.seq < a.sequences ? a.table + int64_t{p.seq} * a.table_width : nullptr;
   const uint32_t lds0 = gemm::lds_addr(lds);
-  int ids[NI];
+  uint32_t kofs[NI], vofs[NI];  // bytes of a lane's chunk from the window's first row
+  if constexpr (KEYS != PAGES) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int r = KEYS == DENSE ? ld_row + i * RPI : lane / CH + i * RPI;
+      const int chunk = (ld_chunk ^ swizzle<D>(ld_row + i * RPI)) * 8;
+      kofs[i] = static_cast<uint32_t>(r * static_cast<int>(a.k_row) + chunk) * 2;
+      vofs[i] = static_cast<uint32_t>(r * static_cast<int>(a.v_row) + chunk) * 2;
+    }
+  }
+  constexpr int NIDS = KEYS == PAGES ? NI : 1;
+  int ids[NIDS] = {};
   bool lacking = false;
 
+  // Pages of tile t's rows, one tile ahead of their use.
   auto load_ids = [&](int t) {
-    if constexpr (PAGED) {
+    if constexpr (KEYS == PAGES16) {
+      const int key = t * KT + wave_s * 16;
+      if (key < p.span) ids[0] = table_entry(table, fast_div(key, a.page_magic, a.page_shift));
+    } else if constexpr (KEYS == PAGES) {
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int key = t * KT + ld_row + i * RPI;
-        ids[i] = key < p.span ? table[fast_div(key, a.page_magic, a.page_shift)] : 0;
+        if (key < p.span) ids[i] = table[fast_div(key, a.page_magic, a.page_shift)];
       }
     }
   };
   auto load_tile = [&](int t, int stage) {
-    const uint32_t dst = lds0 + stage * 2 * TILE + wave * NI * 1024;
+    const uint32_t dst = lds0 + stage * 2 * TILE + wave_s * NI * 1024;
+    if constexpr (KEYS == PAGES) {
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int r = ld_row + i * RPI, key = t * KT + r;
-      const int chunk = (ld_chunk ^ swizzle<D>(r)) * 8;
-      bool in = key < p.span;
-      int64_t ko, vo;
-      if constexpr (PAGED) {
-        const int page = ids[i];
-        if (in && static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.pages)) {
-          in = false;
-          lacking = true;
-        }
+      for (int i = 0; i < NI; ++i) {
+        const int r = ld_row + i * RPI, key = t * KT + r;
+        const int chunk = (ld_chunk ^ swizzle<D>(r)) * 8;
+        const bool in = key < p.span, has = static_cast<uint32_t>(ids[i]) < static_cast<uint32_t>(a.pages);
+        lacking |= in && !has;
         const int slot = key - static_cast<int>(fast_div(key, a.page_magic, a.page_shift)) * a.page_size;
-        ko = page * a.k_page + slot * a.k_row;
-        vo = page * a.v_page + slot * a.v_row;
-      } else {
-        ko = key * a.k_row;
-        vo = key * a.v_row;
+        const void *kp = kZeros, *vp = kZeros;
+        if (in && has) {
+          kp = kbase + ids[i] * a.k_page + slot * a.k_row + chunk;
+          vp = vbase + ids[i] * a.v_page + slot * a.v_row + chunk;
+        }
+        dma16_flat(dst + i * 1024, kp);
+        dma16_flat(dst + TILE + i * 1024, vp);
       }
-      const void* kp = in ? static_cast<const void*>(kbase + ko + chunk) : kZeros;
-      const void* vp = in ? static_cast<const void*>(vbase + vo + chunk) : kZeros;
-      dma16_flat(dst + i * 1024, kp);
-      dma16_flat(dst + TILE + i * 1024, vp);
+    } else {
+      const uint16_t *kp = kbase, *vp = vbase;
+      int rows;
+      if constexpr (KEYS == DENSE) {
+        rows = min(p.span - t * KT, KT);
+        kp += int64_t{t} * KT * a.k_row;
+        vp += int64_t{t} * KT * a.v_row;
+      } else {
+        const int key = t * KT + wave_s * 16, page = __builtin_amdgcn_readfirstlane(ids[0]);
+        rows = min(p.span - key, 16);
+        if (rows > 0) {
+          if (static_cast<uint32_t>(page) < static_cast<uint32_t>(a.pages)) {
+            const int slot = key - static_cast<int>(fast_div(key, a.page_magic, a.page_shift)) * a.page_size;
+            kp += page * a.k_page + slot * a.k_row;
+            vp += page * a.v_page + slot * a.v_row;
+          } else {
+            rows = 0;
+            lacking = true;
+          }
+        }
+      }
+      const v4i kr = rows_rsrc<D>(kp, rows, a.k_row), vr = rows_rsrc<D>(vp, rows, a.v_row);
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        gemm::dma16<true>(dst + i * 1024, kofs[i], kr);
+        gemm::dma16<true>(dst + TILE + i * 1024, vofs[i], vr);
+      }
     }
   };
 
@@ -384,6 +447,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   const int vchunk = 2 * (g & 1) + ((gi & 3) >> 1);
   const uint32_t vread = lds0 + TILE + vrow * ROWB + (gi & 1) * 8;
 
+  wait_all();
   v16f o[OB];
   float m, l;
   // One pass over the keys; true where it has to be made again with care.
@@ -398,10 +462,11 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
       load_tile(t_begin, 0);
       if (t_begin + 1 < t_end) load_ids(t_begin + 1);
     }
+
     for (int t = t_begin; t < t_end; ++t) {
       const int stage = (t - t_begin) & 1;
       // This wave's part of tile t is in LDS, its reads of the other stage are done; then everybody's.
-      __asm__ volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      wait_all();
       gemm::stage_barrier();
       if (t + 1 < t_end) {
         load_tile(t + 1, stage ^ 1);
@@ -441,7 +506,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
           for (int r = 0; r < 16; ++r) {
             const int key = kofs + 32 * b + 8 * (r >> 2) + (r & 3);
             bool sees = static_cast<uint32_t>(key - rr.lo) < width;
-            if constexpr (PAGED && careful) {
+            if constexpr (KEYS != DENSE && careful) {
               if (sees)
                 sees = static_cast<uint32_t>(table[fast_div(key, a.page_magic, a.page_shift)]) <
                        static_cast<uint32_t>(a.pages);
@@ -588,7 +653,7 @@ __global__ __launch_bounds__(256) void attention_join(const Args a) {
   }
 }
 
-template <int DT, int D, bool PAGED>
+template <int DT, int D, int KEYS>
 int launch(const Args& a, hipStream_t st) {
   const bool mods = a.softcap > 0.0f || a.slopes;
   const int64_t blocks = int64_t{a.slots} * a.kv_heads * a.splits;
@@ -596,7 +661,7 @@ int launch(const Args& a, hipStream_t st) {
     set_error("attention: too many tiles for one launch");
     return M5K_EINVAL;
   }
-  launch_kernel(mods ? attention_tile<DT, D, PAGED, true> : attention_tile<DT, D, PAGED, false>,
+  launch_kernel(mods ? attention_tile<DT, D, KEYS, true> : attention_tile<DT, D, KEYS, false>,
                 dim3(static_cast<uint32_t>(blocks)), dim3(THREADS), st, a);
   int rc = launch_status("attention");
   if (rc != M5K_OK || a.splits == 1) return rc;
@@ -605,11 +670,11 @@ int launch(const Args& a, hipStream_t st) {
   return launch_status("attention join");
 }
 
-template <bool PAGED>
+template <int KEYS>
 int launch_typed(const Args& a, int dtype, int head_dim, hipStream_t st) {
   if (dtype == M5K_BF16)
-    return head_dim == 64 ? launch<M5K_BF16, 64, PAGED>(a, st) : launch<M5K_BF16, 128, PAGED>(a, st);
-  return head_dim == 64 ? launch<M5K_F16, 64, PAGED>(a, st) : launch<M5K_F16, 128, PAGED>(a, st);
+    return head_dim == 64 ? launch<M5K_BF16, 64, KEYS>(a, st) : launch<M5K_BF16, 128, KEYS>(a, st);
+  return head_dim == 64 ? launch<M5K_F16, 64, KEYS>(a, st) : launch<M5K_F16, 128, KEYS>(a, st);
 }
 
 // Packed rows per workgroup and the key splits of a launch: as many as bring the workgroups to two a compute unit

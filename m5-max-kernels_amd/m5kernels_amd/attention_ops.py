@@ -109,6 +109,13 @@ def _rows(t, name, aligned=True):
     return t
 
 
+def _apart(t):
+    """`t` [heads, keys, width], copied where its rows overlap or lie further apart than the kernel's windows reach."""
+    if t.shape[1] > 1 and not t.shape[2] <= t.stride(1) <= 1 << 23:
+        return t.contiguous()
+    return t
+
+
 def _heads_tensor(t, name, dtypes):
     if not isinstance(t, torch.Tensor) or t.dim() != 3:
         raise ValueError(f"{name} must be a [heads, tokens, width] tensor")
@@ -371,7 +378,7 @@ def attention(q, k, v, *, causal=False, window=None, document_starts=None, prefi
     out = torch.empty((tokens, heads * width), dtype=q.dtype, device=device)
     if tokens == 0:
         return out
-    q, k, v = _rows(q, "q"), _rows(k, "k"), _rows(v, "v")
+    q, k, v = _rows(q, "q"), _apart(_rows(k, "k")), _apart(_rows(v, "v"))
     qs, ks, vs = _strides(q), _strides(k), _strides(v)
     splits = _splits(0, tokens, heads, kv_heads, documents, keys, _cu_count_of(device.index))
     workspace, n = _workspace(splits, tokens, heads, width, device)
