@@ -205,6 +205,20 @@ __device__ __forceinline__ float score(float x, const Args& a, float scale2, flo
   }
 }
 
+// V^T fragment of k-step c and channel block b: keys 16 c + 8 h + 4 (lane >> 5) .. + 3 from address at[h].
+template <uint32_t ROWB>
+__device__ __forceinline__ v4i value_frag(const uint32_t (&at)[2], int c, int b) {
+  v4i f;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_v4s>((at[h] ^ (b << 6)) + 16 * c * ROWB));
+    const auto y = __builtin_bit_cast(m5k_u32x2, x);
+    f[2 * h] = static_cast<int>(y[0]);
+    f[2 * h + 1] = static_cast<int>(y[1]);
+  }
+  return f;
+}
+
 // Non-finite 16-bit values of a fragment: zero in `clean`; `mark` holds 1 for +inf, 128 for -inf, 16384 for NaN.
 template <int DT>
 __device__ __forceinline__ void split_nonfinite(v4i f, v4i& clean, v4i& mark) {
@@ -305,7 +319,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   constexpr int NI = CH / WAVES;         // load instructions of a wave, each of K and V
   constexpr int QS = D / 16, OB = D / 32;
   constexpr uint32_t TILE = KT * D * 2, ROWB = D * 2;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[4 * TILE];  // K, V of stage 0, K, V of stage 1
+  __shared__ __attribute__((aligned(256))) uint8_t lds[4 * TILE];  // K stages 0 and 1, V stages 0 and 1
   __shared__ int bounds[2 * WAVES];
 
   const Place p = place<KEYS>(a, 32 * WAVES);
@@ -374,225 +388,267 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     }
   }
   constexpr int NIDS = KEYS == PAGES ? NI : 1;
-  int ids[NIDS] = {};
+  int ids[2][NIDS] = {};  // pages of the next tile's keys, and of the tile before it, whose values come next
   bool lacking = false;
 
-  // Pages of tile t's rows, one tile ahead of their use.
-  auto load_ids = [&](int t) {
+  // Unconditional, at the last key where tile t has none: a load under a condition would be waited for at the
+  // condition's end, and with it everything in flight.
+  auto load_ids = [&](int t, int (&to)[NIDS]) __attribute__((always_inline)) {
     if constexpr (KEYS == PAGES16) {
-      const int key = t * KT + wave_s * 16;
-      if (key < p.span) ids[0] = table_entry(table, fast_div(key, a.page_magic, a.page_shift));
+      const int key = min(t * KT + wave_s * 16, p.span - 1);
+      to[0] = table_entry(table, fast_div(key, a.page_magic, a.page_shift));
     } else if constexpr (KEYS == PAGES) {
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        const int key = t * KT + ld_row + i * RPI;
-        if (key < p.span) ids[i] = table[fast_div(key, a.page_magic, a.page_shift)];
+        const int key = min(t * KT + ld_row + i * RPI, p.span - 1);
+        to[i] = table[fast_div(key, a.page_magic, a.page_shift)];
       }
     }
   };
-  auto load_tile = [&](int t, int stage) {
-    const uint32_t dst = lds0 + stage * 2 * TILE + wave_s * NI * 1024;
+  // This wave's 16 rows of tile t of one operand to LDS at dst.
+  auto load_rows = [&](int t, const int (&id)[NIDS], const uint16_t* base, int64_t page_stride, int64_t row_stride,
+                       const uint32_t (&ofs)[NI], uint32_t dst) __attribute__((always_inline)) {
+    dst += wave_s * NI * 1024;
     if constexpr (KEYS == PAGES) {
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int r = ld_row + i * RPI, key = t * KT + r;
         const int chunk = (ld_chunk ^ swizzle<D>(r)) * 8;
-        const bool in = key < p.span, has = static_cast<uint32_t>(ids[i]) < static_cast<uint32_t>(a.pages);
+        const bool in = key < p.span, has = static_cast<uint32_t>(id[i]) < static_cast<uint32_t>(a.pages);
         lacking |= in && !has;
         const int slot = key - static_cast<int>(fast_div(key, a.page_magic, a.page_shift)) * a.page_size;
-        const void *kp = kZeros, *vp = kZeros;
-        if (in && has) {
-          kp = kbase + ids[i] * a.k_page + slot * a.k_row + chunk;
-          vp = vbase + ids[i] * a.v_page + slot * a.v_row + chunk;
-        }
-        dma16_flat(dst + i * 1024, kp);
-        dma16_flat(dst + TILE + i * 1024, vp);
+        const void* at = kZeros;
+        if (in && has) at = base + id[i] * page_stride + slot * row_stride + chunk;
+        dma16_flat(dst + i * 1024, at);
       }
     } else {
-      const uint16_t *kp = kbase, *vp = vbase;
       int rows;
       if constexpr (KEYS == DENSE) {
         rows = min(p.span - t * KT, KT);
-        kp += int64_t{t} * KT * a.k_row;
-        vp += int64_t{t} * KT * a.v_row;
+        base += int64_t{t} * KT * row_stride;
       } else {
-        const int key = t * KT + wave_s * 16, page = __builtin_amdgcn_readfirstlane(ids[0]);
+        const int key = t * KT + wave_s * 16, page = __builtin_amdgcn_readfirstlane(id[0]);
         rows = min(p.span - key, 16);
         if (rows > 0) {
           if (static_cast<uint32_t>(page) < static_cast<uint32_t>(a.pages)) {
             const int slot = key - static_cast<int>(fast_div(key, a.page_magic, a.page_shift)) * a.page_size;
-            kp += page * a.k_page + slot * a.k_row;
-            vp += page * a.v_page + slot * a.v_row;
+            base += page * page_stride + slot * row_stride;
           } else {
             rows = 0;
             lacking = true;
           }
         }
       }
-      const v4i kr = rows_rsrc<D>(kp, rows, a.k_row), vr = rows_rsrc<D>(vp, rows, a.v_row);
+      const v4i rsrc = rows_rsrc<D>(base, rows, row_stride);
 #pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        gemm::dma16<true>(dst + i * 1024, kofs[i], kr);
-        gemm::dma16<true>(dst + TILE + i * 1024, vofs[i], vr);
-      }
+      for (int i = 0; i < NI; ++i) gemm::dma16<true>(dst + i * 1024, ofs[i], rsrc);
     }
   };
 
-  // Fragment addresses.
-  const int krow = lane & 31;
-  const uint32_t kread = lds0 + krow * ROWB;
-  const int ksw = swizzle<D>(krow);
+  // Fragment addresses: chunk c of a row is its chunk 0 XOR 16 c, rows being aligned to their size.
+  const uint32_t kread = lds0 + (lane & 31) * ROWB + ((half ^ swizzle<D>(lane & 31)) << 4);
   const int g = lane >> 4, gi = lane & 15;
-  const int vrow = 4 * half + (gi >> 2);
-  const int vchunk = 2 * (g & 1) + ((gi & 3) >> 1);
-  const uint32_t vread = lds0 + TILE + vrow * ROWB + (gi & 1) * 8;
+  const int vrow = 4 * half + (gi >> 2), vchunk = 2 * (g & 1) + ((gi & 3) >> 1);
+  uint32_t vread[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    vread[h] = lds0 + 2 * TILE + (8 * h + vrow) * ROWB + ((vchunk ^ swizzle<D>(8 * h + vrow)) << 4) + (gi & 1) * 8;
 
   wait_all();
-  v16f o[OB];
+  v16f o[OB], s[2][NB];
+  v4i pf[2 * NB];
   float m, l;
-  // One pass over the keys; true where it has to be made again with care.
-  auto pass = [&](auto with_care) -> bool {
+
+  // Scores of tile t, from K at stage `st`.
+  auto product = [&](v16f (&x)[NB], int st) __attribute__((always_inline)) {
+    uint32_t at = kread + st * TILE;
+    __asm__("" : "+v"(at));  // addresses by XOR, not kept in registers
+#pragma unroll
+    for (int c = 0; c < QS; ++c)
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const v4i kf = *reinterpret_cast<const __attribute__((address_space(3))) v4i*>((at ^ (c << 5)) + b * 32 * ROWB);
+        x[b] = mfma32<DT>(kf, qf[c], c == 0 ? v16f{} : x[b]);
+      }
+  };
+  // Cap, bias and mask of tile t's scores.
+  auto finish = [&](v16f (&x)[NB], int t, auto with_care, uint32_t& sees_bits) __attribute__((always_inline)) {
     constexpr bool careful = decltype(with_care)::value;
-    m = M_FLOOR;
-    l = 0.0f;
-#pragma unroll
-    for (int b = 0; b < OB; ++b) o[b] = v16f{};
-    if (t_begin < t_end) {
-      load_ids(t_begin);
-      load_tile(t_begin, 0);
-      if (t_begin + 1 < t_end) load_ids(t_begin + 1);
-    }
-
-    for (int t = t_begin; t < t_end; ++t) {
-      const int stage = (t - t_begin) & 1;
-      // This wave's part of tile t is in LDS, its reads of the other stage are done; then everybody's.
-      wait_all();
-      gemm::stage_barrier();
-      if (t + 1 < t_end) {
-        load_tile(t + 1, stage ^ 1);
-        if (t + 2 < t_end) load_ids(t + 2);
-      }
-      const int key0 = t * KT;
-      if (key0 + KT <= any_lo || key0 >= any_hi) continue;  // the same for the whole wave
-      const uint32_t kst = kread + stage * 2 * TILE, vst = vread + stage * 2 * TILE;
-
-      v16f s[NB];
-#pragma unroll
-      for (int b = 0; b < NB; ++b) s[b] = v16f{};
-#pragma unroll
-      for (int c = 0; c < QS; ++c) {
-        const uint32_t at = kst + (((2 * c + half) ^ ksw) << 4);
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          const v4i kf = *reinterpret_cast<const __attribute__((address_space(3))) v4i*>(at + b * 32 * ROWB);
-          s[b] = mfma32<DT>(kf, qf[c], s[b]);
-        }
-      }
-
-      uint32_t seen = 0;  // careful mode: the keys of this lane's registers that the row sees
-      const int kofs = key0 + 4 * half;
-      if constexpr (MODS) {
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            s[b][r] = score<MODS>(s[b][r], a, scale2, slope2, rr.pos, kofs + 32 * b + 8 * (r >> 2) + (r & 3));
-      }
-      if (careful || key0 < all_lo || key0 + KT > all_hi) {
-        const uint32_t width = static_cast<uint32_t>(max(rr.hi - rr.lo, 0));
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int key = kofs + 32 * b + 8 * (r >> 2) + (r & 3);
-            bool sees = static_cast<uint32_t>(key - rr.lo) < width;
-            if constexpr (KEYS != DENSE && careful) {
-              if (sees)
-                sees = static_cast<uint32_t>(table[fast_div(key, a.page_magic, a.page_shift)]) <
-                       static_cast<uint32_t>(a.pages);
-            }
-            if constexpr (careful) seen |= static_cast<uint32_t>(sees) << (16 * b + r);
-            s[b][r] = sees ? s[b][r] : -__builtin_inff();
-          }
-      }
-
-      float top = s[0][0];
+    const int key0 = t * KT, kofs0 = key0 + 4 * half;
+    if constexpr (MODS) {
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
-      top = max_halves(top) * unit;
-      if (__builtin_amdgcn_ballot_w64(top > m + LAZY)) {
-        const float next = fmaxf(m, top);
-        const float f = __builtin_amdgcn_exp2f(m - next);
-        m = next;
-        l *= f;
+        for (int r = 0; r < 16; ++r)
+          x[b][r] = score<MODS>(x[b][r], a, scale2, slope2, rr.pos, kofs0 + 32 * b + 8 * (r >> 2) + (r & 3));
+    }
+    if (careful || key0 < all_lo || key0 + KT > all_hi) {
+      const uint32_t width = static_cast<uint32_t>(max(rr.hi - rr.lo, 0));
+      if constexpr (careful) sees_bits = 0;
 #pragma unroll
-        for (int b = 0; b < OB; ++b)
+      for (int b = 0; b < NB; ++b)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) o[b][r] *= f;
-      }
-      v4i pf[2 * NB];
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        float sum = 0.0f;
-#pragma unroll
-        for (int r = 0; r < 16; r += 2) {
-          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], unit, -m));
-          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r + 1], unit, -m));
-          sum += p0;
-          sum += p1;
-          pf[2 * b + (r >> 3)][(r & 7) >> 1] = static_cast<int>(pack2<DT>(p0, p1));
+        for (int r = 0; r < 16; ++r) {
+          const int key = kofs0 + 32 * b + 8 * (r >> 2) + (r & 3);
+          bool sees = static_cast<uint32_t>(key - rr.lo) < width;
+          if constexpr (KEYS != DENSE && careful) {
+            if (sees)
+              sees = static_cast<uint32_t>(table[fast_div(key, a.page_magic, a.page_shift)]) <
+                     static_cast<uint32_t>(a.pages);
+          }
+          if constexpr (careful) sees_bits |= static_cast<uint32_t>(sees) << (16 * b + r);
+          x[b][r] = sees ? x[b][r] : -__builtin_inff();
         }
-        l += sum;
+    }
+  };
+  auto maximum = [&](const v16f (&x)[NB]) __attribute__((always_inline)) {
+    float t0 = x[0][0], t1 = x[0][1];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        t0 = fmaxf(t0, x[b][r]);
+        t1 = fmaxf(t1, x[b][r + 1]);
       }
-
+    return fmaxf(t0, t1);
+  };
+  // Probabilities of a tile against the running maximum, packed for the second product; their sum.
+  auto probabilities = [&](const v16f (&x)[NB]) __attribute__((always_inline)) {
+    float sum[2] = {};
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][r], unit, -m));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][r + 1], unit, -m));
+        sum[0] += p0;
+        sum[1] += p1;
+        pf[2 * b + (r >> 3)][(r & 7) >> 1] = static_cast<int>(pack2<DT>(p0, p1));
+      }
+    l += sum[0] + sum[1];
+  };
+  // O += V^T P of a tile, V at stage `st`.
+  auto accumulate = [&](int st, auto with_care, uint32_t sees_bits) __attribute__((always_inline)) {
+    constexpr bool careful = decltype(with_care)::value;
+    uint32_t at[2] = {vread[0] + st * TILE, vread[1] + st * TILE};
+    __asm__("" : "+v"(at[0]), "+v"(at[1]));
+    if constexpr (!careful) {
+#pragma unroll
+      for (int c = 0; c < 2 * NB; ++c)
+#pragma unroll
+        for (int b = 0; b < OB; ++b) o[b] = mfma32<DT>(value_frag<ROWB>(at, c, b), pf[c], o[b]);
+    } else {
 #pragma unroll
       for (int b = 0; b < OB; ++b) {
         v16f marks = {};
 #pragma unroll
         for (int c = 0; c < 2 * NB; ++c) {
-          v4i vf;
+          v4i clean, mark, see;
+          split_nonfinite<DT>(value_frag<ROWB>(at, c, b), clean, mark);
+          const uint32_t one = pack2<DT>(1.0f, 1.0f);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            // Row 16 c + 8 h + vrow: its swizzle's low bits are (2 h + half) & 3 at D = 128, and rows 8 apart are
-            // alike at D = 64 but for the same two bits.
-            const int sw = swizzle<D>(8 * h + vrow);
-            const uint32_t at = vst + (16 * c + 8 * h) * ROWB + (((4 * b + vchunk) ^ sw) << 4);
-            const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_v4s>(at));
-            const auto y = __builtin_bit_cast(uint2, x);
-            vf[2 * h] = static_cast<int>(y.x);
-            vf[2 * h + 1] = static_cast<int>(y.y);
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t bits = sees_bits >> (8 * c + 2 * w);
+            see[w] = static_cast<int>(((bits & 1u) ? one & 0xFFFFu : 0u) | ((bits & 2u) ? one & 0xFFFF0000u : 0u));
           }
-          if constexpr (careful) {
-            v4i clean, mark, see;
-            split_nonfinite<DT>(vf, clean, mark);
-            const uint32_t one = pack2<DT>(1.0f, 1.0f);
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              const uint32_t bits = seen >> (8 * c + 2 * w);
-              see[w] = static_cast<int>(((bits & 1u) ? one & 0xFFFFu : 0u) | ((bits & 2u) ? one & 0xFFFF0000u : 0u));
-            }
-            marks = mfma32<DT>(mark, see, marks);
-            vf = clean;
-            __builtin_amdgcn_sched_barrier(0);  // rare: few registers rather than overlap
-          }
-          o[b] = mfma32<DT>(vf, pf[c], o[b]);
+          marks = mfma32<DT>(mark, see, marks);
+          o[b] = mfma32<DT>(clean, pf[c], o[b]);
+          __builtin_amdgcn_sched_barrier(0);  // rare: few registers rather than overlap
         }
-        if constexpr (careful) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) o[b][r] += nonfinite_sum(marks[r]);
-        }
+        for (int r = 0; r < 16; ++r) o[b][r] += nonfinite_sum(marks[r]);
       }
     }
-    float check = 0.0f;
-#pragma unroll
-    for (int b = 0; b < OB; ++b)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) check = __builtin_fmaf(o[b][r], 0.0f, check);
-    return __syncthreads_or(lacking || check != 0.0f) != 0;
   };
-  if (pass(std::false_type{})) pass(std::true_type{});
+  // Adopt a tile maximum where a row's exceeds the running one by more than LAZY.
+  auto adopt = [&](float tile_top) __attribute__((always_inline)) {
+    const float t = max_halves(tile_top) * unit;
+    if (__builtin_amdgcn_ballot_w64(t > m + LAZY)) {
+      const float next = fmaxf(m, t), f = __builtin_amdgcn_exp2f(m - next);
+      m = next;
+      l *= f;
+#pragma unroll
+      for (int b = 0; b < OB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[b][r] *= f;
+    }
+  };
+
+  const int first = max(t_begin, any_lo / KT), last = min(t_end, (any_hi + KT - 1) / KT);  // this wave's tiles
+  auto start = [&]() __attribute__((always_inline)) {
+    m = M_FLOOR;
+    l = 0.0f;
+#pragma unroll
+    for (int b = 0; b < OB; ++b) o[b] = v16f{};
+  };
+
+  // Step t turns the scores of tile t into its part of O, and makes the scores of tile t + 1 meanwhile, so that the
+  // matrix cores have work beside the exponentials.  Tile t's K and V are in stage t & 1 of each; step t loads K of
+  // tile t + 2 and V of tile t + 1 over what step t - 1 was the last to read.
+  constexpr std::false_type quick{};
+  auto step = [&](int t, v16f (&x)[NB], v16f (&next)[NB]) __attribute__((always_inline)) {
+    wait_all();
+    gemm::stage_barrier();
+    if (t + 1 < t_end) {
+      load_rows(t + 1, ids[1], vbase, a.v_page, a.v_row, vofs, lds0 + (2 + ((t + 1) & 1)) * TILE);
+      if (t + 2 < t_end) load_rows(t + 2, ids[0], kbase, a.k_page, a.k_row, kofs, lds0 + (t & 1) * TILE);
+    }
+#pragma unroll
+    for (int i = 0; i < NIDS; ++i) ids[1][i] = ids[0][i];
+    load_ids(t + 3, ids[0]);
+    uint32_t none;
+    const bool now = t >= first && t < last, then = t + 1 >= first && t + 1 < last;  // the same for the whole wave
+    if (now && then) {
+      product(next, (t + 1) & 1);
+      probabilities(x);
+      finish(next, t + 1, quick, none);
+      accumulate(t & 1, quick, 0);
+      adopt(maximum(next));
+    } else if (then) {
+      product(next, (t + 1) & 1);
+      finish(next, t + 1, quick, none);
+      adopt(maximum(next));
+    } else if (now) {
+      probabilities(x);
+      accumulate(t & 1, quick, 0);
+    }
+  };
+  start();
+  if (t_begin < t_end) {
+    load_ids(t_begin, ids[1]);
+    load_rows(t_begin, ids[1], kbase, a.k_page, a.k_row, kofs, lds0 + (t_begin & 1) * TILE);
+    load_ids(t_begin + 1, ids[0]);
+    for (int t = t_begin - 1; t < t_end; t += 2) {
+      step(t, s[0], s[1]);
+      if (t + 1 < t_end) step(t + 1, s[1], s[0]);
+    }
+  }
+  float check = 0.0f;
+#pragma unroll
+  for (int b = 0; b < OB; ++b)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) check = __builtin_fmaf(o[b][r], 0.0f, check);
+  if (__syncthreads_or(lacking || check != 0.0f)) {
+    constexpr std::true_type careful{};
+    start();
+    for (int t = t_begin; t < t_end; ++t) {
+      load_ids(t, ids[0]);
+      load_rows(t, ids[0], kbase, a.k_page, a.k_row, kofs, lds0);
+      load_rows(t, ids[0], vbase, a.v_page, a.v_row, vofs, lds0 + 2 * TILE);
+      wait_all();
+      gemm::stage_barrier();
+      if (t >= first && t < last) {
+        uint32_t sees;
+        product(s[0], 0);
+        finish(s[0], t, careful, sees);
+        adopt(maximum(s[0]));
+        probabilities(s[0]);
+        accumulate(0, careful, sees);
+      }
+      wait_all();
+      gemm::stage_barrier();
+    }
+  }
 
   l += other_half(l);
   if (!live) return;
