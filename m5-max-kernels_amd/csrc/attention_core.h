@@ -459,17 +459,43 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   v4i pf[2 * NB];
   float m, l;
 
-  // Scores of tile t, from K at stage `st`.
-  auto product = [&](v16f (&x)[NB], int st) __attribute__((always_inline)) {
+  // Scores of a tile, from K at stage `st`; beside them, where `prob`, the probabilities of the tile before against the
+  // running maximum, packed for the second product, and their sum.  A 32 x 32 x 16 product holds the matrix cores for
+  // 32 cycles, in which the wave issues 8 VALU instructions: each step's fence keeps its share of the exponentials
+  // between its products, and the next step's fragments on their way.
+  auto key_frags = [&](uint32_t at, int c, v4i (&f)[NB]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+      f[b] = *reinterpret_cast<const __attribute__((address_space(3))) v4i*>((at ^ (c << 5)) + b * 32 * ROWB);
+  };
+  auto probabilities = [&](const v16f (&x)[NB], int from, int to, float (&sum)[2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = from; e < to; e += 2) {
+      const int b = e >> 4, r = e & 15;
+      const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][r], unit, -m));
+      const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][r + 1], unit, -m));
+      sum[0] += p0;
+      sum[1] += p1;
+      uint32_t w = pack2<DT>(p0, p1);
+      __asm__ volatile("" : "+v"(w), "+v"(sum[0]), "+v"(sum[1]));  // made here, not where they are read
+      pf[2 * b + (r >> 3)][(r & 7) >> 1] = static_cast<int>(w);
+    }
+  };
+  auto product = [&](v16f (&y)[NB], int st, const v16f (&x)[NB], bool prob) __attribute__((always_inline)) {
     uint32_t at = kread + st * TILE;
     __asm__("" : "+v"(at));  // addresses by XOR, not kept in registers
+    v4i kf[2][NB];
+    float sum[2] = {};
+    key_frags(at, 0, kf[0]);
 #pragma unroll
-    for (int c = 0; c < QS; ++c)
+    for (int c = 0; c < QS; ++c) {
+      if (c + 1 < QS) key_frags(at, c + 1, kf[(c + 1) & 1]);
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const v4i kf = *reinterpret_cast<const __attribute__((address_space(3))) v4i*>((at ^ (c << 5)) + b * 32 * ROWB);
-        x[b] = mfma32<DT>(kf, qf[c], c == 0 ? v16f{} : x[b]);
-      }
+      for (int b = 0; b < NB; ++b) y[b] = mfma32<DT>(kf[c & 1][b], qf[c], c == 0 ? v16f{} : y[b]);
+      if (prob) probabilities(x, c * 32 / QS, (c + 1) * 32 / QS, sum);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (prob) l += sum[0] + sum[1];
   };
   // Cap, bias and mask of tile t's scores.
   auto finish = [&](v16f (&x)[NB], int t, auto with_care, uint32_t& sees_bits) __attribute__((always_inline)) {
@@ -501,64 +527,64 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
         }
     }
   };
-  auto maximum = [&](const v16f (&x)[NB]) __attribute__((always_inline)) {
-    float t0 = x[0][0], t1 = x[0][1];
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int r = 0; r < 16; r += 2) {
-        t0 = fmaxf(t0, x[b][r]);
-        t1 = fmaxf(t1, x[b][r + 1]);
-      }
-    return fmaxf(t0, t1);
-  };
-  // Probabilities of a tile against the running maximum, packed for the second product; their sum.
-  auto probabilities = [&](const v16f (&x)[NB]) __attribute__((always_inline)) {
-    float sum[2] = {};
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int r = 0; r < 16; r += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][r], unit, -m));
-        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][r + 1], unit, -m));
-        sum[0] += p0;
-        sum[1] += p1;
-        pf[2 * b + (r >> 3)][(r & 7) >> 1] = static_cast<int>(pack2<DT>(p0, p1));
-      }
-    l += sum[0] + sum[1];
-  };
-  // O += V^T P of a tile, V at stage `st`.
-  auto accumulate = [&](int st, auto with_care, uint32_t sees_bits) __attribute__((always_inline)) {
-    constexpr bool careful = decltype(with_care)::value;
+  // O += V^T P of a tile, V at stage `st`, in steps of two products as above; beside them the maximum of the scores x.
+  auto accumulate = [&](int st, const v16f (&x)[NB]) __attribute__((always_inline)) -> float {
+    constexpr int STEPS = 2 * NB * OB / 2;
     uint32_t at[2] = {vread[0] + st * TILE, vread[1] + st * TILE};
     __asm__("" : "+v"(at[0]), "+v"(at[1]));
-    if constexpr (!careful) {
+    v4i vf[2][2];
+    float t0 = x[0][0], t1 = x[0][1];
 #pragma unroll
-      for (int c = 0; c < 2 * NB; ++c)
+    for (int j = 0; j < 2; ++j) vf[0][j] = value_frag<ROWB>(at, 0, j);
 #pragma unroll
-        for (int b = 0; b < OB; ++b) o[b] = mfma32<DT>(value_frag<ROWB>(at, c, b), pf[c], o[b]);
-    } else {
+    for (int i = 0; i < STEPS; ++i) {
+      if (i + 1 < STEPS) {
 #pragma unroll
-      for (int b = 0; b < OB; ++b) {
-        v16f marks = {};
-#pragma unroll
-        for (int c = 0; c < 2 * NB; ++c) {
-          v4i clean, mark, see;
-          split_nonfinite<DT>(value_frag<ROWB>(at, c, b), clean, mark);
-          const uint32_t one = pack2<DT>(1.0f, 1.0f);
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const uint32_t bits = sees_bits >> (8 * c + 2 * w);
-            see[w] = static_cast<int>(((bits & 1u) ? one & 0xFFFFu : 0u) | ((bits & 2u) ? one & 0xFFFF0000u : 0u));
-          }
-          marks = mfma32<DT>(mark, see, marks);
-          o[b] = mfma32<DT>(clean, pf[c], o[b]);
-          __builtin_amdgcn_sched_barrier(0);  // rare: few registers rather than overlap
-        }
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[b][r] += nonfinite_sum(marks[r]);
+        for (int j = 0; j < 2; ++j)
+          vf[(i + 1) & 1][j] = value_frag<ROWB>(at, (2 * i + 2) / OB, (2 * i + 2) % OB + j);
       }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int b = 2 * i % OB + j;
+        o[b] = mfma32<DT>(vf[i & 1][j], pf[2 * i / OB], o[b]);
+      }
+#pragma unroll
+      for (int e = i * 32 / STEPS; e < (i + 1) * 32 / STEPS; e += 2) {
+        t0 = fmaxf(t0, x[e >> 4][e & 15]);
+        t1 = fmaxf(t1, x[e >> 4][(e & 15) + 1]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
+    return fmaxf(t0, t1);
+  };
+  // The same with care: non-finite values apart, for the keys in `bits`.
+  auto accumulate_careful = [&](uint32_t bits) __attribute__((always_inline)) {
+#pragma unroll
+    for (int b = 0; b < OB; ++b) {
+      v16f marks = {};
+#pragma unroll
+      for (int c = 0; c < 2 * NB; ++c) {
+        v4i clean, mark, see;
+        split_nonfinite<DT>(value_frag<ROWB>(vread, c, b), clean, mark);
+        const uint32_t one = pack2<DT>(1.0f, 1.0f);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t two = bits >> (8 * c + 2 * w);
+          see[w] = static_cast<int>(((two & 1u) ? one & 0xFFFFu : 0u) | ((two & 2u) ? one & 0xFFFF0000u : 0u));
+        }
+        marks = mfma32<DT>(mark, see, marks);
+        o[b] = mfma32<DT>(clean, pf[c], o[b]);
+        __builtin_amdgcn_sched_barrier(0);  // rare: few registers rather than overlap
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[b][r] += nonfinite_sum(marks[r]);
+    }
+  };
+  auto maximum = [&](const v16f (&x)[NB]) __attribute__((always_inline)) {
+    float t0 = x[0][0];
+#pragma unroll
+    for (int e = 1; e < 32; ++e) t0 = fmaxf(t0, x[e >> 4][e & 15]);
+    return t0;
   };
   // Adopt a tile maximum where a row's exceeds the running one by more than LAZY.
   auto adopt = [&](float tile_top) __attribute__((always_inline)) {
@@ -599,18 +625,18 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     uint32_t none;
     const bool now = t >= first && t < last, then = t + 1 >= first && t + 1 < last;  // the same for the whole wave
     if (now && then) {
-      product(next, (t + 1) & 1);
-      probabilities(x);
+      product(next, (t + 1) & 1, x, true);
       finish(next, t + 1, quick, none);
-      accumulate(t & 1, quick, 0);
-      adopt(maximum(next));
+      adopt(accumulate(t & 1, next));
     } else if (then) {
-      product(next, (t + 1) & 1);
+      product(next, (t + 1) & 1, x, false);
       finish(next, t + 1, quick, none);
       adopt(maximum(next));
     } else if (now) {
-      probabilities(x);
-      accumulate(t & 1, quick, 0);
+      float sum[2] = {};
+      probabilities(x, 0, 32, sum);
+      l += sum[0] + sum[1];
+      accumulate(t & 1, x);
     }
   };
   start();
@@ -639,11 +665,13 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
       gemm::stage_barrier();
       if (t >= first && t < last) {
         uint32_t sees;
-        product(s[0], 0);
+        product(s[0], 0, s[1], false);
         finish(s[0], t, careful, sees);
         adopt(maximum(s[0]));
-        probabilities(s[0]);
-        accumulate(0, careful, sees);
+        float sum[2] = {};
+        probabilities(s[0], 0, 32, sum);
+        l += sum[0] + sum[1];
+        accumulate_careful(sees);
       }
       wait_all();
       gemm::stage_barrier();
