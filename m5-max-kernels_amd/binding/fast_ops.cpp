@@ -1,9 +1,10 @@
 // Native front of the calls that a projection makes, quantize(), gemm() and the Q/K and Q/K/V
-// projections: the argument checks, the output allocation and the launches of a plain call, without the
-// interpreter.
+// projections, and of the attention step behind them (attention_ops.py): the argument checks, the output
+// allocation and the launches of a plain call, without the interpreter.
 //
-// Each function takes a call only if it can see that the Python front (hip.py) would accept it and
-// launch at once: plain CUDA tensors, contiguous, of the right dtypes and shapes, no forced schedule.
+// Each function takes a call only if it can see that the Python front (hip.py, attention_ops.py) would accept it
+// and launch at once: plain CUDA tensors, contiguous (heads and caches: rows that the kernels read in place), of the
+// right dtypes and shapes, no forced schedule.
 // Anything else returns None, and the Python front handles the call and raises what it raises: no error
 // is decided here.  The launches are the same C ABI calls, with the interpreter lock released.
 //
@@ -11,6 +12,7 @@
 // the HIP launch takes about 3 each.  The projections' staged form, two launches, takes
 // 18 to 20 us through Python and 8 to 10 us here; the fused one 10 to 13 and 5 to 6 us.
 #include <Python.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -39,9 +41,9 @@ int dtype_code(at::ScalarType t) {
   }
 }
 
-// A tensor whose storage a kernel may read as it is: exactly torch.Tensor (or Parameter), strided and
-// contiguous on a GPU, and not a wrapper of a transform (vmap, forward or reverse mode of torch.func).
-const at::Tensor* plain(PyObject* o) {
+// A tensor whose storage a kernel may read as it is: exactly torch.Tensor (or Parameter), strided (plain():
+// contiguous) on a GPU, and not a wrapper of a transform (vmap, forward or reverse mode of torch.func).
+const at::Tensor* plain_strided(PyObject* o) {
   if (!THPVariable_CheckExact(o)) return nullptr;
   const at::Tensor& t = THPVariable_Unpack(o);
   const c10::DispatchKeySet keys = t.key_set();
@@ -49,9 +51,14 @@ const at::Tensor* plain(PyObject* o) {
       keys.has_any(c10::DispatchKeySet({c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
                                         c10::DispatchKey::Functionalize, c10::DispatchKey::Python,
                                         c10::DispatchKey::Conjugate, c10::DispatchKey::Negative})) ||
-      !t.has_storage() || !t.is_contiguous())
+      !t.has_storage())
     return nullptr;
   return &t;
+}
+
+const at::Tensor* plain(PyObject* o) {
+  const at::Tensor* t = plain_strided(o);
+  return t && t->is_contiguous() ? t : nullptr;
 }
 
 bool vector_of(const at::Tensor* t, int64_t n, at::ScalarType st, c10::Device d) {
@@ -405,6 +412,304 @@ PyObject* qkv(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- the attention step ---------------------------------------------------------------------------
+
+// Stride in elements, 0 along an axis of one entry.
+int64_t stride(const at::Tensor& t, int d) { return t.size(d) == 1 ? 0 : t.stride(d); }
+
+// Whether the rows (last axis) of a tensor begin at multiples of 16 bytes and are contiguous.
+bool rows16(const at::Tensor& t) {
+  const int last = static_cast<int>(t.dim()) - 1;
+  if (t.size(last) > 1 && t.stride(last) != 1) return false;
+  const int64_t unit = 16 / static_cast<int64_t>(t.element_size());
+  for (int d = 0; d < last; ++d)
+    if (stride(t, d) % unit) return false;
+  return aligned16(t.data_ptr());
+}
+
+// The launches go to the current device.
+bool current(c10::Device d) { return c10::impl::VirtualGuardImpl(d.type()).getDevice().index() == d.index(); }
+
+// A positive finite float as attention_ops.py takes it, `absent` for None; false: let Python look at it.
+bool positive(PyObject* o, float absent, float& out) {
+  if (o == Py_None) {
+    out = absent;
+    return true;
+  }
+  if (!PyFloat_CheckExact(o)) return false;
+  const double v = PyFloat_AS_DOUBLE(o);
+  out = static_cast<float>(v);
+  return v > 0.0 && v < 1e30 && out > 0.0f;
+}
+
+// A positive int below 2^30, 0 for None.
+bool window_of(PyObject* o, int64_t& out) {
+  out = 0;
+  if (o == Py_None) return true;
+  if (!PyLong_CheckExact(o)) return false;
+  int overflow = 0;
+  out = PyLong_AsLongLongAndOverflow(o, &overflow);
+  return !overflow && out > 0 && out < (int64_t{1} << 30);
+}
+
+// An int32 (or other) vector of n entries, null for None; false: let Python look at it.
+template <class T>
+bool optional_vector(PyObject* o, int64_t n, at::ScalarType st, c10::Device d, const T** out) {
+  *out = nullptr;
+  if (o == Py_None) return true;
+  const at::Tensor* t = plain(o);
+  if (!vector_of(t, n, st, d)) return false;
+  *out = static_cast<const T*>(t->data_ptr());
+  return true;
+}
+
+// layout "half" 0, "interleaved" 1, anything else -1.
+int layout_of(PyObject* o) {
+  if (!PyUnicode_Check(o)) return -1;
+  if (PyUnicode_CompareWithASCIIString(o, "half") == 0) return 0;
+  return PyUnicode_CompareWithASCIIString(o, "interleaved") == 0 ? 1 : -1;
+}
+
+const at::Tensor* frequencies_of(PyObject* o, int64_t width, c10::Device d) {
+  const at::Tensor* f = plain(o);
+  return f && f->dim() == 1 && f->scalar_type() == at::kDouble && f->device() == d && f->size(0) >= 1 &&
+                 2 * f->size(0) <= width
+             ? f
+             : nullptr;
+}
+
+// [heads, tokens, width] of a float type with contiguous channels.
+const at::Tensor* heads_of(PyObject* o) {
+  const at::Tensor* t = plain_strided(o);
+  return t && t->dim() == 3 && t->size(0) > 0 && t->size(1) > 0 && t->size(2) > 0 &&
+                 dtype_code(t->scalar_type()) >= 0 && (t->size(2) == 1 || t->stride(2) == 1)
+             ? t
+             : nullptr;
+}
+
+bool half_type(const at::Tensor& t) { return t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16; }
+
+// rope(x, positions, frequencies, layout, magnitude).
+PyObject* rope(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  const at::Tensor* x = nargs == 5 ? heads_of(args[0]) : nullptr;
+  const int layout = nargs == 5 ? layout_of(args[3]) : -1;
+  float magnitude;
+  if (!x || layout < 0 || !current(x->device()) || args[4] == Py_None || !positive(args[4], 1.0f, magnitude))
+    Py_RETURN_NONE;
+  const c10::Device dev = x->device();
+  const int64_t heads = x->size(0), tokens = x->size(1), width = x->size(2);
+  const at::Tensor *p = plain(args[1]), *f = frequencies_of(args[2], width, dev);
+  if (!f || !vector_of(p, tokens, at::kInt, dev)) Py_RETURN_NONE;
+  void* stream = nullptr;
+  if (!stream_of(dev, &stream)) return nullptr;
+  at::Tensor y = empty({heads, tokens, width}, x->scalar_type(), dev);
+  const void* xp = x->data_ptr();
+  const auto* pp = static_cast<const int32_t*>(p->data_ptr());
+  const auto* fp = static_cast<const double*>(f->data_ptr());
+  void* yp = y.data_ptr();
+  const int64_t sh = stride(*x, 0), st = stride(*x, 1), pairs = f->size(0);
+  const int code = dtype_code(x->scalar_type());
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = m5k_rope(xp, code, tokens, heads, width, sh, st, pp, fp, pairs, layout, magnitude, yp, stream);
+  Py_END_ALLOW_THREADS
+  if (rc) return failed("m5k_rope", rc);
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// A paged cache and the vectors that describe its sequences.
+struct Paged {
+  const at::Tensor *k, *v;
+  const int32_t *table, *starts, *context;
+  int64_t sequences, width, pages, kv_heads, page_size, dim;
+};
+
+// Takes args k_cache, v_cache, page_table, query_starts, context_lengths.
+bool paged_of(PyObject* const* args, Paged& out) {
+  const at::Tensor *k = plain_strided(args[0]), *v = plain_strided(args[1]), *t = plain(args[2]);
+  if (!k || !v || !t || k->dim() != 4 || v->sizes() != k->sizes() || v->scalar_type() != k->scalar_type() ||
+      v->device() != k->device() || k->numel() == 0 || k->stride(3) != 1 || v->stride(3) != 1)
+    return false;
+  const c10::Device dev = k->device();
+  if (t->dim() != 2 || t->scalar_type() != at::kInt || t->device() != dev || t->numel() == 0) return false;
+  out = Paged{k, v, static_cast<const int32_t*>(t->data_ptr()), nullptr, nullptr, t->size(0), t->size(1),
+              k->size(0), k->size(1), k->size(2), k->size(3)};
+  return out.page_size <= (1 << 20) && out.width * out.page_size <= (1 << 30) && args[3] != Py_None &&
+         args[4] != Py_None && optional_vector(args[3], out.sequences + 1, at::kInt, dev, &out.starts) &&
+         optional_vector(args[4], out.sequences, at::kInt, dev, &out.context);
+}
+
+bool expanded(const at::Tensor& t) {
+  for (int d = 0; d < t.dim(); ++d)
+    if (t.size(d) > 1 && t.stride(d) == 0) return true;
+  return false;
+}
+
+// paged_append(k, v, k_cache, v_cache, page_table, query_starts, context_lengths, q, frequencies, layout, magnitude):
+// the turned q, or True without one.
+PyObject* paged_append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 11) Py_RETURN_NONE;
+  const at::Tensor *k = heads_of(args[0]), *v = heads_of(args[1]);
+  Paged c;
+  const int layout = layout_of(args[9]);
+  float magnitude;
+  if (!k || !v || layout < 0 || !paged_of(args + 2, c) || !current(k->device()) || args[10] == Py_None ||
+      !positive(args[10], 1.0f, magnitude))
+    Py_RETURN_NONE;
+  const c10::Device dev = k->device();
+  const int64_t tokens = k->size(1);
+  if (v->sizes() != k->sizes() || v->scalar_type() != k->scalar_type() || v->device() != dev ||
+      c.k->device() != dev || c.k->scalar_type() != k->scalar_type() || c.kv_heads != k->size(0) ||
+      c.dim != k->size(2) || expanded(*c.k) || expanded(*c.v))
+    Py_RETURN_NONE;
+  const at::Tensor *f = nullptr, *q = nullptr;
+  if (args[8] != Py_None && !(f = frequencies_of(args[8], c.dim, dev))) Py_RETURN_NONE;
+  if (args[7] != Py_None) {
+    q = heads_of(args[7]);
+    if (!q || !f || q->size(1) != tokens || q->size(2) != c.dim || q->scalar_type() != k->scalar_type() ||
+        q->device() != dev)
+      Py_RETURN_NONE;
+  }
+  void* stream = nullptr;
+  if (!stream_of(dev, &stream)) return nullptr;
+  const int64_t heads = q ? q->size(0) : 0;
+  at::Tensor y;
+  if (q) y = empty({heads, tokens, c.dim}, k->scalar_type(), dev);
+  const void *kp = k->data_ptr(), *vp = v->data_ptr(), *qp = q ? q->data_ptr() : nullptr;
+  void *kc = c.k->data_ptr(), *vc = c.v->data_ptr(), *yp = q ? y.data_ptr() : nullptr;
+  const auto* fp = f ? static_cast<const double*>(f->data_ptr()) : nullptr;
+  const int64_t pairs = f ? f->size(0) : 0;
+  const int code = dtype_code(k->scalar_type());
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = m5k_paged_append(kp, stride(*k, 0), stride(*k, 1), vp, stride(*v, 0), stride(*v, 1), code, tokens, c.kv_heads,
+                        c.dim, kc, stride(*c.k, 0), stride(*c.k, 1), stride(*c.k, 2), vc, stride(*c.v, 0),
+                        stride(*c.v, 1), stride(*c.v, 2), c.pages, c.page_size, c.table, c.width, c.sequences, c.starts,
+                        c.context, qp, heads, q ? stride(*q, 0) : 0, q ? stride(*q, 1) : 0, yp, fp, pairs, layout,
+                        magnitude, stream);
+  Py_END_ALLOW_THREADS
+  if (rc) return failed("m5k_paged_append", rc);
+  if (!q) Py_RETURN_TRUE;
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// What both attention entries share.
+struct Scores {
+  float scale, softcap;
+  int64_t window;
+  const float* slopes;
+  int splits;
+  at::Tensor out, workspace;
+  float* wp;
+  int64_t elems;
+};
+
+// Checks q against the keys' heads and width, and the score options; allocates.  false: let Python look at it.
+bool scores_of(const at::Tensor* q, int64_t kv_heads, int64_t dim, at::ScalarType st, c10::Device dev, PyObject* scale,
+               PyObject* softcap, PyObject* window, PyObject* slopes, bool paged, int64_t sequences, int64_t keys,
+               Scores& s) {
+  if (!q || q->scalar_type() != st || !half_type(*q) || q->device() != dev || !current(dev) || q->size(2) != dim ||
+      q->size(0) % kv_heads || (dim != 64 && dim != 128) || !rows16(*q))
+    return false;
+  const int64_t heads = q->size(0), tokens = q->size(1);
+  if (tokens > (1 << 24) || heads > (1 << 16) || tokens * heads >= (int64_t{1} << 30)) return false;
+  if (!positive(scale, static_cast<float>(1.0 / std::sqrt(static_cast<double>(dim))), s.scale) ||
+      !positive(softcap, 0.0f, s.softcap) || !window_of(window, s.window) ||
+      !optional_vector(slopes, heads, at::kFloat, dev, &s.slopes))
+    return false;
+  if (m5k_attention_splits(paged, tokens, heads, kv_heads, sequences, keys, 0, &s.splits)) return false;
+  s.out = empty({tokens, heads * dim}, st, dev);
+  s.elems = 0;
+  s.wp = nullptr;
+  if (s.splits > 1) {
+    s.elems = s.splits * tokens * heads * (dim + 2);
+    s.workspace = empty({s.elems}, at::kFloat, dev);
+    s.wp = static_cast<float*>(s.workspace.data_ptr());
+  }
+  return true;
+}
+
+// paged_attention(q, k_cache, v_cache, page_table, query_starts, context_lengths, scale, window, softcap, slopes,
+// prefix_lengths).
+PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Paged c;
+  Scores s;
+  const int32_t* prefix;
+  if (nargs != 11 || !paged_of(args + 1, c)) Py_RETURN_NONE;
+  const at::Tensor* q = heads_of(args[0]);
+  const c10::Device dev = c.k->device();
+  if (!optional_vector(args[10], c.sequences, at::kInt, dev, &prefix) || (prefix && args[7] != Py_None) ||
+      !rows16(*c.k) || !rows16(*c.v) ||
+      !scores_of(q, c.kv_heads, c.dim, c.k->scalar_type(), dev, args[6], args[8], args[7], args[9], true, c.sequences,
+                 c.width * c.page_size, s))
+    Py_RETURN_NONE;
+  void* stream = nullptr;
+  if (!stream_of(dev, &stream)) return nullptr;
+  const void *qp = q->data_ptr(), *kp = c.k->data_ptr(), *vp = c.v->data_ptr();
+  void* op = s.out.data_ptr();
+  const int code = dtype_code(q->scalar_type());
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = m5k_paged_attention(qp, code, q->size(1), q->size(0), static_cast<int>(c.dim), stride(*q, 0), stride(*q, 1), kp,
+                           stride(*c.k, 0), stride(*c.k, 1), stride(*c.k, 2), vp, stride(*c.v, 0), stride(*c.v, 1),
+                           stride(*c.v, 2), c.pages, c.page_size, c.kv_heads, c.table, c.width, c.sequences, c.starts,
+                           c.context, s.scale, s.window, s.softcap, s.slopes, prefix, op, s.splits, s.wp, s.elems,
+                           stream);
+  Py_END_ALLOW_THREADS
+  if (rc) return failed("m5k_paged_attention", rc);
+  return THPVariable_Wrap(std::move(s.out));
+  END_HANDLE_TH_ERRORS
+}
+
+// attention(q, k, v, causal, window, document_starts, prefix_lengths, softcap, slopes, scale).
+PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 10 || !PyBool_Check(args[3])) Py_RETURN_NONE;
+  const at::Tensor *q = heads_of(args[0]), *k = heads_of(args[1]), *v = heads_of(args[2]);
+  if (!q || !k || !v || v->sizes() != k->sizes() || v->scalar_type() != k->scalar_type() ||
+      v->device() != k->device() || !rows16(*k) || !rows16(*v))
+    Py_RETURN_NONE;
+  const c10::Device dev = k->device();
+  const int64_t kv_heads = k->size(0), keys = k->size(1), dim = k->size(2), tokens = q->size(1);
+  for (const at::Tensor* t : {k, v})
+    if (keys > 1 && (t->stride(1) < dim || t->stride(1) > (1 << 23))) Py_RETURN_NONE;
+  const bool causal = args[3] == Py_True;
+  const int32_t *starts = nullptr, *prefix;
+  int64_t documents = 0;
+  if (args[5] != Py_None) {
+    const at::Tensor* d = plain(args[5]);
+    if (!d || d->dim() != 1 || d->size(0) < 2 || d->scalar_type() != at::kInt || d->device() != dev || tokens != keys)
+      Py_RETURN_NONE;
+    starts = static_cast<const int32_t*>(d->data_ptr());
+    documents = d->size(0) - 1;
+  }
+  Scores s;
+  if (keys > (1 << 24) || !optional_vector(args[6], documents ? documents : 1, at::kInt, dev, &prefix) ||
+      (prefix && (!causal || args[4] != Py_None)) ||
+      !scores_of(q, kv_heads, dim, k->scalar_type(), dev, args[9], args[7], args[4], args[8], false, documents, keys,
+                 s))
+    Py_RETURN_NONE;
+  void* stream = nullptr;
+  if (!stream_of(dev, &stream)) return nullptr;
+  const void *qp = q->data_ptr(), *kp = k->data_ptr(), *vp = v->data_ptr();
+  void* op = s.out.data_ptr();
+  const int code = dtype_code(q->scalar_type());
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = m5k_attention(qp, code, tokens, q->size(0), static_cast<int>(dim), stride(*q, 0), stride(*q, 1), kp,
+                     stride(*k, 0), stride(*k, 1), vp, stride(*v, 0), stride(*v, 1), keys, kv_heads, s.scale, causal,
+                     s.window, s.softcap, s.slopes, starts, documents, prefix, op, s.splits, s.wp, s.elems, stream);
+  Py_END_ALLOW_THREADS
+  if (rc) return failed("m5k_attention", rc);
+  return THPVariable_Wrap(std::move(s.out));
+  END_HANDLE_TH_ERRORS
+}
+
 // bind(stream_of, splits, staged): the Python callables above.
 PyObject* bind(PyObject*, PyObject* args) {
   PyObject *s, *p, *q;
@@ -424,6 +729,11 @@ PyMethodDef methods[] = {
     {"gemm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(gemm)), METH_FASTCALL, nullptr},
     {"qk", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(qk)), METH_FASTCALL, nullptr},
     {"qkv", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(qkv)), METH_FASTCALL, nullptr},
+    {"rope", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rope)), METH_FASTCALL, nullptr},
+    {"paged_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paged_append)), METH_FASTCALL, nullptr},
+    {"paged_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paged_attention)), METH_FASTCALL,
+     nullptr},
+    {"attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(attention)), METH_FASTCALL, nullptr},
     {"bind", bind, METH_VARARGS, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 

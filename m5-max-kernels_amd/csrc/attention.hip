@@ -53,6 +53,7 @@ extern "C" int m5k_attention_splits(int paged, int64_t tokens, int64_t heads, in
   m5k::clear_error();
   M5K_REQUIRE(splits && tokens > 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && sequences >= 0 && keys >= 0,
               "attention_splits: bad sizes");
+  if (cus <= 0) cus = m5k::device_cus();
   if (cus <= 0) cus = 256;
   *splits = m5k::attn::plan_splits(paged != 0, tokens, static_cast<int>(heads / kv_heads), static_cast<int>(kv_heads),
                                    sequences, keys, cus);

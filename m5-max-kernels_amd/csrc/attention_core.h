@@ -120,8 +120,8 @@ __device__ __forceinline__ int swizzle(int row) {
   else return ((row & 3) << 2) | ((row >> 2) & 3);
 }
 
-// Where keys and values lie.  PAGES16: pages of a multiple of 16 keys, so that the 16 rows of a tile that one wave loads
-// lie in one page and take one address; PAGES: any page size, an address a lane.
+// Where keys and values lie.  PAGES16: pages of a multiple of 16 keys, so that the 16 rows of a tile that one wave
+// loads lie in one page and take one address; PAGES: any page size, an address a lane.
 enum Keys { DENSE = 0, PAGES16 = 1, PAGES = 2 };
 
 // Page id at a position of the table, loaded per lane although it is the same for all: a scalar load would share
@@ -131,8 +131,8 @@ __device__ __forceinline__ int table_entry(const int32_t* table, uint32_t at) {
   return table[at];
 }
 
-// Buffer window of up to `rows` rows of `stride` elements from `p`, reading 0 behind them: rows are at least D apart, so a
-// row behind the last begins behind the window's end.
+// Buffer window of up to `rows` rows of `stride` elements from `p`, reading 0 behind them: rows are at least D apart,
+// so a row behind the last begins behind the window's end.
 template <int D>
 __device__ __forceinline__ v4i rows_rsrc(const uint16_t* p, int rows, int64_t stride) {
   const int64_t n = rows > 0 ? ((rows - 1) * stride + D) * 2 : 0;
@@ -191,33 +191,9 @@ __device__ __forceinline__ float tanh_f32(float y) {
   const float f = __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f);
   return z < 0.0625f ? s : f;
 }
-
-// Scores in base 2 of one accumulator value.
-template <bool MODS>
-__device__ __forceinline__ float score(float x, const Args& a, float scale2, float slope2, int pos, int key) {
-  if constexpr (!MODS) {
-    return x;
-  } else {
-    float t;
-    if (a.softcap > 0.0f) t = tanh_f32(x * (a.scale / a.softcap)) * (a.softcap * LOG2E);
-    else t = x * scale2;
-    return __builtin_fmaf(-slope2, fabsf(static_cast<float>(pos - key)), t);
-  }
-}
-
-// V^T fragment of k-step c and channel block b: keys 16 c + 8 h + 4 (lane >> 5) .. + 3 from address at[h].
-template <uint32_t ROWB>
-__device__ __forceinline__ v4i value_frag(const uint32_t (&at)[2], int c, int b) {
-  v4i f;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_v4s>((at[h] ^ (b << 6)) + 16 * c * ROWB));
-    const auto y = __builtin_bit_cast(m5k_u32x2, x);
-    f[2 * h] = static_cast<int>(y[0]);
-    f[2 * h + 1] = static_cast<int>(y[1]);
-  }
-  return f;
-}
+// Caps up to here take the second form alone, C - 2 C / (e^(2y) + 1) in five instructions: off by C 2^-22, 6e-5 at
+// most (16 heads of 64, 1999 tokens: 72 us with tanh_f32, 38 us).
+constexpr float CAP_SHORT = 128.0f;
 
 // Non-finite 16-bit values of a fragment: zero in `clean`; `mark` holds 1 for +inf, 128 for -inf, 16384 for NaN.
 template <int DT>
@@ -318,6 +294,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   constexpr int RPI = 64 / CH;           // rows of one load instruction
   constexpr int NI = CH / WAVES;         // load instructions of a wave, each of K and V
   constexpr int QS = D / 16, OB = D / 32;
+  constexpr int AHEAD = 1;  // steps of two products between a fragment's read and its use (2: no faster)
   constexpr uint32_t TILE = KT * D * 2, ROWB = D * 2;
   __shared__ __attribute__((aligned(256))) uint8_t lds[4 * TILE];  // K stages 0 and 1, V stages 0 and 1
   __shared__ int bounds[2 * WAVES];
@@ -445,14 +422,20 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     }
   };
 
-  // Fragment addresses: chunk c of a row is its chunk 0 XOR 16 c, rows being aligned to their size.
-  const uint32_t kread = lds0 + (lane & 31) * ROWB + ((half ^ swizzle<D>(lane & 31)) << 4);
+  // Fragment addresses in stage 0 (the other stage and the rows further on are instruction offsets): chunk c of a row
+  // is its chunk 0 XOR 16 c, rows being aligned to their size.
+  uint32_t kread[QS], vread[2][OB];
   const int g = lane >> 4, gi = lane & 15;
   const int vrow = 4 * half + (gi >> 2), vchunk = 2 * (g & 1) + ((gi & 3) >> 1);
-  uint32_t vread[2];
+#pragma unroll
+  for (int c = 0; c < QS; ++c)
+    kread[c] = (lds0 + (lane & 31) * ROWB + ((half ^ swizzle<D>(lane & 31)) << 4)) ^ (c << 5);
 #pragma unroll
   for (int h = 0; h < 2; ++h)
-    vread[h] = lds0 + 2 * TILE + (8 * h + vrow) * ROWB + ((vchunk ^ swizzle<D>(8 * h + vrow)) << 4) + (gi & 1) * 8;
+#pragma unroll
+    for (int b = 0; b < OB; ++b)
+      vread[h][b] =
+          (lds0 + (8 * h + vrow) * ROWB + ((vchunk ^ swizzle<D>(8 * h + vrow)) << 4) + (gi & 1) * 8) ^ (b << 6);
 
   wait_all();
   v16f o[OB], s[2][NB];
@@ -463,10 +446,23 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   // running maximum, packed for the second product, and their sum.  A 32 x 32 x 16 product holds the matrix cores for
   // 32 cycles, in which the wave issues 8 VALU instructions: each step's fence keeps its share of the exponentials
   // between its products, and the next step's fragments on their way.
-  auto key_frags = [&](uint32_t at, int c, v4i (&f)[NB]) __attribute__((always_inline)) {
+  auto key_frags = [&](int st, int c, v4i (&f)[NB]) __attribute__((always_inline)) {
 #pragma unroll
     for (int b = 0; b < NB; ++b)
-      f[b] = *reinterpret_cast<const __attribute__((address_space(3))) v4i*>((at ^ (c << 5)) + b * 32 * ROWB);
+      f[b] = *reinterpret_cast<const __attribute__((address_space(3))) v4i*>(kread[c] + b * 32 * ROWB + st * TILE);
+  };
+  // V^T fragment of k-step c and channel block b: keys 16 c + 8 h + 4 (lane >> 5) .. + 3 for h = 0, 1.
+  auto value_frag = [&](int st, int c, int b) __attribute__((always_inline)) {
+    v4i f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          reinterpret_cast<lds_v4s>(vread[h][b] + 16 * c * ROWB + (2 + st) * TILE));
+      const auto y = __builtin_bit_cast(m5k_u32x2, x);
+      f[2 * h] = static_cast<int>(y[0]);
+      f[2 * h + 1] = static_cast<int>(y[1]);
+    }
+    return f;
   };
   auto probabilities = [&](const v16f (&x)[NB], int from, int to, float (&sum)[2]) __attribute__((always_inline)) {
 #pragma unroll
@@ -482,16 +478,15 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     }
   };
   auto product = [&](v16f (&y)[NB], int st, const v16f (&x)[NB], bool prob) __attribute__((always_inline)) {
-    uint32_t at = kread + st * TILE;
-    __asm__("" : "+v"(at));  // addresses by XOR, not kept in registers
-    v4i kf[2][NB];
+    v4i kf[AHEAD + 1][NB];
     float sum[2] = {};
-    key_frags(at, 0, kf[0]);
+#pragma unroll
+    for (int c = 0; c < AHEAD; ++c) key_frags(st, c, kf[c]);
 #pragma unroll
     for (int c = 0; c < QS; ++c) {
-      if (c + 1 < QS) key_frags(at, c + 1, kf[(c + 1) & 1]);
+      if (c + AHEAD < QS) key_frags(st, c + AHEAD, kf[(c + AHEAD) % (AHEAD + 1)]);
 #pragma unroll
-      for (int b = 0; b < NB; ++b) y[b] = mfma32<DT>(kf[c & 1][b], qf[c], c == 0 ? v16f{} : y[b]);
+      for (int b = 0; b < NB; ++b) y[b] = mfma32<DT>(kf[c % (AHEAD + 1)][b], qf[c], c == 0 ? v16f{} : y[b]);
       if (prob) probabilities(x, c * 32 / QS, (c + 1) * 32 / QS, sum);
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -502,11 +497,33 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     constexpr bool careful = decltype(with_care)::value;
     const int key0 = t * KT, kofs0 = key0 + 4 * half;
     if constexpr (MODS) {
+      // Scores in base 2: capped, or scaled with the bias.  Distances are whole numbers, exact in FP32 up to 2^24.
+      if (a.softcap > 0.0f) {
+        const float cap2 = a.softcap * LOG2E, y = a.scale / a.softcap;
+        if (a.softcap <= CAP_SHORT) {
+          const float y2 = y * (2.0f * LOG2E);
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
+          for (int e = 0; e < 32; ++e) {
+            const float g = __builtin_amdgcn_exp2f(x[e >> 4][e & 15] * y2) + 1.0f;
+            x[e >> 4][e & 15] = __builtin_fmaf(-2.0f * cap2, __builtin_amdgcn_rcpf(g), cap2);
+            if ((e & 7) == 7) __builtin_amdgcn_sched_barrier(0);
+          }
+        } else {
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          x[b][r] = score<MODS>(x[b][r], a, scale2, slope2, rr.pos, kofs0 + 32 * b + 8 * (r >> 2) + (r & 3));
+          for (int e = 0; e < 32; ++e) {
+            x[e >> 4][e & 15] = tanh_f32(x[e >> 4][e & 15] * y) * cap2;
+            if ((e & 3) == 3) __builtin_amdgcn_sched_barrier(0);  // few registers
+          }
+        }
+      }
+      if (a.slopes) {
+        const float apart = static_cast<float>(rr.pos - kofs0), f = a.softcap > 0.0f ? 1.0f : scale2;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const float d = fabsf(apart - static_cast<float>(32 * (e >> 4) + 8 * ((e & 15) >> 2) + (e & 3)));
+          x[e >> 4][e & 15] = __builtin_fmaf(x[e >> 4][e & 15], f, -slope2 * d);
+        }
+      }
     }
     if (careful || key0 < all_lo || key0 + KT > all_hi) {
       const uint32_t width = static_cast<uint32_t>(max(rr.hi - rr.lo, 0));
@@ -530,23 +547,21 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   // O += V^T P of a tile, V at stage `st`, in steps of two products as above; beside them the maximum of the scores x.
   auto accumulate = [&](int st, const v16f (&x)[NB]) __attribute__((always_inline)) -> float {
     constexpr int STEPS = 2 * NB * OB / 2;
-    uint32_t at[2] = {vread[0] + st * TILE, vread[1] + st * TILE};
-    __asm__("" : "+v"(at[0]), "+v"(at[1]));
-    v4i vf[2][2];
+    v4i vf[AHEAD + 1][2];
     float t0 = x[0][0], t1 = x[0][1];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) vf[0][j] = value_frag<ROWB>(at, 0, j);
+    for (int j = 0; j < 2 * AHEAD; ++j) vf[j / 2][j & 1] = value_frag(st, j / OB, j % OB);
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
-      if (i + 1 < STEPS) {
+      if (i + AHEAD < STEPS) {
+        const int n = 2 * (i + AHEAD);
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-          vf[(i + 1) & 1][j] = value_frag<ROWB>(at, (2 * i + 2) / OB, (2 * i + 2) % OB + j);
+        for (int j = 0; j < 2; ++j) vf[(i + AHEAD) % (AHEAD + 1)][j] = value_frag(st, n / OB, n % OB + j);
       }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int b = 2 * i % OB + j;
-        o[b] = mfma32<DT>(vf[i & 1][j], pf[2 * i / OB], o[b]);
+        o[b] = mfma32<DT>(vf[i % (AHEAD + 1)][j], pf[2 * i / OB], o[b]);
       }
 #pragma unroll
       for (int e = i * 32 / STEPS; e < (i + 1) * 32 / STEPS; e += 2) {
@@ -565,7 +580,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
 #pragma unroll
       for (int c = 0; c < 2 * NB; ++c) {
         v4i clean, mark, see;
-        split_nonfinite<DT>(value_frag<ROWB>(vread, c, b), clean, mark);
+        split_nonfinite<DT>(value_frag(0, c, b), clean, mark);
         const uint32_t one = pack2<DT>(1.0f, 1.0f);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
@@ -609,15 +624,17 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   };
 
   // Step t turns the scores of tile t into its part of O, and makes the scores of tile t + 1 meanwhile, so that the
-  // matrix cores have work beside the exponentials.  Tile t's K and V are in stage t & 1 of each; step t loads K of
-  // tile t + 2 and V of tile t + 1 over what step t - 1 was the last to read.
+  // matrix cores have work beside the exponentials.  The i-th step (ODD = i & 1) reads K of tile t + 1 in stage ODD and
+  // V of tile t in stage EVEN; it loads V of tile t + 1 and K of tile t + 2 over what the step before was the last to
+  // read.
   constexpr std::false_type quick{};
-  auto step = [&](int t, v16f (&x)[NB], v16f (&next)[NB]) __attribute__((always_inline)) {
+  auto step = [&](int t, auto odd, v16f (&x)[NB], v16f (&next)[NB]) __attribute__((always_inline)) {
+    constexpr int ODD = decltype(odd)::value, EVEN = 1 - ODD;
     wait_all();
     gemm::stage_barrier();
     if (t + 1 < t_end) {
-      load_rows(t + 1, ids[1], vbase, a.v_page, a.v_row, vofs, lds0 + (2 + ((t + 1) & 1)) * TILE);
-      if (t + 2 < t_end) load_rows(t + 2, ids[0], kbase, a.k_page, a.k_row, kofs, lds0 + (t & 1) * TILE);
+      load_rows(t + 1, ids[1], vbase, a.v_page, a.v_row, vofs, lds0 + (2 + ODD) * TILE);
+      if (t + 2 < t_end) load_rows(t + 2, ids[0], kbase, a.k_page, a.k_row, kofs, lds0 + EVEN * TILE);
     }
 #pragma unroll
     for (int i = 0; i < NIDS; ++i) ids[1][i] = ids[0][i];
@@ -625,28 +642,28 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     uint32_t none;
     const bool now = t >= first && t < last, then = t + 1 >= first && t + 1 < last;  // the same for the whole wave
     if (now && then) {
-      product(next, (t + 1) & 1, x, true);
+      product(next, ODD, x, true);
       finish(next, t + 1, quick, none);
-      adopt(accumulate(t & 1, next));
+      adopt(accumulate(EVEN, next));
     } else if (then) {
-      product(next, (t + 1) & 1, x, false);
+      product(next, ODD, x, false);
       finish(next, t + 1, quick, none);
       adopt(maximum(next));
     } else if (now) {
       float sum[2] = {};
       probabilities(x, 0, 32, sum);
       l += sum[0] + sum[1];
-      accumulate(t & 1, x);
+      accumulate(EVEN, x);
     }
   };
   start();
   if (t_begin < t_end) {
     load_ids(t_begin, ids[1]);
-    load_rows(t_begin, ids[1], kbase, a.k_page, a.k_row, kofs, lds0 + (t_begin & 1) * TILE);
+    load_rows(t_begin, ids[1], kbase, a.k_page, a.k_row, kofs, lds0);
     load_ids(t_begin + 1, ids[0]);
     for (int t = t_begin - 1; t < t_end; t += 2) {
-      step(t, s[0], s[1]);
-      if (t + 1 < t_end) step(t + 1, s[1], s[0]);
+      step(t, std::integral_constant<int, 0>{}, s[0], s[1]);
+      if (t + 1 < t_end) step(t + 1, std::integral_constant<int, 1>{}, s[1], s[0]);
     }
   }
   float check = 0.0f;
@@ -708,32 +725,66 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     }
 }
 
-// Joins the key splits: one wave a (token, head), each split's sum weighted by 2^(m - max m), in split order.
-template <int DT, int D>
+// Joins the key splits of a (token, head), each split's sum weighted by 2^(m - max m).  Lane i holds split i's maximum
+// and total, so that the weights cost one load; the sums' loads then wait for nothing but memory.  Latency bound: with
+// WAVES_ROW = 4 (many splits, so few rows) the waves take a quarter of the splits each and add up in LDS, in wave order
+// (64 splits of 64 rows: 54 us with one wave and a weight at a time).
+template <int DT, int D, int WAVES_ROW>
 __global__ __launch_bounds__(256) void attention_join(const Args a) {
+  constexpr int E = D / 64, ROWS = 4 / WAVES_ROW, BATCH = WAVES_ROW == 1 ? 4 : 16;
+  __shared__ float sums[WAVES_ROW == 1 ? 1 : 4][D];
   const int64_t rows = int64_t{a.tokens} * a.heads;
-  const int64_t at = int64_t{blockIdx.x} * 4 + (threadIdx.x >> 6);
-  if (at >= rows) return;
-  const int lane = threadIdx.x & 63;
-  constexpr int E = D / 64;
-  float top = M_FLOOR;
-  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_ml[2 * (s * rows + at)]);
-  float sum = 0.0f, acc[E] = {};
-  for (int s = 0; s < a.splits; ++s) {
-    const float l = a.part_ml[2 * (s * rows + at) + 1];
-    if (l == 0.0f) continue;
-    const float w = __builtin_amdgcn_exp2f(a.part_ml[2 * (s * rows + at)] - top);
-    sum = __builtin_fmaf(l, w, sum);
-    const float* src = a.part_o + (s * rows + at) * D + lane * E;
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = __builtin_fmaf(src[e], w, acc[e]);
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t at = int64_t{blockIdx.x} * ROWS + wave / WAVES_ROW;
+  if (at >= rows) return;  // whole workgroups where waves share a row
+  float m = M_FLOOR, l = 0.0f;
+  if (lane < a.splits) {
+    const float2 ml = reinterpret_cast<const float2*>(a.part_ml)[lane * rows + at];
+    m = ml.x;
+    l = ml.y;
   }
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  float top = m;
+#pragma unroll
+  for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  const float w = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+  const float total = wave_sum(l * w);
+  const int per = (a.splits + WAVES_ROW - 1) / WAVES_ROW, s0 = wave % WAVES_ROW * per, s1 = min(s0 + per, a.splits);
+  float acc[E] = {};
+  for (int s = s0; s < s1; s += BATCH) {
+    float v[BATCH][E];
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const float* src = a.part_o + (min(s + i, s1 - 1) * rows + at) * D + lane * E;
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[i][e] = src[e];
+    }
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      // A split that saw nothing wrote no sums: whatever lies there is left out.
+      const int from = min(s + i, s1 - 1);
+      const float f = s + i < s1 ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), from)) : 0.0f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = f == 0.0f ? acc[e] : __builtin_fmaf(v[i][e], f, acc[e]);
+    }
+  }
+  if constexpr (WAVES_ROW > 1) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) sums[wave][lane * E + e] = acc[e];
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      acc[e] = sums[0][lane * E + e];
+#pragma unroll
+      for (int i = 1; i < 4; ++i) acc[e] += sums[i][lane * E + e];
+    }
+  }
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
   uint16_t* dst = a.out + at * D + lane * E;
   if constexpr (E == 2) {
-    *reinterpret_cast<uint32_t*>(dst) = sum == 0.0f ? 0u : pack2<DT>(acc[0] * inv, acc[1] * inv);
+    *reinterpret_cast<uint32_t*>(dst) = total == 0.0f ? 0u : pack2<DT>(acc[0] * inv, acc[1] * inv);
   } else {
-    *dst = static_cast<uint16_t>(sum == 0.0f ? 0u : pack2<DT>(acc[0] * inv, 0.0f) & 0xFFFFu);
+    *dst = static_cast<uint16_t>(total == 0.0f ? 0u : pack2<DT>(acc[0] * inv, 0.0f) & 0xFFFFu);
   }
 }
 
@@ -750,7 +801,10 @@ int launch(const Args& a, hipStream_t st) {
   int rc = launch_status("attention");
   if (rc != M5K_OK || a.splits == 1) return rc;
   const int64_t rows = int64_t{a.tokens} * a.heads;
-  launch_kernel(attention_join<DT, D>, dim3(static_cast<uint32_t>((rows + 3) / 4)), dim3(256), st, a);
+  if (a.splits > 8)
+    launch_kernel(attention_join<DT, D, 4>, dim3(static_cast<uint32_t>(rows)), dim3(256), st, a);
+  else
+    launch_kernel(attention_join<DT, D, 1>, dim3(static_cast<uint32_t>((rows + 3) / 4)), dim3(256), st, a);
   return launch_status("attention join");
 }
 

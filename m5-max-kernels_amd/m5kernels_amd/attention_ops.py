@@ -23,8 +23,7 @@ import math
 
 import torch
 
-from . import _lib
-from .hip import _cu_count_of
+from . import _lib, hip
 
 _LAYOUTS = ("half", "interleaved")
 _HALF_DTYPES = (torch.float16, torch.bfloat16)
@@ -154,6 +153,11 @@ def rope(x, positions, frequencies, *, layout="half", magnitude=1.0):
     `magnitude`; the other channels are copied.  Pair j is channels (j, j + pairs) with layout "half", (2j, 2j + 1) with
     "interleaved".  x float16, bfloat16 or float32 in any strides, positions int32 [tokens], frequencies float64
     [pairs] (rope_frequencies).  Computed in FP32 and rounded once; returns a contiguous tensor of x's dtype."""
+    fast = hip._fast
+    if fast is not None:
+        y = fast.rope(x, positions, frequencies, layout, magnitude)
+        if y is not None:
+            return y
     heads, tokens, width = _heads_tensor(x, "x", _FLOAT_DTYPES)
     frequencies, magnitude = _rotation(frequencies, layout, magnitude, width)
     positions = _int_vector(positions, tokens, "positions")
@@ -209,6 +213,12 @@ def paged_append(k, v, k_cache, v_cache, page_table, query_starts, context_lengt
 
     A token whose position is negative (an idle slot: context_lengths 0) or lies behind the table, or whose table entry
     names no page, is not stored.  Two tokens of one call that name the same place leave either's values there."""
+    fast = hip._fast
+    if fast is not None:
+        done = fast.paged_append(k, v, k_cache, v_cache, page_table, query_starts, context_lengths, q, frequencies,
+                                 layout, magnitude)
+        if done is not None:
+            return None if done is True else done
     kv_heads, tokens, width = _heads_tensor(k, "k", _FLOAT_DTYPES)
     if not isinstance(v, torch.Tensor) or v.shape != k.shape or v.dtype != k.dtype:
         raise ValueError("k and v must have the same shape and dtype")
@@ -303,6 +313,12 @@ def paged_attention(q, k_cache, v_cache, page_table, query_starts, context_lengt
     [heads]) then adds -slopes[h] * (distance of j from p).  Returns [tokens, heads * width]; rows that see no key,
     and rows behind the last sequence, are 0.  Keys on pages that a table entry outside [0, pages) would name are
     left out."""
+    fast = hip._fast
+    if fast is not None:
+        out = fast.paged_attention(q, k_cache, v_cache, page_table, query_starts, context_lengths, scale, window,
+                                   softcap, slopes, prefix_lengths)
+        if out is not None:
+            return out
     if prefix_lengths is not None and window is not None:
         raise NotImplementedError("a window and a prefix cannot be combined")
     if not isinstance(k_cache, torch.Tensor) or k_cache.dim() != 4:
@@ -328,7 +344,7 @@ def paged_attention(q, k_cache, v_cache, page_table, query_starts, context_lengt
     q = _rows(q, "q")
     qs = _strides(q)
     pages, page_size = k_cache.shape[0], k_cache.shape[2]
-    splits = _splits(1, tokens, heads, kv_heads, sequences, table_width * page_size, _cu_count_of(device.index))
+    splits = _splits(1, tokens, heads, kv_heads, sequences, table_width * page_size, hip._cu_count_of(device.index))
     workspace, n = _workspace(splits, tokens, heads, width, device)
     with _on(device):
         _lib.call(
@@ -350,6 +366,11 @@ def attention(q, k, v, *, causal=False, window=None, document_starts=None, prefi
     0, as many keys as tokens) confines it to its own document.  `prefix_lengths` (int32 [documents], or [1]; with
     causal, without window) shows every token of a document that many of its first keys too.  Scores as in
     paged_attention.  A row that sees no key, and a row behind the last document, is 0."""
+    fast = hip._fast
+    if fast is not None:
+        out = fast.attention(q, k, v, causal, window, document_starts, prefix_lengths, softcap, slopes, scale)
+        if out is not None:
+            return out
     if prefix_lengths is not None and window is not None:
         raise NotImplementedError("a window and a prefix cannot be combined")
     kv_heads, keys, width = _heads_tensor(k, "k", _HALF_DTYPES)
@@ -380,7 +401,7 @@ def attention(q, k, v, *, causal=False, window=None, document_starts=None, prefi
         return out
     q, k, v = _rows(q, "q"), _apart(_rows(k, "k")), _apart(_rows(v, "v"))
     qs, ks, vs = _strides(q), _strides(k), _strides(v)
-    splits = _splits(0, tokens, heads, kv_heads, documents, keys, _cu_count_of(device.index))
+    splits = _splits(0, tokens, heads, kv_heads, documents, keys, hip._cu_count_of(device.index))
     workspace, n = _workspace(splits, tokens, heads, width, device)
     with _on(device):
         _lib.call(

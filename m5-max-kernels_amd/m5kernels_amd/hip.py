@@ -646,5 +646,21 @@ class _NativeFront:
         module = self._load()
         return None if module is None else module.qkv(*args)
 
+    def rope(self, *args):
+        module = self._load()
+        return None if module is None else module.rope(*args)
+
+    def paged_append(self, *args):
+        module = self._load()
+        return None if module is None else module.paged_append(*args)
+
+    def paged_attention(self, *args):
+        module = self._load()
+        return None if module is None else module.paged_attention(*args)
+
+    def attention(self, *args):
+        module = self._load()
+        return None if module is None else module.attention(*args)
+
 
 _fast = _NativeFront()
