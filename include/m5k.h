@@ -437,8 +437,8 @@ int m5k_attention(const void* q, int dtype, int64_t tokens, int64_t heads, int h
 
 /* Key splits of m5k_attention (paged 0) or m5k_paged_attention (paged 1, keys = table_width * page_size) that
  * fill `cus` compute units (host only; cus <= 0: those of the current device). */
-int m5k_attention_splits(int paged, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t sequences, int64_t keys,
-                         int cus, int* splits);
+int m5k_attention_splits(int paged, int64_t tokens, int64_t heads, int64_t kv_heads, int head_dim, int64_t sequences,
+                         int64_t keys, int cus, int* splits);
 
 /*
  * Attention of new tokens over a paged cache: k_cache, v_cache [pages, kv_heads, page_size, head_dim] by

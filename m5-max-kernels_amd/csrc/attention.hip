@@ -48,15 +48,15 @@ int common(Args& a, const void* q, int dtype, int64_t tokens, int64_t heads, int
 
 }  // namespace
 
-extern "C" int m5k_attention_splits(int paged, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t sequences,
-                                    int64_t keys, int cus, int* splits) {
+extern "C" int m5k_attention_splits(int paged, int64_t tokens, int64_t heads, int64_t kv_heads, int head_dim,
+                                    int64_t sequences, int64_t keys, int cus, int* splits) {
   m5k::clear_error();
   M5K_REQUIRE(splits && tokens > 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && sequences >= 0 && keys >= 0,
               "attention_splits: bad sizes");
   if (cus <= 0) cus = m5k::device_cus();
   if (cus <= 0) cus = 256;
   *splits = m5k::attn::plan_splits(paged != 0, tokens, static_cast<int>(heads / kv_heads), static_cast<int>(kv_heads),
-                                   sequences, keys, cus);
+                                   head_dim, sequences, keys, cus);
   return M5K_OK;
 }
 
@@ -91,7 +91,6 @@ extern "C" int m5k_attention(const void* q, int dtype, int64_t tokens, int64_t h
   a.causal = causal != 0;
   a.starts = document_starts;
   a.sequences = static_cast<int>(documents);
-  a.slots = m5k::attn::plan_slots(false, tokens, a.group, 0);
   return m5k::attn::launch_typed<m5k::attn::DENSE>(a, dtype, head_dim, m5k::as_stream(stream));
 }
 
@@ -134,7 +133,6 @@ extern "C" int m5k_paged_attention(const void* q, int dtype, int64_t tokens, int
   a.keys = static_cast<int>(table_width * page_size);
   a.causal = 1;
   m5k::attn::magic_of(static_cast<uint32_t>(page_size), a.page_magic, a.page_shift);
-  a.slots = m5k::attn::plan_slots(true, tokens, a.group, sequences);
   const bool whole = page_size % 16 == 0 && k_slot >= head_dim && v_slot >= head_dim && k_slot <= (1 << 23) &&
                      v_slot <= (1 << 23);
   const auto run = whole ? m5k::attn::launch_typed<m5k::attn::PAGES16> : m5k::attn::launch_typed<m5k::attn::PAGES>;

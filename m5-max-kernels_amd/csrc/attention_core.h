@@ -124,11 +124,18 @@ __device__ __forceinline__ int swizzle(int row) {
 // loads lie in one page and take one address; PAGES: any page size, an address a lane.
 enum Keys { DENSE = 0, PAGES16 = 1, PAGES = 2 };
 
-// Page id at a position of the table, loaded per lane although it is the same for all: a scalar load would share
-// lgkmcnt with the LDS reads, out of order, and so make each of them wait.
+// Page id at a position of the table, the same for the whole wave.  SCALAR: a scalar load, which leaves vmcnt to the
+// tiles in flight.  Otherwise a load per lane: a scalar one shares lgkmcnt with the LDS reads, out of order, and makes
+// each of them wait.
+template <bool SCALAR>
 __device__ __forceinline__ int table_entry(const int32_t* table, uint32_t at) {
-  __asm__("" : "+v"(at));
-  return table[at];
+  if constexpr (SCALAR) {
+    at = __builtin_amdgcn_readfirstlane(at);
+    return reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(table))[at];
+  } else {
+    __asm__("" : "+v"(at));
+    return table[at];
+  }
 }
 
 // Buffer window of up to `rows` rows of `stride` elements from `p`, reading 0 behind them: rows are at least D apart,
@@ -287,51 +294,62 @@ __device__ __forceinline__ RowRange range_of(const Args& a, const Place& p, int 
   return row_range(s, e, i + p.shift, prefix, a.causal, a.window);
 }
 
-template <int DT, int D, int KEYS, bool MODS>
-__global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
-  constexpr int KT = 64, NB = KT / 32;   // keys of a tile, 32-key blocks
-  constexpr int CH = D / 8;              // 16-byte chunks of a row
-  constexpr int RPI = 64 / CH;           // rows of one load instruction
-  constexpr int NI = CH / WAVES;         // load instructions of a wave, each of K and V
+// FEW = false: the 4 waves take 32 rows each and share key tiles of 64.  FEW: they share 32 rows, for calls that have
+// no more, and take every fourth tile of 32 keys each, through LDS of their own: no barrier in the loop, two tiles a
+// wave in flight, and the keys of a short row are read four tiles at a time.
+template <int DT, int D, int KEYS, bool MODS, bool FEW>
+__global__ __launch_bounds__(THREADS, FEW && D == 128 ? 1 : 2) void attention_tile(const Args a) {
+  constexpr int KT = FEW ? 32 : 64, NB = KT / 32;  // keys of a tile, 32-key blocks
+  constexpr int EL = 16 * NB;                      // scores of a lane
+  constexpr int CH = D / 8;                        // 16-byte chunks of a row
+  constexpr int RPI = 64 / CH;                     // rows of one load instruction
+  constexpr int LOADED = FEW ? KT : KT / WAVES;    // rows of a tile that one wave loads
+  constexpr int GROUPS = LOADED / 16;
+  constexpr int NI = LOADED / RPI;  // its load instructions, each of K and V
   constexpr int QS = D / 16, OB = D / 32;
   constexpr int AHEAD = 1;  // steps of two products between a fragment's read and its use (2: no faster)
-  constexpr uint32_t TILE = KT * D * 2, ROWB = D * 2;
-  __shared__ __attribute__((aligned(256))) uint8_t lds[4 * TILE];  // K stages 0 and 1, V stages 0 and 1
+  constexpr int ROWS = FEW ? 32 : 32 * WAVES;
+  constexpr uint32_t ROWB = D * 2, TILE = KT * ROWB;
+  // K stages 0 and 1, V stages 0 and 1; FEW: those of each wave, later its sums.
+  __shared__ __attribute__((aligned(256))) uint8_t lds[(FEW ? WAVES : 1) * 4 * TILE];
   __shared__ int bounds[2 * WAVES];
 
-  const Place p = place<KEYS>(a, 32 * WAVES);
+  const Place p = place<KEYS>(a, ROWS);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-  const int row0 = p.tile * 32 * WAVES;
+  const int wave_s = __builtin_amdgcn_readfirstlane(wave);
+  const int row0 = p.tile * ROWS;
   if (row0 >= p.rows) return;
-  const int row = row0 + 32 * wave + (lane & 31);
+  const int row = row0 + (FEW ? 0 : 32 * wave) + (lane & 31);
   const bool live = row < p.rows;
   int token, head;
   const RowRange rr = range_of<KEYS>(a, p, min(row, p.rows - 1), token, head);
 
   // Key ranges: of the wave (any row, every row), and of the workgroup.
-  const bool idle = row0 + 32 * wave >= p.rows;
+  const bool idle = !FEW && row0 + 32 * wave >= p.rows;
   const int any_lo = idle ? 0x3FFFFFFF : wave_min_i(rr.lo), any_hi = idle ? 0 : wave_max_i(rr.hi);
   const int all_lo = wave_max_i(rr.lo), all_hi = wave_min_i(rr.hi);
-  if (lane == 0) {
-    bounds[wave] = any_lo;
-    bounds[WAVES + wave] = any_hi;
-  }
-  __syncthreads();
-  int lo = bounds[0], hi = bounds[WAVES];
+  int lo = any_lo, hi = any_hi;
+  if constexpr (!FEW) {
+    if (lane == 0) {
+      bounds[wave] = any_lo;
+      bounds[WAVES + wave] = any_hi;
+    }
+    __syncthreads();
 #pragma unroll
-  for (int w = 1; w < WAVES; ++w) {
-    lo = min(lo, bounds[w]);
-    hi = max(hi, bounds[WAVES + w]);
+    for (int w = 0; w < WAVES; ++w) {
+      lo = min(lo, bounds[w]);
+      hi = max(hi, bounds[WAVES + w]);
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    hi = __builtin_amdgcn_readfirstlane(hi);
   }
-  lo = __builtin_amdgcn_readfirstlane(lo);
-  hi = __builtin_amdgcn_readfirstlane(hi);
   int t_begin = 0, t_end = 0;
   if (lo < hi) {
     t_begin = lo / KT;
     t_end = (hi + KT - 1) / KT;
     if (a.splits > 1) {
-      // At least 4 tiles a split: below, the partial sums cost more than the keys.
-      const int per = max((t_end - t_begin + a.splits - 1) / a.splits, 4);
+      // At least 256 keys a split: below, the partial sums cost more than the keys.
+      const int per = max((t_end - t_begin + a.splits - 1) / a.splits, 256 / KT);
       t_begin = min(t_begin + p.split * per, t_end);
       t_end = min(t_begin + per, t_end);
     }
@@ -347,24 +365,24 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   const float unit = MODS ? 1.0f : scale2;  // what turns score() into base 2
   const float slope2 = MODS && a.slopes ? a.slopes[head] * LOG2E : 0.0f;
 
-  // Loads: instruction i of a wave brings rows wave * 16 + i * RPI + lane / CH of K and of V.
-  const int wave_s = __builtin_amdgcn_readfirstlane(wave);
-  const int ld_row = wave * NI * RPI + lane / CH, ld_chunk = lane % CH;
+  // Loads: instruction i of a wave brings rows first_row + i * RPI + lane / CH of K and of V.
+  const int first_row = FEW ? 0 : wave_s * LOADED;
+  const int ld_row = first_row + lane / CH, ld_chunk = lane % CH;
   const uint16_t* kbase = a.k + int64_t{p.kvh} * a.k_head;
   const uint16_t* vbase = a.v + int64_t{p.kvh} * a.v_head;
   const int32_t* table = KEYS != DENSE && p.seq < a.sequences ? a.table + int64_t{p.seq} * a.table_width : nullptr;
-  const uint32_t lds0 = gemm::lds_addr(lds);
+  const uint32_t lds0 = gemm::lds_addr(lds) + (FEW ? wave_s * 4 * TILE : 0);
   uint32_t kofs[NI], vofs[NI];  // bytes of a lane's chunk from the window's first row
   if constexpr (KEYS != PAGES) {
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const int r = KEYS == DENSE ? ld_row + i * RPI : lane / CH + i * RPI;
+      const int r = KEYS == DENSE ? ld_row + i * RPI : lane / CH + i % (NI / GROUPS) * RPI;  // pages: of 16 rows
       const int chunk = (ld_chunk ^ swizzle<D>(ld_row + i * RPI)) * 8;
       kofs[i] = static_cast<uint32_t>(r * static_cast<int>(a.k_row) + chunk) * 2;
       vofs[i] = static_cast<uint32_t>(r * static_cast<int>(a.v_row) + chunk) * 2;
     }
   }
-  constexpr int NIDS = KEYS == PAGES ? NI : 1;
+  constexpr int NIDS = KEYS == PAGES ? NI : GROUPS;
   int ids[2][NIDS] = {};  // pages of the next tile's keys, and of the tile before it, whose values come next
   bool lacking = false;
 
@@ -372,8 +390,11 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   // condition's end, and with it everything in flight.
   auto load_ids = [&](int t, int (&to)[NIDS]) __attribute__((always_inline)) {
     if constexpr (KEYS == PAGES16) {
-      const int key = min(t * KT + wave_s * 16, p.span - 1);
-      to[0] = table_entry(table, fast_div(key, a.page_magic, a.page_shift));
+#pragma unroll
+      for (int i = 0; i < GROUPS; ++i) {
+        const int key = min(t * KT + first_row + 16 * i, p.span - 1);
+        to[i] = table_entry<FEW>(table, fast_div(key, a.page_magic, a.page_shift));
+      }
     } else if constexpr (KEYS == PAGES) {
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
@@ -385,7 +406,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   // This wave's 16 rows of tile t of one operand to LDS at dst.
   auto load_rows = [&](int t, const int (&id)[NIDS], const uint16_t* base, int64_t page_stride, int64_t row_stride,
                        const uint32_t (&ofs)[NI], uint32_t dst) __attribute__((always_inline)) {
-    dst += wave_s * NI * 1024;
+    dst += FEW ? 0 : wave_s * NI * 1024;
     if constexpr (KEYS == PAGES) {
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
@@ -398,27 +419,30 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
         if (in && has) at = base + id[i] * page_stride + slot * row_stride + chunk;
         dma16_flat(dst + i * 1024, at);
       }
+    } else if constexpr (KEYS == DENSE) {
+      const v4i rsrc = rows_rsrc<D>(base + int64_t{t} * KT * row_stride, min(p.span - t * KT, KT), row_stride);
+#pragma unroll
+      for (int i = 0; i < NI; ++i) gemm::dma16<true>(dst + i * 1024, ofs[i], rsrc);
     } else {
-      int rows;
-      if constexpr (KEYS == DENSE) {
-        rows = min(p.span - t * KT, KT);
-        base += int64_t{t} * KT * row_stride;
-      } else {
-        const int key = t * KT + wave_s * 16, page = __builtin_amdgcn_readfirstlane(id[0]);
-        rows = min(p.span - key, 16);
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) {
+        const int key = t * KT + first_row + 16 * g, page = __builtin_amdgcn_readfirstlane(id[g]);
+        const uint16_t* at = base;
+        int rows = min(p.span - key, 16);
         if (rows > 0) {
           if (static_cast<uint32_t>(page) < static_cast<uint32_t>(a.pages)) {
             const int slot = key - static_cast<int>(fast_div(key, a.page_magic, a.page_shift)) * a.page_size;
-            base += page * page_stride + slot * row_stride;
+            at += page * page_stride + slot * row_stride;
           } else {
             rows = 0;
             lacking = true;
           }
         }
-      }
-      const v4i rsrc = rows_rsrc<D>(base, rows, row_stride);
+        const v4i rsrc = rows_rsrc<D>(at, rows, row_stride);
+        constexpr int PER = NI / GROUPS;
 #pragma unroll
-      for (int i = 0; i < NI; ++i) gemm::dma16<true>(dst + i * 1024, ofs[i], rsrc);
+        for (int i = 0; i < PER; ++i) gemm::dma16<true>(dst + (g * PER + i) * 1024, ofs[g * PER + i], rsrc);
+      }
     }
   };
 
@@ -487,7 +511,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
       if (c + AHEAD < QS) key_frags(st, c + AHEAD, kf[(c + AHEAD) % (AHEAD + 1)]);
 #pragma unroll
       for (int b = 0; b < NB; ++b) y[b] = mfma32<DT>(kf[c % (AHEAD + 1)][b], qf[c], c == 0 ? v16f{} : y[b]);
-      if (prob) probabilities(x, c * 32 / QS, (c + 1) * 32 / QS, sum);
+      if (prob) probabilities(x, c * EL / QS, (c + 1) * EL / QS, sum);
       __builtin_amdgcn_sched_barrier(0);
     }
     if (prob) l += sum[0] + sum[1];
@@ -503,14 +527,14 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
         if (a.softcap <= CAP_SHORT) {
           const float y2 = y * (2.0f * LOG2E);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
+          for (int e = 0; e < EL; ++e) {
             const float g = __builtin_amdgcn_exp2f(x[e >> 4][e & 15] * y2) + 1.0f;
             x[e >> 4][e & 15] = __builtin_fmaf(-2.0f * cap2, __builtin_amdgcn_rcpf(g), cap2);
             if ((e & 7) == 7) __builtin_amdgcn_sched_barrier(0);
           }
         } else {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
+          for (int e = 0; e < EL; ++e) {
             x[e >> 4][e & 15] = tanh_f32(x[e >> 4][e & 15] * y) * cap2;
             if ((e & 3) == 3) __builtin_amdgcn_sched_barrier(0);  // few registers
           }
@@ -519,7 +543,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
       if (a.slopes) {
         const float apart = static_cast<float>(rr.pos - kofs0), f = a.softcap > 0.0f ? 1.0f : scale2;
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
+        for (int e = 0; e < EL; ++e) {
           const float d = fabsf(apart - static_cast<float>(32 * (e >> 4) + 8 * ((e & 15) >> 2) + (e & 3)));
           x[e >> 4][e & 15] = __builtin_fmaf(x[e >> 4][e & 15], f, -slope2 * d);
         }
@@ -564,7 +588,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
         o[b] = mfma32<DT>(vf[i % (AHEAD + 1)][j], pf[2 * i / OB], o[b]);
       }
 #pragma unroll
-      for (int e = i * 32 / STEPS; e < (i + 1) * 32 / STEPS; e += 2) {
+      for (int e = i * EL / STEPS; e < (i + 1) * EL / STEPS; e += 2) {
         t0 = fmaxf(t0, x[e >> 4][e & 15]);
         t1 = fmaxf(t1, x[e >> 4][(e & 15) + 1]);
       }
@@ -598,7 +622,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   auto maximum = [&](const v16f (&x)[NB]) __attribute__((always_inline)) {
     float t0 = x[0][0];
 #pragma unroll
-    for (int e = 1; e < 32; ++e) t0 = fmaxf(t0, x[e >> 4][e & 15]);
+    for (int e = 1; e < EL; ++e) t0 = fmaxf(t0, x[e >> 4][e & 15]);
     return t0;
   };
   // Adopt a tile maximum where a row's exceeds the running one by more than LAZY.
@@ -651,13 +675,46 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
       adopt(maximum(next));
     } else if (now) {
       float sum[2] = {};
-      probabilities(x, 0, 32, sum);
+      probabilities(x, 0, EL, sum);
       l += sum[0] + sum[1];
       accumulate(EVEN, x);
     }
   };
+  // FEW: this wave's tile t from stage ST, its next one (4 further on) on its way to the other stage.
+  auto own_tile = [&](int t, auto stage) __attribute__((always_inline)) {
+    constexpr int ST = decltype(stage)::value;
+    if (t + WAVES < t_end) {
+      __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last reads of that stage
+      load_rows(t + WAVES, ids[0], kbase, a.k_page, a.k_row, kofs, lds0 + (1 - ST) * TILE);
+      load_rows(t + WAVES, ids[0], vbase, a.v_page, a.v_row, vofs, lds0 + (3 - ST) * TILE);
+      load_ids(t + 2 * WAVES, ids[0]);
+      gemm::wait_stage<2 * NI>();
+    } else {
+      gemm::wait_stage<0>();
+    }
+    uint32_t none;
+    product(s[0], ST, s[0], false);
+    finish(s[0], t, quick, none);
+    adopt(maximum(s[0]));
+    float sum[2] = {};
+    probabilities(s[0], 0, EL, sum);
+    l += sum[0] + sum[1];
+    accumulate(ST, s[0]);
+  };
   start();
-  if (t_begin < t_end) {
+  if constexpr (FEW) {
+    int t = t_begin + wave_s;
+    if (t < t_end) {
+      load_ids(t, ids[0]);
+      load_rows(t, ids[0], kbase, a.k_page, a.k_row, kofs, lds0);
+      load_rows(t, ids[0], vbase, a.v_page, a.v_row, vofs, lds0 + 2 * TILE);
+      load_ids(t + WAVES, ids[0]);
+    }
+    for (; t < t_end; t += 2 * WAVES) {
+      own_tile(t, std::integral_constant<int, 0>{});
+      if (t + WAVES < t_end) own_tile(t + WAVES, std::integral_constant<int, 1>{});
+    }
+  } else if (t_begin < t_end) {
     load_ids(t_begin, ids[1]);
     load_rows(t_begin, ids[1], kbase, a.k_page, a.k_row, kofs, lds0);
     load_ids(t_begin + 1, ids[0]);
@@ -671,31 +728,95 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   for (int b = 0; b < OB; ++b)
 #pragma unroll
     for (int r = 0; r < 16; ++r) check = __builtin_fmaf(o[b][r], 0.0f, check);
+  wait_all();
   if (__syncthreads_or(lacking || check != 0.0f)) {
     constexpr std::true_type careful{};
     start();
     for (int t = t_begin; t < t_end; ++t) {
+      if (FEW && ((t - t_begin) & (WAVES - 1)) != wave_s) continue;
       load_ids(t, ids[0]);
       load_rows(t, ids[0], kbase, a.k_page, a.k_row, kofs, lds0);
       load_rows(t, ids[0], vbase, a.v_page, a.v_row, vofs, lds0 + 2 * TILE);
       wait_all();
-      gemm::stage_barrier();
+      if constexpr (!FEW) gemm::stage_barrier();
       if (t >= first && t < last) {
         uint32_t sees;
         product(s[0], 0, s[1], false);
         finish(s[0], t, careful, sees);
         adopt(maximum(s[0]));
         float sum[2] = {};
-        probabilities(s[0], 0, 32, sum);
+        probabilities(s[0], 0, EL, sum);
         l += sum[0] + sum[1];
         accumulate_careful(sees);
       }
       wait_all();
-      gemm::stage_barrier();
+      if constexpr (!FEW) gemm::stage_barrier();
     }
+    if constexpr (FEW) __syncthreads();
   }
 
   l += other_half(l);
+  if constexpr (FEW) {
+    // The waves' sums joined in LDS, in wave order: a row's sums in rows of D + 4 floats (16 bytes a lane without bank
+    // conflicts), its maximum and total behind the last row.  Then 8 threads a row.
+    constexpr int SUMS = (D + 4) * 4, AREA = 4 * TILE;
+    static_assert(32 * SUMS + 256 <= AREA, "a wave's sums fit in its tiles");
+    uint8_t* mine = lds + wave * AREA;
+    float* ml = reinterpret_cast<float*>(mine + 32 * SUMS) + 2 * (lane & 31);
+    if (half == 0) {
+      ml[0] = m;
+      ml[1] = l;
+    }
+#pragma unroll
+    for (int b = 0; b < OB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        *reinterpret_cast<float4*>(mine + (lane & 31) * SUMS + (32 * b + 2 * r + 4 * half) * 4) =
+            make_float4(o[b][r], o[b][r + 1], o[b][r + 2], o[b][r + 3]);
+    __syncthreads();
+    constexpr int E = D / 8;
+    const int r = threadIdx.x >> 3, c = (threadIdx.x & 7) * E;
+    if (row0 + r >= p.rows) return;
+    float top = M_FLOOR, total = 0.0f, acc[E] = {};
+    float w[WAVES];
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) {
+      w[i] = *reinterpret_cast<const float*>(lds + i * AREA + 32 * SUMS + 8 * r);
+      top = fmaxf(top, w[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) {
+      w[i] = __builtin_amdgcn_exp2f(w[i] - top);
+      total = __builtin_fmaf(*reinterpret_cast<const float*>(lds + i * AREA + 32 * SUMS + 8 * r + 4), w[i], total);
+      const float* src = reinterpret_cast<const float*>(lds + i * AREA + r * SUMS) + c;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = __builtin_fmaf(src[e], w[i], acc[e]);
+    }
+    int t_out, h_out;
+    range_of<KEYS>(a, p, row0 + r, t_out, h_out);
+    if (a.splits > 1) {
+      const int64_t at = (int64_t{p.split} * a.tokens + t_out) * a.heads + h_out;
+      if (c == 0) {
+        a.part_ml[2 * at] = top;
+        a.part_ml[2 * at + 1] = total;
+      }
+#pragma unroll
+      for (int e = 0; e < E; e += 4)
+        *reinterpret_cast<float4*>(a.part_o + at * D + c + e) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
+      return;
+    }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    uint16_t* op = a.out + (int64_t{t_out} * a.heads + h_out) * D + c;
+#pragma unroll
+    for (int e = 0; e < E; e += 8) {
+      uint32_t v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        v[i] = total == 0.0f ? 0u : pack2<DT>(acc[e + 2 * i] * inv, acc[e + 2 * i + 1] * inv);
+      *reinterpret_cast<uint4*>(op + e) = make_uint4(v[0], v[1], v[2], v[3]);
+    }
+    return;
+  }
   if (!live) return;
   if (a.splits > 1) {
     const int64_t at = (int64_t{p.split} * a.tokens + token) * a.heads + head;
@@ -788,16 +909,51 @@ __global__ __launch_bounds__(256) void attention_join(const Args a) {
   }
 }
 
+// How a call is launched.  `few`: sequences of no more than 32 packed rows on average, or fewer tiles of 128 rows than
+// compute units (128 tokens, 56 heads of 128: 8.7 us with tiles of 128 rows, 6.3 us with `few`; 1999 tokens, 4 key
+// heads of 64, prefix and cap, 252 tiles: 43.8 and 35.6 us; chunks of 830 tokens, 16 heads of 64, 144 tiles: 33.8 and
+// 23.9 us).
+struct Plan {
+  bool few;
+  int slots;
+};
+inline Plan plan(bool paged, int64_t tokens, int group, int kv_heads, int64_t sequences, int cus) {
+  const int64_t rows = tokens * group, own = paged ? sequences : 1;
+  const int64_t tiles = (rows / (32 * WAVES) + own) * kv_heads;
+  const bool few = rows <= 32 * own || tiles < cus;
+  const int64_t r = few ? 32 : 32 * WAVES;
+  return Plan{few, static_cast<int>(paged ? rows / r + sequences + 1 : (rows + r - 1) / r)};
+}
+
+// Key splits: as many as bring the workgroups to what the compute units hold at once (two each; one of `few` with heads
+// of 128), each over at least 256 keys of the longest span; twice as many were slower (chunks of 830 tokens over 4008
+// keys: 24 and 34 us).  Sequences of few rows that fill the chip unsplit still differ in length, and the longest ends
+// last: two splits of them where a span can be long enough to pay for the join (64 tokens over 0 to 8190 keys, 8 key
+// heads: 177 and 158 us).
+inline int plan_splits(bool paged, int64_t tokens, int group, int kv_heads, int head_dim, int64_t sequences,
+                       int64_t keys, int cus) {
+  const Plan p = plan(paged, tokens, group, kv_heads, sequences, cus);
+  // Slots that have rows: of a paged launch about half a tile a sequence on top of the whole ones.
+  const int64_t r = p.few ? 32 : 32 * WAVES, whole = tokens * group / r, own = tokens < sequences ? tokens : sequences;
+  const int64_t tiles = !paged ? p.slots : whole + own / 2 > own ? whole + own / 2 : own;
+  const int64_t busy = (tiles > 0 ? tiles : 1) * kv_heads;
+  int64_t n = (p.few && head_dim == 128 ? 1 : 2) * int64_t{cus} / busy;
+  const int64_t most = keys / 256;
+  if (paged && p.few && n < 2 && keys >= 4096 && busy <= 4 * int64_t{cus}) n = 2;
+  n = n < most ? n : most;
+  return static_cast<int>(n < 1 ? 1 : n > 64 ? 64 : n);
+}
+
 template <int DT, int D, int KEYS>
-int launch(const Args& a, hipStream_t st) {
+int launch(Args& a, hipStream_t st) {
   const bool mods = a.softcap > 0.0f || a.slopes;
+  const Plan p = plan(KEYS != DENSE, a.tokens, a.group, a.kv_heads, a.sequences, device_cus());
+  a.slots = p.slots;
   const int64_t blocks = int64_t{a.slots} * a.kv_heads * a.splits;
-  if (blocks > 0x7FFFFFFF) {
-    set_error("attention: too many tiles for one launch");
-    return M5K_EINVAL;
-  }
-  launch_kernel(mods ? attention_tile<DT, D, KEYS, true> : attention_tile<DT, D, KEYS, false>,
-                dim3(static_cast<uint32_t>(blocks)), dim3(THREADS), st, a);
+  M5K_REQUIRE(blocks <= INT32_MAX, "attention: too many tiles for one launch");
+  auto kernel = p.few ? (mods ? attention_tile<DT, D, KEYS, true, true> : attention_tile<DT, D, KEYS, false, true>)
+                      : (mods ? attention_tile<DT, D, KEYS, true, false> : attention_tile<DT, D, KEYS, false, false>);
+  launch_kernel(kernel, dim3(static_cast<uint32_t>(blocks)), dim3(THREADS), st, a);
   int rc = launch_status("attention");
   if (rc != M5K_OK || a.splits == 1) return rc;
   const int64_t rows = int64_t{a.tokens} * a.heads;
@@ -809,27 +965,10 @@ int launch(const Args& a, hipStream_t st) {
 }
 
 template <int KEYS>
-int launch_typed(const Args& a, int dtype, int head_dim, hipStream_t st) {
+int launch_typed(Args& a, int dtype, int head_dim, hipStream_t st) {
   if (dtype == M5K_BF16)
     return head_dim == 64 ? launch<M5K_BF16, 64, KEYS>(a, st) : launch<M5K_BF16, 128, KEYS>(a, st);
   return head_dim == 64 ? launch<M5K_F16, 64, KEYS>(a, st) : launch<M5K_F16, 128, KEYS>(a, st);
-}
-
-// Packed rows per workgroup and the key splits of a launch: as many as bring the workgroups to two a compute unit
-// (what its LDS holds), each over at least 256 keys of the longest span.
-inline int plan_slots(bool paged, int64_t tokens, int group, int64_t sequences) {
-  const int64_t r = 32 * WAVES;
-  return static_cast<int>(paged ? tokens * group / r + sequences + 1 : (tokens * group + r - 1) / r);
-}
-inline int plan_splits(bool paged, int64_t tokens, int group, int kv_heads, int64_t sequences, int64_t keys, int cus) {
-  // Tiles that have rows: a paged launch has a spare slot a sequence.
-  const int64_t r = 32 * WAVES, whole = tokens * group / r, at_least = tokens < sequences ? tokens : sequences;
-  const int64_t tiles = paged ? (whole > at_least ? whole : at_least) : (tokens * group + r - 1) / r;
-  const int64_t busy = (tiles > 0 ? tiles : 1) * kv_heads;
-  int64_t n = 2 * int64_t{cus} / busy;
-  const int64_t most = keys / 256;
-  n = n < most ? n : most;
-  return static_cast<int>(n < 1 ? 1 : n > 64 ? 64 : n);
 }
 
 inline void magic_of(uint32_t d, uint32_t& magic, uint32_t& shift) {

@@ -262,9 +262,9 @@ def paged_append(k, v, k_cache, v_cache, page_table, query_starts, context_lengt
 
 
 @functools.lru_cache(maxsize=4096)
-def _splits(paged, tokens, heads, kv_heads, sequences, keys, cus):
+def _splits(paged, tokens, heads, kv_heads, width, sequences, keys, cus):
     n = ctypes.c_int(0)
-    _lib.call("m5k_attention_splits", paged, tokens, heads, kv_heads, sequences, keys, cus, ctypes.byref(n))
+    _lib.call("m5k_attention_splits", paged, tokens, heads, kv_heads, width, sequences, keys, cus, ctypes.byref(n))
     return n.value
 
 
@@ -344,7 +344,8 @@ def paged_attention(q, k_cache, v_cache, page_table, query_starts, context_lengt
     q = _rows(q, "q")
     qs = _strides(q)
     pages, page_size = k_cache.shape[0], k_cache.shape[2]
-    splits = _splits(1, tokens, heads, kv_heads, sequences, table_width * page_size, hip._cu_count_of(device.index))
+    splits = _splits(1, tokens, heads, kv_heads, width, sequences, table_width * page_size,
+                     hip._cu_count_of(device.index))
     workspace, n = _workspace(splits, tokens, heads, width, device)
     with _on(device):
         _lib.call(
@@ -401,7 +402,7 @@ def attention(q, k, v, *, causal=False, window=None, document_starts=None, prefi
         return out
     q, k, v = _rows(q, "q"), _apart(_rows(k, "k")), _apart(_rows(v, "v"))
     qs, ks, vs = _strides(q), _strides(k), _strides(v)
-    splits = _splits(0, tokens, heads, kv_heads, documents, keys, hip._cu_count_of(device.index))
+    splits = _splits(0, tokens, heads, kv_heads, width, documents, keys, hip._cu_count_of(device.index))
     workspace, n = _workspace(splits, tokens, heads, width, device)
     with _on(device):
         _lib.call(

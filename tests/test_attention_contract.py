@@ -159,7 +159,7 @@ def test_c_entries_refuse_without_launching():
                       (dict(keys=-1), b"keys"), (dict(starts=p, docs=1, keys=5), b"documents"),
                       (dict(prefix=p), b"causal"), (dict(prefix=p, causal=1, window=2), b"combined")):
         assert attention(**bad) == 1 and text in lib.m5k_last_error(), (bad, lib.m5k_last_error())
-    assert lib.m5k_attention_splits(0, 4, 3, 2, 0, 4, 256, ctypes.byref(n)) == 1
+    assert lib.m5k_attention_splits(0, 4, 3, 2, 64, 0, 4, 256, ctypes.byref(n)) == 1
 
     def rope(pairs=2, d=8, x=p, heads=2):
         return lib.m5k_rope(x, _lib.F32, 4, heads, d, 8, 8, p, p, pairs, 0, s, p, None)
@@ -169,10 +169,11 @@ def test_c_entries_refuse_without_launching():
 
 
 def test_split_rule():
-    """Enough rows: no split.  Few rows: up to two workgroups a compute unit, over 256 keys at least each."""
+    """Enough rows: no split.  Few rows: as many workgroups as run at once, over 256 keys at least each."""
     plan = lambda *a: module._splits(*a, 256)  # noqa: E731
-    assert plan(0, 4096, 56, 56, 0, 4096) == 1
-    assert plan(0, 1, 8, 8, 0, 255) == 1
-    assert plan(1, 1, 64, 8, 1, 131072) == 64
-    assert plan(1, 64, 64, 8, 64, 8192) == 1
-    assert 1 < plan(1, 8, 64, 8, 8, 8192) <= 32
+    assert plan(0, 4096, 56, 56, 128, 0, 4096) == 1
+    assert plan(0, 1, 8, 8, 128, 0, 255) == 1
+    assert plan(1, 1, 64, 8, 128, 1, 131072) == 32
+    assert plan(1, 1, 64, 8, 64, 1, 131072) == 64
+    assert plan(1, 64, 64, 8, 128, 64, 8192) == 2 and plan(1, 64, 64, 8, 128, 64, 2048) == 1
+    assert 1 < plan(1, 8, 64, 8, 64, 8, 8192) <= 32
