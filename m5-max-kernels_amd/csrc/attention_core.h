@@ -163,7 +163,7 @@ __device__ __forceinline__ RowRange row_range(int s, int e, int p, int prefix, i
   return RowRange{lo, hi, p};
 }
 
-// The last b in [0, n) with starts[b] + pad * b ... <= x, by binary search over a nondecreasing key(b); 0 if none.
+// The last b in [0, n) with key(b) <= x, by binary search over a nondecreasing key; 0 if there is none.
 template <class Key>
 __device__ __forceinline__ int last_not_above(int n, int x, Key key) {
   int lo = 0, hi = n;
@@ -261,7 +261,16 @@ __device__ __forceinline__ Place place(const Args& a, int rows_per_tile) {
     const int T = a.tokens, B = a.sequences;
     auto start = [&](int b) { return b == 0 ? 0 : min(max(a.starts[b], 0), T); };
     auto first = [&](int b) { return static_cast<int>(int64_t{start(b)} * a.group / rows_per_tile) + b; };
-    p.seq = last_not_above(B + 1, slot, first);
+    // The last b with first(b) <= slot, 64 probes at a time.
+    int lo = 0, left = B + 1;
+    while (left > 1) {
+      const int apart = (left + 63) >> 6, probe = static_cast<int>(threadIdx.x & 63) * apart;
+      const bool below = probe < left && first(lo + probe) <= slot;
+      const int at = max(__popcll(__builtin_amdgcn_ballot_w64(below)) - 1, 0) * apart;
+      lo += at;
+      left = min(apart, left - at);
+    }
+    p.seq = __builtin_amdgcn_readfirstlane(lo);
     p.token0 = start(p.seq);
     p.tile = slot - first(p.seq);
     const int end = p.seq == B ? T : start(p.seq + 1);
@@ -295,10 +304,11 @@ __device__ __forceinline__ RowRange range_of(const Args& a, const Place& p, int 
 }
 
 // FEW = false: the 4 waves take 32 rows each and share key tiles of 64.  FEW: they share 32 rows, for calls that have
-// no more, and take every fourth tile of 32 keys each, through LDS of their own: no barrier in the loop, two tiles a
-// wave in flight, and the keys of a short row are read four tiles at a time.
+// no more, and take every fourth tile of 32 keys each, through LDS of their own: no barrier in the loop, and the keys
+// of a short row are read four tiles at a time.  One K and one V tile a wave: with two of each, one workgroup a compute
+// unit, 64 tokens over 300 keys took 36 us instead of 24, over 1000 keys of 256 sequences 199 instead of 183.
 template <int DT, int D, int KEYS, bool MODS, bool FEW>
-__global__ __launch_bounds__(THREADS, FEW && D == 128 ? 1 : 2) void attention_tile(const Args a) {
+__global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   constexpr int KT = FEW ? 32 : 64, NB = KT / 32;  // keys of a tile, 32-key blocks
   constexpr int EL = 16 * NB;                      // scores of a lane
   constexpr int CH = D / 8;                        // 16-byte chunks of a row
@@ -310,8 +320,11 @@ __global__ __launch_bounds__(THREADS, FEW && D == 128 ? 1 : 2) void attention_ti
   constexpr int AHEAD = 1;  // steps of two products between a fragment's read and its use (2: no faster)
   constexpr int ROWS = FEW ? 32 : 32 * WAVES;
   constexpr uint32_t ROWB = D * 2, TILE = KT * ROWB;
-  // K stages 0 and 1, V stages 0 and 1; FEW: those of each wave, later its sums.
-  __shared__ __attribute__((aligned(256))) uint8_t lds[(FEW ? WAVES : 1) * 4 * TILE];
+  // K stages 0 and 1, V stages 0 and 1.  FEW: one K and one V tile of each wave, later its sums, in rows of D + 4
+  // floats (16 bytes a lane without bank conflicts), and their maxima and totals.
+  constexpr uint32_t SUMS = (D + 4) * 4, AREA = 32 * SUMS + 256, VTILE = FEW ? TILE : 2 * TILE;
+  static_assert(AREA >= 2 * TILE || !FEW, "a wave's tiles fit in its area");
+  __shared__ __attribute__((aligned(256))) uint8_t lds[FEW ? WAVES * AREA : 4 * TILE];
   __shared__ int bounds[2 * WAVES];
 
   const Place p = place<KEYS>(a, ROWS);
@@ -371,7 +384,7 @@ __global__ __launch_bounds__(THREADS, FEW && D == 128 ? 1 : 2) void attention_ti
   const uint16_t* kbase = a.k + int64_t{p.kvh} * a.k_head;
   const uint16_t* vbase = a.v + int64_t{p.kvh} * a.v_head;
   const int32_t* table = KEYS != DENSE && p.seq < a.sequences ? a.table + int64_t{p.seq} * a.table_width : nullptr;
-  const uint32_t lds0 = gemm::lds_addr(lds) + (FEW ? wave_s * 4 * TILE : 0);
+  const uint32_t lds0 = gemm::lds_addr(lds) + (FEW ? wave_s * AREA : 0);
   uint32_t kofs[NI], vofs[NI];  // bytes of a lane's chunk from the window's first row
   if constexpr (KEYS != PAGES) {
 #pragma unroll
@@ -481,7 +494,7 @@ __global__ __launch_bounds__(THREADS, FEW && D == 128 ? 1 : 2) void attention_ti
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          reinterpret_cast<lds_v4s>(vread[h][b] + 16 * c * ROWB + (2 + st) * TILE));
+          reinterpret_cast<lds_v4s>(vread[h][b] + 16 * c * ROWB + VTILE + st * TILE));
       const auto y = __builtin_bit_cast(m5k_u32x2, x);
       f[2 * h] = static_cast<int>(y[0]);
       f[2 * h + 1] = static_cast<int>(y[1]);
@@ -680,26 +693,30 @@ __global__ __launch_bounds__(THREADS, FEW && D == 128 ? 1 : 2) void attention_ti
       accumulate(EVEN, x);
     }
   };
-  // FEW: this wave's tile t from stage ST, its next one (4 further on) on its way to the other stage.
-  auto own_tile = [&](int t, auto stage) __attribute__((always_inline)) {
-    constexpr int ST = decltype(stage)::value;
-    if (t + WAVES < t_end) {
-      __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last reads of that stage
-      load_rows(t + WAVES, ids[0], kbase, a.k_page, a.k_row, kofs, lds0 + (1 - ST) * TILE);
-      load_rows(t + WAVES, ids[0], vbase, a.v_page, a.v_row, vofs, lds0 + (3 - ST) * TILE);
-      load_ids(t + 2 * WAVES, ids[0]);
-      gemm::wait_stage<2 * NI>();
-    } else {
-      gemm::wait_stage<0>();
+  // FEW: this wave's tile t.  The K of its next one (WAVES further on) is loaded as soon as this one's has been read, V
+  // likewise, so that one of the two is on its way through every phase.  Loads end in the order of their issue.
+  auto own_tile = [&](int t) __attribute__((always_inline)) {
+    const bool more = t + WAVES < t_end;
+    gemm::wait_stage<NI>();  // K, behind which V was issued
+    product(s[0], 0, s[0], false);
+    if (more) {
+      __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      load_rows(t + WAVES, ids[0], kbase, a.k_page, a.k_row, kofs, lds0);
     }
     uint32_t none;
-    product(s[0], ST, s[0], false);
     finish(s[0], t, quick, none);
     adopt(maximum(s[0]));
     float sum[2] = {};
     probabilities(s[0], 0, EL, sum);
     l += sum[0] + sum[1];
-    accumulate(ST, s[0]);
+    if (more) gemm::wait_stage<NI>();
+    else gemm::wait_stage<0>();
+    accumulate(0, s[0]);
+    if (more) {
+      __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      load_rows(t + WAVES, ids[0], vbase, a.v_page, a.v_row, vofs, lds0 + VTILE);
+      load_ids(t + 2 * WAVES, ids[0]);
+    }
   };
   start();
   if constexpr (FEW) {
@@ -707,13 +724,10 @@ __global__ __launch_bounds__(THREADS, FEW && D == 128 ? 1 : 2) void attention_ti
     if (t < t_end) {
       load_ids(t, ids[0]);
       load_rows(t, ids[0], kbase, a.k_page, a.k_row, kofs, lds0);
-      load_rows(t, ids[0], vbase, a.v_page, a.v_row, vofs, lds0 + 2 * TILE);
+      load_rows(t, ids[0], vbase, a.v_page, a.v_row, vofs, lds0 + VTILE);
       load_ids(t + WAVES, ids[0]);
     }
-    for (; t < t_end; t += 2 * WAVES) {
-      own_tile(t, std::integral_constant<int, 0>{});
-      if (t + WAVES < t_end) own_tile(t + WAVES, std::integral_constant<int, 1>{});
-    }
+    for (; t < t_end; t += WAVES) own_tile(t);
   } else if (t_begin < t_end) {
     load_ids(t_begin, ids[1]);
     load_rows(t_begin, ids[1], kbase, a.k_page, a.k_row, kofs, lds0);
@@ -736,7 +750,7 @@ __global__ __launch_bounds__(THREADS, FEW && D == 128 ? 1 : 2) void attention_ti
       if (FEW && ((t - t_begin) & (WAVES - 1)) != wave_s) continue;
       load_ids(t, ids[0]);
       load_rows(t, ids[0], kbase, a.k_page, a.k_row, kofs, lds0);
-      load_rows(t, ids[0], vbase, a.v_page, a.v_row, vofs, lds0 + 2 * TILE);
+      load_rows(t, ids[0], vbase, a.v_page, a.v_row, vofs, lds0 + VTILE);
       wait_all();
       if constexpr (!FEW) gemm::stage_barrier();
       if (t >= first && t < last) {
@@ -757,10 +771,7 @@ __global__ __launch_bounds__(THREADS, FEW && D == 128 ? 1 : 2) void attention_ti
 
   l += other_half(l);
   if constexpr (FEW) {
-    // The waves' sums joined in LDS, in wave order: a row's sums in rows of D + 4 floats (16 bytes a lane without bank
-    // conflicts), its maximum and total behind the last row.  Then 8 threads a row.
-    constexpr int SUMS = (D + 4) * 4, AREA = 4 * TILE;
-    static_assert(32 * SUMS + 256 <= AREA, "a wave's sums fit in its tiles");
+    // The waves' sums joined in LDS, in wave order, by 8 threads a row.
     uint8_t* mine = lds + wave * AREA;
     float* ml = reinterpret_cast<float*>(mine + 32 * SUMS) + 2 * (lane & 31);
     if (half == 0) {
@@ -909,37 +920,41 @@ __global__ __launch_bounds__(256) void attention_join(const Args a) {
   }
 }
 
-// How a call is launched.  `few`: sequences of no more than 32 packed rows on average, or fewer tiles of 128 rows than
-// compute units (128 tokens, 56 heads of 128: 8.7 us with tiles of 128 rows, 6.3 us with `few`; 1999 tokens, 4 key
-// heads of 64, prefix and cap, 252 tiles: 43.8 and 35.6 us; chunks of 830 tokens, 16 heads of 64, 144 tiles: 33.8 and
-// 23.9 us).
+// How a call is launched.  `few`: sequences of no more than 32 packed rows on average; or fewer tiles of 128 rows than
+// compute units, where 32-row workgroups fill them better (two run on one at once), the keys are not so many that the
+// other form's key splits cost nothing beside them, and not so few that a second round of workgroups costs more than
+// it brings.  With tiles of 128 rows and with `few`: 128 tokens, 56 heads of 128: 8.7 and 5.8 us; 300 tokens: 12.8 and
+// 15.8; 1024 tokens, 16 heads: 33.8 and 18.0; 1999 tokens, 4 key heads of 64, prefix and cap: 43.8 and 32.2; 9914
+// tokens, one head: 71 and 98.
 struct Plan {
   bool few;
   int slots;
 };
-inline Plan plan(bool paged, int64_t tokens, int group, int kv_heads, int64_t sequences, int cus) {
+inline Plan plan(bool paged, int64_t tokens, int group, int kv_heads, int64_t sequences, int64_t keys, int cus) {
   const int64_t rows = tokens * group, own = paged ? sequences : 1;
-  const int64_t tiles = (rows / (32 * WAVES) + own) * kv_heads;
-  const bool few = rows <= 32 * own || tiles < cus;
+  const int64_t tiles = (rows / (32 * WAVES) + own) * kv_heads, thin = (rows / 32 + own) * kv_heads;
+  const bool few = rows <= 32 * own || (tiles < cus && thin <= (keys < 512 ? 2 : 4) * cus && keys <= 4096);
   const int64_t r = few ? 32 : 32 * WAVES;
   return Plan{few, static_cast<int>(paged ? rows / r + sequences + 1 : (rows + r - 1) / r)};
 }
 
-// Key splits: as many as bring the workgroups to what the compute units hold at once (two each; one of `few` with heads
-// of 128), each over at least 256 keys of the longest span; twice as many were slower (chunks of 830 tokens over 4008
-// keys: 24 and 34 us).  Sequences of few rows that fill the chip unsplit still differ in length, and the longest ends
-// last: two splits of them where a span can be long enough to pay for the join (64 tokens over 0 to 8190 keys, 8 key
-// heads: 177 and 158 us).
+// Key splits: as many as bring the workgroups to two a compute unit, what it holds at once, each over at least 256 keys
+// of the longest span; twice as many were slower (2048 tokens, 8 heads: 22 and 36 us).  Full workgroups of `few` to
+// one: their waves split the keys already, and the sums of 32 rows cost as much as their keys (2000 tokens, 4 query
+// heads on one key head, 250 workgroups: 19 us, 26 us in two splits).  Single tokens of many sequences differ in length, and the
+// longest ends last: two splits at least where a span can be long enough to pay for the join (64 tokens over 0 to 8190
+// keys, 8 key heads: 177 and 158 us).
 inline int plan_splits(bool paged, int64_t tokens, int group, int kv_heads, int head_dim, int64_t sequences,
                        int64_t keys, int cus) {
-  const Plan p = plan(paged, tokens, group, kv_heads, sequences, cus);
+  const Plan p = plan(paged, tokens, group, kv_heads, sequences, keys, cus);
   // Slots that have rows: of a paged launch about half a tile a sequence on top of the whole ones.
   const int64_t r = p.few ? 32 : 32 * WAVES, whole = tokens * group / r, own = tokens < sequences ? tokens : sequences;
   const int64_t tiles = !paged ? p.slots : whole + own / 2 > own ? whole + own / 2 : own;
   const int64_t busy = (tiles > 0 ? tiles : 1) * kv_heads;
-  int64_t n = (p.few && head_dim == 128 ? 1 : 2) * int64_t{cus} / busy;
+  const bool full = p.few && tokens * group > 32 * (paged ? sequences : 1);
+  int64_t n = (full ? 1 : 2) * int64_t{cus} / busy;
   const int64_t most = keys / 256;
-  if (paged && p.few && n < 2 && keys >= 4096 && busy <= 4 * int64_t{cus}) n = 2;
+  if (paged && p.few && n < 2 && keys >= 4096 && busy <= 4 * int64_t{cus} && tokens <= sequences) n = 2;
   n = n < most ? n : most;
   return static_cast<int>(n < 1 ? 1 : n > 64 ? 64 : n);
 }
@@ -947,7 +962,7 @@ inline int plan_splits(bool paged, int64_t tokens, int group, int kv_heads, int 
 template <int DT, int D, int KEYS>
 int launch(Args& a, hipStream_t st) {
   const bool mods = a.softcap > 0.0f || a.slopes;
-  const Plan p = plan(KEYS != DENSE, a.tokens, a.group, a.kv_heads, a.sequences, device_cus());
+  const Plan p = plan(KEYS != DENSE, a.tokens, a.group, a.kv_heads, a.sequences, a.keys, device_cus());
   a.slots = p.slots;
   const int64_t blocks = int64_t{a.slots} * a.kv_heads * a.splits;
   M5K_REQUIRE(blocks <= INT32_MAX, "attention: too many tiles for one launch");

@@ -173,7 +173,7 @@ def test_split_rule():
     plan = lambda *a: module._splits(*a, 256)  # noqa: E731
     assert plan(0, 4096, 56, 56, 128, 0, 4096) == 1
     assert plan(0, 1, 8, 8, 128, 0, 255) == 1
-    assert plan(1, 1, 64, 8, 128, 1, 131072) == 32
-    assert plan(1, 1, 64, 8, 64, 1, 131072) == 64
+    assert plan(1, 1, 64, 8, 128, 1, 131072) == plan(1, 1, 64, 8, 64, 1, 131072) == 64
+    assert plan(0, 5000, 4, 1, 128, 0, 5000) == 3
     assert plan(1, 64, 64, 8, 128, 64, 8192) == 2 and plan(1, 64, 64, 8, 128, 64, 2048) == 1
     assert 1 < plan(1, 8, 64, 8, 64, 8, 8192) <= 32
