@@ -425,7 +425,7 @@ int m5k_shift_split_condition(const void* gamma, const void* scale, int param_dt
  *   nondecreasing from 0; needs keys == tokens) keeps the row's own document.  A row that sees no key is 0;
  *   so is a row behind the last document.  What a masked key or value holds does not matter, NaN included.
  *   prefix_lengths: int32 [documents], or [1] without document_starts; only with causal, not with window.
- *   splits: key ranges joined by a second launch (m5k_attention_splits gives the number that pays); above 1
+ *   splits: key ranges joined by a second launch (m5k_attention_plan gives the number that pays); above 1
  *   workspace holds splits * tokens * heads * (head_dim + 2) floats that the call may overwrite.
  */
 int m5k_attention(const void* q, int dtype, int64_t tokens, int64_t heads, int head_dim, int64_t q_head,
@@ -435,10 +435,12 @@ int m5k_attention(const void* q, int dtype, int64_t tokens, int64_t heads, int h
                   const int32_t* prefix_lengths, void* out, int splits, float* workspace, int64_t workspace_elems,
                   void* stream);
 
-/* Key splits of m5k_attention (paged 0) or m5k_paged_attention (paged 1, keys = table_width * page_size) that
- * fill `cus` compute units (host only; cus <= 0: those of the current device). */
-int m5k_attention_splits(int paged, int64_t tokens, int64_t heads, int64_t kv_heads, int head_dim, int64_t sequences,
-                         int64_t keys, int cus, int* splits);
+/* The plan of m5k_attention (paged 0, sequences = documents) or m5k_paged_attention (paged 1,
+ * keys = table_width * page_size) on `cus` compute units (host only; cus <= 0: those of the current device): the key
+ * splits that pay, and whether the waves of a workgroup share 32 rows (few 1) or take 32 each (few 0; few may be
+ * NULL). */
+int m5k_attention_plan(int paged, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t sequences, int64_t keys,
+                       int cus, int* splits, int* few);
 
 /*
  * Attention of new tokens over a paged cache: k_cache, v_cache [pages, kv_heads, page_size, head_dim] by

@@ -621,8 +621,7 @@ bool scores_of(const at::Tensor* q, int64_t kv_heads, int64_t dim, at::ScalarTyp
       !positive(softcap, 0.0f, s.softcap) || !window_of(window, s.window) ||
       !optional_vector(slopes, heads, at::kFloat, dev, &s.slopes))
     return false;
-  if (m5k_attention_splits(paged, tokens, heads, kv_heads, static_cast<int>(dim), sequences, keys, 0, &s.splits))
-    return false;
+  if (m5k_attention_plan(paged, tokens, heads, kv_heads, sequences, keys, 0, &s.splits, nullptr)) return false;
   s.out = empty({tokens, heads * dim}, st, dev);
   s.elems = 0;
   s.wp = nullptr;

@@ -48,15 +48,16 @@ int common(Args& a, const void* q, int dtype, int64_t tokens, int64_t heads, int
 
 }  // namespace
 
-extern "C" int m5k_attention_splits(int paged, int64_t tokens, int64_t heads, int64_t kv_heads, int head_dim,
-                                    int64_t sequences, int64_t keys, int cus, int* splits) {
+extern "C" int m5k_attention_plan(int paged, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t sequences,
+                                  int64_t keys, int cus, int* splits, int* few) {
   m5k::clear_error();
   M5K_REQUIRE(splits && tokens > 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && sequences >= 0 && keys >= 0,
-              "attention_splits: bad sizes");
+              "attention_plan: bad sizes");
   if (cus <= 0) cus = m5k::device_cus();
   if (cus <= 0) cus = 256;
-  *splits = m5k::attn::plan_splits(paged != 0, tokens, static_cast<int>(heads / kv_heads), static_cast<int>(kv_heads),
-                                   head_dim, sequences, keys, cus);
+  const int group = static_cast<int>(heads / kv_heads), kvh = static_cast<int>(kv_heads);
+  *splits = m5k::attn::plan_splits(paged != 0, tokens, group, kvh, sequences, keys, cus);
+  if (few) *few = m5k::attn::plan(paged != 0, tokens, group, kvh, sequences, keys, cus).few;
   return M5K_OK;
 }
 

@@ -944,8 +944,8 @@ inline Plan plan(bool paged, int64_t tokens, int group, int kv_heads, int64_t se
 // heads on one key head, 250 workgroups: 19 us, 26 us in two splits).  Single tokens of many sequences differ in length, and the
 // longest ends last: two splits at least where a span can be long enough to pay for the join (64 tokens over 0 to 8190
 // keys, 8 key heads: 177 and 158 us).
-inline int plan_splits(bool paged, int64_t tokens, int group, int kv_heads, int head_dim, int64_t sequences,
-                       int64_t keys, int cus) {
+inline int plan_splits(bool paged, int64_t tokens, int group, int kv_heads, int64_t sequences, int64_t keys,
+                       int cus) {
   const Plan p = plan(paged, tokens, group, kv_heads, sequences, keys, cus);
   // Slots that have rows: of a paged launch about half a tile a sequence on top of the whole ones.
   const int64_t r = p.few ? 32 : 32 * WAVES, whole = tokens * group / r, own = tokens < sequences ? tokens : sequences;

@@ -77,7 +77,7 @@ SIGNATURES = {
     "m5k_projection_qk_rope": [_p, _p, _i32, _i64, _i64, _i64, _p, _p, _p, _p, _p, _i32, _f32, _p, _p],
     "m5k_qk_norm_rope": [_p, _i64, _i64, _p, _p, _p, _i32, _f32, _p, _p],
     "m5k_qkv_norm_rope": [_p, _i64, _i64, _p, _p, _p, _p, _i32, _f32, _p, _p, _p, _p],
-    "m5k_attention_splits": [_i32, _i64, _i64, _i64, _i32, _i64, _i64, _i32, _p],
+    "m5k_attention_plan": [_i32, _i64, _i64, _i64, _i64, _i64, _i32, _p, _p],
     "m5k_attention": [
         _p, _i32, _i64, _i64, _i32, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _f32, _i32, _i64, _f32, _p,
         _p, _i64, _p, _p, _i32, _p, _i64, _p,

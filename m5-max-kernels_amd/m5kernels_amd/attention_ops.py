@@ -262,10 +262,12 @@ def paged_append(k, v, k_cache, v_cache, page_table, query_starts, context_lengt
 
 
 @functools.lru_cache(maxsize=4096)
-def _splits(paged, tokens, heads, kv_heads, width, sequences, keys, cus):
-    n = ctypes.c_int(0)
-    _lib.call("m5k_attention_splits", paged, tokens, heads, kv_heads, width, sequences, keys, cus, ctypes.byref(n))
-    return n.value
+def _plan(paged, tokens, heads, kv_heads, sequences, keys, cus):
+    """(key splits, whether waves share rows) of a call (m5k_attention_plan; host only)."""
+    n, few = ctypes.c_int(0), ctypes.c_int(0)
+    _lib.call("m5k_attention_plan", paged, tokens, heads, kv_heads, sequences, keys, cus, ctypes.byref(n),
+              ctypes.byref(few))
+    return n.value, bool(few.value)
 
 
 def _scores(q, heads, width, scale, softcap, window, slopes):
@@ -344,8 +346,7 @@ def paged_attention(q, k_cache, v_cache, page_table, query_starts, context_lengt
     q = _rows(q, "q")
     qs = _strides(q)
     pages, page_size = k_cache.shape[0], k_cache.shape[2]
-    splits = _splits(1, tokens, heads, kv_heads, width, sequences, table_width * page_size,
-                     hip._cu_count_of(device.index))
+    splits, _ = _plan(1, tokens, heads, kv_heads, sequences, table_width * page_size, hip._cu_count_of(device.index))
     workspace, n = _workspace(splits, tokens, heads, width, device)
     with _on(device):
         _lib.call(
@@ -402,7 +403,7 @@ def attention(q, k, v, *, causal=False, window=None, document_starts=None, prefi
         return out
     q, k, v = _rows(q, "q"), _apart(_rows(k, "k")), _apart(_rows(v, "v"))
     qs, ks, vs = _strides(q), _strides(k), _strides(v)
-    splits = _splits(0, tokens, heads, kv_heads, width, documents, keys, hip._cu_count_of(device.index))
+    splits, _ = _plan(0, tokens, heads, kv_heads, documents, keys, hip._cu_count_of(device.index))
     workspace, n = _workspace(splits, tokens, heads, width, device)
     with _on(device):
         _lib.call(

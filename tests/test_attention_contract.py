@@ -154,12 +154,13 @@ def test_c_entries_refuse_without_launching():
     for bad, text in ((dict(q=None), b"null"), (dict(dtype=_lib.F32), b"dtype"), (dict(d=96), b"head_dim"),
                       (dict(heads=3), b"multiple"), (dict(tokens=0), b"positive"), (dict(qt=63), b"aligned"),
                       (dict(q=ctypes.c_void_p(68)), b"aligned"), (dict(scale=0.0), b"scale"),
-                      (dict(cap=-1.0), b"softcap"), (dict(scale=float("nan")), b"scale"), (dict(window=-1), b"window"), (dict(splits=0), b"splits"),
+                      (dict(cap=-1.0), b"softcap"), (dict(scale=float("nan")), b"scale"),
+                      (dict(window=-1), b"window"), (dict(splits=0), b"splits"),
                       (dict(splits=2), b"workspace"), (dict(splits=2, ws=p, n=100), b"workspace"),
                       (dict(keys=-1), b"keys"), (dict(starts=p, docs=1, keys=5), b"documents"),
                       (dict(prefix=p), b"causal"), (dict(prefix=p, causal=1, window=2), b"combined")):
         assert attention(**bad) == 1 and text in lib.m5k_last_error(), (bad, lib.m5k_last_error())
-    assert lib.m5k_attention_splits(0, 4, 3, 2, 64, 0, 4, 256, ctypes.byref(n)) == 1
+    assert lib.m5k_attention_plan(0, 4, 3, 2, 0, 4, 256, ctypes.byref(n), None) == 1
 
     def rope(pairs=2, d=8, x=p, heads=2):
         return lib.m5k_rope(x, _lib.F32, 4, heads, d, 8, 8, p, p, pairs, 0, s, p, None)
@@ -168,12 +169,15 @@ def test_c_entries_refuse_without_launching():
         assert rope(**bad) == 1 and b"rope" in lib.m5k_last_error()
 
 
-def test_split_rule():
-    """Enough rows: no split.  Few rows: as many workgroups as run at once, over 256 keys at least each."""
-    plan = lambda *a: module._splits(*a, 256)  # noqa: E731
-    assert plan(0, 4096, 56, 56, 128, 0, 4096) == 1
-    assert plan(0, 1, 8, 8, 128, 0, 255) == 1
-    assert plan(1, 1, 64, 8, 128, 1, 131072) == plan(1, 1, 64, 8, 64, 1, 131072) == 64
-    assert plan(0, 5000, 4, 1, 128, 0, 5000) == 3
-    assert plan(1, 64, 64, 8, 128, 64, 8192) == 2 and plan(1, 64, 64, 8, 128, 64, 2048) == 1
-    assert 1 < plan(1, 8, 64, 8, 64, 8, 8192) <= 32
+def test_plan():
+    """Enough rows: tiles of 128, no split.  Few rows: waves share them, and as many workgroups as run at once split the
+    keys, over 256 at least each."""
+    plan = lambda *a: module._plan(*a, 256)  # noqa: E731
+    assert plan(0, 4096, 56, 56, 0, 4096) == (1, False)
+    assert plan(0, 1, 8, 8, 0, 255) == (1, True)
+    assert plan(1, 1, 64, 8, 1, 131072) == (64, True)
+    assert plan(1, 64, 64, 8, 64, 8192) == (2, True) and plan(1, 64, 64, 8, 64, 2048) == (1, True)
+    splits, few = plan(1, 8, 64, 8, 8, 8192)
+    assert 1 < splits <= 32 and few
+    assert plan(0, 5000, 4, 1, 0, 5000) == (3, False) and plan(0, 2000, 4, 1, 0, 2000) == (1, True)
+    assert plan(0, 300, 56, 56, 0, 300) == (1, False) and plan(0, 128, 56, 56, 0, 128) == (1, True)

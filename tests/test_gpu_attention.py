@@ -93,7 +93,7 @@ def test_documents_with_bias_and_window(device):
 @pytest.mark.parametrize("d", [64, 128])
 def test_key_splits(tokens, keys, d, device):
     """Few rows over many keys: the keys are split and the parts joined."""
-    assert attn_module._splits(0, tokens, 8, 2, d, 0, keys, 256) > 1
+    assert attn_module._plan(0, tokens, 8, 2, 0, keys, 256)[0] > 1
     _dense(device, 8, 2, tokens, keys, d, BF16, causal=True)
     _dense(device, 8, 2, tokens, keys, d, BF16, causal=True, window=300)
 
@@ -212,7 +212,7 @@ def test_idle_slots_and_rows_behind(device):
 
 
 def test_long_context_is_split(device):
-    assert attn_module._splits(1, 1, 8, 1, 128, 1, 9000, 256) > 1
+    assert attn_module._plan(1, 1, 8, 1, 1, 9000, 256)[0] > 1
     _paged(device, 8, 1, 128, BF16, 64, [1], [8765])
     _paged(device, 8, 1, 64, BF16, 16, [2, 1], [3000, 40], behind=3)
 
