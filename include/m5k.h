@@ -4,7 +4,8 @@
  * Every entry point takes device pointers to row-major, contiguous buffers,
  * 64-bit sizes and an opaque HIP stream (hipStream_t passed as void*; NULL is
  * the default stream). Launches are asynchronous on that stream. Inputs are
- * never written. The library never allocates device memory: the caller owns
+ * never written, but for the caches that m5k_paged_append fills; the attention
+ * entries take rows by strides. The library never allocates device memory: the caller owns
  * every buffer, outputs included.
  *
  * Return value: 0 on success; a nonzero M5K_E* code otherwise, with a

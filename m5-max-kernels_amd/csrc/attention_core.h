@@ -49,7 +49,7 @@ struct Args {
   const float* slopes;
   uint16_t* out;
   float *part_o, *part_ml;
-  int tokens, keys, heads, kv_heads, group, sequences, pages, page_size, window, causal, splits, slots;
+  int tokens, keys, heads, kv_heads, group, sequences, pages, page_size, window, causal, splits, slots, spread, cus;
   uint32_t page_magic, page_shift, group_magic, group_shift;
   float scale, softcap;
 };
@@ -240,13 +240,28 @@ struct Place {
 
 template <int KEYS>
 __device__ __forceinline__ Place place(const Args& a, int rows_per_tile) {
-  int item = gemm::xcd_logical(blockIdx.x, gridDim.x);
   Place p;
-  p.split = item % a.splits;
-  item /= a.splits;
-  p.kvh = item / a.slots;
-  // Later tiles see more keys under a causal mask: they go first.
-  const int slot = a.slots - 1 - item % a.slots;
+  int slot;
+  if (a.spread) {
+    // Tiles of unequal work, and heads that do not divide among the XCDs: in turn over the XCDs, longest first under a
+    // causal mask; what a compute unit gets as its second workgroup of a grid that is resident at once is the
+    // shortest left.  (6000 causal tokens, 12 query heads on 3 key heads: 189 us by XCDs, whose parts of a head differ
+    // in work, 129 us.)
+    const int total = gridDim.x, id = blockIdx.x;
+    int item = total <= 2 * a.cus && id >= a.cus ? total - 1 - (id - a.cus) : id;
+    p.kvh = item % a.kv_heads;
+    item /= a.kv_heads;
+    p.split = item % a.splits;
+    slot = item / a.splits;
+  } else {
+    // One XCD after the other takes whole heads, so that a head's keys stay in its L2.
+    int item = gemm::xcd_logical(blockIdx.x, gridDim.x);
+    p.split = item % a.splits;
+    item /= a.splits;
+    p.kvh = item / a.slots;
+    slot = item % a.slots;
+  }
+  slot = a.slots - 1 - slot;  // later tiles see more keys under a causal mask: they go first
   if constexpr (KEYS == DENSE) {
     p.seq = 0;
     p.tile = slot;
@@ -964,6 +979,8 @@ int launch(Args& a, hipStream_t st) {
   const bool mods = a.softcap > 0.0f || a.slopes;
   const Plan p = plan(KEYS != DENSE, a.tokens, a.group, a.kv_heads, a.sequences, a.keys, device_cus());
   a.slots = p.slots;
+  a.cus = device_cus();
+  a.spread = a.kv_heads % 8 != 0 && (KEYS != DENSE || a.causal || a.starts);
   const int64_t blocks = int64_t{a.slots} * a.kv_heads * a.splits;
   M5K_REQUIRE(blocks <= INT32_MAX, "attention: too many tiles for one launch");
   auto kernel = p.few ? (mods ? attention_tile<DT, D, KEYS, true, true> : attention_tile<DT, D, KEYS, false, true>)
