@@ -390,7 +390,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     for (int s = 0; s < QS; ++s) qf[s] = *reinterpret_cast<const v4i*>(qp + 16 * s);
   }
   const float scale2 = a.scale * LOG2E;
-  const float unit = MODS ? 1.0f : scale2;  // what turns score() into base 2
+  const float unit = MODS ? 1.0f : scale2;  // what turns finished scores into base 2
   const float slope2 = MODS && a.slopes ? a.slopes[head] * LOG2E : 0.0f;
 
   // Loads: instruction i of a wave brings rows first_row + i * RPI + lane / CH of K and of V.
@@ -431,7 +431,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
       }
     }
   };
-  // This wave's 16 rows of tile t of one operand to LDS at dst.
+  // This wave's rows of tile t of one operand to LDS at dst.
   auto load_rows = [&](int t, const int (&id)[NIDS], const uint16_t* base, int64_t page_stride, int64_t row_stride,
                        const uint32_t (&ofs)[NI], uint32_t dst) __attribute__((always_inline)) {
     dst += FEW ? 0 : wave_s * NI * 1024;
@@ -935,12 +935,14 @@ __global__ __launch_bounds__(256) void attention_join(const Args a) {
   }
 }
 
-// How a call is launched.  `few`: sequences of no more than 32 packed rows on average; or fewer tiles of 128 rows than
-// compute units, where 32-row workgroups fill them better (two run on one at once), the keys are not so many that the
-// other form's key splits cost nothing beside them, and not so few that a second round of workgroups costs more than
-// it brings.  With tiles of 128 rows and with `few`: 128 tokens, 56 heads of 128: 8.7 and 5.8 us; 300 tokens: 12.8 and
-// 15.8; 1024 tokens, 16 heads: 33.8 and 18.0; 1999 tokens, 4 key heads of 64, prefix and cap: 43.8 and 32.2; 9914
-// tokens, one head: 71 and 98.
+// How a call is launched.  `few`: sequences of no more than 32 packed rows on average that are fewer, with their key
+// heads, than the workgroups that run at once (more are as well off with one wave at work in tiles of 128 rows: 64
+// tokens over 0 to 8190 keys, 8 key heads, 160 us against 170 us); or fewer tiles of 128 rows than compute units,
+// where 32-row workgroups fill them better (two run on one at once), the keys are not so many that the other form's key
+// splits cost nothing beside them, and not so few that a second round of workgroups costs more than it brings.  With
+// tiles of 128 rows and with `few`: 128 tokens, 56 heads of 128: 8.7 and 5.8 us; 300 tokens: 12.8 and 15.8; 1024
+// tokens, 16 heads: 33.8 and 18.0; 1999 tokens, 4 key heads of 64, prefix and cap: 43.8 and 32.2; 9914 tokens, one
+// head: 71 and 98.
 struct Plan {
   bool few;
   int slots;
@@ -948,7 +950,8 @@ struct Plan {
 inline Plan plan(bool paged, int64_t tokens, int group, int kv_heads, int64_t sequences, int64_t keys, int cus) {
   const int64_t rows = tokens * group, own = paged ? sequences : 1;
   const int64_t tiles = (rows / (32 * WAVES) + own) * kv_heads, thin = (rows / 32 + own) * kv_heads;
-  const bool few = rows <= 32 * own || (tiles < cus && thin <= (keys < 512 ? 2 : 4) * cus && keys <= 4096);
+  const bool few = (rows <= 32 * own && own * kv_heads < 2 * cus) ||
+                   (tiles < cus && thin <= (keys < 512 ? 2 : 4) * cus && keys <= 4096);
   const int64_t r = few ? 32 : 32 * WAVES;
   return Plan{few, static_cast<int>(paged ? rows / r + sequences + 1 : (rows + r - 1) / r)};
 }
@@ -956,9 +959,7 @@ inline Plan plan(bool paged, int64_t tokens, int group, int kv_heads, int64_t se
 // Key splits: as many as bring the workgroups to two a compute unit, what it holds at once, each over at least 256 keys
 // of the longest span; twice as many were slower (2048 tokens, 8 heads: 22 and 36 us).  Full workgroups of `few` to
 // one: their waves split the keys already, and the sums of 32 rows cost as much as their keys (2000 tokens, 4 query
-// heads on one key head, 250 workgroups: 19 us, 26 us in two splits).  Single tokens of many sequences differ in length, and the
-// longest ends last: two splits at least where a span can be long enough to pay for the join (64 tokens over 0 to 8190
-// keys, 8 key heads: 177 and 158 us).
+// heads on one key head, 250 workgroups: 19 us, 26 us in two splits).
 inline int plan_splits(bool paged, int64_t tokens, int group, int kv_heads, int64_t sequences, int64_t keys,
                        int cus) {
   const Plan p = plan(paged, tokens, group, kv_heads, sequences, keys, cus);
@@ -969,7 +970,6 @@ inline int plan_splits(bool paged, int64_t tokens, int group, int kv_heads, int6
   const bool full = p.few && tokens * group > 32 * (paged ? sequences : 1);
   int64_t n = (full ? 1 : 2) * int64_t{cus} / busy;
   const int64_t most = keys / 256;
-  if (paged && p.few && n < 2 && keys >= 4096 && busy <= 4 * int64_t{cus} && tokens <= sequences) n = 2;
   n = n < most ? n : most;
   return static_cast<int>(n < 1 ? 1 : n > 64 ? 64 : n);
 }

@@ -1,8 +1,9 @@
 """m5kernels_amd: the quantized projection hot path of m5-max-kernels on MI355X (gfx950).
 
 Python op contracts mirror the reference package ``m5kernels`` (quantize, gemm, rotate,
-...) on torch tensors; every computation runs in libm5k.so, hand-written HIP kernels
-behind a C ABI (include/m5k.h).  There is no CPU fallback.
+...) on torch tensors; the attention step that the projections feed (rope, paged_append,
+paged_attention, attention) stands beside them.  Every computation runs in libm5k.so,
+hand-written HIP kernels behind a C ABI (include/m5k.h).  There is no CPU fallback.
 """
 
 from .hip import gemm, gemm_i8_accumulators, quantize

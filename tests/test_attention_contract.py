@@ -176,7 +176,7 @@ def test_plan():
     assert plan(0, 4096, 56, 56, 0, 4096) == (1, False)
     assert plan(0, 1, 8, 8, 0, 255) == (1, True)
     assert plan(1, 1, 64, 8, 1, 131072) == (64, True)
-    assert plan(1, 64, 64, 8, 64, 8192) == (2, True) and plan(1, 64, 64, 8, 64, 2048) == (1, True)
+    assert plan(1, 64, 64, 8, 64, 8192) == (1, False) and plan(1, 32, 64, 8, 32, 2048) == (2, True)
     splits, few = plan(1, 8, 64, 8, 8, 8192)
     assert 1 < splits <= 32 and few
     assert plan(0, 5000, 4, 1, 0, 5000) == (3, False) and plan(0, 2000, 4, 1, 0, 2000) == (1, True)
