@@ -4,7 +4,8 @@
 // read and written once.  A thread owns a chunk of 8 channels (16 bytes of a 16-bit type) of one token and walks over
 // heads with it, so that the chunk's sines and cosines, the only arithmetic of note, are made once for all of them.
 // In the half layout the partner channels are R away: a second load, which the thread that owns them brings into the
-// cache as well.
+// cache as well.  9914 tokens of 56 heads of 128 in BF16 take 54 us, 5.3 TB/s read and written, the rate of a copy; 64
+// tokens appended 5.3 us, a chain of dependent loads (sequence, page, row).
 //
 // Angles.  p f_j / 2 pi is reduced to a fraction of a turn in 64 bits: at position 10^6 an FP32 angle would be off by
 // 0.06 rad, the 64-bit fraction by 10^-10.  The fraction's nearest quarter turn is taken off in 64 bits too and the
