@@ -27,8 +27,8 @@
 // behind the length and rows of pages that the cache lacks read as zeros instead.
 //
 // What bounds it.  Long prompts: the card's power and the issue of products beside exponentials (9914 tokens, 56 heads
-// of 128: 2.55 ms, 1.1 PFLOP/s, matrix cores busy 64% of the cycles, no LDS bank conflicts).  Single tokens: the cache's
-// bytes (131073 keys, 8 key heads of 128: 95 us and 5 us of joining, 5.6 TB/s).  Heads of 64: the exponentials.
+// of 128: 2.55 ms, 1.1 PFLOP/s, matrix cores busy 64% of the cycles, no LDS bank conflicts).  Single tokens: the
+// cache's bytes (131073 keys, 8 key heads of 128: 95 us and 5 us of joining, 5.6 TB/s).  Heads of 64: the exponentials.
 #pragma once
 
 #include "gemm_core.h"
