@@ -13,7 +13,6 @@ pass, ``work`` the bytes and operations that a pass cannot do without, ``exact``
 
 from __future__ import annotations
 
-import functools
 import math
 import sys
 from pathlib import Path
@@ -219,7 +218,6 @@ def run(s):
     return _OWN[s["case"]["kind"]](s, s["case"]) if own else _PLAIN[s["case"]["kind"]](s, s["case"])
 
 
-@functools.lru_cache(maxsize=None)
 def _package():
     path = str(Path(__file__).resolve().parent.parent / "m5-max-kernels_amd")
     if path not in sys.path:
