@@ -31,6 +31,7 @@
 // cache's bytes (131073 keys, 8 key heads of 128: 95 us and 5 us of joining, 5.6 TB/s).  Heads of 64: the exponentials.
 #pragma once
 
+#include "attention_place.h"
 #include "gemm_core.h"
 #include "m5k_common.h"
 
@@ -274,26 +275,16 @@ __device__ __forceinline__ Place place(const Args& a, int rows_per_tile) {
     p.span = a.keys;
     p.shift = a.keys - a.tokens;
   } else {
-    // Sequence b owns the slots from (starts[b] * G / R) + b on: at least as many as it has tiles, and the first of
-    // them is known without the lengths of the sequences before it.  The tokens behind the last sequence are
-    // sequence number `sequences`, which sees nothing.
     const int T = a.tokens, B = a.sequences;
-    auto start = [&](int b) { return b == 0 ? 0 : min(max(a.starts[b], 0), T); };
-    auto first = [&](int b) { return static_cast<int>(int64_t{start(b)} * a.group / rows_per_tile) + b; };
-    // The last b with first(b) <= slot, 64 probes at a time.
-    int lo = 0, left = B + 1;
-    while (left > 1) {
-      const int apart = (left + 63) >> 6, probe = static_cast<int>(threadIdx.x & 63) * apart;
-      const bool below = probe < left && first(lo + probe) <= slot;
-      const int at = max(__popcll(__builtin_amdgcn_ballot_w64(below)) - 1, 0) * apart;
-      lo += at;
-      left = min(apart, left - at);
-    }
-    p.seq = __builtin_amdgcn_readfirstlane(lo);
-    p.token0 = start(p.seq);
-    p.tile = slot - first(p.seq);
-    const int end = p.seq == B ? T : start(p.seq + 1);
-    const int n = max(0, end - p.token0);
+    const auto probes = [&](int lo, int left, int apart) {
+      const int probe = static_cast<int>(threadIdx.x & 63) * apart;
+      const bool below = probe < left && first_slot(a.starts, lo + probe, T, a.group, rows_per_tile) <= slot;
+      return __popcll(__builtin_amdgcn_ballot_w64(below));
+    };
+    p.seq = __builtin_amdgcn_readfirstlane(sequence_of_slot(B + 1, probes));
+    p.token0 = start_of(a.starts, p.seq, T);
+    p.tile = slot - first_slot(a.starts, p.seq, T, a.group, rows_per_tile);
+    const int n = tokens_of(a.starts, p.seq, B, T);
     p.rows = n * a.group;
     const int ctx = p.seq == B ? 0 : a.context[p.seq];
     p.span = min(max(ctx, 0), a.keys);
@@ -349,8 +340,8 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   const Place p = place<KEYS>(a, ROWS);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
   const int wave_s = __builtin_amdgcn_readfirstlane(wave);
+  if (!tile_has_rows(p.tile, p.rows, ROWS)) return;
   const int row0 = p.tile * ROWS;
-  if (row0 >= p.rows) return;
   const int row = row0 + (FEW ? 0 : 32 * wave) + (lane & 31);
   const bool live = row < p.rows;
   int token, head;
