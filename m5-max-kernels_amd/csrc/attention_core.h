@@ -16,10 +16,16 @@
 // octet s of P is its operand for keys 16 s .. 16 s + 15, and V^T is read in the same order, two groups of 4 keys,
 // by ds_read_b64_tr_b16 (the transpose of a 4 x 16 block on the way out of LDS).  P never leaves registers.
 //
-// Softmax.  Running maximum and sum in FP32 in base 2: p = exp2(t - m), t = scale * log2(e) * score.  The maximum
-// is raised, and O and the sum rescaled, only where a row's tile maximum exceeds it by more than 8: p stays below 2^8,
-// the quotient of O and the sum does not depend on m, and most tiles skip the rescale.  P is rounded to the inputs'
+// Softmax.  Running maximum m and sum in FP32: p = exp2(unit (x - m)), x the score, unit = scale * log2(e).  The maximum
+// is raised, and O and the sum rescaled, only where a row's tile maximum exceeds it by more than 8 / unit: p stays below
+// 2^8, the quotient of O and the sum does not depend on m, and most tiles skip the rescale.  P is rounded to the inputs'
 // type for the matrix cores (as the second product's operand has to be); the sum takes the unrounded p.
+//
+// Scores of any size.  The loop has one multiply-add a score, x unit - (m unit), off by the rounding of m unit: 2^-5 at
+// 2^20, and past 2^27 enough to take p out of range.  Rows that end there run again in careful mode (below), with
+// unit (x - m).  Splits and waves are joined by unit (m - m') of the unscaled maxima.  A row that sees no key ends with a
+// sum of 0 and the maximum it began with, and is 0; one that sees keys of score -inf alone leaves a maximum of -inf, and
+// is NaN if every part of it does.
 //
 // NaN and infinities.  A masked key's score is replaced, whatever it was, but its value row still meets the product
 // as 0 * v.  A wave whose sums end non-finite makes its workgroup run again in careful mode: non-finite values
@@ -42,7 +48,8 @@ using gemm::v16f;
 using gemm::v4i;
 
 constexpr int WAVES = 4, THREADS = 64 * WAVES;
-constexpr float M_FLOOR = -1e30f;  // running maximum before any key: finite, so that no difference is NaN
+constexpr float M_FLOOR = -3.40282347e38f;  // running maximum before any key: finite, so that no difference is NaN
+constexpr float FAR = 1048576.0f;           // maximum, in base 2, from which the careful mode takes over
 constexpr float LAZY = 8.0f;       // log2 of how far a tile maximum may pass the running one unadopted
 constexpr float LOG2E = 1.44269504088896340736f;
 
@@ -385,7 +392,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     for (int s = 0; s < QS; ++s) qf[s] = *reinterpret_cast<const v4i*>(qp + 16 * s);
   }
   const float scale2 = a.scale * LOG2E;
-  const float unit = MODS ? 1.0f : scale2;  // what turns finished scores into base 2
+  const float unit = MODS ? 1.0f : scale2;  // what turns finished scores into base 2, launch_unit()
   const float slope2 = MODS && a.slopes ? a.slopes[head] * LOG2E : 0.0f;
 
   // Loads: instruction i of a wave brings rows first_row + i * RPI + lane / CH of K and of V.
@@ -487,7 +494,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   wait_all();
   v16f o[OB], s[2][NB];
   v4i pf[2 * NB];
-  float m, l;
+  float m, m2, l;  // maximum, the same in base 2, sum
 
   // Scores of a tile, from K at stage `st`; beside them, where `prob`, the probabilities of the tile before against the
   // running maximum, packed for the second product, and their sum.  A 32 x 32 x 16 product holds the matrix cores for
@@ -511,17 +518,25 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     }
     return f;
   };
-  auto probabilities = [&](const v16f (&x)[NB], int from, int to, float (&sum)[2]) __attribute__((always_inline)) {
+  constexpr std::false_type quick{};
+  constexpr std::true_type careful{};
+  auto weight = [&](float x, auto with_care) __attribute__((always_inline)) {
+    float t = __builtin_fmaf(x, unit, -m2);
+    if constexpr (decltype(with_care)::value) t = fabsf(m2) < FAR ? t : (x - m) * unit;
+    return __builtin_amdgcn_exp2f(t);
+  };
+  auto probabilities = [&](const v16f (&x)[NB], int from, int to, float (&sum)[2], auto with_care)
+                           __attribute__((always_inline)) {
 #pragma unroll
     for (int e = from; e < to; e += 2) {
       const int b = e >> 4, r = e & 15;
-      const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][r], unit, -m));
-      const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][r + 1], unit, -m));
+      const float p0 = weight(x[b][r], with_care), p1 = weight(x[b][r + 1], with_care);
       sum[0] += p0;
       sum[1] += p1;
       uint32_t w = pack2<DT>(p0, p1);
       __asm__ volatile("" : "+v"(w), "+v"(sum[0]), "+v"(sum[1]));  // made here, not where they are read
       pf[2 * b + (r >> 3)][(r & 7) >> 1] = static_cast<int>(w);
+      if constexpr (decltype(with_care)::value) __builtin_amdgcn_sched_barrier(0);  // rare: few registers
     }
   };
   auto product = [&](v16f (&y)[NB], int st, const v16f (&x)[NB], bool prob) __attribute__((always_inline)) {
@@ -534,7 +549,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
       if (c + AHEAD < QS) key_frags(st, c + AHEAD, kf[(c + AHEAD) % (AHEAD + 1)]);
 #pragma unroll
       for (int b = 0; b < NB; ++b) y[b] = mfma32<DT>(kf[c % (AHEAD + 1)][b], qf[c], c == 0 ? v16f{} : y[b]);
-      if (prob) probabilities(x, c * EL / QS, (c + 1) * EL / QS, sum);
+      if (prob) probabilities(x, c * EL / QS, (c + 1) * EL / QS, sum, quick);
       __builtin_amdgcn_sched_barrier(0);
     }
     if (prob) l += sum[0] + sum[1];
@@ -650,10 +665,11 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   };
   // Adopt a tile maximum where a row's exceeds the running one by more than LAZY.
   auto adopt = [&](float tile_top) __attribute__((always_inline)) {
-    const float t = max_halves(tile_top) * unit;
-    if (__builtin_amdgcn_ballot_w64(t > m + LAZY)) {
-      const float next = fmaxf(m, t), f = __builtin_amdgcn_exp2f(m - next);
+    const float t = max_halves(tile_top);
+    if (__builtin_amdgcn_ballot_w64((t - m) * unit > LAZY)) {
+      const float next = fmaxf(m, t), f = __builtin_amdgcn_exp2f((m - next) * unit);
       m = next;
+      m2 = fmaxf(m * unit, M_FLOOR);  // finite: a masked score, -inf, stays one
       l *= f;
 #pragma unroll
       for (int b = 0; b < OB; ++b)
@@ -664,7 +680,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
 
   const int first = max(t_begin, any_lo / KT), last = min(t_end, (any_hi + KT - 1) / KT);  // this wave's tiles
   auto start = [&]() __attribute__((always_inline)) {
-    m = M_FLOOR;
+    m = m2 = M_FLOOR;
     l = 0.0f;
 #pragma unroll
     for (int b = 0; b < OB; ++b) o[b] = v16f{};
@@ -674,7 +690,6 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   // matrix cores have work beside the exponentials.  The i-th step (ODD = i & 1) reads K of tile t + 1 in stage ODD and
   // V of tile t in stage EVEN; it loads V of tile t + 1 and K of tile t + 2 over what the step before was the last to
   // read.
-  constexpr std::false_type quick{};
   auto step = [&](int t, auto odd, v16f (&x)[NB], v16f (&next)[NB]) __attribute__((always_inline)) {
     constexpr int ODD = decltype(odd)::value, EVEN = 1 - ODD;
     wait_all();
@@ -698,7 +713,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
       adopt(maximum(next));
     } else if (now) {
       float sum[2] = {};
-      probabilities(x, 0, EL, sum);
+      probabilities(x, 0, EL, sum, quick);
       l += sum[0] + sum[1];
       accumulate(EVEN, x);
     }
@@ -717,7 +732,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     finish(s[0], t, quick, none);
     adopt(maximum(s[0]));
     float sum[2] = {};
-    probabilities(s[0], 0, EL, sum);
+    probabilities(s[0], 0, EL, sum, quick);
     l += sum[0] + sum[1];
     if (more) gemm::wait_stage<NI>();
     else gemm::wait_stage<0>();
@@ -752,9 +767,16 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   for (int b = 0; b < OB; ++b)
 #pragma unroll
     for (int r = 0; r < 16; ++r) check = __builtin_fmaf(o[b][r], 0.0f, check);
+  // Whether the row saw a key here: one of its tiles of this wave meets its interval.
+  bool saw;
+  {
+    const int from = max(t_begin, rr.lo / KT), to = min(t_end, (rr.hi + KT - 1) / KT);
+    saw = from + (FEW ? (wave - (from - t_begin)) & (WAVES - 1) : 0) < to;
+  }
+  const bool far = !MODS && m != M_FLOOR && !(fabsf(m2) < FAR);
   wait_all();
-  if (__syncthreads_or(lacking || check != 0.0f)) {
-    constexpr std::true_type careful{};
+  if (__syncthreads_or(lacking || far || check != 0.0f)) {
+    saw = false;
     start();
     for (int t = t_begin; t < t_end; ++t) {
       if (FEW && ((t - t_begin) & (WAVES - 1)) != wave_s) continue;
@@ -769,17 +791,20 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
         finish(s[0], t, careful, sees);
         adopt(maximum(s[0]));
         float sum[2] = {};
-        probabilities(s[0], 0, EL, sum);
+        probabilities(s[0], 0, EL, sum, careful);
         l += sum[0] + sum[1];
         accumulate_careful(sees);
+        saw |= sees != 0;
       }
       wait_all();
       if constexpr (!FEW) gemm::stage_barrier();
     }
     if constexpr (FEW) __syncthreads();
+    saw = (__builtin_amdgcn_ballot_w64(saw) >> (lane & 31)) & 0x100000001ull;  // in either half's keys
   }
 
   l += other_half(l);
+  if (l == 0.0f && saw) m = -__builtin_inff();
   if constexpr (FEW) {
     // The waves' sums joined in LDS, in wave order, by 8 threads a row.
     uint8_t* mine = lds + wave * AREA;
@@ -800,14 +825,16 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     if (row0 + r >= p.rows) return;
     float top = M_FLOOR, total = 0.0f, acc[E] = {};
     float w[WAVES];
+    bool lost = false;
 #pragma unroll
     for (int i = 0; i < WAVES; ++i) {
       w[i] = *reinterpret_cast<const float*>(lds + i * AREA + 32 * SUMS + 8 * r);
       top = fmaxf(top, w[i]);
+      lost |= w[i] < M_FLOOR;
     }
 #pragma unroll
     for (int i = 0; i < WAVES; ++i) {
-      w[i] = __builtin_amdgcn_exp2f(w[i] - top);
+      w[i] = __builtin_amdgcn_exp2f((w[i] - top) * unit);
       total = __builtin_fmaf(*reinterpret_cast<const float*>(lds + i * AREA + 32 * SUMS + 8 * r + 4), w[i], total);
       const float* src = reinterpret_cast<const float*>(lds + i * AREA + r * SUMS) + c;
 #pragma unroll
@@ -815,10 +842,11 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     }
     int t_out, h_out;
     range_of<KEYS>(a, p, row0 + r, t_out, h_out);
+    lost = lost && total == 0.0f;
     if (a.splits > 1) {
       const int64_t at = (int64_t{p.split} * a.tokens + t_out) * a.heads + h_out;
       if (c == 0) {
-        a.part_ml[2 * at] = top;
+        a.part_ml[2 * at] = lost ? -__builtin_inff() : top;
         a.part_ml[2 * at + 1] = total;
       }
 #pragma unroll
@@ -826,14 +854,14 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
         *reinterpret_cast<float4*>(a.part_o + at * D + c + e) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
       return;
     }
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total, none = lost ? __builtin_nanf("") : 0.0f;
     uint16_t* op = a.out + (int64_t{t_out} * a.heads + h_out) * D + c;
 #pragma unroll
     for (int e = 0; e < E; e += 8) {
       uint32_t v[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        v[i] = total == 0.0f ? 0u : pack2<DT>(acc[e + 2 * i] * inv, acc[e + 2 * i + 1] * inv);
+        v[i] = total == 0.0f ? pack2<DT>(none, none) : pack2<DT>(acc[e + 2 * i] * inv, acc[e + 2 * i + 1] * inv);
       *reinterpret_cast<uint4*>(op + e) = make_uint4(v[0], v[1], v[2], v[3]);
     }
     return;
@@ -854,20 +882,26 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
             make_float4(o[b][r], o[b][r + 1], o[b][r + 2], o[b][r + 3]);
     return;
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l, none = m < M_FLOOR ? __builtin_nanf("") : 0.0f;
+  const uint32_t nones = pack2<DT>(none, none);
   uint16_t* op = a.out + (int64_t{token} * a.heads + head) * D + 4 * half;
 #pragma unroll
   for (int b = 0; b < OB; ++b)
 #pragma unroll
     for (int r = 0; r < 16; r += 4) {
-      const uint2 w = l == 0.0f ? make_uint2(0u, 0u)
+      const uint2 w = l == 0.0f ? make_uint2(nones, nones)
                                 : make_uint2(pack2<DT>(o[b][r] * inv, o[b][r + 1] * inv),
                                              pack2<DT>(o[b][r + 2] * inv, o[b][r + 3] * inv));
       *reinterpret_cast<uint2*>(op + 32 * b + 2 * r) = w;
     }
 }
 
-// Joins the key splits of a (token, head), each split's sum weighted by 2^(m - max m).  Lane i holds split i's maximum
+// unit of a launch's kernels.
+__device__ __forceinline__ float launch_unit(const Args& a) {
+  return a.softcap > 0.0f || a.slopes ? 1.0f : a.scale * LOG2E;
+}
+
+// Joins the key splits of a (token, head), each split's sum weighted by 2^(unit (m - max m)).  Lane i holds split i's maximum
 // and total, so that the weights cost one load; the sums' loads then wait for nothing but memory.  Latency bound: with
 // WAVES_ROW = 4 (many splits, so few rows) the waves take a quarter of the splits each and add up in LDS, in wave order
 // (64 splits of 64 rows: 54 us with one wave and a weight at a time).
@@ -888,7 +922,8 @@ __global__ __launch_bounds__(256) void attention_join(const Args a) {
   float top = m;
 #pragma unroll
   for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-  const float w = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+  const float w = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f((m - top) * launch_unit(a));
+  const bool lost = __builtin_amdgcn_ballot_w64(m < M_FLOOR) != 0;
   const float total = wave_sum(l * w);
   const int per = (a.splits + WAVES_ROW - 1) / WAVES_ROW, s0 = wave % WAVES_ROW * per, s1 = min(s0 + per, a.splits);
   float acc[E] = {};
@@ -921,13 +956,12 @@ __global__ __launch_bounds__(256) void attention_join(const Args a) {
       for (int i = 1; i < 4; ++i) acc[e] += sums[i][lane * E + e];
     }
   }
-  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total, none = lost ? __builtin_nanf("") : 0.0f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = total == 0.0f ? none : acc[e] * inv;
   uint16_t* dst = a.out + at * D + lane * E;
-  if constexpr (E == 2) {
-    *reinterpret_cast<uint32_t*>(dst) = total == 0.0f ? 0u : pack2<DT>(acc[0] * inv, acc[1] * inv);
-  } else {
-    *dst = static_cast<uint16_t>(total == 0.0f ? 0u : pack2<DT>(acc[0] * inv, 0.0f) & 0xFFFFu);
-  }
+  if constexpr (E == 2) *reinterpret_cast<uint32_t*>(dst) = pack2<DT>(acc[0], acc[1]);
+  else *dst = static_cast<uint16_t>(pack2<DT>(acc[0], 0.0f) & 0xFFFFu);
 }
 
 // How a call is launched.  `few`: sequences of no more than 32 packed rows on average that are fewer, with their key

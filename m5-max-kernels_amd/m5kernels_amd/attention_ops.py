@@ -312,9 +312,9 @@ def paged_attention(q, k_cache, v_cache, page_table, query_starts, context_lengt
     are the last n of its context_lengths[b] keys; a token at position p sees keys j <= p, of them with `window` those
     with p - j < window, and with `prefix_lengths` (int32 [sequences]) also every j below the prefix.  Scores are
     scale * q . k (scale defaults to width ** -0.5); `softcap` c turns s into c * tanh(s / c); `slopes` (float32
-    [heads]) then adds -slopes[h] * (distance of j from p).  Returns [tokens, heads * width]; rows that see no key,
-    and rows behind the last sequence, are 0.  Keys on pages that a table entry outside [0, pages) would name are
-    left out."""
+    [heads]) then adds -slopes[h] * (distance of j from p).  Scores are FP32 numbers of any size.  Returns
+    [tokens, heads * width]; rows that see no key, and rows behind the last sequence, are 0; rows that see only keys of
+    score -inf are NaN.  Keys on pages that a table entry outside [0, pages) would name are left out."""
     fast = hip._fast
     if fast is not None:
         out = fast.paged_attention(q, k_cache, v_cache, page_table, query_starts, context_lengths, scale, window,

@@ -1,0 +1,117 @@
+"""Scores of every size: huge ones, ones far below zero, infinite ones, in each form that a call can take."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import m5kernels_amd as m5
+from m5kernels_amd import attention_ops, hip
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16 = torch.bfloat16, torch.float16
+# name -> (query heads, key heads, tokens, keys, splits): waves that share 32 rows, tiles of 128 rows, each split or not.
+FORMS = {"few": (4, 2, 40, 150, False), "few split": (4, 2, 3, 3000, True), "tiles": (256, 256, 130, 150, False),
+         "tiles split": (3, 1, 47, 4500, True)}
+
+
+def _shape(form):
+    hq, hkv, tokens, keys, split = FORMS[form]
+    got = attention_ops._plan(0, tokens, hq, hkv, 0, keys, hip._cu_count_of(0))
+    assert got[1] == form.startswith("few") and (got[0] > 1) == split, got
+    return hq, hkv, tokens, keys
+
+
+def _whole(seed, lo, hi, *shape):
+    """Whole numbers lo..hi as float64."""
+    g = torch.Generator().manual_seed(seed)
+    return torch.randint(lo, hi + 1, shape, generator=g).double()
+
+
+def _softmax(score, visible):
+    """Softmax over the visible keys in 64 bits: 0 where a row sees none, NaN where it sees infinities only."""
+    p = torch.softmax(score.masked_fill(~visible, -math.inf), -1)
+    return torch.where(visible.any(-1, keepdim=True), p, 0.0)
+
+
+def _causal(tokens, keys):
+    return torch.arange(keys)[None, :] <= torch.arange(tokens)[:, None] + keys - tokens
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("dtype,d,shift", [(F16, 64, 12), (F16, 128, 26), (BF16, 64, 21), (BF16, 64, 40),
+                                           (BF16, 128, 110)])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_huge_scores(sign, dtype, d, shift, biased, form, device):
+    """Scores are multiples of 2^shift, all positive or all negative (down to below -10^35), and exact: q and k are
+    whole numbers times a power of two.  Keys but a row's best weigh less than e^-4096, so that the output is the
+    mean of the values of its best keys: n of them add up in FP32 to n 2^-24 of max |v|, n at most the keys, and
+    each weight, a power of two that need not be whole, is rounded for the product by half a step."""
+    hq, hkv, tokens, keys = _shape(form)
+    up, down = shift // 2, shift - shift // 2
+    q = (_whole(0, 1, 3, hq, tokens, d) * 2.0 ** up).to(dtype)
+    k = (sign * _whole(1, 1, 3, hkv, keys, d) * 2.0 ** down).to(dtype)
+    v = torch.randn(hkv, keys, d, generator=torch.Generator().manual_seed(2)).to(dtype)
+    slopes = torch.zeros(hq) if biased else None
+    got = m5.attention(q.to(device), k.to(device), v.to(device), causal=True, scale=1.0,
+                       slopes=None if slopes is None else slopes.to(device)).cpu().double().view(tokens, hq, d)
+    for h in range(0, hq, max(1, hq // 4)):
+        score = q[h].double() @ k[h * hkv // hq].double().T
+        vh = v[h * hkv // hq].double()
+        p, half = _softmax(score, _causal(tokens, keys)), torch.finfo(dtype).eps / 2
+        want = p @ vh
+        bound = half * (want.abs() + p @ vh.abs()) + keys * 2.0 ** -24 * vh.abs().max()
+        assert torch.isfinite(got[:, h]).all()
+        assert ((got[:, h] - want).abs() <= bound * 1.01).all()
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("d,dtype", [(64, F16), (128, BF16)])
+def test_scores_of_minus_infinity(d, dtype, form, device):
+    """Keys of score -inf weigh nothing beside finite ones; a row that sees only such keys is NaN, as the quotient of
+    two zeros is; a row that sees no key is 0."""
+    hq, hkv, tokens, keys = _shape(form)
+    g = torch.Generator().manual_seed(3)
+    q, k, v = (torch.randn(h, n, d, generator=g).to(dtype) for h, n in ((hq, tokens), (hkv, keys), (hkv, keys)))
+    q[:, :, 0] = q[:, :, 0].abs() + 0.5
+    at = keys - tokens + tokens // 2  # what half of the rows see without them
+    k[:, :at, 0] = -math.inf
+    cut = torch.zeros_like(k)
+    cut[:, at:] = k[:, at:]
+    got = m5.attention(q.to(device), k.to(device), v.to(device), causal=True).cpu().view(tokens, hq, d)
+    assert torch.isnan(got[:tokens // 2]).all()
+    want = m5.attention(q[:, tokens // 2:].to(device), k[:, at:].to(device), v[:, at:].to(device),
+                        causal=True).cpu().view(-1, hq, d)
+    rest = got[tokens // 2:].double()
+    # Two runs of the same softmax: each rounds its probabilities and its output by half a step, and its sums by less.
+    assert (rest - want.double()).abs().max() <= 4 * torch.finfo(dtype).eps / 2 * v.double().abs().max()
+    k[:] = -math.inf
+    k[:, :, 1:] = 0.0
+    lost = m5.attention(q.to(device), k[:, :1].to(device), v[:, :1].to(device), causal=True).cpu().view(tokens, hq, d)
+    assert (lost[:-1] == 0).all() and torch.isnan(lost[-1]).all()
+
+
+@pytest.mark.parametrize("page", [16, 24])
+def test_scores_of_minus_infinity_on_pages(page, device):
+    """The same over a cache: a sequence whose keys all score -inf, one whose visible keys lie on pages that the cache
+    lacks (0), one that has a finite key behind them."""
+    hkv, d, width = 2, 64, 6
+    g = torch.Generator().manual_seed(4)
+    kc, vc = (torch.randn(3 * width, hkv, page, d, generator=g).to(BF16) for _ in range(2))
+    q = torch.randn(4, 3, d, generator=g).to(BF16)
+    q[:, :, 0] = q[:, :, 0].abs() + 0.5
+    table = torch.arange(3 * width, dtype=torch.int32).view(3, width).clone()
+    kc[:2 * width, :, :, 0] = -math.inf
+    table[1] = -1
+    last = 5 * page + 3
+    kc[2 * width:, :, :, 0] = -math.inf
+    kc[2 * width + 5, :, 2, 0] = 0.0  # the last key of the third sequence
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
+    got = m5.paged_attention(q.to(device), kc.to(device), vc.to(device), table.to(device), ints(0, 1, 2, 3),
+                             ints(last, last, last)).cpu().view(3, 4, d)
+    assert torch.isnan(got[0]).all() and (got[1] == 0).all()
+    assert torch.equal(got[2], vc[2 * width + 5, :, 2].repeat_interleave(2, 0))
