@@ -50,6 +50,9 @@ using gemm::v4i;
 constexpr int WAVES = 4, THREADS = 64 * WAVES;
 constexpr float M_FLOOR = -3.40282347e38f;  // running maximum before any key: finite, so that no difference is NaN
 constexpr float FAR = 1048576.0f;           // maximum, in base 2, from which the careful mode takes over
+// Least factor on a part that a row saw: an infinity in it stays one (times 0 it would be NaN, and left out it would be
+// lost); finite parts of so little weight vanish beside the sum all the same, which is about 1 or more.
+constexpr float LEAST = 0x1p-126f;
 constexpr float LAZY = 8.0f;       // log2 of how far a tile maximum may pass the running one unadopted
 constexpr float LOG2E = 1.44269504088896340736f;
 
@@ -667,7 +670,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   auto adopt = [&](float tile_top) __attribute__((always_inline)) {
     const float t = max_halves(tile_top);
     if (__builtin_amdgcn_ballot_w64((t - m) * unit > LAZY)) {
-      const float next = fmaxf(m, t), f = __builtin_amdgcn_exp2f((m - next) * unit);
+      const float next = fmaxf(m, t), f = fmaxf(__builtin_amdgcn_exp2f((m - next) * unit), LEAST);
       m = next;
       m2 = fmaxf(m * unit, M_FLOOR);  // finite: a masked score, -inf, stays one
       l *= f;
@@ -834,7 +837,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     }
 #pragma unroll
     for (int i = 0; i < WAVES; ++i) {
-      w[i] = __builtin_amdgcn_exp2f((w[i] - top) * unit);
+      w[i] = fmaxf(__builtin_amdgcn_exp2f((w[i] - top) * unit), LEAST);
       total = __builtin_fmaf(*reinterpret_cast<const float*>(lds + i * AREA + 32 * SUMS + 8 * r + 4), w[i], total);
       const float* src = reinterpret_cast<const float*>(lds + i * AREA + r * SUMS) + c;
 #pragma unroll
@@ -873,7 +876,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
       a.part_ml[2 * at] = m;
       a.part_ml[2 * at + 1] = l;
     }
-    if (l == 0.0f) return;  // nothing seen here: the sums are not read
+    if (l == 0.0f && m == M_FLOOR) return;  // nothing seen here: the sums are not read
 #pragma unroll
     for (int b = 0; b < OB; ++b)
 #pragma unroll
@@ -922,7 +925,8 @@ __global__ __launch_bounds__(256) void attention_join(const Args a) {
   float top = m;
 #pragma unroll
   for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-  const float w = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f((m - top) * launch_unit(a));
+  const float w =
+      l == 0.0f && m == M_FLOOR ? 0.0f : fmaxf(__builtin_amdgcn_exp2f((m - top) * launch_unit(a)), LEAST);
   const bool lost = __builtin_amdgcn_ballot_w64(m < M_FLOOR) != 0;
   const float total = wave_sum(l * w);
   const int per = (a.splits + WAVES_ROW - 1) / WAVES_ROW, s0 = wave % WAVES_ROW * per, s1 = min(s0 + per, a.splits);

@@ -115,3 +115,27 @@ def test_scores_of_minus_infinity_on_pages(page, device):
                              ints(last, last, last)).cpu().view(3, 4, d)
     assert torch.isnan(got[0]).all() and (got[1] == 0).all()
     assert torch.equal(got[2], vc[2 * width + 5, :, 2].repeat_interleave(2, 0))
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("low", ["first", "last"])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf])
+@pytest.mark.parametrize("d,dtype", [(64, F16), (128, BF16)])
+def test_infinite_values_of_little_weight(d, dtype, bad, low, form, device):
+    """An infinity that a row sees is its output, however small the weight (here e^-256, which FP32 has no number for),
+    and whichever tile, wave or split meets it; the other channels stay what they are.  Half of the keys have that
+    weight, so that whole tiles, waves and splits have no other."""
+    hq, hkv, tokens, keys = _shape(form)
+    q = torch.ones(hq, tokens, d, dtype=dtype)
+    k = (_whole(5, 0, 3, hkv, keys, 1) / d).to(dtype).repeat(1, 1, d)
+    v = torch.randn(hkv, keys, d, generator=torch.Generator().manual_seed(6)).to(dtype)
+    half = keys // 2
+    k[:, :half] = k[:, :half] if low == "last" else -256 / d
+    k[:, half:] = k[:, half:] if low == "first" else -256 / d
+    want = m5.attention(q.to(device), k.to(device), v.to(device), scale=1.0).cpu().view(tokens, hq, d)
+    assert torch.isfinite(want).all()
+    v[:, 40 if low == "first" else keys - 50, 5] = bad
+    got = m5.attention(q.to(device), k.to(device), v.to(device), scale=1.0).cpu().view(tokens, hq, d)
+    assert (got[:, :, 5] == bad).all()
+    got[:, :, 5] = want[:, :, 5]
+    assert torch.equal(got, want)
