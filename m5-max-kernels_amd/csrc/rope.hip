@@ -156,8 +156,9 @@ __global__ __launch_bounds__(256) void rope_rows(const Args a) {
     } else if constexpr (INTERLEAVED && V == 8) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        out[2 * i] = x[2 * i] * cs[i] - x[2 * i + 1] * sn[i];
-        out[2 * i + 1] = x[2 * i + 1] * cs[i] + x[2 * i] * sn[i];
+        const bool turns = c0 + 2 * i < 2 * a.pairs;  // else copied as it is: times 0, a partner's infinity is NaN
+        out[2 * i] = turns ? x[2 * i] * cs[i] - x[2 * i + 1] * sn[i] : x[2 * i];
+        out[2 * i + 1] = turns ? x[2 * i + 1] * cs[i] + x[2 * i] * sn[i] : x[2 * i + 1];
       }
     } else {
       float partner[V];
