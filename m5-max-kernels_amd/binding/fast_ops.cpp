@@ -19,6 +19,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
 
+#include <cfloat>
 #include <cmath>
 #include <mutex>
 #include <unordered_map>
@@ -622,6 +623,7 @@ bool scores_of(const at::Tensor* q, int64_t kv_heads, int64_t dim, at::ScalarTyp
       !positive(softcap, 0.0f, s.softcap) || !window_of(window, s.window) ||
       !optional_vector(slopes, heads, at::kFloat, dev, &s.slopes))
     return false;
+  if (s.scale < FLT_MIN || (s.softcap != 0.0f && (s.softcap < FLT_MIN || s.scale / s.softcap > 1e37f))) return false;
   if (m5k_attention_plan(paged, tokens, heads, kv_heads, sequences, keys, 0, &s.splits, nullptr)) return false;
   s.out = empty({tokens, heads * dim}, st, dev);
   s.elems = 0;

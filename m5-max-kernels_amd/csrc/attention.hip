@@ -18,8 +18,11 @@ int common(Args& a, const void* q, int dtype, int64_t tokens, int64_t heads, int
               "attention: too many tokens");
   M5K_REQUIRE(q_head % 8 == 0 && q_token % 8 == 0 && m5k::aligned16(q) && m5k::aligned16(out),
               "attention: q and out rows must be 16-byte aligned");
-  M5K_REQUIRE(scale > 0.0f && scale < 1e30f && softcap >= 0.0f && softcap < 1e30f,
+  M5K_REQUIRE(scale >= 0x1p-126f && scale < 1e30f && softcap >= 0.0f && softcap < 1e30f,
               "attention: scale must be positive, softcap nonnegative, both finite");
+  // A subnormal cap and an infinite quotient turn scores of 0 into NaN.
+  M5K_REQUIRE(softcap == 0.0f || (softcap >= 0x1p-126f && scale / softcap <= 1.0001e37f),
+              "attention: softcap must be 0 or a normal number, scale / softcap at most 1e37");
   M5K_REQUIRE(window >= 0 && window < (1 << 30), "attention: bad window");
   M5K_REQUIRE(!(window && prefix), "attention: a window and a prefix cannot be combined");
   M5K_REQUIRE(splits >= 1 && splits <= 64, "attention: splits must be in [1, 64]");

@@ -30,6 +30,8 @@ _HALF_DTYPES = (torch.float16, torch.bfloat16)
 _FLOAT_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 HEAD_DIMS = (64, 128)
 _WINDOW_MAX = (1 << 30) - 1
+_F32_LEAST = 2.0 ** -126
+_RATIO_MAX = 1e37  # scale / softcap: what a score is multiplied by before the cap's tanh, finite with its log2(e)
 
 
 def rope_frequencies(rotary_dim, base=10000.0, *, scaling=None, factor=1.0, original_length=None, fast=32.0, slow=1.0,
@@ -135,6 +137,14 @@ def _positive(v, name):
     if not _lib.is_real(v) or not math.isfinite(v) or not 0 < v < 1e30:
         raise ValueError(f"{name} must be a positive finite real scalar")
     return float(v)
+
+
+def _normal(v, name):
+    """A positive scalar that FP32, in which the kernels take it, has a normal number for."""
+    v = _positive(v, name)
+    if v < _F32_LEAST:
+        raise ValueError(f"{name} must be at least 2^-126")
+    return v
 
 
 def _rotation(frequencies, layout, magnitude, width):
@@ -271,8 +281,13 @@ def _plan(paged, tokens, heads, kv_heads, sequences, keys, cus):
 
 
 def _scores(q, heads, width, scale, softcap, window, slopes):
-    scale = 1.0 / math.sqrt(width) if scale is None else _positive(scale, "scale")
-    softcap = 0.0 if softcap is None else _positive(softcap, "softcap")
+    scale = 1.0 / math.sqrt(width) if scale is None else _normal(scale, "scale")
+    if softcap is None:
+        softcap = 0.0
+    else:
+        softcap = _normal(softcap, "softcap")
+        if scale / softcap > _RATIO_MAX:
+            raise ValueError(f"scale / softcap must be at most {_RATIO_MAX:g}")
     if window is None:
         window = 0
     elif not _lib.is_int(window) or window <= 0:
@@ -312,7 +327,8 @@ def paged_attention(q, k_cache, v_cache, page_table, query_starts, context_lengt
     are the last n of its context_lengths[b] keys; a token at position p sees keys j <= p, of them with `window` those
     with p - j < window, and with `prefix_lengths` (int32 [sequences]) also every j below the prefix.  Scores are
     scale * q . k (scale defaults to width ** -0.5); `softcap` c turns s into c * tanh(s / c); `slopes` (float32
-    [heads]) then adds -slopes[h] * (distance of j from p).  Scores are FP32 numbers of any size.  Returns
+    [heads]) then adds -slopes[h] * (distance of j from p).  Scores are FP32 numbers of any size; scale and c are normal
+    ones, scale / c at most 1e37.  Returns
     [tokens, heads * width]; rows that see no key, and rows behind the last sequence, are 0; rows that see only keys of
     score -inf are NaN.  Keys on pages that a table entry outside [0, pages) would name are left out."""
     fast = hip._fast

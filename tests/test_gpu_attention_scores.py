@@ -139,3 +139,21 @@ def test_infinite_values_of_little_weight(d, dtype, bad, low, form, device):
     assert (got[:, :, 5] == bad).all()
     got[:, :, 5] = want[:, :, 5]
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("scale,softcap", [(2.0 ** -126, 2.0 ** -126), (0.125, 1e-20), (1e29, 1.0)])
+def test_smallest_and_largest_scales(scale, softcap, device):
+    """A cap of next to nothing leaves the mean of the values; caps and scales without a normal FP32 number are refused
+    by either front."""
+    q, k, v = (torch.randn(2, n, 64, generator=torch.Generator().manual_seed(n)).to(BF16) for n in (5, 90, 90))
+    q[0] = 0.0  # a score of 0 stays one
+    got = m5.attention(q.to(device), k.to(device), v.to(device), scale=scale, softcap=softcap).cpu().double()
+    score = q.double() @ k.double().transpose(1, 2) * scale
+    want = torch.softmax(softcap * torch.tanh(score / softcap), -1) @ v.double()
+    bound = 2.0 ** -8 * (want.abs() + v.double().abs().mean(1, keepdim=True)) + 2.0 ** -14
+    if softcap == 1.0:  # weights of up to e^2 the mean's, off by the cap's 2^-22 and half a step
+        bound = bound * 8
+    assert ((got.view(5, 2, 64).transpose(0, 1) - want).abs() <= bound).all()
+    for bad in (dict(softcap=1e-50), dict(scale=1e-50), dict(softcap=2.0 ** -127), dict(scale=4.0, softcap=2.0 ** -126)):
+        with pytest.raises(ValueError, match="scale|softcap"):
+            m5.attention(q.to(device), k.to(device), v.to(device), **bad)
