@@ -121,11 +121,15 @@ def load(path: Path | str | None = None) -> ctypes.CDLL:
     return lib
 
 
+# What hip._NativeFront asks of the native front.
+FRONT_CALLS = ("bind", "quantize", "gemm", "qk", "qkv", "rope", "paged_append", "paged_attention", "attention")
+
+
 def load_fast():
     """The native front of quantize(), gemm(), the projections and the attention step
     (binding/fast_ops.cpp), linked against libm5k.so, or None where the libraries have not been built.
-    One that does not load, or that was compiled for another C ABI or another torch (left from an older
-    build), warns: the same kernels then run with the checks in Python."""
+    One that does not load, that was compiled for another C ABI or another torch, or that lacks a call (left
+    from an older build), warns: the same kernels then run with the checks in Python."""
     if not (FAST_PATH.exists() and LIB_PATH.exists()) or _current_raw_stream is None:
         return None
     spec = importlib.util.spec_from_file_location("m5k_fast", FAST_PATH)
@@ -140,6 +144,10 @@ def load_fast():
     if built_for != running:
         warnings.warn(f"{FAST_PATH.name} was compiled for (C ABI, torch) {built_for}, this process has {running}; "
                       "build the package again", RuntimeWarning)
+        return None
+    lacking = [name for name in FRONT_CALLS if not hasattr(module, name)]
+    if lacking:
+        warnings.warn(f"{FAST_PATH.name} lacks {', '.join(lacking)}; build the package again", RuntimeWarning)
         return None
     return module
 
