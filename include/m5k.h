@@ -480,6 +480,7 @@ int m5k_rope(const void* x, int dtype, int64_t tokens, int64_t heads, int64_t he
  * q (or NULL) [heads, tokens, head_dim] is turned too, into q_out [heads, tokens, head_dim] contiguous, whose rows
  * behind the last sequence become 0.  A token whose position is negative or lies behind the table, or whose table
  * entry is outside [0, pages), is not stored; nothing else in the cache is written.
+ * Two tokens that name the same place leave a mixture there, each channel of each head one token's or the other's.
  */
 int m5k_paged_append(const void* k, int64_t k_head, int64_t k_token, const void* v, int64_t v_head, int64_t v_token,
                      int dtype, int64_t tokens, int64_t kv_heads, int64_t head_dim, void* k_cache, int64_t kc_page,

@@ -222,7 +222,8 @@ def paged_append(k, v, k_cache, v_cache, page_table, query_starts, context_lengt
     launch and returned (contiguous; rows behind the last sequence are 0); otherwise None is returned.
 
     A token whose position is negative (an idle slot: context_lengths 0) or lies behind the table, or whose table entry
-    names no page, is not stored.  Two tokens of one call that name the same place leave either's values there."""
+    names no page, is not stored.  Where two tokens of one call name the same place, what lies there is unspecified:
+    each channel of each head is one token's or the other's, in the keys and the values by themselves."""
     fast = hip._fast
     if fast is not None:
         done = fast.paged_append(k, v, k_cache, v_cache, page_table, query_starts, context_lengths, q, frequencies,

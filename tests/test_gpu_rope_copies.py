@@ -1,5 +1,5 @@
 """Channels behind the rotated ones are copied: whatever their neighbours hold, they keep their values, infinities, NaN
-and the sign of a zero included, in rope() and on the way into a cache."""
+and the sign of a zero included, in rope() and on the way into a cache; what two tokens for one place leave there."""
 
 from __future__ import annotations
 
@@ -59,3 +59,15 @@ def test_copied_channels_of_stored_keys(layout, device):
     _same(stored[..., rotary:], k[..., rotary:])
     _same(q.cpu()[..., rotary:], k[..., rotary:])
     _same(torch.cat([vc[0], vc[1]], 1)[:, :29].cpu(), k)
+
+
+def test_tokens_for_one_place(device):
+    """Two sequences whose tables name the same page: each element is one token's or the other's, the rest untouched."""
+    k, v = (torch.randn(3, 40, 64, generator=torch.Generator().manual_seed(n)).to(BF16) for n in (1, 2))
+    kc, vc = (torch.zeros(4, 3, 32, 64, dtype=BF16, device=device) for _ in range(2))
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
+    table = torch.tensor([[2], [2]], dtype=torch.int32, device=device)
+    m5.paged_append(k.to(device), v.to(device), kc, vc, table, ints(0, 20, 40), ints(20, 20))
+    for cache, new in ((kc.cpu(), k), (vc.cpu(), v)):
+        assert ((cache[2, :, :20] == new[:, :20]) | (cache[2, :, :20] == new[:, 20:])).all()
+        assert (cache[2, :, 20:] == 0).all() and (cache[[0, 1, 3]] == 0).all()
