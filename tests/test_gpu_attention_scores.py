@@ -157,3 +157,34 @@ def test_smallest_and_largest_scales(scale, softcap, device):
     for bad in (dict(softcap=1e-50), dict(scale=1e-50), dict(softcap=2.0 ** -127), dict(scale=4.0, softcap=2.0 ** -126)):
         with pytest.raises(ValueError, match="scale|softcap"):
             m5.attention(q.to(device), k.to(device), v.to(device), **bad)
+
+
+@pytest.mark.parametrize("form", ["few", "few split", "tiles", "tiles split"])
+@pytest.mark.parametrize("d,dtype", [(64, F16), (128, BF16)])
+@pytest.mark.parametrize("softcap", [3.0, 127.0, 129.0, 200.0, 500.0])
+def test_caps_that_bite(softcap, d, dtype, form, device):
+    """Scores of both signs from far below the cap to five times it.  They are exact: q is one whole number a row, k
+    whole numbers times a power of two, and q . k is below 2^24 steps.  So the capped score is off by what tanh and its
+    product cost: the short form (caps to 128) by 2^-22 cap, the long one by its exponential, reciprocal, sum and
+    result, four steps of at most 2^-23 cap, and either by the roundings of the argument (2^-23 of y sech^2 y, below
+    half of that again), the scaling to base 2 and the difference from the maximum (2^-23 cap each): 2^-20 cap in
+    all.  A weight is then off by that much twice (its own score and the sum's), its rounding adds half a step."""
+    hq, hkv, tokens, keys = _shape(form)
+    q, k = torch.zeros(hq, tokens, d), torch.zeros(hkv, keys, d)
+    q[:, :, 0] = _whole(7, -4, 4, hq, tokens).float()
+    k[:, :, 0] = _whole(8, -64, 64, hkv, keys).float() * 2.0 ** round(math.log2(5 * softcap / 256))
+    q, k = q.to(dtype), k.to(dtype)
+    v = torch.randn(hkv, keys, d, generator=torch.Generator().manual_seed(9)).to(dtype)
+    got = m5.attention(q.to(device), k.to(device), v.to(device), scale=1.0, softcap=softcap).cpu().double()
+    got, half, off = got.view(tokens, hq, d), torch.finfo(dtype).eps / 2, 2.0 ** -20 * softcap + keys * 2.0 ** -24
+    bites = 0
+    for h in range(0, hq, max(1, hq // 4)):
+        score, vh = q[h].double() @ k[h * hkv // hq].double().T, v[h * hkv // hq].double()
+        p = torch.softmax(softcap * torch.tanh(score / softcap), -1)
+        tiny = keys * 2.0 ** -25 if dtype == F16 else 0.0  # probabilities below float16's normal range
+        slack = (half + 2 * off) * (p @ vh.abs()) + tiny * vh.abs().max()
+        want = p @ vh
+        bound = slack + half * (want.abs() + slack)
+        assert ((got[:, h] - want).abs() <= bound).all()
+        bites += int(((torch.softmax(score, -1) @ vh - want).abs() > 4 * bound).sum())
+    assert bites > 0  # without the cap the outputs are others
