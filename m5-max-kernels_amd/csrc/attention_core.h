@@ -325,8 +325,15 @@ __device__ __forceinline__ RowRange range_of(const Args& a, const Place& p, int 
 
 // FEW = false: the 4 waves take 32 rows each and share key tiles of 64.  FEW: they share 32 rows, for calls that have
 // no more, and take every fourth tile of 32 keys each, through LDS of their own: no barrier in the loop, and the keys
-// of a short row are read four tiles at a time.  One K and one V tile a wave: with two of each, one workgroup a compute
-// unit, 64 tokens over 300 keys took 36 us instead of 24, over 1000 keys of 256 sequences 199 instead of 183.
+// of a short row are read four tiles at a time.
+//
+// Tiles of K and V that a wave of FEW holds: one of each, so that two or three workgroups run on a compute unit at once
+// (two of each at heads of 128, one workgroup: 64 tokens over 300 keys 36 us instead of 24).  Two of each where an
+// address a lane (PAGES) makes the loads long and heads of 64 leave room for two workgroups: with one and with two, 830
+// tokens of three sequences, window and cap, pages of 24, 16 heads: 27.4 and 24.2 us; 8 chunks of 64 tokens over 1564
+// keys, 16 heads: 32.2 and 26.5; 63 single tokens over 1 to 4000 keys, 8 key heads: 72.6 and 57.8; single tokens over
+// 1000 keys, one key head: 480 of them 28.2 and 24.7, but 508, which just fill the chip, 28.6 and 36.7.  By whole
+// addresses (pages of 16, dense) two of each gained 10% in some calls and lost 3 to 12% in others.
 template <int DT, int D, int KEYS, bool MODS, bool FEW>
 __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   constexpr int KT = FEW ? 32 : 64, NB = KT / 32;  // keys of a tile, 32-key blocks
@@ -339,11 +346,11 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   constexpr int QS = D / 16, OB = D / 32;
   constexpr int AHEAD = 1;  // steps of two products between a fragment's read and its use (2: no faster)
   constexpr int ROWS = FEW ? 32 : 32 * WAVES;
-  constexpr uint32_t ROWB = D * 2, TILE = KT * ROWB;
-  // K stages 0 and 1, V stages 0 and 1.  FEW: one K and one V tile of each wave, later its sums, in rows of D + 4
-  // floats (16 bytes a lane without bank conflicts), and their maxima and totals.
-  constexpr uint32_t SUMS = (D + 4) * 4, AREA = 32 * SUMS + 256, VTILE = FEW ? TILE : 2 * TILE;
-  static_assert(AREA >= 2 * TILE || !FEW, "a wave's tiles fit in its area");
+  constexpr int STAGES = FEW && !(KEYS == PAGES && D == 64) ? 1 : 2;  // tiles of K, and of V, in LDS
+  constexpr uint32_t ROWB = D * 2, TILE = KT * ROWB, VTILE = STAGES * TILE;
+  // K stages, V stages.  FEW: those of each wave, later its sums, in rows of D + 4 floats (16 bytes a lane without bank
+  // conflicts), and their maxima and totals.
+  constexpr uint32_t SUMS = (D + 4) * 4, JOIN = 32 * SUMS + 256, AREA = JOIN > 2 * VTILE ? JOIN : 2 * VTILE;
   __shared__ __attribute__((aligned(256))) uint8_t lds[FEW ? WAVES * AREA : 4 * TILE];
   __shared__ int bounds[2 * WAVES];
 
@@ -721,15 +728,30 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
       accumulate(EVEN, x);
     }
   };
-  // FEW: this wave's tile t.  The K of its next one (WAVES further on) is loaded as soon as this one's has been read, V
-  // likewise, so that one of the two is on its way through every phase.  Loads end in the order of their issue.
-  auto own_tile = [&](int t) __attribute__((always_inline)) {
+  // FEW: this wave's tile t, from stage ST.  With two stages the next one (WAVES further on) is on its way to the other
+  // meanwhile.  With one the K of the next is loaded as soon as this one's has been read, V likewise, so that one of the
+  // two is on its way through every phase.  Loads end in the order of their issue.
+  auto own_tile = [&](int t, auto stage) __attribute__((always_inline)) {
+    constexpr int ST = decltype(stage)::value;
     const bool more = t + WAVES < t_end;
-    gemm::wait_stage<NI>();  // K, behind which V was issued
-    product(s[0], 0, s[0], false);
-    if (more) {
-      __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      load_rows(t + WAVES, ids[0], kbase, a.k_page, a.k_row, kofs, lds0);
+    if constexpr (STAGES == 2) {
+      if (more) {
+        __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last reads of that stage
+        load_rows(t + WAVES, ids[0], kbase, a.k_page, a.k_row, kofs, lds0 + (1 - ST) * TILE);
+        load_rows(t + WAVES, ids[0], vbase, a.v_page, a.v_row, vofs, lds0 + VTILE + (1 - ST) * TILE);
+        load_ids(t + 2 * WAVES, ids[0]);
+        gemm::wait_stage<2 * NI>();
+      } else {
+        gemm::wait_stage<0>();
+      }
+      product(s[0], ST, s[0], false);
+    } else {
+      gemm::wait_stage<NI>();  // K, behind which V was issued
+      product(s[0], ST, s[0], false);
+      if (more) {
+        __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        load_rows(t + WAVES, ids[0], kbase, a.k_page, a.k_row, kofs, lds0);
+      }
     }
     uint32_t none;
     finish(s[0], t, quick, none);
@@ -737,13 +759,17 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     float sum[2] = {};
     probabilities(s[0], 0, EL, sum, quick);
     l += sum[0] + sum[1];
-    if (more) gemm::wait_stage<NI>();
-    else gemm::wait_stage<0>();
-    accumulate(0, s[0]);
-    if (more) {
-      __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      load_rows(t + WAVES, ids[0], vbase, a.v_page, a.v_row, vofs, lds0 + VTILE);
-      load_ids(t + 2 * WAVES, ids[0]);
+    if constexpr (STAGES == 1) {
+      if (more) gemm::wait_stage<NI>();
+      else gemm::wait_stage<0>();
+    }
+    accumulate(ST, s[0]);
+    if constexpr (STAGES == 1) {
+      if (more) {
+        __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        load_rows(t + WAVES, ids[0], vbase, a.v_page, a.v_row, vofs, lds0 + VTILE);
+        load_ids(t + 2 * WAVES, ids[0]);
+      }
     }
   };
   start();
@@ -755,7 +781,10 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
       load_rows(t, ids[0], vbase, a.v_page, a.v_row, vofs, lds0 + VTILE);
       load_ids(t + WAVES, ids[0]);
     }
-    for (; t < t_end; t += WAVES) own_tile(t);
+    for (; t < t_end; t += STAGES * WAVES) {
+      own_tile(t, std::integral_constant<int, 0>{});
+      if (STAGES == 2 && t + WAVES < t_end) own_tile(t + WAVES, std::integral_constant<int, STAGES - 1>{});
+    }
   } else if (t_begin < t_end) {
     load_ids(t_begin, ids[1]);
     load_rows(t_begin, ids[1], kbase, a.k_page, a.k_row, kofs, lds0);
