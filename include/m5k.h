@@ -426,6 +426,8 @@ int m5k_shift_split_condition(const void* gamma, const void* scale, int param_dt
  *   nondecreasing from 0; needs keys == tokens) keeps the row's own document.  A row that sees no key is 0;
  *   so is a row behind the last document.  What a masked key or value holds does not matter, NaN included.
  *   Scores are FP32 numbers of any size; a row that sees only keys of score -infinity is NaN.
+ *   Infinities and NaN in values that a row sees are in its output, however small their weight.  Sums of weights, up to
+ *   2^8, times values are FP32 numbers: values up to 2^119 over the number of keys.
  *   scale and a softcap other than 0 are normal FP32 numbers, scale / softcap at most 1e37.
  *   prefix_lengths: int32 [documents], or [1] without document_starts; only with causal, not with window.
  *   splits: key ranges joined by a second launch (m5k_attention_plan gives the number that pays); above 1

@@ -50,9 +50,6 @@ using gemm::v4i;
 constexpr int WAVES = 4, THREADS = 64 * WAVES;
 constexpr float M_FLOOR = -3.40282347e38f;  // running maximum before any key: finite, so that no difference is NaN
 constexpr float FAR = 1048576.0f;           // maximum, in base 2, from which the careful mode takes over
-// Least factor on a part that a row saw: an infinity in it stays one (times 0 it would be NaN, and left out it would be
-// lost); finite parts of so little weight vanish beside the sum all the same, which is about 1 or more.
-constexpr float LEAST = 0x1p-126f;
 constexpr float LAZY = 8.0f;       // log2 of how far a tile maximum may pass the running one unadopted
 constexpr float LOG2E = 1.44269504088896340736f;
 
@@ -216,6 +213,12 @@ __device__ __forceinline__ float tanh_f32(float y) {
 // Caps up to here take the second form alone, C - 2 C / (e^(2y) + 1) in five instructions: off by C 2^-22, 6e-5 at
 // most (16 heads of 64, 1999 tokens: 72 us with tanh_f32, 38 us).
 constexpr float CAP_SHORT = 128.0f;
+
+// acc + sum * f, f the weight of a sum.  Infinities and NaN that a row saw stay, also where f is below FP32's range: times
+// 0 an infinity would be NaN.
+__device__ __forceinline__ float add_scaled(float acc, float sum, float f) {
+  return fabsf(sum) < __builtin_inff() ? __builtin_fmaf(sum, f, acc) : acc + sum;
+}
 
 // Non-finite 16-bit values of a fragment: zero in `clean`; `mark` holds 1 for +inf, 128 for -inf, 16384 for NaN.
 template <int DT>
@@ -674,17 +677,17 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     return t0;
   };
   // Adopt a tile maximum where a row's exceeds the running one by more than LAZY.
-  auto adopt = [&](float tile_top) __attribute__((always_inline)) {
+  auto adopt = [&](float tile_top, auto with_care) __attribute__((always_inline)) {
     const float t = max_halves(tile_top);
     if (__builtin_amdgcn_ballot_w64((t - m) * unit > LAZY)) {
-      const float next = fmaxf(m, t), f = fmaxf(__builtin_amdgcn_exp2f((m - next) * unit), LEAST);
+      const float next = fmaxf(m, t), f = __builtin_amdgcn_exp2f((m - next) * unit);
       m = next;
       m2 = fmaxf(m * unit, M_FLOOR);  // finite: a masked score, -inf, stays one
       l *= f;
 #pragma unroll
       for (int b = 0; b < OB; ++b)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o[b][r] *= f;
+        for (int r = 0; r < 16; ++r) o[b][r] = decltype(with_care)::value ? add_scaled(0.0f, o[b][r], f) : o[b][r] * f;
     }
   };
 
@@ -716,11 +719,11 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     if (now && then) {
       product(next, ODD, x, true);
       finish(next, t + 1, quick, none);
-      adopt(accumulate(EVEN, next));
+      adopt(accumulate(EVEN, next), quick);
     } else if (then) {
       product(next, ODD, x, false);
       finish(next, t + 1, quick, none);
-      adopt(maximum(next));
+      adopt(maximum(next), quick);
     } else if (now) {
       float sum[2] = {};
       probabilities(x, 0, EL, sum, quick);
@@ -755,7 +758,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     }
     uint32_t none;
     finish(s[0], t, quick, none);
-    adopt(maximum(s[0]));
+    adopt(maximum(s[0]), quick);
     float sum[2] = {};
     probabilities(s[0], 0, EL, sum, quick);
     l += sum[0] + sum[1];
@@ -821,7 +824,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
         uint32_t sees;
         product(s[0], 0, s[1], false);
         finish(s[0], t, careful, sees);
-        adopt(maximum(s[0]));
+        adopt(maximum(s[0]), careful);
         float sum[2] = {};
         probabilities(s[0], 0, EL, sum, careful);
         l += sum[0] + sum[1];
@@ -866,11 +869,11 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     }
 #pragma unroll
     for (int i = 0; i < WAVES; ++i) {
-      w[i] = fmaxf(__builtin_amdgcn_exp2f((w[i] - top) * unit), LEAST);
+      w[i] = __builtin_amdgcn_exp2f((w[i] - top) * unit);
       total = __builtin_fmaf(*reinterpret_cast<const float*>(lds + i * AREA + 32 * SUMS + 8 * r + 4), w[i], total);
       const float* src = reinterpret_cast<const float*>(lds + i * AREA + r * SUMS) + c;
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = __builtin_fmaf(src[e], w[i], acc[e]);
+      for (int e = 0; e < E; ++e) acc[e] = add_scaled(acc[e], src[e], w[i]);
     }
     int t_out, h_out;
     range_of<KEYS>(a, p, row0 + r, t_out, h_out);
@@ -954,29 +957,43 @@ __global__ __launch_bounds__(256) void attention_join(const Args a) {
   float top = m;
 #pragma unroll
   for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-  const float w =
-      l == 0.0f && m == M_FLOOR ? 0.0f : fmaxf(__builtin_amdgcn_exp2f((m - top) * launch_unit(a)), LEAST);
+  const float w = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f((m - top) * launch_unit(a));
+  const uint64_t saw = __builtin_amdgcn_ballot_w64(l != 0.0f || m != M_FLOOR);  // splits that wrote sums
   const bool lost = __builtin_amdgcn_ballot_w64(m < M_FLOOR) != 0;
   const float total = wave_sum(l * w);
   const int per = (a.splits + WAVES_ROW - 1) / WAVES_ROW, s0 = wave % WAVES_ROW * per, s1 = min(s0 + per, a.splits);
-  float acc[E] = {};
-  for (int s = s0; s < s1; s += BATCH) {
-    float v[BATCH][E];
+  float acc[E];
+  auto add_up = [&](auto with_care) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < BATCH; ++i) {
-      const float* src = a.part_o + (min(s + i, s1 - 1) * rows + at) * D + lane * E;
+    for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+    for (int s = s0; s < s1; s += BATCH) {
+      float v[BATCH][E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) v[i][e] = src[e];
+      for (int i = 0; i < BATCH; ++i) {
+        const float* src = a.part_o + (min(s + i, s1 - 1) * rows + at) * D + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[i][e] = src[e];
+      }
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        // A split that saw nothing wrote no sums: whatever lies there is left out.
+        const int from = min(s + i, s1 - 1);
+        const float f = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), from));
+        const bool take = s + i < s1 && ((saw >> from) & 1);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float next =
+              decltype(with_care)::value ? add_scaled(acc[e], v[i][e], f) : __builtin_fmaf(v[i][e], f, acc[e]);
+          acc[e] = take ? next : acc[e];
+        }
+      }
     }
+  };
+  add_up(std::false_type{});
+  float check = 0.0f;
 #pragma unroll
-    for (int i = 0; i < BATCH; ++i) {
-      // A split that saw nothing wrote no sums: whatever lies there is left out.
-      const int from = min(s + i, s1 - 1);
-      const float f = s + i < s1 ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), from)) : 0.0f;
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = f == 0.0f ? acc[e] : __builtin_fmaf(v[i][e], f, acc[e]);
-    }
-  }
+  for (int e = 0; e < E; ++e) check = __builtin_fmaf(acc[e], 0.0f, check);
+  if (__builtin_amdgcn_ballot_w64(check != 0.0f)) add_up(std::true_type{});  // rare: a sum is not finite
   if constexpr (WAVES_ROW > 1) {
 #pragma unroll
     for (int e = 0; e < E; ++e) sums[wave][lane * E + e] = acc[e];

@@ -188,3 +188,39 @@ def test_caps_that_bite(softcap, d, dtype, form, device):
         assert ((got[:, h] - want).abs() <= bound).all()
         bites += int(((torch.softmax(score, -1) @ vh - want).abs() > 4 * bound).sum())
     assert bites > 0  # without the cap the outputs are others
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("low", ["first", "last"])
+@pytest.mark.parametrize("infinite", [False, True])
+def test_huge_values_of_little_weight(infinite, low, form, device):
+    """Finite values of weight e^-256 (2^-369) leave nothing in the output, also where infinities in another channel are
+    kept.  They are as large as the sums hold: keys times 2^8, the largest weight against a running maximum, times 2^104
+    is below 2^128 with 4500 keys."""
+    hq, hkv, tokens, keys = _shape(form)
+    q, half = torch.ones(hq, tokens, 64, dtype=BF16), keys // 2
+    k = (_whole(5, 0, 3, hkv, keys, 1) / 64).to(BF16).repeat(1, 1, 64)
+    v = torch.randn(hkv, keys, 64, generator=torch.Generator().manual_seed(6)).to(BF16)
+    little = slice(0, half) if low == "first" else slice(half, keys)
+    k[:, little] = -4.0
+    v[:, 40 if low == "first" else keys - 50, 5] = math.inf if infinite else 0.0
+    v[:, :, 6:8] = 0.0
+    want = m5.attention(q.to(device), k.to(device), v.to(device), scale=1.0).view(tokens, hq, 64)
+    v[:, little, 6], v[:, little, 7] = 2.0 ** 100, -2.0 ** 104
+    got = m5.attention(q.to(device), k.to(device), v.to(device), scale=1.0).view(tokens, hq, 64)
+    assert (got[..., 6:] == want[..., 6:]).all() and (got[..., 6:8] == 0).all()
+    assert torch.equal(got[..., :6], want[..., :6])
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("low", ["first", "last"])
+def test_nan_of_little_weight(low, form, device):
+    hq, hkv, tokens, keys = _shape(form)
+    q, half = torch.ones(hq, tokens, 64, dtype=F16), keys // 2
+    k = (_whole(5, 0, 3, hkv, keys, 1) / 64).to(F16).repeat(1, 1, 64)
+    v = torch.randn(hkv, keys, 64, generator=torch.Generator().manual_seed(6)).to(F16)
+    k[:, :half] = k[:, :half] if low == "last" else -4.0
+    k[:, half:] = k[:, half:] if low == "first" else -4.0
+    v[:, 40 if low == "first" else keys - 50, 5] = math.nan
+    got = m5.attention(q.to(device), k.to(device), v.to(device), scale=1.0).view(tokens, hq, 64)
+    assert torch.isnan(got[..., 5]).all() and torch.isfinite(got[..., :5]).all() and torch.isfinite(got[..., 6:]).all()
