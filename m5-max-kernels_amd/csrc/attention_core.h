@@ -797,11 +797,12 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
       if (t + 1 < t_end) step(t + 1, std::integral_constant<int, 1>{}, s[1], s[0]);
     }
   }
-  float check = 0.0f;
+  float checks[4] = {};  // NaN from any sum that is not finite, in four chains
 #pragma unroll
   for (int b = 0; b < OB; ++b)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) check = __builtin_fmaf(o[b][r], 0.0f, check);
+    for (int r = 0; r < 16; ++r) checks[r & 3] = __builtin_fmaf(o[b][r], 0.0f, checks[r & 3]);
+  const float check = (checks[0] + checks[1]) + (checks[2] + checks[3]);
   // Whether the row saw a key here: one of its tiles of this wave meets its interval.
   bool saw;
   {
@@ -867,13 +868,26 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
       top = fmaxf(top, w[i]);
       lost |= w[i] < M_FLOOR;
     }
+    auto add_up = [&](int i, auto with_care) __attribute__((always_inline)) {
+      const float* src = reinterpret_cast<const float*>(lds + i * AREA + r * SUMS) + c;
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        acc[e] = decltype(with_care)::value ? add_scaled(acc[e], src[e], w[i]) : __builtin_fmaf(src[e], w[i], acc[e]);
+    };
 #pragma unroll
     for (int i = 0; i < WAVES; ++i) {
       w[i] = __builtin_amdgcn_exp2f((w[i] - top) * unit);
       total = __builtin_fmaf(*reinterpret_cast<const float*>(lds + i * AREA + 32 * SUMS + 8 * r + 4), w[i], total);
-      const float* src = reinterpret_cast<const float*>(lds + i * AREA + r * SUMS) + c;
+      add_up(i, quick);
+    }
+    float odd[2] = {};
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = add_scaled(acc[e], src[e], w[i]);
+    for (int e = 0; e < E; ++e) odd[e & 1] = __builtin_fmaf(acc[e], 0.0f, odd[e & 1]);
+    if (__builtin_amdgcn_ballot_w64(odd[0] + odd[1] != 0.0f)) {  // rare: a sum is not finite
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < WAVES; ++i) add_up(i, careful);
     }
     int t_out, h_out;
     range_of<KEYS>(a, p, row0 + r, t_out, h_out);
