@@ -10,8 +10,9 @@
 //
 // Measured on a [1, 256] activation: quantize 7.3 -> 4.6 us of host time, gemm 9.4 -> 4.4 us, of which
 // the HIP launch takes about 3 each.  The projections' staged form, two launches, takes
-// 18 to 20 us through Python and 8 to 10 us here; the fused one 10 to 13 and 5 to 6 us.  rope takes 24
-// and 4.5 us, paged_append 36 and 5.5, attention of 128 tokens 29 and under 6, each with its kernel.
+// 18 to 20 us through Python and 8 to 10 us here; the fused one 10 to 13 and 5 to 6 us.  Calls of the
+// attention step back to back, each with its kernel: rope of one token 9.5 and 4.7 us, paged_append of 64
+// tokens 18 and 5.6, attention of 128 tokens 14.4 and 6.6, which is its kernel.
 #include <Python.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/Dtype.h>

@@ -16,16 +16,16 @@
 // octet s of P is its operand for keys 16 s .. 16 s + 15, and V^T is read in the same order, two groups of 4 keys,
 // by ds_read_b64_tr_b16 (the transpose of a 4 x 16 block on the way out of LDS).  P never leaves registers.
 //
-// Softmax.  Running maximum m and sum in FP32: p = exp2(unit (x - m)), x the score, unit = scale * log2(e).  The maximum
-// is raised, and O and the sum rescaled, only where a row's tile maximum exceeds it by more than 8 / unit: p stays below
-// 2^8, the quotient of O and the sum does not depend on m, and most tiles skip the rescale.  P is rounded to the inputs'
-// type for the matrix cores (as the second product's operand has to be); the sum takes the unrounded p.
+// Softmax.  Running maximum m and sum in FP32: p = exp2(unit (x - m)), x the score, unit = scale * log2(e).  The
+// maximum is raised, and O and the sum rescaled, only where a row's tile maximum exceeds it by more than 8 / unit: p
+// stays below 2^8, the quotient of O and the sum does not depend on m, and most tiles skip the rescale.  P is rounded
+// to the inputs' type for the matrix cores (as the second product's operand has to be); the sum takes the unrounded p.
 //
 // Scores of any size.  The loop has one multiply-add a score, x unit - (m unit), off by the rounding of m unit: 2^-5 at
 // 2^20, and past 2^27 enough to take p out of range.  Rows that end there run again in careful mode (below), with
-// unit (x - m).  Splits and waves are joined by unit (m - m') of the unscaled maxima.  A row that sees no key ends with a
-// sum of 0 and the maximum it began with, and is 0; one that sees keys of score -inf alone leaves a maximum of -inf, and
-// is NaN if every part of it does.
+// unit (x - m).  Splits and waves are joined by unit (m - m') of the unscaled maxima.  A row that sees no key ends with
+// a sum of 0 and the maximum it began with, and is 0; one that sees keys of score -inf alone leaves a maximum of -inf,
+// and is NaN if every part of it does.
 //
 // NaN and infinities.  A masked key's score is replaced, whatever it was, but its value row still meets the product
 // as 0 * v.  A wave whose sums end non-finite makes its workgroup run again in careful mode: non-finite values
@@ -33,8 +33,13 @@
 // behind the length and rows of pages that the cache lacks read as zeros instead.
 //
 // What bounds it.  Long prompts: the card's power and the issue of products beside exponentials (9914 tokens, 56 heads
-// of 128: 2.55 ms, 1.1 PFLOP/s, matrix cores busy 64% of the cycles, no LDS bank conflicts).  Single tokens: the
-// cache's bytes (131073 keys, 8 key heads of 128: 95 us and 5 us of joining, 5.6 TB/s).  Heads of 64: the exponentials.
+// of 128: 2.51 to 2.64 ms by the card, 1.1 PFLOP/s, matrix cores busy 64% of the cycles, no LDS bank conflicts).
+// Single tokens: the cache's bytes (131073 keys, 8 key heads of 128: 94 to 100 us and 5 us of joining, 5.5 TB/s).
+// Heads of 64: the exponentials.
+//
+// Registers.  Tiles of 128 rows with heads of 128 use 241 to 256, all there are for two waves a SIMD.  With a cap or a
+// bias 8 to 10 of them go to memory and come back inside the loop, 34 by pages of no multiple of 16 (chunks of up to
+// 1024 tokens over up to 8192 keys, bias: 232 us in pages of 64, 536 in pages of 24; without the bias 182 and 251).
 #pragma once
 
 #include "attention_place.h"
@@ -214,8 +219,8 @@ __device__ __forceinline__ float tanh_f32(float y) {
 // most (16 heads of 64, 1999 tokens: 72 us with tanh_f32, 38 us).
 constexpr float CAP_SHORT = 128.0f;
 
-// acc + sum * f, f the weight of a sum.  Infinities and NaN that a row saw stay, also where f is below FP32's range: times
-// 0 an infinity would be NaN.
+// acc + sum * f, f the weight of a sum.  Infinities and NaN that a row saw stay, also where f is below FP32's range:
+// times 0 an infinity would be NaN.
 __device__ __forceinline__ float add_scaled(float acc, float sum, float f) {
   return fabsf(sum) < __builtin_inff() ? __builtin_fmaf(sum, f, acc) : acc + sum;
 }
@@ -732,8 +737,8 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     }
   };
   // FEW: this wave's tile t, from stage ST.  With two stages the next one (WAVES further on) is on its way to the other
-  // meanwhile.  With one the K of the next is loaded as soon as this one's has been read, V likewise, so that one of the
-  // two is on its way through every phase.  Loads end in the order of their issue.
+  // meanwhile.  With one the K of the next is loaded as soon as this one's has been read, V likewise, so that one of
+  // the two is on its way through every phase.  Loads end in the order of their issue.
   auto own_tile = [&](int t, auto stage) __attribute__((always_inline)) {
     constexpr int ST = decltype(stage)::value;
     const bool more = t + WAVES < t_end;
@@ -950,10 +955,10 @@ __device__ __forceinline__ float launch_unit(const Args& a) {
   return a.softcap > 0.0f || a.slopes ? 1.0f : a.scale * LOG2E;
 }
 
-// Joins the key splits of a (token, head), each split's sum weighted by 2^(unit (m - max m)).  Lane i holds split i's maximum
-// and total, so that the weights cost one load; the sums' loads then wait for nothing but memory.  Latency bound: with
-// WAVES_ROW = 4 (many splits, so few rows) the waves take a quarter of the splits each and add up in LDS, in wave order
-// (64 splits of 64 rows: 54 us with one wave and a weight at a time).
+// Joins the key splits of a (token, head), each split's sum weighted by 2^(unit (m - max m)).  Lane i holds split i's
+// maximum and total, so that the weights cost one load; the sums' loads then wait for nothing but memory.  Latency
+// bound: with WAVES_ROW = 4 (many splits, so few rows) the waves take a quarter of the splits each and add up in LDS,
+// in wave order (64 splits of 64 rows: 54 us with one wave and a weight at a time).
 template <int DT, int D, int WAVES_ROW>
 __global__ __launch_bounds__(256) void attention_join(const Args a) {
   constexpr int E = D / 64, ROWS = 4 / WAVES_ROW, BATCH = WAVES_ROW == 1 ? 4 : 16;
@@ -1029,13 +1034,19 @@ __global__ __launch_bounds__(256) void attention_join(const Args a) {
 }
 
 // How a call is launched.  `few`: sequences of no more than 32 packed rows on average that are fewer, with their key
-// heads, than the workgroups that run at once (more are as well off with one wave at work in tiles of 128 rows: 64
-// tokens over 0 to 8190 keys, 8 key heads, 160 us against 170 us); or fewer tiles of 128 rows than compute units,
-// where 32-row workgroups fill them better (two run on one at once), the keys are not so many that the other form's key
-// splits cost nothing beside them, and not so few that a second round of workgroups costs more than it brings.  With
-// tiles of 128 rows and with `few`: 128 tokens, 56 heads of 128: 8.7 and 5.8 us; 300 tokens: 12.8 and 15.8; 1024
-// tokens, 16 heads: 33.8 and 18.0; 1999 tokens, 4 key heads of 64, prefix and cap: 43.8 and 32.2; 9914 tokens, one
-// head: 71 and 98.
+// heads, than the workgroups that run at once; or fewer tiles of 128 rows than compute units, where 32-row workgroups
+// fill them better (two run on one at once), the keys are not so many that the other form's key splits cost nothing
+// beside them, and not so few that a second round of workgroups costs more than it brings.  With tiles of 128 rows and
+// with `few`: 128 tokens, 56 heads of 128: 8.7 and 6.5 us; 300 tokens: 12.8 and 15.8; 1024 tokens, 16 heads: 33.8 and
+// 18.0; 1999 tokens, 4 key heads of 64, prefix and cap: 43.8 and 32.2; 9914 tokens, one head: 71 and 98.
+//
+// The first limit is no crossing of the forms.  Single tokens of 8 key heads of 128, with tiles and with `few`, over
+// 300 / 1000 / 4000 keys each: 32 sequences 14, 13 / 29, 28 / 98, 98 us; 63: 20, 17 / 45, 42 / 177, 176; 64: 20, 18 /
+// 46, 44 / 182, 180; 65: 26, 21 / 63, 50 / 248, 209; 128: 34, 31 / 99, 95 / 355, 352; 256: 68, 62 / 191, 184.  Two key
+// heads, 256 sequences: 20, 21 / 46, 48 / 183, 205; 400: 30, 27 / 82, 82 / 289, 304.  64 of unequal lengths up to 8190,
+// evenly spread: 161, 170; at random: 228, 236 and 208, 201; spread over the logarithm: 146, 105; 65 of these: 148, 97.
+// Beyond the limit `few` is mostly the better one, by up to a third; tiles are where lengths are spread evenly, and
+// where few key heads just fill the chip.  The limit has not been moved to what these say.
 struct Plan {
   bool few;
   int slots;

@@ -1,13 +1,13 @@
 // Where the rows of a paged attention call lie: the integer arithmetic that gives a workgroup its sequence, tile and
 // tokens, apart from the kernels so that a host compiler takes it too.
 //
-// The packed rows (token * G + head of its group) of a sequence are cut into tiles of R.  Sequence b owns the slots from
-// (starts[b] * G / R) + b on: at least as many as it has tiles, and the first of them is known without the lengths of the
-// sequences before it.  The tokens behind the last sequence are sequence number `sequences`, which sees nothing.
+// The packed rows (token * G + head of its group) of a sequence are cut into tiles of R.  Sequence b owns the slots
+// from (starts[b] * G / R) + b on: at least as many as it has tiles, and the first of them is known without the lengths
+// of the sequences before it.  The tokens behind the last sequence are sequence number `sequences`, which sees nothing.
 //
-// Starts lie on the device and nothing checks them.  In any order and of any value they are taken as cut to [0, tokens]; a
-// slot then finds some sequence, perhaps one that does not own it, and has rows only if its tile is one of that
-// sequence's: every row that is read or written is a row of the call.
+// Starts lie on the device and nothing checks them.  In any order and of any value they are taken as cut to [0,
+// tokens]; a slot then finds some sequence, perhaps one that does not own it, and has rows only if its tile is one of
+// that sequence's: every row that is read or written is a row of the call.
 #pragma once
 
 #include <stdint.h>
@@ -38,8 +38,8 @@ M5K_PLACE int first_slot(const int32_t* starts, int b, int tokens, int group, in
   return static_cast<int>(int64_t{start_of(starts, b, tokens)} * group / rows_per_tile) + b;
 }
 
-// The last b of [0, n) whose first slot does not lie behind a slot, 64 probes at a time: count(lo, left, apart) says for
-// how many of lo, lo + apart, ... below lo + left (64 at most) that holds.  Ascending starts make those the first ones.
+// The last b of [0, n) whose first slot does not lie behind a slot, 64 probes at a time: count(lo, left, apart) says
+// for how many of lo, lo + apart, ... below lo + left (64 at most) that holds.  Ascending starts make those the first.
 template <class Count>
 M5K_PLACE int sequence_of_slot(int n, Count count) {
   int lo = 0, left = n;
