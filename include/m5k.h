@@ -440,6 +440,19 @@ int m5k_attention(const void* q, int dtype, int64_t tokens, int64_t heads, int h
                   const int32_t* prefix_lengths, void* out, int splits, float* workspace, int64_t workspace_elems,
                   void* stream);
 
+/*
+ * m5k_attention with a window (above 0) of which the first `sinks` keys of the row's document stay visible: of the keys
+ * that the other masks leave, those with p - j < window (and j - p < window without causal), and those below the
+ * document's first key + sinks.  sinks 0: m5k_attention.  The plan's keys: at most window (twice it without causal)
+ * + sinks + 64.
+ */
+int m5k_attention_sinks(const void* q, int dtype, int64_t tokens, int64_t heads, int head_dim, int64_t q_head,
+                        int64_t q_token, const void* k, int64_t k_head, int64_t k_key, const void* v, int64_t v_head,
+                        int64_t v_key, int64_t keys, int64_t kv_heads, float scale, int causal, int64_t window,
+                        int64_t sinks, float softcap, const float* slopes, const int32_t* document_starts,
+                        int64_t documents, const int32_t* prefix_lengths, void* out, int splits, float* workspace,
+                        int64_t workspace_elems, void* stream);
+
 /* The plan of m5k_attention (paged 0, sequences = documents) or m5k_paged_attention (paged 1,
  * keys = table_width * page_size) on `cus` compute units (host only; cus <= 0: those of the current device): the key
  * splits that pay, and whether the waves of a workgroup share 32 rows (few 1) or take 32 each (few 0; few may be
@@ -463,6 +476,36 @@ int m5k_paged_attention(const void* q, int dtype, int64_t tokens, int64_t heads,
                         int64_t sequences, const int32_t* query_starts, const int32_t* context_lengths, float scale,
                         int64_t window, float softcap, const float* slopes, const int32_t* prefix_lengths, void* out,
                         int splits, float* workspace, int64_t workspace_elems, void* stream);
+
+/* m5k_paged_attention with a window of which the first `sinks` keys of each sequence stay visible (as in
+ * m5k_attention_sinks). */
+int m5k_paged_attention_sinks(const void* q, int dtype, int64_t tokens, int64_t heads, int head_dim, int64_t q_head,
+                              int64_t q_token, const void* k_cache, int64_t k_page, int64_t k_head, int64_t k_slot,
+                              const void* v_cache, int64_t v_page, int64_t v_head, int64_t v_slot, int64_t pages,
+                              int64_t page_size, int64_t kv_heads, const int32_t* page_table, int64_t table_width,
+                              int64_t sequences, const int32_t* query_starts, const int32_t* context_lengths,
+                              float scale, int64_t window, int64_t sinks, float softcap, const float* slopes,
+                              const int32_t* prefix_lengths, void* out, int splits, float* workspace,
+                              int64_t workspace_elems, void* stream);
+
+/*
+ * A cache in 8 bits.  Codes [pages, kv_heads, page_size, head_dim], E4M3 (mode M5K_QUANT_FP8) or INT8 in [-127, 127]
+ * (M5K_QUANT_INT8), by strides in bytes; exponents [pages, kv_heads, page_size / block] bytes, the last axis
+ * contiguous, ke_page and ke_head apart.  A code of a block of `block` tokens (a multiple of 16 that divides
+ * page_size) and head stands for code * 2^(exponent - 127); under exponent 255 every code is NaN.
+ *
+ * m5k_paged_attention_codes: m5k_paged_attention_sinks over such a cache, whose values are taken in q's dtype (exact in
+ * BF16 down to its subnormals; in FP16 rounded, to an infinity above its range).  Rows of codes are 16-byte aligned,
+ * head_dim to 2^23 bytes apart.
+ */
+int m5k_paged_attention_codes(
+    const void* q, int dtype, int64_t tokens, int64_t heads, int head_dim, int64_t q_head, int64_t q_token, int mode,
+    const void* k_codes, int64_t k_page, int64_t k_head, int64_t k_slot, const uint8_t* k_exponents, int64_t ke_page,
+    int64_t ke_head, const void* v_codes, int64_t v_page, int64_t v_head, int64_t v_slot, const uint8_t* v_exponents,
+    int64_t ve_page, int64_t ve_head, int64_t block, int64_t pages, int64_t page_size, int64_t kv_heads,
+    const int32_t* page_table, int64_t table_width, int64_t sequences, const int32_t* query_starts,
+    const int32_t* context_lengths, float scale, int64_t window, int64_t sinks, float softcap, const float* slopes,
+    const int32_t* prefix_lengths, void* out, int splits, float* workspace, int64_t workspace_elems, void* stream);
 
 /*
  * Rotary positions: y = x with channel pairs of the first 2 * pairs channels turned by
@@ -492,6 +535,39 @@ int m5k_paged_append(const void* k, int64_t k_head, int64_t k_token, const void*
                      const int32_t* context_lengths, const void* q, int64_t heads, int64_t q_head, int64_t q_token,
                      void* q_out, const double* frequencies, int64_t pairs, int interleaved, float magnitude,
                      void* stream);
+
+/*
+ * m5k_paged_append into a cache in 8 bits (layout: see m5k_paged_attention_codes; block at most 128; the caches are
+ * written, with their exponents).  A block's exponent is the least e with max |x| <= 448 * 2^e (FP8) or 127 * 2^e
+ * (INT8) over the new tokens in it and, where the block holds older ones (at positions below context - n), at least
+ * the exponent that it has; a code is x / 2^e to the nearest, ties to even, and where the exponent grows the older
+ * codes are rounded again under it.  Slots behind the context stay as they are.  A block that gets an infinity or NaN
+ * takes exponent 255.
+ * Keys are turned in 64 bits; q, in 32, as m5k_rope's.  head_dim 64 or 128; rows of k, v and q 16-byte aligned.
+ * Two tokens that name the same place, or two sequences that name the same block, leave unspecified codes there.
+ */
+int m5k_paged_append_codes(
+    const void* k, int64_t k_head, int64_t k_token, const void* v, int64_t v_head, int64_t v_token, int dtype,
+    int64_t tokens, int64_t kv_heads, int64_t head_dim, int mode, void* k_codes, int64_t kc_page, int64_t kc_head,
+    int64_t kc_slot, uint8_t* k_exponents, int64_t ke_page, int64_t ke_head, void* v_codes, int64_t vc_page,
+    int64_t vc_head, int64_t vc_slot, uint8_t* v_exponents, int64_t ve_page, int64_t ve_head, int64_t block,
+    int64_t pages, int64_t page_size, const int32_t* page_table, int64_t table_width, int64_t sequences,
+    const int32_t* query_starts, const int32_t* context_lengths, const void* q, int64_t heads, int64_t q_head,
+    int64_t q_token, void* q_out, const double* frequencies, int64_t pairs, int interleaved, float magnitude,
+    void* stream);
+
+/*
+ * Read a cache in 8 bits back: k, v [kv_heads, tokens, head_dim] (F32, F16 or BF16, contiguous, 16-byte aligned) are
+ * the values of the last n of each sequence's context_lengths[b] keys, n = query_starts[b + 1] - query_starts[b]: what
+ * m5k_paged_append_codes with the same arguments wrote.  Rows behind the last sequence, at negative positions, behind
+ * the table or on no page are 0.
+ */
+int m5k_paged_read(int mode, const void* k_codes, int64_t kc_page, int64_t kc_head, int64_t kc_slot,
+                   const uint8_t* k_exponents, int64_t ke_page, int64_t ke_head, const void* v_codes, int64_t vc_page,
+                   int64_t vc_head, int64_t vc_slot, const uint8_t* v_exponents, int64_t ve_page, int64_t ve_head,
+                   int64_t block, int64_t pages, int64_t page_size, int64_t kv_heads, int64_t head_dim,
+                   const int32_t* page_table, int64_t table_width, int64_t sequences, const int32_t* query_starts,
+                   const int32_t* context_lengths, int64_t tokens, void* k, void* v, int dtype, void* stream);
 
 #ifdef __cplusplus
 }

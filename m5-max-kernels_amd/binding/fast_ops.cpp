@@ -550,11 +550,38 @@ bool expanded(const at::Tensor& t) {
   return false;
 }
 
-// paged_append(k, v, k_cache, v_cache, page_table, query_starts, context_lengths, q, frequencies, layout, magnitude):
-// the turned q, or True without one.
+// A cache in 8 bits: its codes' mode and the exponents of their blocks.
+struct Codes {
+  const at::Tensor *k, *v;
+  uint8_t *ke, *ve;
+  int64_t block;
+  int mode;
+};
+
+// Takes args k_scales, v_scales beside the cache; false: let Python look at it.
+bool codes_of(PyObject* const* args, const Paged& c, Codes& out) {
+  const at::Tensor *k = plain_strided(args[0]), *v = plain_strided(args[1]);
+  const at::ScalarType st = c.k->scalar_type();
+  if (!k || !v || (st != at::kByte && st != at::kChar) || k->dim() != 3 || v->sizes() != k->sizes() ||
+      k->scalar_type() != at::kByte || v->scalar_type() != at::kByte || k->device() != c.k->device() ||
+      v->device() != c.k->device() || k->size(0) != c.pages || k->size(1) != c.kv_heads || k->size(2) == 0 ||
+      c.page_size % k->size(2) || (c.dim != 64 && c.dim != 128) || !rows16(*c.k) || !rows16(*c.v))
+    return false;
+  const int64_t block = c.page_size / k->size(2);
+  if (block % 16 || block > 128 || (k->size(2) > 1 && (k->stride(2) != 1 || v->stride(2) != 1))) return false;
+  for (const at::Tensor* t : {c.k, c.v})
+    if (t->stride(2) < c.dim || t->stride(2) > (1 << 23)) return false;
+  out = Codes{k, v, static_cast<uint8_t*>(k->data_ptr()), static_cast<uint8_t*>(v->data_ptr()), block,
+              st == at::kByte ? M5K_QUANT_FP8 : M5K_QUANT_INT8};
+  return true;
+}
+
+// paged_append(k, v, k_cache, v_cache, page_table, query_starts, context_lengths, q, frequencies, layout, magnitude
+// [, k_scales, v_scales]): the turned q, or True without one.
 PyObject* paged_append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  if (nargs != 11) Py_RETURN_NONE;
+  if (nargs != 11 && nargs != 13) Py_RETURN_NONE;
+  const bool coded = nargs == 13 && (args[11] != Py_None || args[12] != Py_None);
   const at::Tensor *k = heads_of(args[0]), *v = heads_of(args[1]);
   Paged c;
   const int layout = layout_of(args[9]);
@@ -565,15 +592,18 @@ PyObject* paged_append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const c10::Device dev = k->device();
   const int64_t tokens = k->size(1);
   if (v->sizes() != k->sizes() || v->scalar_type() != k->scalar_type() || v->device() != dev ||
-      c.k->device() != dev || c.k->scalar_type() != k->scalar_type() || c.kv_heads != k->size(0) ||
+      c.k->device() != dev || (!coded && c.k->scalar_type() != k->scalar_type()) || c.kv_heads != k->size(0) ||
       c.dim != k->size(2) || expanded(*c.k) || expanded(*c.v))
+    Py_RETURN_NONE;
+  Codes e{};
+  if (coded && (!codes_of(args + 11, c, e) || expanded(*e.k) || expanded(*e.v) || !rows16(*k) || !rows16(*v)))
     Py_RETURN_NONE;
   const at::Tensor *f = nullptr, *q = nullptr;
   if (args[8] != Py_None && !(f = frequencies_of(args[8], c.dim, dev))) Py_RETURN_NONE;
   if (args[7] != Py_None) {
     q = heads_of(args[7]);
     if (!q || !f || q->size(1) != tokens || q->size(2) != c.dim || q->scalar_type() != k->scalar_type() ||
-        q->device() != dev)
+        q->device() != dev || (coded && !rows16(*q)))
       Py_RETURN_NONE;
   }
   void* stream = nullptr;
@@ -587,6 +617,19 @@ PyObject* paged_append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const int64_t pairs = f ? f->size(0) : 0;
   const int code = dtype_code(k->scalar_type());
   int rc;
+  if (coded) {
+    Py_BEGIN_ALLOW_THREADS
+    rc = m5k_paged_append_codes(kp, stride(*k, 0), stride(*k, 1), vp, stride(*v, 0), stride(*v, 1), code, tokens,
+                                c.kv_heads, c.dim, e.mode, kc, stride(*c.k, 0), stride(*c.k, 1), stride(*c.k, 2), e.ke,
+                                stride(*e.k, 0), stride(*e.k, 1), vc, stride(*c.v, 0), stride(*c.v, 1),
+                                stride(*c.v, 2), e.ve, stride(*e.v, 0), stride(*e.v, 1), e.block, c.pages, c.page_size,
+                                c.table, c.width, c.sequences, c.starts, c.context, qp, heads, q ? stride(*q, 0) : 0,
+                                q ? stride(*q, 1) : 0, yp, fp, pairs, layout, magnitude, stream);
+    Py_END_ALLOW_THREADS
+    if (rc) return failed("m5k_paged_append_codes", rc);
+    if (!q) Py_RETURN_TRUE;
+    return THPVariable_Wrap(std::move(y));
+  }
   Py_BEGIN_ALLOW_THREADS
   rc = m5k_paged_append(kp, stride(*k, 0), stride(*k, 1), vp, stride(*v, 0), stride(*v, 1), code, tokens, c.kv_heads,
                         c.dim, kc, stride(*c.k, 0), stride(*c.k, 1), stride(*c.k, 2), vc, stride(*c.v, 0),
@@ -600,10 +643,45 @@ PyObject* paged_append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// paged_read(k_cache, v_cache, page_table, query_starts, context_lengths, tokens, k_scales, v_scales, dtype): (k, v).
+PyObject* paged_read(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Paged c;
+  Codes e;
+  if (nargs != 9 || !paged_of(args, c) || !codes_of(args + 6, c, e) || !current(c.k->device()) ||
+      !PyLong_CheckExact(args[5]) || !THPDtype_Check(args[8]))
+    Py_RETURN_NONE;
+  int overflow = 0;
+  const int64_t tokens = PyLong_AsLongLongAndOverflow(args[5], &overflow);
+  const at::ScalarType st = reinterpret_cast<THPDtype*>(args[8])->scalar_type;
+  const int code = dtype_code(st);
+  if (overflow || tokens <= 0 || tokens > (1 << 28) || code < 0) Py_RETURN_NONE;
+  const c10::Device dev = c.k->device();
+  void* stream = nullptr;
+  if (!stream_of(dev, &stream)) return nullptr;
+  at::Tensor k = empty({c.kv_heads, tokens, c.dim}, st, dev), v = empty({c.kv_heads, tokens, c.dim}, st, dev);
+  const void *kc = c.k->data_ptr(), *vc = c.v->data_ptr();
+  void *kp = k.data_ptr(), *vp = v.data_ptr();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = m5k_paged_read(e.mode, kc, stride(*c.k, 0), stride(*c.k, 1), stride(*c.k, 2), e.ke, stride(*e.k, 0),
+                      stride(*e.k, 1), vc, stride(*c.v, 0), stride(*c.v, 1), stride(*c.v, 2), e.ve, stride(*e.v, 0),
+                      stride(*e.v, 1), e.block, c.pages, c.page_size, c.kv_heads, c.dim, c.table, c.width, c.sequences,
+                      c.starts, c.context, tokens, kp, vp, code, stream);
+  Py_END_ALLOW_THREADS
+  if (rc) return failed("m5k_paged_read", rc);
+  PyObject* pair = PyTuple_New(2);
+  if (!pair) return nullptr;
+  PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(k)));
+  PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(std::move(v)));
+  return pair;
+  END_HANDLE_TH_ERRORS
+}
+
 // What both attention entries share.
 struct Scores {
   float scale, softcap;
-  int64_t window;
+  int64_t window, sinks;
   const float* slopes;
   int splits;
   at::Tensor out, workspace;
@@ -613,8 +691,8 @@ struct Scores {
 
 // Checks q against the keys' heads and width, and the score options; allocates.  false: let Python look at it.
 bool scores_of(const at::Tensor* q, int64_t kv_heads, int64_t dim, at::ScalarType st, c10::Device dev, PyObject* scale,
-               PyObject* softcap, PyObject* window, PyObject* slopes, bool paged, int64_t sequences, int64_t keys,
-               Scores& s) {
+               PyObject* softcap, PyObject* window, PyObject* sinks, PyObject* slopes, bool paged, bool causal,
+               int64_t sequences, int64_t keys, Scores& s) {
   if (!q || q->scalar_type() != st || !half_type(*q) || q->device() != dev || !current(dev) || q->size(2) != dim ||
       q->size(0) % kv_heads || (dim != 64 && dim != 128) || !rows16(*q))
     return false;
@@ -622,10 +700,13 @@ bool scores_of(const at::Tensor* q, int64_t kv_heads, int64_t dim, at::ScalarTyp
   if (tokens > (1 << 24) || heads > (1 << 16) || tokens * heads >= (int64_t{1} << 30)) return false;
   if (!positive(scale, static_cast<float>(1.0 / std::sqrt(static_cast<double>(dim))), s.scale) ||
       !positive(softcap, 0.0f, s.softcap) || !window_of(window, s.window) ||
+      !window_of(sinks, s.sinks) || (s.sinks && !s.window) ||
       !optional_vector(slopes, heads, at::kFloat, dev, &s.slopes))
     return false;
   if (s.scale < FLT_MIN || (s.softcap != 0.0f && (s.softcap < FLT_MIN || s.scale / s.softcap > 1e37f))) return false;
-  if (m5k_attention_plan(paged, tokens, heads, kv_heads, sequences, keys, 0, &s.splits, nullptr)) return false;
+  // Keys that the plan counts a row to see.
+  const int64_t seen = (causal ? 1 : 2) * s.window + s.sinks + 64, reach = s.sinks && seen < keys ? seen : keys;
+  if (m5k_attention_plan(paged, tokens, heads, kv_heads, sequences, reach, 0, &s.splits, nullptr)) return false;
   s.out = empty({tokens, heads * dim}, st, dev);
   s.elems = 0;
   s.wp = nullptr;
@@ -638,19 +719,23 @@ bool scores_of(const at::Tensor* q, int64_t kv_heads, int64_t dim, at::ScalarTyp
 }
 
 // paged_attention(q, k_cache, v_cache, page_table, query_starts, context_lengths, scale, window, softcap, slopes,
-// prefix_lengths).
+// prefix_lengths [, sinks, k_scales, v_scales]).
 PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   Paged c;
   Scores s;
   const int32_t* prefix;
-  if (nargs != 11 || !paged_of(args + 1, c)) Py_RETURN_NONE;
+  if ((nargs != 11 && nargs != 14) || !paged_of(args + 1, c)) Py_RETURN_NONE;
+  Codes e{};
+  const bool coded = nargs == 14 && (args[12] != Py_None || args[13] != Py_None);
+  if (coded && !codes_of(args + 12, c, e)) Py_RETURN_NONE;
   const at::Tensor* q = heads_of(args[0]);
   const c10::Device dev = c.k->device();
   if (!optional_vector(args[10], c.sequences, at::kInt, dev, &prefix) || (prefix && args[7] != Py_None) ||
       !rows16(*c.k) || !rows16(*c.v) ||
-      !scores_of(q, c.kv_heads, c.dim, c.k->scalar_type(), dev, args[6], args[8], args[7], args[9], true, c.sequences,
-                 c.width * c.page_size, s))
+      !q || !scores_of(q, c.kv_heads, c.dim, coded ? q->scalar_type() : c.k->scalar_type(), dev, args[6], args[8],
+                       args[7], nargs == 14 ? args[11] : Py_None, args[9], true, true, c.sequences,
+                       c.width * c.page_size, s))
     Py_RETURN_NONE;
   void* stream = nullptr;
   if (!stream_of(dev, &stream)) return nullptr;
@@ -658,22 +743,34 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   void* op = s.out.data_ptr();
   const int code = dtype_code(q->scalar_type());
   int rc;
+  if (coded) {
+    Py_BEGIN_ALLOW_THREADS
+    rc = m5k_paged_attention_codes(
+        qp, code, q->size(1), q->size(0), static_cast<int>(c.dim), stride(*q, 0), stride(*q, 1), e.mode, kp,
+        stride(*c.k, 0), stride(*c.k, 1), stride(*c.k, 2), e.ke, stride(*e.k, 0), stride(*e.k, 1), vp, stride(*c.v, 0),
+        stride(*c.v, 1), stride(*c.v, 2), e.ve, stride(*e.v, 0), stride(*e.v, 1), e.block, c.pages, c.page_size,
+        c.kv_heads, c.table, c.width, c.sequences, c.starts, c.context, s.scale, s.window, s.sinks, s.softcap, s.slopes,
+        prefix, op, s.splits, s.wp, s.elems, stream);
+    Py_END_ALLOW_THREADS
+    if (rc) return failed("m5k_paged_attention_codes", rc);
+    return THPVariable_Wrap(std::move(s.out));
+  }
   Py_BEGIN_ALLOW_THREADS
-  rc = m5k_paged_attention(qp, code, q->size(1), q->size(0), static_cast<int>(c.dim), stride(*q, 0), stride(*q, 1), kp,
-                           stride(*c.k, 0), stride(*c.k, 1), stride(*c.k, 2), vp, stride(*c.v, 0), stride(*c.v, 1),
-                           stride(*c.v, 2), c.pages, c.page_size, c.kv_heads, c.table, c.width, c.sequences, c.starts,
-                           c.context, s.scale, s.window, s.softcap, s.slopes, prefix, op, s.splits, s.wp, s.elems,
-                           stream);
+  rc = m5k_paged_attention_sinks(
+      qp, code, q->size(1), q->size(0), static_cast<int>(c.dim), stride(*q, 0), stride(*q, 1), kp, stride(*c.k, 0),
+      stride(*c.k, 1), stride(*c.k, 2), vp, stride(*c.v, 0), stride(*c.v, 1), stride(*c.v, 2), c.pages, c.page_size,
+      c.kv_heads, c.table, c.width, c.sequences, c.starts, c.context, s.scale, s.window, s.sinks, s.softcap, s.slopes,
+      prefix, op, s.splits, s.wp, s.elems, stream);
   Py_END_ALLOW_THREADS
-  if (rc) return failed("m5k_paged_attention", rc);
+  if (rc) return failed("m5k_paged_attention_sinks", rc);
   return THPVariable_Wrap(std::move(s.out));
   END_HANDLE_TH_ERRORS
 }
 
-// attention(q, k, v, causal, window, document_starts, prefix_lengths, softcap, slopes, scale).
+// attention(q, k, v, causal, window, document_starts, prefix_lengths, softcap, slopes, scale [, sinks]).
 PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  if (nargs != 10 || !PyBool_Check(args[3])) Py_RETURN_NONE;
+  if ((nargs != 10 && nargs != 11) || !PyBool_Check(args[3])) Py_RETURN_NONE;
   const at::Tensor *q = heads_of(args[0]), *k = heads_of(args[1]), *v = heads_of(args[2]);
   if (!q || !k || !v || v->sizes() != k->sizes() || v->scalar_type() != k->scalar_type() ||
       v->device() != k->device() || !rows16(*k) || !rows16(*v))
@@ -695,8 +792,8 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   Scores s;
   if (keys > (1 << 24) || !optional_vector(args[6], documents ? documents : 1, at::kInt, dev, &prefix) ||
       (prefix && (!causal || args[4] != Py_None)) ||
-      !scores_of(q, kv_heads, dim, k->scalar_type(), dev, args[9], args[7], args[4], args[8], false, documents, keys,
-                 s))
+      !scores_of(q, kv_heads, dim, k->scalar_type(), dev, args[9], args[7], args[4], nargs == 11 ? args[10] : Py_None,
+                 args[8], false, causal, documents, keys, s))
     Py_RETURN_NONE;
   void* stream = nullptr;
   if (!stream_of(dev, &stream)) return nullptr;
@@ -705,11 +802,12 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const int code = dtype_code(q->scalar_type());
   int rc;
   Py_BEGIN_ALLOW_THREADS
-  rc = m5k_attention(qp, code, tokens, q->size(0), static_cast<int>(dim), stride(*q, 0), stride(*q, 1), kp,
-                     stride(*k, 0), stride(*k, 1), vp, stride(*v, 0), stride(*v, 1), keys, kv_heads, s.scale, causal,
-                     s.window, s.softcap, s.slopes, starts, documents, prefix, op, s.splits, s.wp, s.elems, stream);
+  rc = m5k_attention_sinks(qp, code, tokens, q->size(0), static_cast<int>(dim), stride(*q, 0), stride(*q, 1), kp,
+                           stride(*k, 0), stride(*k, 1), vp, stride(*v, 0), stride(*v, 1), keys, kv_heads, s.scale,
+                           causal, s.window, s.sinks, s.softcap, s.slopes, starts, documents, prefix, op, s.splits,
+                           s.wp, s.elems, stream);
   Py_END_ALLOW_THREADS
-  if (rc) return failed("m5k_attention", rc);
+  if (rc) return failed("m5k_attention_sinks", rc);
   return THPVariable_Wrap(std::move(s.out));
   END_HANDLE_TH_ERRORS
 }
@@ -735,6 +833,7 @@ PyMethodDef methods[] = {
     {"qkv", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(qkv)), METH_FASTCALL, nullptr},
     {"rope", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rope)), METH_FASTCALL, nullptr},
     {"paged_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paged_append)), METH_FASTCALL, nullptr},
+    {"paged_read", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paged_read)), METH_FASTCALL, nullptr},
     {"paged_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paged_attention)), METH_FASTCALL,
      nullptr},
     {"attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(attention)), METH_FASTCALL, nullptr},

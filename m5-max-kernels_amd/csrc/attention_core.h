@@ -69,6 +69,12 @@ struct Args {
   int tokens, keys, heads, kv_heads, group, sequences, pages, page_size, window, causal, splits, slots, spread, cus;
   uint32_t page_magic, page_shift, group_magic, group_shift;
   float scale, softcap;
+  int sinks;
+  int64_t reach;  // keys that a row can see, for the plan
+  // Codes: exponent bytes of each block of tokens, strides in bytes.
+  const uint8_t *k_exp, *v_exp;
+  int64_t ke_page, ke_head, ve_page, ve_head;
+  uint32_t block_magic, block_shift;
 };
 
 // n / d of 0 <= n < 2^31 by one multiplication: magic = ceil(2^(31 + shift) / d), shift = ceil(log2 d).  The excess
@@ -141,6 +147,9 @@ __device__ __forceinline__ int swizzle(int row) {
 // loads lie in one page and take one address; PAGES: any page size, an address a lane.
 enum Keys { DENSE = 0, PAGES16 = 1, PAGES = 2 };
 
+// What a cache holds: 16-bit values, or codes of 8 bits under a block's power of two.
+enum Codes { NO_CODES = 0, E4M3 = 1, INT8 = 2 };
+
 // Page id at a position of the table, the same for the whole wave.  SCALAR: a scalar load, which leaves vmcnt to the
 // tiles in flight.  Otherwise a load per lane: a scalar one shares lgkmcnt with the LDS reads, out of order, and makes
 // each of them wait.
@@ -157,27 +166,85 @@ __device__ __forceinline__ int table_entry(const int32_t* table, uint32_t at) {
 
 // Buffer window of up to `rows` rows of `stride` elements from `p`, reading 0 behind them: rows are at least D apart,
 // so a row behind the last begins behind the window's end.
-template <int D>
-__device__ __forceinline__ v4i rows_rsrc(const uint16_t* p, int rows, int64_t stride) {
-  const int64_t n = rows > 0 ? ((rows - 1) * stride + D) * 2 : 0;
+template <int D, class Elem>
+__device__ __forceinline__ v4i rows_rsrc(const Elem* p, int rows, int64_t stride) {
+  const int64_t n = rows > 0 ? ((rows - 1) * stride + D) * static_cast<int64_t>(sizeof(Elem)) : 0;
   return gemm::buffer_rsrc(p, static_cast<uint32_t>(n));
+}
+
+constexpr int NEVER = 0x3FFFFFFF;  // behind every key
+
+// An exponent byte, the same for the whole wave.  SCALAR: see table_entry.
+template <bool SCALAR>
+__device__ __forceinline__ int exponent_byte(const uint8_t* at) {
+  if constexpr (SCALAR) {
+    const uintptr_t p = reinterpret_cast<uintptr_t>(at);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(p));
+    const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(p >> 32));
+    const uintptr_t word = (static_cast<uintptr_t>(hi) << 32) | (lo & ~3u);
+    const uint32_t w = *reinterpret_cast<const __attribute__((address_space(4))) uint32_t*>(word);
+    return static_cast<int>((w >> (8 * (lo & 3u))) & 0xFFu);
+  } else {
+    return *at;
+  }
+}
+
+// Two codes, bytes 2 HI and 2 HI + 1 of a word, times a power of two, as 16-bit values.
+template <int DT, int CODES, bool HI>
+__device__ __forceinline__ uint32_t code_pair(int w, float scale) {
+  if constexpr (CODES == E4M3) {
+    const auto f = __builtin_amdgcn_cvt_pk_f32_fp8(w, HI);
+    return pack2<DT>(f[0] * scale, f[1] * scale);
+  } else {
+    const int w0 = HI ? w << 8 : w << 24, w1 = HI ? w : w << 16;
+    return pack2<DT>(static_cast<float>(w0 >> 24) * scale, static_cast<float>(w1 >> 24) * scale);
+  }
+}
+
+// 16 codes times 2^(e - 127), in order, as 16-bit values.  Exact in BF16, which has more bits than a code and FP32's
+// range; rounded once to FP16, which only numbers below 2^-14 need.  e = 255: NaN.
+template <int DT, int CODES>
+__device__ __forceinline__ void expand16(v4i c, int e, v4i (&x)[2]) {
+  // 2^-127 has no exponent field of its own in FP32.
+  const float scale = __uint_as_float(e == 0 ? 0x00400000u : e == 255 ? 0x7FC00000u : static_cast<uint32_t>(e) << 23);
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    x[w >> 1][2 * (w & 1)] = static_cast<int>(code_pair<DT, CODES, false>(c[w], scale));
+    x[w >> 1][2 * (w & 1) + 1] = static_cast<int>(code_pair<DT, CODES, true>(c[w], scale));
+  }
 }
 
 struct RowRange {
   int lo, hi;  // visible keys; lo > hi where there are none
   int pos;     // position on the key axis, for the distance bias
+  int slo, shi;  // SINKS: further visible keys, before lo; slo > shi where there are none
 };
 
-// The interval of a row at position p of a span [s, e) of keys.
-__device__ __forceinline__ RowRange row_range(int s, int e, int p, int prefix, int causal, int window) {
-  int lo = s, hi = e;
+// The interval of a row at position p of a span [s, e) of keys, and with SINKS the span's first keys where the window
+// has left them behind.
+template <bool SINKS>
+__device__ __forceinline__ RowRange row_range(int s, int e, int p, int prefix, int causal, int window, int sinks) {
+  int lo = s, hi = e, slo = NEVER, shi = 0;
   if (causal) hi = min(e, max(p + 1, s + prefix));
+  const int kept = min(hi, s + sinks);
   if (window) {
     lo = max(lo, p - window + 1);
     if (!causal) hi = min(hi, p + window);
   }
-  if (hi <= lo) { lo = 0x3FFFFFFF; hi = 0; }
-  return RowRange{lo, hi, p};
+  if constexpr (SINKS) {
+    if (hi <= lo) {
+      lo = s;
+      hi = kept;
+    } else if (kept >= lo) {
+      lo = s;
+      hi = max(hi, kept);
+    } else if (kept > s) {
+      slo = s;
+      shi = kept;
+    }
+  }
+  if (hi <= lo) { lo = NEVER; hi = 0; }
+  return RowRange{lo, hi, p, slo, shi};
 }
 
 // The last b in [0, n) with key(b) <= x, by binary search over a nondecreasing key; 0 if there is none.
@@ -312,7 +379,7 @@ __device__ __forceinline__ Place place(const Args& a, int rows_per_tile) {
 }
 
 // The row range, and the token and query head of packed row r (r < p.rows).
-template <int KEYS>
+template <int KEYS, bool SINKS>
 __device__ __forceinline__ RowRange range_of(const Args& a, const Place& p, int r, int& token, int& head) {
   const int i = a.group == 1 ? r : static_cast<int>(fast_div(r, a.group_magic, a.group_shift));
   head = p.kvh * a.group + r - i * a.group;
@@ -327,8 +394,8 @@ __device__ __forceinline__ RowRange range_of(const Args& a, const Place& p, int 
   } else if (a.prefix && (KEYS == DENSE || p.seq < a.sequences)) {
     prefix = a.prefix[p.seq];
   }
-  prefix = min(max(prefix, 0), 0x3FFFFFFF);
-  return row_range(s, e, i + p.shift, prefix, a.causal, a.window);
+  prefix = min(max(prefix, 0), NEVER);
+  return row_range<SINKS>(s, e, i + p.shift, prefix, a.causal, a.window, a.sinks);
 }
 
 // FEW = false: the 4 waves take 32 rows each and share key tiles of 64.  FEW: they share 32 rows, for calls that have
@@ -342,11 +409,19 @@ __device__ __forceinline__ RowRange range_of(const Args& a, const Place& p, int 
 // keys, 16 heads: 32.2 and 26.5; 63 single tokens over 1 to 4000 keys, 8 key heads: 72.6 and 57.8; single tokens over
 // 1000 keys, one key head: 480 of them 28.2 and 24.7, but 508, which just fill the chip, 28.6 and 36.7.  By whole
 // addresses (pages of 16, dense) two of each gained 10% in some calls and lost 3 to 12% in others.
-template <int DT, int D, int KEYS, bool MODS, bool FEW>
+//
+// SINKS: rows see their span's first keys beside their window.  The workgroup's tiles are those of the first keys, then
+// those of the windows: `t` counts them, real(t) is where tile t lies.
+//
+// CODES: K and V are codes of 8 bits with an exponent byte a block of tokens.  A wave's codes go to LDS as they are, by
+// the loads above, and from there, times their scale, to the tile of 16-bit values that the products read: by the wave
+// that loaded them, so that no barrier stands between and each code is expanded once a workgroup.
+template <int DT, int D, int KEYS, bool MODS, bool FEW, bool SINKS, int CODES>
 __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
+  static_assert(CODES == NO_CODES || KEYS == PAGES16, "codes lie in pages of a multiple of 16");
   constexpr int KT = FEW ? 32 : 64, NB = KT / 32;  // keys of a tile, 32-key blocks
   constexpr int EL = 16 * NB;                      // scores of a lane
-  constexpr int CH = D / 8;                        // 16-byte chunks of a row
+  constexpr int CH = CODES ? D / 16 : D / 8;       // 16-byte chunks of a row, as it lies in memory
   constexpr int RPI = 64 / CH;                     // rows of one load instruction
   constexpr int LOADED = FEW ? KT : KT / WAVES;    // rows of a tile that one wave loads
   constexpr int GROUPS = LOADED / 16;
@@ -358,9 +433,14 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   constexpr uint32_t ROWB = D * 2, TILE = KT * ROWB, VTILE = STAGES * TILE;
   // K stages, V stages.  FEW: those of each wave, later its sums, in rows of D + 4 floats (16 bytes a lane without bank
   // conflicts), and their maxima and totals.
-  constexpr uint32_t SUMS = (D + 4) * 4, JOIN = 32 * SUMS + 256, AREA = JOIN > 2 * VTILE ? JOIN : 2 * VTILE;
-  __shared__ __attribute__((aligned(256))) uint8_t lds[FEW ? WAVES * AREA : 4 * TILE];
-  __shared__ int bounds[2 * WAVES];
+  // CODES: behind them a wave's codes of one tile of K and one of V.
+  constexpr uint32_t RAW = CODES ? LOADED * D : 0;
+  constexpr uint32_t HELD = 2 * VTILE + 2 * RAW;
+  constexpr uint32_t SUMS = (D + 4) * 4, JOIN = 32 * SUMS + 256, AREA = JOIN > HELD ? JOIN : HELD;
+  __shared__ __attribute__((aligned(256))) uint8_t lds[FEW ? WAVES * AREA : 4 * TILE + 2 * WAVES * RAW];
+  // Bounds of the waves' rows.  CODES: where the codes come later, since two workgroups' LDS fills the compute unit.
+  __shared__ int bounds_own[FEW || CODES ? 1 : SINKS ? 5 * WAVES : 2 * WAVES];
+  int* const bounds = CODES ? reinterpret_cast<int*>(lds) : bounds_own;
 
   const Place p = place<KEYS>(a, ROWS);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
@@ -370,11 +450,12 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   const int row = row0 + (FEW ? 0 : 32 * wave) + (lane & 31);
   const bool live = row < p.rows;
   int token, head;
-  const RowRange rr = range_of<KEYS>(a, p, min(row, p.rows - 1), token, head);
+  const RowRange rr = range_of<KEYS, SINKS>(a, p, min(row, p.rows - 1), token, head);
 
   // Key ranges: of the wave (any row, every row), and of the workgroup.
   const bool idle = !FEW && row0 + 32 * wave >= p.rows;
-  const int any_lo = idle ? 0x3FFFFFFF : wave_min_i(rr.lo), any_hi = idle ? 0 : wave_max_i(rr.hi);
+  int any_lo = idle ? NEVER : wave_min_i(rr.lo);
+  const int any_hi = idle ? 0 : wave_max_i(rr.hi);
   const int all_lo = wave_max_i(rr.lo), all_hi = wave_min_i(rr.hi);
   int lo = any_lo, hi = any_hi;
   if constexpr (!FEW) {
@@ -391,10 +472,56 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     lo = __builtin_amdgcn_readfirstlane(lo);
     hi = __builtin_amdgcn_readfirstlane(hi);
   }
+  // First keys that lie before the windows of all rows have tiles of their own, `kept` of them from `kept_tile` on; the
+  // others (of documents that begin inside the workgroup's rows) are taken with the windows.
+  int kept = 0, kept_tile = 0;
+  bool with_window = true;
+  if constexpr (SINKS) {
+    with_window = rr.shi > lo / KT * KT;
+    const bool has = rr.slo < rr.shi && !idle;
+    any_lo = wave_min_i(has && with_window ? min(rr.lo, rr.slo) : idle ? NEVER : rr.lo);
+    const int own_lo = wave_min_i(has && !with_window ? rr.slo : NEVER);
+    int s_lo = own_lo, s_hi = wave_max_i(has && !with_window ? rr.shi : 0);
+    lo = any_lo;
+    if constexpr (!FEW) {
+      if (lane == 0) {
+        bounds[2 * WAVES + wave] = any_lo;
+        bounds[3 * WAVES + wave] = s_lo;
+        bounds[4 * WAVES + wave] = s_hi;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        lo = min(lo, bounds[2 * WAVES + w]);
+        s_lo = min(s_lo, bounds[3 * WAVES + w]);
+        s_hi = max(s_hi, bounds[4 * WAVES + w]);
+      }
+      lo = __builtin_amdgcn_readfirstlane(lo);
+      s_lo = __builtin_amdgcn_readfirstlane(s_lo);
+      s_hi = __builtin_amdgcn_readfirstlane(s_hi);
+    }
+    if (s_lo < s_hi) {
+      kept_tile = s_lo / KT;
+      kept = (s_hi + KT - 1) / KT - kept_tile;
+      if (kept_tile + kept > lo / KT) {  // one stretch of tiles after all
+        kept = 0;
+        lo = min(lo, s_lo);
+        any_lo = min(any_lo, own_lo);
+        with_window = true;
+      }
+    }
+  }
+  if constexpr (CODES && !FEW) __syncthreads();  // the bounds have been read
+  // Tile t lies at real(t), and a window's tile T is tile t = T - ahead.
+  const int window_tile = SINKS ? lo / KT : 0, ahead = window_tile - kept;
+  auto real = [&](int t) __attribute__((always_inline)) {
+    if constexpr (SINKS) return t < kept ? kept_tile + t : t + ahead;
+    else return t;
+  };
   int t_begin = 0, t_end = 0;
   if (lo < hi) {
-    t_begin = lo / KT;
-    t_end = (hi + KT - 1) / KT;
+    t_begin = SINKS ? 0 : lo / KT;
+    t_end = (hi + KT - 1) / KT - (SINKS ? ahead : 0);
     if (a.splits > 1) {
       // At least 256 keys a split: below, the partial sums cost more than the keys.
       const int per = max((t_end - t_begin + a.splits - 1) / a.splits, 256 / KT);
@@ -416,8 +543,11 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   // Loads: instruction i of a wave brings rows first_row + i * RPI + lane / CH of K and of V.
   const int first_row = FEW ? 0 : wave_s * LOADED;
   const int ld_row = first_row + lane / CH, ld_chunk = lane % CH;
-  const uint16_t* kbase = a.k + int64_t{p.kvh} * a.k_head;
-  const uint16_t* vbase = a.v + int64_t{p.kvh} * a.v_head;
+  using Elem = std::conditional_t<CODES != NO_CODES, uint8_t, uint16_t>;
+  const Elem* kbase = reinterpret_cast<const Elem*>(a.k) + int64_t{p.kvh} * a.k_head;
+  const Elem* vbase = reinterpret_cast<const Elem*>(a.v) + int64_t{p.kvh} * a.v_head;
+  const uint8_t* kexp = CODES ? a.k_exp + int64_t{p.kvh} * a.ke_head : nullptr;
+  const uint8_t* vexp = CODES ? a.v_exp + int64_t{p.kvh} * a.ve_head : nullptr;
   const int32_t* table = KEYS != DENSE && p.seq < a.sequences ? a.table + int64_t{p.seq} * a.table_width : nullptr;
   const uint32_t lds0 = gemm::lds_addr(lds) + (FEW ? wave_s * AREA : 0);
   uint32_t kofs[NI], vofs[NI];  // bytes of a lane's chunk from the window's first row
@@ -425,13 +555,14 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int r = KEYS == DENSE ? ld_row + i * RPI : lane / CH + i % (NI / GROUPS) * RPI;  // pages: of 16 rows
-      const int chunk = (ld_chunk ^ swizzle<D>(ld_row + i * RPI)) * 8;
-      kofs[i] = static_cast<uint32_t>(r * static_cast<int>(a.k_row) + chunk) * 2;
-      vofs[i] = static_cast<uint32_t>(r * static_cast<int>(a.v_row) + chunk) * 2;
+      const int chunk = CODES ? ld_chunk * 16 : (ld_chunk ^ swizzle<D>(ld_row + i * RPI)) * 8;
+      kofs[i] = static_cast<uint32_t>(r * static_cast<int>(a.k_row) + chunk) * sizeof(Elem);
+      vofs[i] = static_cast<uint32_t>(r * static_cast<int>(a.v_row) + chunk) * sizeof(Elem);
     }
   }
   constexpr int NIDS = KEYS == PAGES ? NI : GROUPS;
   int ids[2][NIDS] = {};  // pages of the next tile's keys, and of the tile before it, whose values come next
+  int ek[GROUPS] = {}, ev[GROUPS] = {};  // CODES: exponents of the codes on their way
   bool lacking = false;
 
   // Unconditional, at the last key where tile t has none: a load under a condition would be waited for at the
@@ -440,21 +571,22 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     if constexpr (KEYS == PAGES16) {
 #pragma unroll
       for (int i = 0; i < GROUPS; ++i) {
-        const int key = min(t * KT + first_row + 16 * i, p.span - 1);
+        const int key = min(real(t) * KT + first_row + 16 * i, p.span - 1);
         to[i] = table_entry<FEW>(table, fast_div(key, a.page_magic, a.page_shift));
       }
     } else if constexpr (KEYS == PAGES) {
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        const int key = min(t * KT + ld_row + i * RPI, p.span - 1);
+        const int key = min(real(t) * KT + ld_row + i * RPI, p.span - 1);
         to[i] = table[fast_div(key, a.page_magic, a.page_shift)];
       }
     }
   };
   // This wave's rows of tile t of one operand to LDS at dst.
-  auto load_rows = [&](int t, const int (&id)[NIDS], const uint16_t* base, int64_t page_stride, int64_t row_stride,
+  auto load_rows = [&](int u, const int (&id)[NIDS], const Elem* base, int64_t page_stride, int64_t row_stride,
                        const uint32_t (&ofs)[NI], uint32_t dst) __attribute__((always_inline)) {
-    dst += FEW ? 0 : wave_s * NI * 1024;
+    const int t = real(u);
+    dst += FEW || CODES ? 0 : wave_s * NI * 1024;
     if constexpr (KEYS == PAGES) {
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
@@ -475,7 +607,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g) {
         const int key = t * KT + first_row + 16 * g, page = __builtin_amdgcn_readfirstlane(id[g]);
-        const uint16_t* at = base;
+        const Elem* at = base;
         int rows = min(p.span - key, 16);
         if (rows > 0) {
           if (static_cast<uint32_t>(page) < static_cast<uint32_t>(a.pages)) {
@@ -490,6 +622,44 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
         constexpr int PER = NI / GROUPS;
 #pragma unroll
         for (int i = 0; i < PER; ++i) gemm::dma16<true>(dst + (g * PER + i) * 1024, ofs[g * PER + i], rsrc);
+      }
+    }
+  };
+
+  // CODES: exponents of the groups of 16 keys that this wave loads of tile t, 0 where there is no page.  FEW: as the
+  // aligned word around each, by a scalar load (see table_entry); the word's other bytes share the byte's allocation.
+  const uint32_t raw_k = FEW ? lds0 + 2 * VTILE : lds0 + 4 * TILE + wave_s * 2 * RAW, raw_v = raw_k + RAW;
+  auto load_exps = [&](int u, const int (&id)[NIDS], const uint8_t* base, int64_t page_stride, int (&to)[GROUPS])
+                       __attribute__((always_inline)) {
+    if constexpr (CODES) {
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) {
+        const int key = real(u) * KT + first_row + 16 * g;
+        const int slot = key - static_cast<int>(fast_div(key, a.page_magic, a.page_shift)) * a.page_size;
+        const bool has = key < p.span && static_cast<uint32_t>(id[g]) < static_cast<uint32_t>(a.pages);
+        const uint8_t* at = has ? base + id[g] * page_stride + fast_div(slot, a.block_magic, a.block_shift)
+                                : reinterpret_cast<const uint8_t*>(kZeros);
+        to[g] = exponent_byte<FEW>(at);
+      }
+    }
+  };
+  // This wave's codes at `raw`, times their scale, to its rows of the 16-bit tile at `dst`.
+  auto expand = [&](uint32_t raw, const int (&exps)[GROUPS], uint32_t dst) __attribute__((always_inline)) {
+    if constexpr (CODES) {
+      constexpr int PER = NI / GROUPS;
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) {
+        const int e = __builtin_amdgcn_readfirstlane(exps[g]);
+#pragma unroll
+        for (int i = g * PER; i < (g + 1) * PER; ++i) {
+          const v4i c = *reinterpret_cast<const __attribute__((address_space(3))) v4i*>(raw + i * 1024 + lane * 16);
+          v4i x[2];
+          expand16<DT, CODES>(c, e, x);
+          const int r = ld_row + i * RPI;
+          const uint32_t at = dst + r * ROWB + (((2 * ld_chunk) ^ swizzle<D>(r)) << 4);
+          *reinterpret_cast<__attribute__((address_space(3))) v4i*>(at) = x[0];
+          *reinterpret_cast<__attribute__((address_space(3))) v4i*>(at ^ 16) = x[1];
+        }
       }
     }
   };
@@ -575,7 +745,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   // Cap, bias and mask of tile t's scores.
   auto finish = [&](v16f (&x)[NB], int t, auto with_care, uint32_t& sees_bits) __attribute__((always_inline)) {
     constexpr bool careful = decltype(with_care)::value;
-    const int key0 = t * KT, kofs0 = key0 + 4 * half;
+    const int key0 = real(t) * KT, kofs0 = key0 + 4 * half;
     if constexpr (MODS) {
       // Scores in base 2: capped, or scaled with the bias.  Distances are whole numbers, exact in FP32 up to 2^24.
       if (a.softcap > 0.0f) {
@@ -607,6 +777,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     }
     if (careful || key0 < all_lo || key0 + KT > all_hi) {
       const uint32_t width = static_cast<uint32_t>(max(rr.hi - rr.lo, 0));
+      const uint32_t first_keys = SINKS ? static_cast<uint32_t>(max(rr.shi - rr.slo, 0)) : 0;
       if constexpr (careful) sees_bits = 0;
 #pragma unroll
       for (int b = 0; b < NB; ++b)
@@ -614,6 +785,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
         for (int r = 0; r < 16; ++r) {
           const int key = kofs0 + 32 * b + 8 * (r >> 2) + (r & 3);
           bool sees = static_cast<uint32_t>(key - rr.lo) < width;
+          if constexpr (SINKS) sees |= static_cast<uint32_t>(key - rr.slo) < first_keys;
           if constexpr (KEYS != DENSE && careful) {
             if (sees)
               sees = static_cast<uint32_t>(table[fast_div(key, a.page_magic, a.page_shift)]) <
@@ -696,7 +868,13 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     }
   };
 
-  const int first = max(t_begin, any_lo / KT), last = min(t_end, (any_hi + KT - 1) / KT);  // this wave's tiles
+  // This wave's tiles.
+  const int first = max(t_begin, any_lo / KT - (SINKS ? ahead : 0));
+  const int last = min(t_end, (any_hi + KT - 1) / KT - (SINKS ? ahead : 0));
+  auto mine = [&](int t) __attribute__((always_inline)) {
+    if constexpr (SINKS) return (t >= first && t < last) || (t >= t_begin && t < min(kept, t_end) && !idle);
+    else return t >= first && t < last;
+  };
   auto start = [&]() __attribute__((always_inline)) {
     m = m2 = M_FLOOR;
     l = 0.0f;
@@ -712,15 +890,26 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     constexpr int ODD = decltype(odd)::value, EVEN = 1 - ODD;
     wait_all();
     gemm::stage_barrier();
-    if (t + 1 < t_end) {
+    if constexpr (CODES) {
+      // The codes of V of tile t + 1 and K of t + 2 are here: expand them, and load those of a tile further on.
+      if (t + 1 < t_end) expand(raw_v, ev, lds0 + (2 + ODD) * TILE);
+      if (t + 2 < t_end) {
+        expand(raw_k, ek, lds0 + EVEN * TILE);
+        __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        load_exps(t + 2, ids[1], vexp, a.ve_page, ev);
+        load_exps(t + 3, ids[0], kexp, a.ke_page, ek);
+        load_rows(t + 2, ids[1], vbase, a.v_page, a.v_row, vofs, raw_v);
+        if (t + 3 < t_end) load_rows(t + 3, ids[0], kbase, a.k_page, a.k_row, kofs, raw_k);
+      }
+    } else if (t + 1 < t_end) {
       load_rows(t + 1, ids[1], vbase, a.v_page, a.v_row, vofs, lds0 + (2 + ODD) * TILE);
       if (t + 2 < t_end) load_rows(t + 2, ids[0], kbase, a.k_page, a.k_row, kofs, lds0 + EVEN * TILE);
     }
 #pragma unroll
     for (int i = 0; i < NIDS; ++i) ids[1][i] = ids[0][i];
-    load_ids(t + 3, ids[0]);
+    load_ids(t + (CODES ? 4 : 3), ids[0]);
     uint32_t none;
-    const bool now = t >= first && t < last, then = t + 1 >= first && t + 1 < last;  // the same for the whole wave
+    const bool now = mine(t), then = mine(t + 1);  // the same for the whole wave
     if (now && then) {
       product(next, ODD, x, true);
       finish(next, t + 1, quick, none);
@@ -742,7 +931,16 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   auto own_tile = [&](int t, auto stage) __attribute__((always_inline)) {
     constexpr int ST = decltype(stage)::value;
     const bool more = t + WAVES < t_end;
-    if constexpr (STAGES == 2) {
+    if constexpr (CODES) {
+      gemm::wait_stage<NI>();  // K, behind which V was issued
+      expand(raw_k, ek, lds0);
+      __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (more) {
+        load_exps(t + WAVES, ids[0], kexp, a.ke_page, ek);
+        load_rows(t + WAVES, ids[0], kbase, a.k_page, a.k_row, kofs, raw_k);
+      }
+      product(s[0], 0, s[0], false);
+    } else if constexpr (STAGES == 2) {
       if (more) {
         __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last reads of that stage
         load_rows(t + WAVES, ids[0], kbase, a.k_page, a.k_row, kofs, lds0 + (1 - ST) * TILE);
@@ -771,8 +969,17 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
       if (more) gemm::wait_stage<NI>();
       else gemm::wait_stage<0>();
     }
+    if constexpr (CODES) {
+      expand(raw_v, ev, lds0 + VTILE);
+      __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (more) {
+        load_exps(t + WAVES, ids[0], vexp, a.ve_page, ev);
+        load_rows(t + WAVES, ids[0], vbase, a.v_page, a.v_row, vofs, raw_v);
+        load_ids(t + 2 * WAVES, ids[0]);
+      }
+    }
     accumulate(ST, s[0]);
-    if constexpr (STAGES == 1) {
+    if constexpr (STAGES == 1 && !CODES) {
       if (more) {
         __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         load_rows(t + WAVES, ids[0], vbase, a.v_page, a.v_row, vofs, lds0 + VTILE);
@@ -785,8 +992,10 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     int t = t_begin + wave_s;
     if (t < t_end) {
       load_ids(t, ids[0]);
-      load_rows(t, ids[0], kbase, a.k_page, a.k_row, kofs, lds0);
-      load_rows(t, ids[0], vbase, a.v_page, a.v_row, vofs, lds0 + VTILE);
+      load_exps(t, ids[0], kexp, a.ke_page, ek);
+      load_exps(t, ids[0], vexp, a.ve_page, ev);
+      load_rows(t, ids[0], kbase, a.k_page, a.k_row, kofs, CODES ? raw_k : lds0);
+      load_rows(t, ids[0], vbase, a.v_page, a.v_row, vofs, CODES ? raw_v : lds0 + VTILE);
       load_ids(t + WAVES, ids[0]);
     }
     for (; t < t_end; t += STAGES * WAVES) {
@@ -795,8 +1004,23 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     }
   } else if (t_begin < t_end) {
     load_ids(t_begin, ids[1]);
-    load_rows(t_begin, ids[1], kbase, a.k_page, a.k_row, kofs, lds0);
-    load_ids(t_begin + 1, ids[0]);
+    if constexpr (CODES) {
+      load_ids(t_begin + 1, ids[0]);
+      load_exps(t_begin, ids[1], kexp, a.ke_page, ek);
+      load_exps(t_begin, ids[1], vexp, a.ve_page, ev);
+      load_rows(t_begin, ids[1], kbase, a.k_page, a.k_row, kofs, raw_k);
+      wait_all();
+      expand(raw_k, ek, lds0);
+      __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      load_exps(t_begin + 1, ids[0], kexp, a.ke_page, ek);
+      load_rows(t_begin, ids[1], vbase, a.v_page, a.v_row, vofs, raw_v);
+      if (t_begin + 1 < t_end) load_rows(t_begin + 1, ids[0], kbase, a.k_page, a.k_row, kofs, raw_k);
+      ids[1][0] = ids[0][0];
+      load_ids(t_begin + 2, ids[0]);
+    } else {
+      load_rows(t_begin, ids[1], kbase, a.k_page, a.k_row, kofs, lds0);
+      load_ids(t_begin + 1, ids[0]);
+    }
     for (int t = t_begin - 1; t < t_end; t += 2) {
       step(t, std::integral_constant<int, 0>{}, s[0], s[1]);
       if (t + 1 < t_end) step(t + 1, std::integral_constant<int, 1>{}, s[1], s[0]);
@@ -811,22 +1035,50 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   // Whether the row saw a key here: one of its tiles of this wave meets its interval.
   bool saw;
   {
-    const int from = max(t_begin, rr.lo / KT), to = min(t_end, (rr.hi + KT - 1) / KT);
-    saw = from + (FEW ? (wave - (from - t_begin)) & (WAVES - 1) : 0) < to;
+    auto meets = [&](int from, int to) __attribute__((always_inline)) {
+      from = max(t_begin, from);
+      to = min(t_end, to);
+      return from + (FEW ? (wave - (from - t_begin)) & (WAVES - 1) : 0) < to;
+    };
+    if constexpr (SINKS) {
+      const int shift = with_window ? ahead : kept_tile;
+      saw = meets(rr.lo / KT - ahead, (rr.hi + KT - 1) / KT - ahead) ||
+            (rr.slo < rr.shi && meets(rr.slo / KT - shift, (rr.shi + KT - 1) / KT - shift));
+    } else {
+      saw = meets(rr.lo / KT, (rr.hi + KT - 1) / KT);
+    }
   }
   const bool far = !MODS && m != M_FLOOR && !(fabsf(m2) < FAR);
   wait_all();
-  if (__syncthreads_or(lacking || far || check != 0.0f)) {
+  bool again = lacking || far || check != 0.0f;
+  if constexpr (CODES && !FEW) {  // in LDS of its own: the reduction's would be more than two workgroups have
+    __syncthreads();
+    const bool any = __builtin_amdgcn_ballot_w64(again) != 0;
+    if (lane == 0) bounds[wave] = any;
+    __syncthreads();
+    again = (bounds[0] | bounds[1] | bounds[2] | bounds[3]) != 0;
+    if (again) __syncthreads();
+  } else {
+    again = __syncthreads_or(again);
+  }
+  if (again) {
     saw = false;
     start();
     for (int t = t_begin; t < t_end; ++t) {
       if (FEW && ((t - t_begin) & (WAVES - 1)) != wave_s) continue;
       load_ids(t, ids[0]);
-      load_rows(t, ids[0], kbase, a.k_page, a.k_row, kofs, lds0);
-      load_rows(t, ids[0], vbase, a.v_page, a.v_row, vofs, lds0 + VTILE);
+      load_exps(t, ids[0], kexp, a.ke_page, ek);
+      load_exps(t, ids[0], vexp, a.ve_page, ev);
+      load_rows(t, ids[0], kbase, a.k_page, a.k_row, kofs, CODES ? raw_k : lds0);
+      load_rows(t, ids[0], vbase, a.v_page, a.v_row, vofs, CODES ? raw_v : lds0 + VTILE);
       wait_all();
+      if constexpr (CODES) {
+        expand(raw_k, ek, lds0);
+        expand(raw_v, ev, lds0 + VTILE);
+        wait_all();
+      }
       if constexpr (!FEW) gemm::stage_barrier();
-      if (t >= first && t < last) {
+      if (mine(t)) {
         uint32_t sees;
         product(s[0], 0, s[1], false);
         finish(s[0], t, careful, sees);
@@ -895,7 +1147,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
       for (int i = 0; i < WAVES; ++i) add_up(i, careful);
     }
     int t_out, h_out;
-    range_of<KEYS>(a, p, row0 + r, t_out, h_out);
+    range_of<KEYS, SINKS>(a, p, row0 + r, t_out, h_out);
     lost = lost && total == 0.0f;
     if (a.splits > 1) {
       const int64_t at = (int64_t{p.split} * a.tokens + t_out) * a.heads + h_out;
@@ -1078,34 +1330,45 @@ inline int plan_splits(bool paged, int64_t tokens, int group, int kv_heads, int6
   return static_cast<int>(n < 1 ? 1 : n > 64 ? 64 : n);
 }
 
-template <int DT, int D, int KEYS>
+// The second launch of a call in key splits (attention.hip).
+int launch_join(const Args& a, int dtype, int head_dim, hipStream_t st);
+
+template <int DT, int D, int KEYS, bool SINKS, int CODES>
 int launch(Args& a, hipStream_t st) {
   const bool mods = a.softcap > 0.0f || a.slopes;
-  const Plan p = plan(KEYS != DENSE, a.tokens, a.group, a.kv_heads, a.sequences, a.keys, device_cus());
+  const Plan p = plan(KEYS != DENSE, a.tokens, a.group, a.kv_heads, a.sequences, a.reach, device_cus());
   a.slots = p.slots;
   a.cus = device_cus();
   a.spread = a.kv_heads % 8 != 0 && (KEYS != DENSE || a.causal || a.starts);
   const int64_t blocks = int64_t{a.slots} * a.kv_heads * a.splits;
   M5K_REQUIRE(blocks <= INT32_MAX, "attention: too many tiles for one launch");
-  auto kernel = p.few ? (mods ? attention_tile<DT, D, KEYS, true, true> : attention_tile<DT, D, KEYS, false, true>)
-                      : (mods ? attention_tile<DT, D, KEYS, true, false> : attention_tile<DT, D, KEYS, false, false>);
+  auto kernel = p.few ? (mods ? attention_tile<DT, D, KEYS, true, true, SINKS, CODES>
+                              : attention_tile<DT, D, KEYS, false, true, SINKS, CODES>)
+                      : (mods ? attention_tile<DT, D, KEYS, true, false, SINKS, CODES>
+                              : attention_tile<DT, D, KEYS, false, false, SINKS, CODES>);
   launch_kernel(kernel, dim3(static_cast<uint32_t>(blocks)), dim3(THREADS), st, a);
   int rc = launch_status("attention");
   if (rc != M5K_OK || a.splits == 1) return rc;
-  const int64_t rows = int64_t{a.tokens} * a.heads;
-  if (a.splits > 8)
-    launch_kernel(attention_join<DT, D, 4>, dim3(static_cast<uint32_t>(rows)), dim3(256), st, a);
-  else
-    launch_kernel(attention_join<DT, D, 1>, dim3(static_cast<uint32_t>((rows + 3) / 4)), dim3(256), st, a);
-  return launch_status("attention join");
+  return launch_join(a, DT, D, st);
 }
 
-template <int KEYS>
-int launch_typed(Args& a, int dtype, int head_dim, hipStream_t st) {
-  if (dtype == M5K_BF16)
-    return head_dim == 64 ? launch<M5K_BF16, 64, KEYS>(a, st) : launch<M5K_BF16, 128, KEYS>(a, st);
-  return head_dim == 64 ? launch<M5K_F16, 64, KEYS>(a, st) : launch<M5K_F16, 128, KEYS>(a, st);
-}
+// One translation unit each (attention_*.hip), so that they compile side by side.
+template <int KEYS, bool SINKS, int CODES>
+int launch_typed(Args& a, int dtype, int head_dim, hipStream_t st);
+
+#define M5K_ATTENTION_UNIT(KEYS, SINKS, CODES)                                                          \
+  namespace m5k {                                                                                       \
+  namespace attn {                                                                                      \
+  template <>                                                                                           \
+  int launch_typed<KEYS, SINKS, CODES>(Args & a, int dtype, int head_dim, hipStream_t st) {             \
+    if (dtype == M5K_BF16)                                                                              \
+      return head_dim == 64 ? launch<M5K_BF16, 64, KEYS, SINKS, CODES>(a, st)                           \
+                            : launch<M5K_BF16, 128, KEYS, SINKS, CODES>(a, st);                         \
+    return head_dim == 64 ? launch<M5K_F16, 64, KEYS, SINKS, CODES>(a, st)                              \
+                          : launch<M5K_F16, 128, KEYS, SINKS, CODES>(a, st);                            \
+  }                                                                                                     \
+  }                                                                                                     \
+  }
 
 inline void magic_of(uint32_t d, uint32_t& magic, uint32_t& shift) {
   shift = 0;

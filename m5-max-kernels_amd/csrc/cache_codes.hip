@@ -1,0 +1,568 @@
+// A paged cache in 8 bits: written as it is quantised, and read back.
+//
+// A block of up to 128 tokens of one head shares a power of two 2^e: the least that brings the block's largest
+// magnitude to Q or below (Q = 448 for E4M3, 127 for INT8).  x 2^-e is exact, so that a code, the nearest of its format
+// with ties to even, depends on nothing but the value and e, and code 2^e is exact in BF16.  A power of two costs E4M3
+// nothing (its relative step is the same everywhere) and INT8 up to one bit of eight.
+//
+// Append.  A workgroup has one block of one operand and walks over heads: 8 channels a thread and pass, all of the
+// block's rows in its registers between the maximum and the codes, so that each value is read once.  Only the block
+// that a sequence's first new token falls into can hold older ones; it keeps the larger exponent, and where that grows
+// the old codes are rounded again under it.  Keys are turned in 64 bits: in 32, about one code in 10^6, next to a
+// border, would be another one than the formula's.  The result enters FP32 rounded to odd, which a second rounding to
+// fewer bits cannot tell from the 64-bit number.  Sines and cosines stand in LDS for all heads of the walk.
+#include "attention_place.h"
+#include "m5k_common.h"
+
+namespace m5k {
+namespace {
+
+constexpr int THREADS = 256;
+constexpr int BLOCK_MAX = 128;  // tokens of a block
+
+// ---- codes ----------------------------------------------------------------------------------------
+
+// Exponent byte of a block whose largest magnitude is `top`, infinity where a value is not finite.  Q = m 2^k: the
+// mantissa of `top` above m's carries into the exponent.
+template <int MODE>
+__device__ __forceinline__ int exponent_of(float top) {
+  if (top == __builtin_inff()) return 255;
+  constexpr uint32_t MANTISSA = MODE == M5K_QUANT_FP8 ? 0x600000u : 0x7E0000u;  // 1.75 2^8, 1.984375 2^6
+  constexpr int K = MODE == M5K_QUANT_FP8 ? 8 : 6;
+  const int e = static_cast<int>((__float_as_uint(top) + (0x7FFFFFu - MANTISSA)) >> 23) - K;
+  return e < 0 ? 0 : e;
+}
+
+// 2^(127 - byte) and 2^(byte - 127).
+__device__ __forceinline__ float unit_of(int byte) {
+  return __uint_as_float(byte >= 254 ? 0x00400000u : static_cast<uint32_t>(254 - byte) << 23);
+}
+__device__ __forceinline__ float scale_of(int byte) {
+  return __uint_as_float(byte == 0 ? 0x00400000u : byte == 255 ? 0x7FC00000u : static_cast<uint32_t>(byte) << 23);
+}
+
+// Codes of 8 values whose magnitudes are at most Q.
+template <int MODE>
+__device__ __forceinline__ uint2 encode8(const float (&x)[8]) {
+  uint32_t w[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if constexpr (MODE == M5K_QUANT_FP8) {
+      int c = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i], x[4 * i + 1], 0, false);
+      w[i] = static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2], x[4 * i + 3], c, true));
+    } else {
+      uint32_t t[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) t[j] = __float_as_uint(x[4 * i + j] + 0x1.8p23f);  // a whole number, ties to even
+      w[i] = __builtin_amdgcn_perm(t[1], t[0], 0x0C0C0400u) | __builtin_amdgcn_perm(t[3], t[2], 0x04000C0Cu);
+    }
+  }
+  return make_uint2(w[0], w[1]);
+}
+
+// What 4 codes stand for before their scale.
+template <int MODE>
+__device__ __forceinline__ void decode4(uint32_t w, float (&x)[4]) {
+  if constexpr (MODE == M5K_QUANT_FP8) {
+    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w), false);
+    const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w), true);
+    x[0] = lo[0];
+    x[1] = lo[1];
+    x[2] = hi[0];
+    x[3] = hi[1];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = static_cast<float>(static_cast<int>(w << (24 - 8 * j)) >> 24);
+  }
+}
+
+// ---- turns ----------------------------------------------------------------------------------------
+
+// Cosine and sine of a, times magnitude, to a few units of 64 bits' last place while a stays below 2^30: the nearest
+// multiple of pi / 2 taken off in two parts, Taylor series of the rest (first terms left out below 1e-17).
+__device__ __forceinline__ double2 turn64(double a, double magnitude) {
+  const double q = rint(a * 0.63661977236758134308);  // 2 / pi
+  double r = __builtin_fma(-q, 1.57079632679489655800, a);
+  r = __builtin_fma(-q, 6.12323399573676603587e-17, r);
+  const double z = r * r;
+  double s = 1.0 / 355687428096000.0;
+  s = __builtin_fma(z, s, -1.0 / 1307674368000.0);
+  s = __builtin_fma(z, s, 1.0 / 6227020800.0);
+  s = __builtin_fma(z, s, -1.0 / 39916800.0);
+  s = __builtin_fma(z, s, 1.0 / 362880.0);
+  s = __builtin_fma(z, s, -1.0 / 5040.0);
+  s = __builtin_fma(z, s, 1.0 / 120.0);
+  s = __builtin_fma(z, s, -1.0 / 6.0);
+  s = __builtin_fma(r * z, s, r);
+  double c = 1.0 / 20922789888000.0;
+  c = __builtin_fma(z, c, -1.0 / 87178291200.0);
+  c = __builtin_fma(z, c, 1.0 / 479001600.0);
+  c = __builtin_fma(z, c, -1.0 / 3628800.0);
+  c = __builtin_fma(z, c, 1.0 / 40320.0);
+  c = __builtin_fma(z, c, -1.0 / 720.0);
+  c = __builtin_fma(z, c, 1.0 / 24.0);
+  c = __builtin_fma(z, c, -0.5);
+  c = __builtin_fma(z, c, 1.0);
+  const int quarter = static_cast<int>(static_cast<int64_t>(q) & 3);
+  const double cosine = quarter & 1 ? s : c, sine = quarter & 1 ? c : s;
+  return make_double2(quarter == 1 || quarter == 2 ? -cosine * magnitude : cosine * magnitude,
+                      quarter >= 2 ? -sine * magnitude : sine * magnitude);
+}
+
+// FP32 rounded to odd: cut off, with the last bit set where anything was.
+__device__ __forceinline__ float round_to_odd(double v) {
+  const float f = static_cast<float>(v);
+  const double back = f;
+  if (!(fabs(v) < __builtin_inf()) || back == v) return f;
+  const uint32_t u = __float_as_uint(f);
+  return __uint_as_float((u - (fabs(back) > fabs(v) ? 1u : 0u)) | 1u);
+}
+
+// ---- append ---------------------------------------------------------------------------------------
+
+struct Operand {
+  const void* src;
+  uint8_t *codes, *exps;
+  int64_t src_head, src_token, page, head, slot, exp_page, exp_head;
+};
+
+struct AppendArgs {
+  Operand op[2];  // K, V
+  const void* q;
+  void* q_out;
+  int64_t q_head, q_token;
+  const int32_t *table, *starts, *context;
+  const double* frequencies;
+  int64_t table_width;
+  int tokens, kv_heads, heads, pairs, interleaved, sequences, pages, page_size, block, walk, groups, slots;
+  double magnitude;
+};
+
+// First block slot of a sequence: it owns floor(n / block) + 2 slots for its n tokens at least, and they touch no more
+// blocks than that, wherever the first one falls.
+__device__ __forceinline__ int first_block_slot(const AppendArgs& a, int b) {
+  return attn::start_of(a.starts, b, a.tokens) / a.block + 2 * b;
+}
+
+// Channels c0 .. c0 + 7 of a row, turned: `turns` holds the row's cosines and sines a pair.  put(i, own, other, turn,
+// turns) gets each channel, its partner, and what they are multiplied by.
+template <int DT, class F>
+__device__ __forceinline__ void turned8(const void* src, int64_t row, int c0, const double2* turns, int pairs,
+                                        bool interleaved, const float (&x)[8], F put) {
+  float other[8];
+  if (interleaved) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) other[i] = x[i ^ 1];
+  } else if (pairs % 8 == 0) {  // a chunk's partners are a chunk
+    if (c0 < 2 * pairs) load8<DT>(src, row + (c0 < pairs ? c0 + pairs : c0 - pairs), other);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int d = c0 + i;
+      other[i] = d < 2 * pairs ? load_elem<DT>(src, row + (d < pairs ? d + pairs : d - pairs)) : 0.0f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int d = c0 + i;
+    if (d >= 2 * pairs) {
+      put(i, x[i], 0.0f, make_double2(1.0, 0.0), false);
+    } else {
+      const double2 t = turns[interleaved ? d >> 1 : d < pairs ? d : d - pairs];
+      put(i, x[i], other[i], make_double2(t.x, (interleaved ? i & 1 : d >= pairs) ? t.y : -t.y), true);
+    }
+  }
+}
+
+// 8 values as DT at element `at`, 16-byte aligned.
+template <int DT>
+__device__ __forceinline__ void store8(void* p, int64_t at, const float (&x)[8]) {
+  if constexpr (DT == M5K_F32) {
+    float4* d = reinterpret_cast<float4*>(static_cast<float*>(p) + at);
+    d[0] = make_float4(x[0], x[1], x[2], x[3]);
+    d[1] = make_float4(x[4], x[5], x[6], x[7]);
+  } else {
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (DT == M5K_BF16) u[i] = f32x2_to_bf16x2(x[2 * i], x[2 * i + 1]);
+      else u[i] = f32_to_f16_bits(x[2 * i]) | (f32_to_f16_bits(x[2 * i + 1]) << 16);
+    }
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + at) = make_uint4(u[0], u[1], u[2], u[3]);
+  }
+}
+
+// PASSES: passes of THREADS threads over the block's rows.  TURNED: K and Q are turned.
+template <int DT, int D, int MODE, int PASSES, bool TURNED>
+__global__ __launch_bounds__(THREADS) void append_codes(const AppendArgs a) {
+  constexpr int CH = D / 8, RPP = THREADS / CH;  // 8-channel chunks of a row, rows of a pass
+  __shared__ double2 turns[TURNED ? PASSES * RPP * (D / 2) : 1];
+  __shared__ float tops[2][4];
+  const int tid = threadIdx.x, c0 = tid % CH * 8, row = tid / CH;
+  const int role = blockIdx.y / a.groups < 2 ? blockIdx.y / a.groups : 2;  // K, V, Q
+  const int walk0 = (blockIdx.y - role * a.groups) * a.walk;
+  const int head1 = min(walk0 + a.walk, role == 2 ? a.heads : a.kv_heads);
+
+  if (role == 2) {
+    // Rows of q by token; those behind the last sequence are 0.
+    if constexpr (TURNED) {
+      const int token0 = blockIdx.x * (PASSES * RPP);
+      if (token0 >= a.tokens) return;
+      for (int i = tid; i < PASSES * RPP * a.pairs; i += THREADS) {
+        const int r = i / a.pairs, token = token0 + r;
+        if (token >= a.tokens) break;
+        int lo = 0, hi = a.sequences;
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (a.starts[mid] <= token) lo = mid;
+          else hi = mid;
+        }
+        const int s = a.starts[lo], e = a.starts[lo + 1];
+        const bool known = token >= s && token < e;
+        const double position = known ? a.context[lo] - (e - token) : 0;
+        const double2 turn = turn64(position * a.frequencies[i - r * a.pairs], a.magnitude);
+        turns[i] = known ? turn : make_double2(__builtin_nan(""), 0.0);
+      }
+      __syncthreads();
+      for (int h = walk0; h < head1; ++h) {
+#pragma unroll
+        for (int pass = 0; pass < PASSES; ++pass) {
+          const int r = pass * RPP + row, token = token0 + r;
+          if (token >= a.tokens) continue;
+          const double2* t = turns + r * a.pairs;
+          const bool known = t[0].x == t[0].x;
+          const int64_t at = h * a.q_head + token * a.q_token;
+          float x[8], y[8];
+          load8<DT>(a.q, at + c0, x);
+          turned8<DT>(a.q, at, c0, t, a.pairs, a.interleaved, x,
+                      [&](int i, float own, float other, double2 u, bool turn) {
+            y[i] = !known ? 0.0f : turn ? own * static_cast<float>(u.x) + other * static_cast<float>(u.y) : own;
+          });
+          store8<DT>(a.q_out, (int64_t{h} * a.tokens + token) * D + c0, y);
+        }
+      }
+    }
+    return;
+  }
+
+  const Operand& op = a.op[role];
+  const int slot = blockIdx.x;
+  if (slot >= a.slots) return;
+  const auto probes = [&](int lo, int left, int apart) {
+    const int probe = (tid & 63) * apart;
+    const bool below = probe < left && first_block_slot(a, lo + probe) <= slot;
+    return __popcll(__builtin_amdgcn_ballot_w64(below));
+  };
+  const int b = __builtin_amdgcn_readfirstlane(attn::sequence_of_slot(a.sequences, probes));
+  const int n = attn::tokens_of(a.starts, b, a.sequences, a.tokens), context = a.context[b];
+  if (n == 0 || context <= 0) return;
+  const int start = attn::start_of(a.starts, b, a.tokens), p_new = context - n;  // position of the first new token
+  const int p0 = max(p_new, 0), tile = slot - first_block_slot(a, b);
+  const int base = (p0 / a.block + tile) * a.block;  // position of the block's first token
+  if (tile < 0 || base < 0 || base >= context || base / a.page_size >= a.table_width) return;
+  const int page = a.table[b * a.table_width + base / a.page_size];
+  if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.pages)) return;
+  const int slot0 = base % a.page_size;
+  const bool has_old = base < p_new;
+  const bool turn = TURNED && role == 0;
+  if constexpr (TURNED) {
+    if (turn) {
+      for (int i = tid; i < a.block * a.pairs; i += THREADS) {
+        const int r = i / a.pairs, p = base + r;
+        if (p < p0 || p >= context) continue;
+        turns[i] = turn64(static_cast<double>(p) * a.frequencies[i - r * a.pairs], a.magnitude);
+      }
+      __syncthreads();
+    }
+  }
+  for (int h = walk0; h < head1; ++h) {
+    uint8_t* exp = op.exps + page * op.exp_page + h * op.exp_head + slot0 / a.block;
+    uint8_t* codes = op.codes + page * op.page + h * op.head + slot0 * op.slot + c0;
+    const int before = has_old ? *exp : 0;
+    float x[PASSES][8], top = 0.0f;
+#pragma unroll
+    for (int pass = 0; pass < PASSES; ++pass) {
+      const int r = pass * RPP + row, p = base + r;
+      if (r >= a.block || p < p0 || p >= context) continue;
+      const int64_t at = h * op.src_head + (start + (p - p_new)) * op.src_token;
+      load8<DT>(op.src, at + c0, x[pass]);
+      if constexpr (TURNED) {
+        if (turn) {
+          float y[8];
+          turned8<DT>(op.src, at, c0, turns + r * a.pairs, a.pairs, a.interleaved, x[pass],
+                      [&](int i, float own, float other, double2 u, bool turns_it) {
+                        y[i] = turns_it ? round_to_odd(__builtin_fma(static_cast<double>(own), u.x, other * u.y)) : own;
+                      });
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[pass][i] = y[i];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        top = fmaxf(top, fabsf(x[pass][i]) < __builtin_inff() ? fabsf(x[pass][i]) : __builtin_inff());
+    }
+    top = wave_max(top);
+    if ((tid & 63) == 0) tops[h & 1][tid >> 6] = top;
+    __syncthreads();  // the other slot is written behind the next head's barrier at the earliest
+    top = fmaxf(fmaxf(tops[h & 1][0], tops[h & 1][1]), fmaxf(tops[h & 1][2], tops[h & 1][3]));
+    const int after = max(exponent_of<MODE>(top), before);
+    const float unit = unit_of(after);
+#pragma unroll
+    for (int pass = 0; pass < PASSES; ++pass) {
+      const int r = pass * RPP + row, p = base + r;
+      if (r >= a.block || p >= context) continue;
+      uint2* to = reinterpret_cast<uint2*>(codes + r * op.slot);
+      float y[8];
+      if (p >= p0) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = after == 255 ? 0.0f : x[pass][i] * unit;
+      } else {
+        if (after == before || after == 255) continue;
+        const uint2 w = *to;
+        float lo[4], hi[4];
+        decode4<MODE>(w.x, lo);
+        decode4<MODE>(w.y, hi);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = __builtin_ldexpf(i < 4 ? lo[i & 3] : hi[i & 3], before - after);
+      }
+      *to = encode8<MODE>(y);
+    }
+    if (tid == 0) *exp = static_cast<uint8_t>(after);
+  }
+}
+
+// ---- read -----------------------------------------------------------------------------------------
+
+struct ReadArgs {
+  const uint8_t *codes[2], *exps[2];
+  int64_t page[2], head[2], slot[2], exp_page[2], exp_head[2];
+  void* out[2];
+  const int32_t *table, *starts, *context;
+  int64_t table_width;
+  int tokens, kv_heads, sequences, pages, page_size, block, walk, groups;
+};
+
+// A thread has 16 channels of one token and walks over heads: 16 bytes in, 16 values out.  Memory bound.
+template <int DT, int D, int MODE>
+__global__ __launch_bounds__(THREADS) void read_codes(const ReadArgs a) {
+  constexpr int CH = D / 16;
+  const int64_t unit = int64_t{blockIdx.x} * THREADS + threadIdx.x;
+  const int token = static_cast<int>(unit / CH), c0 = static_cast<int>(unit % CH) * 16;
+  if (token >= a.tokens) return;
+  const int which = blockIdx.y >= a.groups, head0 = (blockIdx.y - which * a.groups) * a.walk;
+  const int head1 = min(head0 + a.walk, a.kv_heads);
+  int lo = 0, hi = a.sequences;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a.starts[mid] <= token) lo = mid;
+    else hi = mid;
+  }
+  const int s = a.starts[lo], e = a.starts[lo + 1];
+  bool known = token >= s && token < e;
+  const int position = known ? a.context[lo] - (e - token) : -1;
+  const int page_at = position / a.page_size;
+  known = known && position >= 0 && page_at < a.table_width;
+  const int page = known ? a.table[lo * a.table_width + page_at] : -1;
+  known = known && static_cast<uint32_t>(page) < static_cast<uint32_t>(a.pages);
+  const int at = position - page_at * a.page_size;
+  for (int h = head0; h < head1; ++h) {
+    uint4 w = make_uint4(0, 0, 0, 0);
+    float scale = 0.0f;
+    if (known) {
+      w = *reinterpret_cast<const uint4*>(a.codes[which] + page * a.page[which] + h * a.head[which] +
+                                          at * a.slot[which] + c0);
+      scale = scale_of(a.exps[which][page * a.exp_page[which] + h * a.exp_head[which] + at / a.block]);
+    }
+    float x[2][8];
+    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float v[4];
+      decode4<MODE>(words[i], v);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[i >> 1][4 * (i & 1) + j] = v[j] * scale;
+    }
+    const int64_t to = (int64_t{h} * a.tokens + token) * D + c0;
+    store8<DT>(a.out[which], to, x[0]);
+    store8<DT>(a.out[which], to + 8, x[1]);
+  }
+}
+
+// ---- launches -------------------------------------------------------------------------------------
+
+int walk_of(int64_t workgroups, int heads) {
+  // Heads a workgroup: as many as leave the chip about eight workgroups a compute unit.
+  const int64_t w = workgroups * heads / (8 * 256);
+  return static_cast<int>(w < 1 ? 1 : w > 8 ? 8 : w);
+}
+
+template <int DT, int D, int MODE, int PASSES>
+int append_passes(AppendArgs& a, hipStream_t st) {
+  constexpr int ROWS = PASSES * THREADS / (D / 8);
+  a.slots = a.tokens / a.block + 2 * a.sequences;
+  a.walk = walk_of(int64_t{a.tokens} / a.block + a.sequences, 2 * a.kv_heads + a.heads);
+  a.groups = (a.kv_heads + a.walk - 1) / a.walk;
+  const int q_groups = (a.heads + a.walk - 1) / a.walk, q_slots = a.heads ? (a.tokens + ROWS - 1) / ROWS : 0;
+  const dim3 grid(static_cast<uint32_t>(a.slots > q_slots ? a.slots : q_slots),
+                  static_cast<uint32_t>(2 * a.groups + q_groups));
+  M5K_REQUIRE(grid.y <= 65535, "paged_append: too many heads for one launch");
+  auto kernel = a.pairs ? append_codes<DT, D, MODE, PASSES, true> : append_codes<DT, D, MODE, PASSES, false>;
+  launch_kernel(kernel, grid, dim3(THREADS), st, a);
+  return launch_status("paged_append");
+}
+
+template <int DT, int D, int MODE>
+int append_block(AppendArgs& a, hipStream_t st) {
+  const int rows = THREADS / (D / 8);
+  if (a.block <= rows) return append_passes<DT, D, MODE, 1>(a, st);
+  if (a.block <= 2 * rows) return append_passes<DT, D, MODE, 2>(a, st);
+  if (a.block <= 4 * rows) return append_passes<DT, D, MODE, 4>(a, st);
+  if constexpr (D == 128) return append_passes<DT, D, MODE, 8>(a, st);
+  return M5K_EINVAL;
+}
+
+template <int DT>
+int append_typed(AppendArgs& a, int mode, int head_dim, hipStream_t st) {
+  if (mode == M5K_QUANT_FP8)
+    return head_dim == 64 ? append_block<DT, 64, M5K_QUANT_FP8>(a, st) : append_block<DT, 128, M5K_QUANT_FP8>(a, st);
+  return head_dim == 64 ? append_block<DT, 64, M5K_QUANT_INT8>(a, st) : append_block<DT, 128, M5K_QUANT_INT8>(a, st);
+}
+
+template <int DT>
+int read_typed(const ReadArgs& a, int mode, int head_dim, hipStream_t st) {
+  const int64_t blocks = (int64_t{a.tokens} * (head_dim / 16) + THREADS - 1) / THREADS;
+  const dim3 grid(static_cast<uint32_t>(blocks), static_cast<uint32_t>(2 * a.groups));
+  auto kernel = mode == M5K_QUANT_FP8
+                    ? (head_dim == 64 ? read_codes<DT, 64, M5K_QUANT_FP8> : read_codes<DT, 128, M5K_QUANT_FP8>)
+                    : (head_dim == 64 ? read_codes<DT, 64, M5K_QUANT_INT8> : read_codes<DT, 128, M5K_QUANT_INT8>);
+  launch_kernel(kernel, grid, dim3(THREADS), st, a);
+  return launch_status("paged_read");
+}
+
+int check_cache(const char* what, int mode, int64_t head_dim, const void* k, const void* v, const void* ke,
+                const void* ve, const int64_t (&strides)[6], int64_t block, int64_t pages, int64_t page_size,
+                int64_t kv_heads, const int32_t* table, int64_t table_width, int64_t sequences, const int32_t* starts,
+                const int32_t* context, int64_t tokens) {
+  M5K_REQUIRE(k && v && ke && ve && table && starts && context, "%s: null pointer", what);
+  M5K_REQUIRE(mode == M5K_QUANT_FP8 || mode == M5K_QUANT_INT8, "%s: codes must be FP8 or INT8", what);
+  M5K_REQUIRE(head_dim == 64 || head_dim == 128, "%s: head_dim must be 64 or 128", what);
+  M5K_REQUIRE(kv_heads > 0 && kv_heads <= 16384, "%s: bad number of heads", what);
+  M5K_REQUIRE(pages > 0 && pages <= INT32_MAX && page_size > 0 && page_size <= (1 << 20) && table_width > 0 &&
+                  table_width * page_size <= (1 << 30) && sequences > 0 && sequences <= (1 << 24),
+              "%s: a sequence may have up to 2^30 keys in pages of up to 2^20", what);
+  M5K_REQUIRE(block > 0 && block <= BLOCK_MAX && block % 16 == 0 && page_size % block == 0,
+              "%s: a block must be 16 to 128 tokens, a multiple of 16, and divide the page", what);
+  M5K_REQUIRE(tokens > 0 && tokens <= (1 << 28), "%s: bad number of tokens", what);
+  bool rows = aligned16(k) && aligned16(v);
+  for (int64_t s : strides) rows = rows && s % 16 == 0;
+  M5K_REQUIRE(rows, "%s: rows of codes must be 16-byte aligned", what);
+  return M5K_OK;
+}
+
+}  // namespace
+}  // namespace m5k
+
+extern "C" int m5k_paged_append_codes(
+    const void* k, int64_t k_head, int64_t k_token, const void* v, int64_t v_head, int64_t v_token, int dtype,
+    int64_t tokens, int64_t kv_heads, int64_t head_dim, int mode, void* k_codes, int64_t kc_page, int64_t kc_head,
+    int64_t kc_slot, uint8_t* k_exponents, int64_t ke_page, int64_t ke_head, void* v_codes, int64_t vc_page,
+    int64_t vc_head, int64_t vc_slot, uint8_t* v_exponents, int64_t ve_page, int64_t ve_head, int64_t block,
+    int64_t pages, int64_t page_size, const int32_t* page_table, int64_t table_width, int64_t sequences,
+    const int32_t* query_starts, const int32_t* context_lengths, const void* q, int64_t heads, int64_t q_head,
+    int64_t q_token, void* q_out, const double* frequencies, int64_t pairs, int interleaved, float magnitude,
+    void* stream) {
+  using namespace m5k;
+  clear_error();
+  M5K_REQUIRE(dtype == M5K_F32 || dtype == M5K_F16 || dtype == M5K_BF16,
+              "paged_append: dtype must be f32, f16 or bf16");
+  if (int rc = check_cache("paged_append", mode, head_dim, k_codes, v_codes, k_exponents, v_exponents,
+                           {kc_page, kc_head, kc_slot, vc_page, vc_head, vc_slot}, block, pages, page_size, kv_heads,
+                           page_table, table_width, sequences, query_starts, context_lengths, tokens))
+    return rc;
+  M5K_REQUIRE(k && v, "paged_append: null pointer");
+  M5K_REQUIRE(pairs >= 0 && 2 * pairs <= head_dim && (pairs == 0 || frequencies),
+              "paged_append: 2 * pairs must fit in head_dim");
+  M5K_REQUIRE(!q || (q_out && heads > 0 && heads <= 16384 && pairs > 0),
+              "paged_append: q needs q_out, heads and a rotation");
+  const int64_t unit = dtype == M5K_F32 ? 4 : 8;
+  M5K_REQUIRE(aligned16(k) && aligned16(v) && k_head % unit == 0 && k_token % unit == 0 && v_head % unit == 0 &&
+                  v_token % unit == 0 && (!q || (aligned16(q) && q_head % unit == 0 && q_token % unit == 0)),
+              "paged_append: rows must be 16-byte aligned");
+  AppendArgs a = {};
+  a.op[0] = Operand{k,       static_cast<uint8_t*>(k_codes), k_exponents, k_head, k_token, kc_page, kc_head, kc_slot,
+                    ke_page, ke_head};
+  a.op[1] = Operand{v,       static_cast<uint8_t*>(v_codes), v_exponents, v_head, v_token, vc_page, vc_head, vc_slot,
+                    ve_page, ve_head};
+  a.q = q;
+  a.q_out = q_out;
+  a.q_head = q_head;
+  a.q_token = q_token;
+  a.table = page_table;
+  a.starts = query_starts;
+  a.context = context_lengths;
+  a.frequencies = frequencies;
+  a.table_width = table_width;
+  a.tokens = static_cast<int>(tokens);
+  a.kv_heads = static_cast<int>(kv_heads);
+  a.heads = q ? static_cast<int>(heads) : 0;
+  a.pairs = static_cast<int>(pairs);
+  a.interleaved = interleaved != 0;
+  a.sequences = static_cast<int>(sequences);
+  a.pages = static_cast<int>(pages);
+  a.page_size = static_cast<int>(page_size);
+  a.block = static_cast<int>(block);
+  a.magnitude = magnitude;
+  const int dim = static_cast<int>(head_dim);
+  if (dtype == M5K_BF16) return append_typed<M5K_BF16>(a, mode, dim, as_stream(stream));
+  if (dtype == M5K_F16) return append_typed<M5K_F16>(a, mode, dim, as_stream(stream));
+  return append_typed<M5K_F32>(a, mode, dim, as_stream(stream));
+}
+
+extern "C" int m5k_paged_read(int mode, const void* k_codes, int64_t kc_page, int64_t kc_head, int64_t kc_slot,
+                              const uint8_t* k_exponents, int64_t ke_page, int64_t ke_head, const void* v_codes,
+                              int64_t vc_page, int64_t vc_head, int64_t vc_slot, const uint8_t* v_exponents,
+                              int64_t ve_page, int64_t ve_head, int64_t block, int64_t pages, int64_t page_size,
+                              int64_t kv_heads, int64_t head_dim, const int32_t* page_table, int64_t table_width,
+                              int64_t sequences, const int32_t* query_starts, const int32_t* context_lengths,
+                              int64_t tokens, void* k, void* v, int dtype, void* stream) {
+  using namespace m5k;
+  clear_error();
+  M5K_REQUIRE(dtype == M5K_F32 || dtype == M5K_F16 || dtype == M5K_BF16, "paged_read: dtype must be f32, f16 or bf16");
+  if (int rc = check_cache("paged_read", mode, head_dim, k_codes, v_codes, k_exponents, v_exponents,
+                           {kc_page, kc_head, kc_slot, vc_page, vc_head, vc_slot}, block, pages, page_size, kv_heads,
+                           page_table, table_width, sequences, query_starts, context_lengths, tokens))
+    return rc;
+  M5K_REQUIRE(k && v && aligned16(k) && aligned16(v), "paged_read: outputs must be 16-byte aligned");
+  ReadArgs a = {};
+  a.codes[0] = static_cast<const uint8_t*>(k_codes);
+  a.codes[1] = static_cast<const uint8_t*>(v_codes);
+  a.exps[0] = k_exponents;
+  a.exps[1] = v_exponents;
+  const int64_t strides[5][2] = {{kc_page, vc_page}, {kc_head, vc_head}, {kc_slot, vc_slot}, {ke_page, ve_page},
+                                 {ke_head, ve_head}};
+  for (int i = 0; i < 2; ++i) {
+    a.page[i] = strides[0][i];
+    a.head[i] = strides[1][i];
+    a.slot[i] = strides[2][i];
+    a.exp_page[i] = strides[3][i];
+    a.exp_head[i] = strides[4][i];
+  }
+  a.out[0] = k;
+  a.out[1] = v;
+  a.table = page_table;
+  a.starts = query_starts;
+  a.context = context_lengths;
+  a.table_width = table_width;
+  a.tokens = static_cast<int>(tokens);
+  a.kv_heads = static_cast<int>(kv_heads);
+  a.sequences = static_cast<int>(sequences);
+  a.pages = static_cast<int>(pages);
+  a.page_size = static_cast<int>(page_size);
+  a.block = static_cast<int>(block);
+  a.walk = walk_of((tokens * (head_dim / 16) + THREADS - 1) / THREADS, 2 * a.kv_heads);
+  a.groups = (a.kv_heads + a.walk - 1) / a.walk;
+  const int dim = static_cast<int>(head_dim);
+  if (dtype == M5K_BF16) return read_typed<M5K_BF16>(a, mode, dim, as_stream(stream));
+  if (dtype == M5K_F16) return read_typed<M5K_F16>(a, mode, dim, as_stream(stream));
+  return read_typed<M5K_F32>(a, mode, dim, as_stream(stream));
+}

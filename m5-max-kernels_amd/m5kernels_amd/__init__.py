@@ -2,7 +2,7 @@
 
 Python op contracts mirror the reference package ``m5kernels`` (quantize, gemm, rotate,
 ...) on torch tensors; the attention step that the projections feed (rope, paged_append,
-paged_attention, attention) stands beside them.  Every computation runs in libm5k.so,
+paged_read, paged_attention, attention) stands beside them.  Every computation runs in libm5k.so,
 hand-written HIP kernels behind a C ABI (include/m5k.h).  There is no CPU fallback.
 """
 
@@ -10,7 +10,7 @@ from .hip import gemm, gemm_i8_accumulators, quantize
 from .qk_rope import projection_qk_rope, projection_qkv_rope, qk_norm_rope
 from .hadamard import SUPPORTED_BLOCK_SIZES, rotate, rotate_quantize
 from .rms_quant import rms_quantize
-from .attention_ops import attention, paged_append, paged_attention, rope, rope_frequencies
+from .attention_ops import attention, paged_append, paged_attention, paged_read, rope, rope_frequencies
 from .chains import gate_chain, norm_shift_split_gemm, shift_split_condition
 from .norm_hadamard import (
     fused_gated_residual_norm_hadamard_quantize,
@@ -40,6 +40,7 @@ __all__ = [
     "rope_frequencies",
     "rope",
     "paged_append",
+    "paged_read",
     "paged_attention",
     "attention",
 ]

@@ -86,10 +86,30 @@ SIGNATURES = {
         _p, _i32, _i64, _i64, _i32, _i64, _i64, *_rows3, *_rows3, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _f32, _i64,
         _f32, _p, _p, _p, _i32, _p, _i64, _p,
     ],
+    "m5k_attention_sinks": [
+        _p, _i32, _i64, _i64, _i32, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _f32, _i32, _i64, _i64,
+        _f32, _p, _p, _i64, _p, _p, _i32, _p, _i64, _p,
+    ],
+    "m5k_paged_attention_sinks": [
+        _p, _i32, _i64, _i64, _i32, _i64, _i64, *_rows3, *_rows3, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _f32, _i64,
+        _i64, _f32, _p, _p, _p, _i32, _p, _i64, _p,
+    ],
+    "m5k_paged_attention_codes": [
+        _p, _i32, _i64, _i64, _i32, _i64, _i64, _i32, *_rows3, _p, _i64, _i64, *_rows3, _p, _i64, _i64, _i64, _i64,
+        _i64, _i64, _p, _i64, _i64, _p, _p, _f32, _i64, _i64, _f32, _p, _p, _p, _i32, _p, _i64, _p,
+    ],
     "m5k_rope": [_p, _i32, _i64, _i64, _i64, _i64, _i64, _p, _p, _i64, _i32, _f32, _p, _p],
     "m5k_paged_append": [
         _p, _i64, _i64, _p, _i64, _i64, _i32, _i64, _i64, _i64, *_rows3, *_rows3, _i64, _i64, _p, _i64, _i64, _p, _p,
         _p, _i64, _i64, _i64, _p, _p, _i64, _i32, _f32, _p,
+    ],
+    "m5k_paged_append_codes": [
+        _p, _i64, _i64, _p, _i64, _i64, _i32, _i64, _i64, _i64, _i32, *_rows3, _p, _i64, _i64, *_rows3, _p, _i64, _i64,
+        _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _i64, _i64, _i64, _p, _p, _i64, _i32, _f32, _p,
+    ],
+    "m5k_paged_read": [
+        _i32, *_rows3, _p, _i64, _i64, *_rows3, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p, _p,
+        _i64, _p, _p, _i32, _p,
     ],
 }
 
@@ -122,7 +142,8 @@ def load(path: Path | str | None = None) -> ctypes.CDLL:
 
 
 # What hip._NativeFront asks of the native front.
-FRONT_CALLS = ("bind", "quantize", "gemm", "qk", "qkv", "rope", "paged_append", "paged_attention", "attention")
+FRONT_CALLS = ("bind", "quantize", "gemm", "qk", "qkv", "rope", "paged_append", "paged_read", "paged_attention",
+               "attention")
 
 
 def load_fast():

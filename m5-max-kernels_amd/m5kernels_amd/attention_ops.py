@@ -12,6 +12,12 @@ from 0, says where each begins.  ``context_lengths`` int32 [sequences] counts th
 new tokens included, and ``page_table`` int32 [sequences, width] names the pages that hold them.  All of them stay on
 the device: a call reads no length back, so it can be captured into a graph and replayed with other lengths.
 Nothing is checked that only the device knows; the kernels stay inside every buffer whatever the values.
+
+A cache may be held in 8 bits: k_cache and v_cache are then codes, uint8 (E4M3) or int8 (in [-127, 127]), and k_scales
+and v_scales uint8 [pages, kv_heads, page_size / block] are the exponent bytes of the power-of-two scales (as
+quantize's "mxint8" has them) that the codes of `block` tokens of a page and head share: a code stands for
+code * 2^(byte - 127), under byte 255 for NaN.  A block is 16 to 128 tokens, a multiple of 16 that divides the page;
+heads are 64 or 128 wide.  paged_append writes such a cache, paged_read reads it back, paged_attention attends over it.
 """
 
 from __future__ import annotations
@@ -28,7 +34,9 @@ from . import _lib, hip
 _LAYOUTS = ("half", "interleaved")
 _HALF_DTYPES = (torch.float16, torch.bfloat16)
 _FLOAT_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
+_CODE_MODES = {torch.uint8: _lib.QUANT_FP8, torch.int8: _lib.QUANT_INT8}
 HEAD_DIMS = (64, 128)
+BLOCK_MAX = 128
 _WINDOW_MAX = (1 << 30) - 1
 _F32_LEAST = 2.0 ** -126
 _RATIO_MAX = 1e37  # scale / softcap: what a score is multiplied by before the cap's tanh, finite with its log2(e)
@@ -184,9 +192,9 @@ def rope(x, positions, frequencies, *, layout="half", magnitude=1.0):
     return y
 
 
-def _cache(t, name, like, kv_heads, width):
-    if not isinstance(t, torch.Tensor) or t.dim() != 4 or t.dtype != like.dtype:
-        raise ValueError(f"{name} must be a [pages, kv_heads, page_size, width] tensor of {like.dtype}")
+def _cache(t, name, dtype, kv_heads, width):
+    if not isinstance(t, torch.Tensor) or t.dim() != 4 or t.dtype != dtype:
+        raise ValueError(f"{name} must be a [pages, kv_heads, page_size, width] tensor of {dtype}")
     if t.shape[1] != kv_heads or t.shape[3] != width or not all(t.shape):
         raise ValueError(f"{name} must have nonempty shape [pages, {kv_heads}, page_size, {width}]")
     if not t.is_cuda:
@@ -195,6 +203,39 @@ def _cache(t, name, like, kv_heads, width):
     if t.stride(3) != 1:
         raise ValueError(f"{name} channels must be contiguous")
     return s
+
+
+def _aligned_rows(t, s, name):
+    unit = 16 // t.element_size()
+    if t.data_ptr() % 16 or any(x % unit for x in s[:3]):
+        raise ValueError(f"{name} rows must start at multiples of 16 bytes")
+
+
+def _codes(k_cache, v_cache, k_scales, v_scales):
+    """Of a cache in 8 bits: its mode, block and scales' strides, checked; None for one in 16 or 32."""
+    if k_scales is None and v_scales is None:
+        return None
+    for t, scales, name in ((k_cache, k_scales, "k"), (v_cache, v_scales, "v")):
+        if not isinstance(t, torch.Tensor) or t.dim() != 4 or t.dtype not in _CODE_MODES or not all(t.shape):
+            raise ValueError(f"{name}_cache with scales must be a nonempty [pages, kv_heads, page_size, width] tensor "
+                             "of uint8 or int8 codes")
+        if not isinstance(scales, torch.Tensor) or scales.dim() != 3 or scales.dtype != torch.uint8:
+            raise ValueError(f"{name}_scales must be a uint8 [pages, kv_heads, page_size / block] tensor")
+    if k_scales.shape != v_scales.shape or k_scales.shape[:2] != k_cache.shape[:2] or not k_scales.shape[2]:
+        raise ValueError("k_scales and v_scales must have the same shape, with the caches' pages and heads")
+    page_size, blocks = k_cache.shape[2], k_scales.shape[2]
+    if page_size % blocks:
+        raise ValueError("the blocks that the scales count must divide the page")
+    if page_size // blocks % 16 or page_size // blocks > BLOCK_MAX:
+        raise NotImplementedError(f"a block must be 16 to {BLOCK_MAX} tokens, a multiple of 16")
+    if k_cache.shape[3] not in HEAD_DIMS:
+        raise NotImplementedError("a cache in 8 bits has heads of 64 or 128 channels")
+    for scales, name in ((k_scales, "k_scales"), (v_scales, "v_scales")):
+        if not scales.is_cuda:
+            raise ValueError(f"{name} must be a ROCm device tensor (got {scales.device}); there is no CPU path")
+        if blocks > 1 and scales.stride(2) != 1:
+            raise ValueError(f"{name} of a page must be contiguous")
+    return _CODE_MODES[k_cache.dtype], page_size // blocks, _strides(k_scales), _strides(v_scales)
 
 
 def _paged(k_cache, v_cache, page_table, query_starts, context_lengths):
@@ -212,7 +253,7 @@ def _paged(k_cache, v_cache, page_table, query_starts, context_lengths):
 
 
 def paged_append(k, v, k_cache, v_cache, page_table, query_starts, context_lengths, *, q=None, frequencies=None,
-                 layout="half", magnitude=1.0):
+                 layout="half", magnitude=1.0, k_scales=None, v_scales=None):
     """Write new keys and values into a paged cache, the keys turned to their positions on the way.
 
     k, v [kv_heads, tokens, width] (float16, bfloat16 or float32, any strides); k_cache, v_cache
@@ -223,21 +264,33 @@ def paged_append(k, v, k_cache, v_cache, page_table, query_starts, context_lengt
 
     A token whose position is negative (an idle slot: context_lengths 0) or lies behind the table, or whose table entry
     names no page, is not stored.  Where two tokens of one call name the same place, what lies there is unspecified:
-    each channel of each head is one token's or the other's, in the keys and the values by themselves."""
+    each channel of each head is one token's or the other's, in the keys and the values by themselves.
+
+    With `k_scales` and `v_scales` the caches are codes, and they and the scales are written.  A block's scale is the
+    least power of two 2^e with max |x| <= 448 * 2^e (E4M3; INT8: 127 * 2^e) over its tokens of this call, or, where it
+    holds older tokens (positions below context_lengths[b] - n), the scale that it has, if that is larger; a code is
+    x / 2^e to the nearest, ties to even.  Where the scale grows, the older tokens' codes are rounded again under it.
+    Slots behind the context stay as they are.  A block that gets an infinity or NaN reads as NaN until it is written
+    from its first slot on.  Keys are turned in 64 bits, and their codes rounded from that.  Where two sequences of a
+    call write into one block, its codes are unspecified."""
     fast = hip._fast
     if fast is not None:
         done = fast.paged_append(k, v, k_cache, v_cache, page_table, query_starts, context_lengths, q, frequencies,
-                                 layout, magnitude)
+                                 layout, magnitude, k_scales, v_scales)
         if done is not None:
             return None if done is True else done
     kv_heads, tokens, width = _heads_tensor(k, "k", _FLOAT_DTYPES)
     if not isinstance(v, torch.Tensor) or v.shape != k.shape or v.dtype != k.dtype:
         raise ValueError("k and v must have the same shape and dtype")
-    ks = _cache(k_cache, "k_cache", k, kv_heads, width)
-    vs = _cache(v_cache, "v_cache", k, kv_heads, width)
-    for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+    codes = _codes(k_cache, v_cache, k_scales, v_scales)
+    ks = _cache(k_cache, "k_cache", k_cache.dtype if codes else k.dtype, kv_heads, width)
+    vs = _cache(v_cache, "v_cache", k_cache.dtype if codes else k.dtype, kv_heads, width)
+    for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache"), (k_scales, "k_scales"), (v_scales, "v_scales")):
+        if t is not None and any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
             raise ValueError(f"{name} must not be an expanded view: it is written")
+    if codes:
+        _aligned_rows(k_cache, ks, "k_cache")
+        _aligned_rows(v_cache, vs, "v_cache")
     page_table, query_starts, context_lengths = _paged(k_cache, v_cache, page_table, query_starts, context_lengths)
     pairs, heads, q_out, qs = 0, 0, None, (0, 0)
     if frequencies is not None:
@@ -253,15 +306,27 @@ def paged_append(k, v, k_cache, v_cache, page_table, query_starts, context_lengt
             raise ValueError("q must have k's tokens and width")
     device = _device(k, (v, "v"), (k_cache, "k_cache"), (v_cache, "v_cache"), (page_table, "page_table"),
                      (query_starts, "query_starts"), (context_lengths, "context_lengths"), (q, "q"),
-                     (frequencies, "frequencies"))
+                     (frequencies, "frequencies"), (k_scales, "k_scales"), (v_scales, "v_scales"))
+    aligned = codes is not None
     if q is not None:
-        q = _rows(q, "q", aligned=False)
+        q = _rows(q, "q", aligned)
         qs = _strides(q)
         q_out = torch.empty((heads, tokens, width), dtype=k.dtype, device=device)
-    k, v = _rows(k, "k", aligned=False), _rows(v, "v", aligned=False)
+    k, v = _rows(k, "k", aligned), _rows(v, "v", aligned)
     if tokens == 0:
         return q_out
     kr, vr = _strides(k), _strides(v)
+    if codes:
+        mode, block, ke, ve = codes
+        with _on(device):
+            _lib.call(
+                "m5k_paged_append_codes", _lib.ptr(k), kr[0], kr[1], _lib.ptr(v), vr[0], vr[1], _lib.dtype_code(k),
+                tokens, kv_heads, width, mode, _lib.ptr(k_cache), ks[0], ks[1], ks[2], _lib.ptr(k_scales), ke[0], ke[1],
+                _lib.ptr(v_cache), vs[0], vs[1], vs[2], _lib.ptr(v_scales), ve[0], ve[1], block, k_cache.shape[0],
+                k_cache.shape[2], _lib.ptr(page_table), page_table.shape[1], page_table.shape[0],
+                _lib.ptr(query_starts), _lib.ptr(context_lengths), _lib.ptr(q), heads, qs[0], qs[1], _lib.ptr(q_out),
+                _lib.ptr(frequencies), pairs, int(layout == "interleaved"), float(magnitude), _lib.stream_of(k))
+        return q_out
     with _on(device):
         _lib.call(
             "m5k_paged_append", _lib.ptr(k), kr[0], kr[1], _lib.ptr(v), vr[0], vr[1], _lib.dtype_code(k), tokens,
@@ -272,6 +337,51 @@ def paged_append(k, v, k_cache, v_cache, page_table, query_starts, context_lengt
     return q_out
 
 
+def paged_read(k_cache, v_cache, page_table, query_starts, context_lengths, tokens, *, k_scales, v_scales,
+               dtype=torch.bfloat16):
+    """Keys and values of a cache in 8 bits as (k, v), fresh [kv_heads, tokens, width] tensors of `dtype` (bfloat16,
+    float16 or float32).
+
+    Arguments are paged_append's: of sequence b the last n = query_starts[b + 1] - query_starts[b] of its
+    context_lengths[b] keys, so that the call with paged_append's arguments gives what that call stored.  `tokens` is
+    how many rows come back: query_starts[-1], or more where the host does not know it (rows behind it are 0).  Rows that paged_append would not store are 0 too.  Values are exact in float32, and in bfloat16 down to its
+    subnormals; in float16 they are rounded, to an infinity above its range."""
+    fast = hip._fast
+    if fast is not None:
+        done = fast.paged_read(k_cache, v_cache, page_table, query_starts, context_lengths, tokens, k_scales, v_scales,
+                               dtype)
+        if done is not None:
+            return done
+    if k_scales is None or v_scales is None:
+        raise ValueError("paged_read reads caches in 8 bits: it needs k_scales and v_scales")
+    mode, block, ke, ve = _codes(k_cache, v_cache, k_scales, v_scales)
+    kv_heads, width = k_cache.shape[1], k_cache.shape[3]
+    ks = _cache(k_cache, "k_cache", k_cache.dtype, kv_heads, width)
+    vs = _cache(v_cache, "v_cache", k_cache.dtype, kv_heads, width)
+    _aligned_rows(k_cache, ks, "k_cache")
+    _aligned_rows(v_cache, vs, "v_cache")
+    if dtype not in _FLOAT_DTYPES:
+        raise ValueError("dtype must be bfloat16, float16 or float32")
+    if not _lib.is_int(tokens) or tokens < 0:
+        raise ValueError("tokens must be a nonnegative integer")
+    if tokens > 1 << 28:
+        raise NotImplementedError("paged_read supports up to 2^28 tokens")
+    page_table, query_starts, context_lengths = _paged(k_cache, v_cache, page_table, query_starts, context_lengths)
+    device = _device(k_cache, (v_cache, "v_cache"), (k_scales, "k_scales"), (v_scales, "v_scales"),
+                     (page_table, "page_table"), (query_starts, "query_starts"), (context_lengths, "context_lengths"))
+    k, v = (torch.empty((kv_heads, tokens, width), dtype=dtype, device=device) for _ in range(2))
+    if tokens == 0:
+        return k, v
+    with _on(device):
+        _lib.call(
+            "m5k_paged_read", mode, _lib.ptr(k_cache), ks[0], ks[1], ks[2], _lib.ptr(k_scales), ke[0], ke[1],
+            _lib.ptr(v_cache), vs[0], vs[1], vs[2], _lib.ptr(v_scales), ve[0], ve[1], block, k_cache.shape[0],
+            k_cache.shape[2], kv_heads, width, _lib.ptr(page_table), page_table.shape[1], page_table.shape[0],
+            _lib.ptr(query_starts), _lib.ptr(context_lengths), tokens, _lib.ptr(k), _lib.ptr(v), _lib.dtype_code(k),
+            _lib.stream_of(k))
+    return k, v
+
+
 @functools.lru_cache(maxsize=4096)
 def _plan(paged, tokens, heads, kv_heads, sequences, keys, cus):
     """(key splits, whether waves share rows) of a call (m5k_attention_plan; host only)."""
@@ -279,6 +389,21 @@ def _plan(paged, tokens, heads, kv_heads, sequences, keys, cus):
     _lib.call("m5k_attention_plan", paged, tokens, heads, kv_heads, sequences, keys, cus, ctypes.byref(n),
               ctypes.byref(few))
     return n.value, bool(few.value)
+
+
+def _first_keys(sinks, window):
+    if sinks is None:
+        return 0
+    if not _lib.is_int(sinks) or sinks <= 0:
+        raise ValueError("sinks must be a positive integer")
+    if window is None:
+        raise ValueError("sinks need a window")
+    return min(int(sinks), _WINDOW_MAX)
+
+
+def _reach(keys, window, sinks, causal):
+    """Keys that the plan counts a row to see."""
+    return min(keys, (1 if causal else 2) * window + sinks + 64) if sinks else keys
 
 
 def _scores(q, heads, width, scale, softcap, window, slopes):
@@ -320,22 +445,26 @@ def _workspace(splits, tokens, heads, width, device):
 
 
 def paged_attention(q, k_cache, v_cache, page_table, query_starts, context_lengths, *, scale=None, window=None,
-                    softcap=None, slopes=None, prefix_lengths=None):
+                    softcap=None, slopes=None, prefix_lengths=None, sinks=None, k_scales=None, v_scales=None):
     """Attention of new tokens, single ones or chunks, over a paged cache that holds their keys and values already.
 
     q [heads, tokens, width] (bfloat16 or float16, width 64 or 128); caches [pages, kv_heads, page_size, width] of the
     same dtype, any page_size, channels contiguous and rows at multiples of 16 bytes.  The n new tokens of sequence b
     are the last n of its context_lengths[b] keys; a token at position p sees keys j <= p, of them with `window` those
-    with p - j < window, and with `prefix_lengths` (int32 [sequences]) also every j below the prefix.  Scores are
+    with p - j < window and with `sinks` (a number; it needs a window) the sequence's first ones too, j < sinks, and
+    with `prefix_lengths` (int32 [sequences]) also every j below the prefix.  Scores are
     scale * q . k (scale defaults to width ** -0.5); `softcap` c turns s into c * tanh(s / c); `slopes` (float32
     [heads]) then adds -slopes[h] * (distance of j from p).  Scores are FP32 numbers of any size; scale and c are normal
     ones, scale / c at most 1e37.  Returns
     [tokens, heads * width]; rows that see no key, and rows behind the last sequence, are 0; rows that see only keys of
-    score -inf are NaN.  Keys on pages that a table entry outside [0, pages) would name are left out."""
+    score -inf are NaN.  Keys on pages that a table entry outside [0, pages) would name are left out.
+
+    With `k_scales` and `v_scales` the caches are codes; keys and values are taken in q's dtype, as paged_read gives
+    them."""
     fast = hip._fast
     if fast is not None:
         out = fast.paged_attention(q, k_cache, v_cache, page_table, query_starts, context_lengths, scale, window,
-                                   softcap, slopes, prefix_lengths)
+                                   softcap, slopes, prefix_lengths, sinks, k_scales, v_scales)
         if out is not None:
             return out
     if prefix_lengths is not None and window is not None:
@@ -343,51 +472,61 @@ def paged_attention(q, k_cache, v_cache, page_table, query_starts, context_lengt
     if not isinstance(k_cache, torch.Tensor) or k_cache.dim() != 4:
         raise ValueError("k_cache must be a [pages, kv_heads, page_size, width] tensor")
     kv_heads, width = k_cache.shape[1], k_cache.shape[3]
-    ks = _cache(k_cache, "k_cache", k_cache, kv_heads, width)
-    vs = _cache(v_cache, "v_cache", k_cache, kv_heads, width)
-    for t, s, name in ((k_cache, ks, "k_cache"), (v_cache, vs, "v_cache")):
-        if t.data_ptr() % 16 or any(x % 8 for x in s[:3]):
-            raise ValueError(f"{name} rows must start at multiples of 16 bytes")
-    heads, tokens = _query(q, kv_heads, width, k_cache.dtype)
+    codes = _codes(k_cache, v_cache, k_scales, v_scales)
+    ks = _cache(k_cache, "k_cache", k_cache.dtype, kv_heads, width)
+    vs = _cache(v_cache, "v_cache", k_cache.dtype, kv_heads, width)
+    _aligned_rows(k_cache, ks, "k_cache")
+    _aligned_rows(v_cache, vs, "v_cache")
+    if codes and k_cache.shape[2] > 1 and not all(width <= s[2] <= 1 << 23 for s in (ks, vs)):
+        raise NotImplementedError("rows of codes must be width to 2^23 bytes apart")
+    heads, tokens = _query(q, kv_heads, width, k_cache.dtype if codes is None else getattr(q, "dtype", None))
     page_table, query_starts, context_lengths = _paged(k_cache, v_cache, page_table, query_starts, context_lengths)
     sequences, table_width = page_table.shape
+    sinks = _first_keys(sinks, window)
     scale, softcap, window, slopes = _scores(q, heads, width, scale, softcap, window, slopes)
     if prefix_lengths is not None:
         prefix_lengths = _int_vector(prefix_lengths, sequences, "prefix_lengths")
     device = _device(q, (k_cache, "k_cache"), (v_cache, "v_cache"), (page_table, "page_table"),
                      (query_starts, "query_starts"), (context_lengths, "context_lengths"), (slopes, "slopes"),
-                     (prefix_lengths, "prefix_lengths"))
+                     (prefix_lengths, "prefix_lengths"), (k_scales, "k_scales"), (v_scales, "v_scales"))
     out = torch.empty((tokens, heads * width), dtype=q.dtype, device=device)
     if tokens == 0:
         return out
     q = _rows(q, "q")
     qs = _strides(q)
     pages, page_size = k_cache.shape[0], k_cache.shape[2]
-    splits, _ = _plan(1, tokens, heads, kv_heads, sequences, table_width * page_size, hip._cu_count_of(device.index))
+    splits, _ = _plan(1, tokens, heads, kv_heads, sequences, _reach(table_width * page_size, window, sinks, True),
+                      hip._cu_count_of(device.index))
     workspace, n = _workspace(splits, tokens, heads, width, device)
+    name, mode, k_more, v_more = "m5k_paged_attention_sinks", (), (), ()
+    if codes:
+        mode, block, ke, ve = codes
+        name, mode = "m5k_paged_attention_codes", (mode,)
+        k_more, v_more = (_lib.ptr(k_scales), ke[0], ke[1]), (_lib.ptr(v_scales), ve[0], ve[1], block)
     with _on(device):
         _lib.call(
-            "m5k_paged_attention", _lib.ptr(q), _lib.dtype_code(q), tokens, heads, width, qs[0], qs[1],
-            _lib.ptr(k_cache), ks[0], ks[1], ks[2], _lib.ptr(v_cache), vs[0], vs[1], vs[2], pages, page_size, kv_heads,
+            name, _lib.ptr(q), _lib.dtype_code(q), tokens, heads, width, qs[0], qs[1], *mode, _lib.ptr(k_cache), ks[0],
+            ks[1], ks[2], *k_more, _lib.ptr(v_cache), vs[0], vs[1], vs[2], *v_more, pages, page_size, kv_heads,
             _lib.ptr(page_table), table_width, sequences, _lib.ptr(query_starts), _lib.ptr(context_lengths), scale,
-            window, softcap, _lib.ptr(slopes), _lib.ptr(prefix_lengths), _lib.ptr(out), splits, _lib.ptr(workspace), n,
-            _lib.stream_of(q))
+            window, sinks, softcap, _lib.ptr(slopes), _lib.ptr(prefix_lengths), _lib.ptr(out), splits,
+            _lib.ptr(workspace), n, _lib.stream_of(q))
     return out
 
 
 def attention(q, k, v, *, causal=False, window=None, document_starts=None, prefix_lengths=None, softcap=None,
-              slopes=None, scale=None):
+              slopes=None, scale=None, sinks=None):
     """softmax(scores) V of q [heads, tokens, width] over k, v [kv_heads, keys, width] (bfloat16 or float16, width 64 or
     128, any strides): [tokens, heads * width].
 
     Token i stands at key position p = i + keys - tokens.  `causal` shows it keys j <= p; `window` those with
-    p - j < window (and, without causal, j - p < window).  `document_starts` (int32 [documents + 1], nondecreasing from
+    p - j < window (and, without causal, j - p < window), and with `sinks` (a number; it needs a window) the first ones
+    of the row's document, or of all keys, too.  `document_starts` (int32 [documents + 1], nondecreasing from
     0, as many keys as tokens) confines it to its own document.  `prefix_lengths` (int32 [documents], or [1]; with
     causal, without window) shows every token of a document that many of its first keys too.  Scores as in
     paged_attention.  A row that sees no key, and a row behind the last document, is 0."""
     fast = hip._fast
     if fast is not None:
-        out = fast.attention(q, k, v, causal, window, document_starts, prefix_lengths, softcap, slopes, scale)
+        out = fast.attention(q, k, v, causal, window, document_starts, prefix_lengths, softcap, slopes, scale, sinks)
         if out is not None:
             return out
     if prefix_lengths is not None and window is not None:
@@ -400,6 +539,7 @@ def attention(q, k, v, *, causal=False, window=None, document_starts=None, prefi
         raise NotImplementedError("attention supports up to 2^24 keys")
     if not isinstance(causal, bool):
         raise ValueError("causal must be a boolean")
+    sinks = _first_keys(sinks, window)
     scale, softcap, window, slopes = _scores(q, heads, width, scale, softcap, window, slopes)
     documents = 0
     if document_starts is not None:
@@ -420,12 +560,13 @@ def attention(q, k, v, *, causal=False, window=None, document_starts=None, prefi
         return out
     q, k, v = _rows(q, "q"), _apart(_rows(k, "k")), _apart(_rows(v, "v"))
     qs, ks, vs = _strides(q), _strides(k), _strides(v)
-    splits, _ = _plan(0, tokens, heads, kv_heads, documents, keys, hip._cu_count_of(device.index))
+    splits, _ = _plan(0, tokens, heads, kv_heads, documents, _reach(keys, window, sinks, causal),
+                      hip._cu_count_of(device.index))
     workspace, n = _workspace(splits, tokens, heads, width, device)
     with _on(device):
         _lib.call(
-            "m5k_attention", _lib.ptr(q), _lib.dtype_code(q), tokens, heads, width, qs[0], qs[1], _lib.ptr(k), ks[0],
-            ks[1], _lib.ptr(v), vs[0], vs[1], keys, kv_heads, scale, int(causal), window, softcap, _lib.ptr(slopes),
-            _lib.ptr(document_starts), documents, _lib.ptr(prefix_lengths), _lib.ptr(out), splits,
+            "m5k_attention_sinks", _lib.ptr(q), _lib.dtype_code(q), tokens, heads, width, qs[0], qs[1], _lib.ptr(k),
+            ks[0], ks[1], _lib.ptr(v), vs[0], vs[1], keys, kv_heads, scale, int(causal), window, sinks, softcap,
+            _lib.ptr(slopes), _lib.ptr(document_starts), documents, _lib.ptr(prefix_lengths), _lib.ptr(out), splits,
             _lib.ptr(workspace), n, _lib.stream_of(q))
     return out

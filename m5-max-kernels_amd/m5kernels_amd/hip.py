@@ -654,6 +654,10 @@ class _NativeFront:
         module = self._load()
         return None if module is None else module.paged_append(*args)
 
+    def paged_read(self, *args):
+        module = self._load()
+        return None if module is None else module.paged_read(*args)
+
     def paged_attention(self, *args):
         module = self._load()
         return None if module is None else module.paged_attention(*args)

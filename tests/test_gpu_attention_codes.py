@@ -1,0 +1,262 @@
+"""paged_attention over a cache in 8 bits against a plain form in 64 bits: the same reference and slack as for 16-bit
+caches, on the values that the codes stand for (exact in the inputs' type)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import attention_reference as ref
+import cache_codes_reference as codes
+import m5kernels_amd as m5
+from attention_sinks_reference import paged
+from m5kernels_amd import _lib, hip
+from m5kernels_amd import attention_ops as module
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, U8, I8 = torch.bfloat16, torch.float16, torch.uint8, torch.int8
+
+
+def _ints(*values):
+    return torch.tensor(values, dtype=torch.int32)
+
+
+def _case(new, context, *, hq=8, hkv=2, d=64, page=32, block=16, mode=U8, dtype=BF16, seed=0):
+    need = [-(-max(c, 0) // page) for c in context]
+    pages = sum(need) + 2
+    g = torch.Generator().manual_seed(seed)
+    order = torch.randperm(pages, generator=g).to(torch.int32)
+    table = torch.full((len(new), max(need) + 1), -1, dtype=torch.int32)
+    at = 0
+    for b, n in enumerate(need):
+        table[b, :n] = order[at:at + n]
+        at += n
+    q = torch.randn(hq, sum(new), d, generator=g).to(dtype)
+    kc, ks = codes.held(seed + 1, pages, hkv, page, d, block, mode, 0.5)
+    vc, vs = codes.held(seed + 2, pages, hkv, page, d, block, mode, 0.5)
+    return dict(q=q, k=kc, v=vc, ks=ks, vs=vs, table=table, starts=torch.tensor([0, *new]).cumsum(0).to(torch.int32),
+                context=_ints(*context))
+
+
+def _got(c, device, **options):
+    moved = {n: o.to(device) if isinstance(o, torch.Tensor) else o for n, o in options.items()}
+    t = {n: x.to(device) for n, x in c.items()}
+    return m5.paged_attention(t["q"], t["k"], t["v"], t["table"], t["starts"], t["context"], k_scales=t["ks"],
+                              v_scales=t["vs"], **moved)
+
+
+def _want(c, **options):
+    k, v = (codes.cache(c[n], c[n + "s"]).to(c["q"].dtype) for n in "kv")
+    return paged(c["q"], k, v, c["table"], c["starts"], c["context"], **options)
+
+
+def _check(c, device, **options):
+    got = _got(c, device, **options)
+    assert got.dtype == c["q"].dtype
+    excess = ref.close(got, *_want(c, **options))
+    assert excess <= 0, excess
+
+
+@pytest.mark.parametrize("mode", [U8, I8])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("d,page,block", [(64, 16, 16), (64, 48, 48), (128, 64, 64), (128, 96, 32), (128, 256, 128)])
+def test_single_tokens(d, page, block, dtype, mode, device):
+    _check(_case([1] * 9, [1, 0, 15, 16, 17, 64, 65, 200, 333], d=d, page=page, block=block, mode=mode, dtype=dtype),
+           device)
+
+
+@pytest.mark.parametrize("mode", [U8, I8])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("d,page,block", [(64, 16, 16), (64, 48, 48), (128, 64, 64), (128, 96, 32), (128, 256, 128)])
+def test_chunks(d, page, block, dtype, mode, device):
+    _check(_case([70, 1, 0, 129, 33], [70, 300, 10, 260, 1000], d=d, page=page, block=block, mode=mode, dtype=dtype),
+           device)
+
+
+def _forms(tokens, heads, kv_heads, sequences, keys):
+    return module._plan(1, tokens, heads, kv_heads, sequences, keys, 256)
+
+
+@pytest.mark.parametrize("mode,dtype", [(U8, BF16), (I8, F16), (I8, BF16)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_tiles_of_128_rows(d, dtype, mode, device):
+    """Rows enough for the form whose waves share key tiles, unsplit, with and without the rest of the options."""
+    c = _case([700, 350, 1], [900, 350, 40], hq=128, hkv=64, d=d, mode=mode, dtype=dtype, page=32, block=32)
+    splits, few = _forms(1051, 128, 64, 3, c["table"].shape[1] * 32)
+    assert not few and splits == 1
+    _check(c, device)
+    _check(c, device, softcap=20.0, slopes=torch.exp2(-8 * torch.arange(1, 129).float() / 128))
+
+
+@pytest.mark.parametrize("mode", [U8, I8])
+@pytest.mark.parametrize("new,context", [([1], [5000]), ([2], [4097]), ([33, 1], [3000, 700]), ([300], [9000])])
+@pytest.mark.parametrize("d", [64, 128])
+def test_key_splits(new, context, d, mode, device):
+    c = _case(new, context, d=d, mode=mode, page=64, block=64)
+    assert _forms(sum(new), 8, 2, len(new), c["table"].shape[1] * 64)[0] > 1
+    _check(c, device)
+    _check(c, device, window=300)
+
+
+@pytest.mark.parametrize("options", [
+    dict(window=1), dict(window=65), dict(softcap=5.0), dict(softcap=1000.0), dict(scale=0.3),
+    dict(slopes=torch.exp2(-torch.arange(1, 9).float())), dict(prefix_lengths=_ints(0, 250, 3, 64)),
+    dict(window=40, sinks=5), dict(window=40, sinks=5, softcap=30.0), dict(window=100, sinks=300)])
+@pytest.mark.parametrize("new", [[1, 1, 1, 1], [90, 1, 37, 150]])
+def test_options(new, options, device):
+    _check(_case(new, [300, 310, 37, 400], d=128), device, **options)
+    _check(_case(new, [300, 310, 37, 400], d=64, mode=I8, dtype=F16), device, **options)
+
+
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (7, 1), (14, 2), (5, 5), (64, 2)])
+def test_shared_heads(hq, hkv, device):
+    _check(_case([1, 20], [200, 100], hq=hq, hkv=hkv, d=128), device)
+
+
+def test_padded_batch(device):
+    """Idle slots, rows behind the last sequence, a context shorter than its tokens."""
+    c = _case([1, 0, 5, 1], [40, 0, 3, 0], d=64)
+    c["q"] = torch.cat([c["q"], torch.ones(8, 6, 64, dtype=BF16)], 1)
+    got = _got(c, device).cpu().view(13, 8, 64)
+    assert not got[7:].any() and not got[6].any() and not got[1:3].any() and got[:1].any() and got[3:6].any()
+    _check(c, device)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new", [[1, 1], [130, 60]])
+def test_lacking_pages_and_lost_blocks(new, d, device):
+    """Keys on no page are left out; a block of NaN reaches the rows that see it, and no others."""
+    c = _case(new, [300, 200], d=d, page=32, block=16)
+    c["table"][0, 3], c["table"][1, 0] = -1, 5000
+    _check(c, device)
+    lost = int(c["table"][0, 5])  # positions 160 .. 175 of the first sequence
+    c["vs"][lost, 1, 0] = 255
+    got, want = _got(c, device).cpu(), _want(c)[0]
+    position = torch.arange(300 - new[0], 300)
+    sees = torch.zeros(sum(new), dtype=torch.bool)
+    sees[:new[0]] = position >= 160
+    heads = got.view(sum(new), 8, d)
+    assert heads[sees][:, 4:].isnan().all()
+    assert torch.isfinite(heads[:, :4]).all() and torch.isfinite(heads[~sees]).all()
+    c["vs"][lost, 1, 0] = c["vs"][lost, 1, 1]
+    c["ks"][lost, 1, 0] = 255
+    heads = _got(c, device).cpu().view(sum(new), 8, d)
+    assert heads[sees][:, 4:].isnan().all()
+    assert torch.isfinite(heads[:, :4]).all() and torch.isfinite(heads[~sees]).all()
+    del want
+
+
+def test_window_behind_a_lost_block(device):
+    """A NaN block that the window has left behind is not seen."""
+    c = _case([1], [400], d=128, page=16, block=16)
+    want = _got(c, device, window=100)
+    c["vs"][int(c["table"][0, 2])] = 255
+    c["ks"][int(c["table"][0, 3])] = 255
+    assert torch.equal(_got(c, device, window=100), want)
+    assert _got(c, device, window=100, sinks=40).isnan().all()
+
+
+@pytest.mark.parametrize("mode", [U8, I8])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_small_and_large_values(dtype, mode, device):
+    """Blocks whose values are far apart: values of 2^-20 (FP16 rounds them) beside others of 2^10."""
+    c = _case([1, 40], [100, 90], d=64, mode=mode, dtype=dtype)
+    c["vs"][:, :, 0] = 127 - 26
+    c["vs"][:, :, 1] = 127 + 3
+    c["ks"][:, :, 0] = 127 - 10
+    _check(c, device)
+
+
+def test_appended(device):
+    """The operators together: chunks, then single tokens, written into 8 bits and attended over, against 64 bits on the
+    values that the reference cache holds."""
+    g = torch.Generator().manual_seed(0)
+    hq, hkv, d, page, block = 14, 2, 128, 32, 16
+    pages = 40
+    table = torch.randperm(pages, generator=g)[:36].reshape(3, 12).to(torch.int32)
+    cpu = {n: torch.zeros(pages, hkv, page, d, dtype=U8) for n in ("k", "v")}
+    exps = {n: torch.zeros(pages, hkv, page // block, dtype=U8) for n in ("k", "v")}
+    c, e = ({n: t.to(device) for n, t in x.items()} for x in (cpu, exps))
+    f, _ = m5.rope_frequencies(96, device="cpu")
+    context = torch.zeros(3, dtype=torch.int32)
+    for step in range(7):
+        new = [[200, 3, 64], [100, 1, 1]][step] if step < 2 else [1, 1, step % 2]
+        starts = torch.tensor([0, *new]).cumsum(0).to(torch.int32)
+        context = context + torch.tensor(new, dtype=torch.int32)
+        t = sum(new)
+        q, k, v = (torch.randn(h, t, d, generator=g).to(BF16) for h in (hq, hkv, hkv))
+        tables = [x.to(device) for x in (table, starts, context)]
+        turned = m5.paged_append(k.to(device), v.to(device), c["k"], c["v"], *tables, q=q.to(device),
+                                 frequencies=f.to(device), k_scales=e["k"], v_scales=e["v"])
+        positions = torch.cat([torch.arange(int(n) - m, int(n)) for n, m in zip(context, new)])
+        codes.append(ref.rotate(k, positions, f), cpu["k"], exps["k"], table, starts, context)
+        codes.append(v.double(), cpu["v"], exps["v"], table, starts, context)
+        values = [codes.cache(cpu[n], exps[n]).to(BF16) for n in "kv"]
+        for options in ({}, dict(window=50, sinks=4)):
+            got = m5.paged_attention(turned, c["k"], c["v"], *tables, k_scales=e["k"], v_scales=e["v"], **options)
+            assert ref.close(got, *paged(turned.cpu(), *values, table, starts, context, **options)) <= 0
+
+
+@pytest.mark.parametrize("sinks", [None, 4])
+def test_both_fronts(sinks, device, monkeypatch):
+    front = _lib.load_fast()
+    if front is None:
+        pytest.skip("the native front is not built")
+    c = {n: t.to(device) for n, t in _case([1, 30], [900, 41], d=128).items()}
+    got = front.paged_attention(c["q"], c["k"], c["v"], c["table"], c["starts"], c["context"], None,
+                                16 if sinks else None, None, None, None, sinks, c["ks"], c["vs"])
+    monkeypatch.setattr(hip, "_fast", None)
+    want = m5.paged_attention(c["q"], c["k"], c["v"], c["table"], c["starts"], c["context"], k_scales=c["ks"],
+                              v_scales=c["vs"], window=16 if sinks else None, sinks=sinks)
+    assert got is not None and torch.equal(got, want)
+
+
+def test_views_and_refusals_on_the_device(device):
+    c = {n: t.to(device) for n, t in _case([1, 30], [100, 41], d=64, hkv=2).items()}
+    want = m5.paged_attention(c["q"], c["k"], c["v"], c["table"], c["starts"], c["context"], k_scales=c["ks"],
+                              v_scales=c["vs"])
+    slot = torch.zeros(c["k"].shape[0], 32, 6, 64, dtype=U8, device=device)  # slots before heads, K and V side by side
+    slot[:, :, 1:3], slot[:, :, 3:5] = c["k"].transpose(1, 2), c["v"].transpose(1, 2)
+    exps = torch.zeros(c["k"].shape[0], 4, 2, dtype=U8, device=device)
+    exps[:, :2], exps[:, 2:] = c["ks"], c["vs"]
+    got = m5.paged_attention(c["q"], slot[:, :, 1:3].transpose(1, 2), slot[:, :, 3:5].transpose(1, 2), c["table"],
+                             c["starts"], c["context"], k_scales=exps[:, :2], v_scales=exps[:, 2:])
+    assert torch.equal(got, want)
+    with pytest.raises(ValueError, match="contiguous"):
+        bad = torch.zeros(c["k"].shape[0], 2, 4, dtype=U8, device=device)[:, :, ::2]
+        m5.paged_attention(c["q"], c["k"], c["v"], c["table"], c["starts"], c["context"], k_scales=bad, v_scales=bad)
+    with pytest.raises(ValueError, match="dtype"):
+        m5.paged_attention(c["q"].float(), c["k"], c["v"], c["table"], c["starts"], c["context"], k_scales=c["ks"],
+                           v_scales=c["vs"])
+
+
+def test_graphs_and_streams(device):
+    """Two captured calls that run in turn, replayed with other lengths: each as the eager call."""
+    one, two = _case([1, 1], [2000, 700], d=128), _case([40, 1], [300, 2100], d=128, seed=9)
+    sides = [{n: t.to(device) for n, t in c.items()} for c in (one, two)]
+
+    def call(c):
+        return m5.paged_attention(c["q"], c["k"], c["v"], c["table"], c["starts"], c["context"], k_scales=c["ks"],
+                                  v_scales=c["vs"], window=500, sinks=4)
+
+    graphs, outs = [], []
+    for c in sides:
+        call(c)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(call(c))
+        graphs.append(graph)
+    for step in range(3):
+        for c in sides:
+            c["context"] -= 7
+        for graph in graphs:
+            graph.replay()
+        for c, out in zip(sides, outs):
+            assert torch.equal(out, call(c))
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        got = call(sides[0])
+    torch.cuda.current_stream().wait_stream(stream)
+    assert torch.equal(got, call(sides[0]))
