@@ -453,8 +453,8 @@ int m5k_attention_sinks(const void* q, int dtype, int64_t tokens, int64_t heads,
                         int64_t documents, const int32_t* prefix_lengths, void* out, int splits, float* workspace,
                         int64_t workspace_elems, void* stream);
 
-/* The plan of m5k_attention (paged 0, sequences = documents) or m5k_paged_attention (paged 1,
- * keys = table_width * page_size) on `cus` compute units (host only; cus <= 0: those of the current device): the key
+/* The plan of m5k_attention (paged 0, sequences = documents), m5k_paged_attention (paged 1,
+ * keys = table_width * page_size) or m5k_paged_attention_codes (paged 2) on `cus` compute units (host only; cus <= 0: those of the current device): the key
  * splits that pay, and whether the waves of a workgroup share 32 rows (few 1) or take 32 each (few 0; few may be
  * NULL). */
 int m5k_attention_plan(int paged, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t sequences, int64_t keys,

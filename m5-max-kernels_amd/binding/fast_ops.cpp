@@ -691,7 +691,7 @@ struct Scores {
 
 // Checks q against the keys' heads and width, and the score options; allocates.  false: let Python look at it.
 bool scores_of(const at::Tensor* q, int64_t kv_heads, int64_t dim, at::ScalarType st, c10::Device dev, PyObject* scale,
-               PyObject* softcap, PyObject* window, PyObject* sinks, PyObject* slopes, bool paged, bool causal,
+               PyObject* softcap, PyObject* window, PyObject* sinks, PyObject* slopes, int paged, bool causal,
                int64_t sequences, int64_t keys, Scores& s) {
   if (!q || q->scalar_type() != st || !half_type(*q) || q->device() != dev || !current(dev) || q->size(2) != dim ||
       q->size(0) % kv_heads || (dim != 64 && dim != 128) || !rows16(*q))
@@ -734,7 +734,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (!optional_vector(args[10], c.sequences, at::kInt, dev, &prefix) || (prefix && args[7] != Py_None) ||
       !rows16(*c.k) || !rows16(*c.v) ||
       !q || !scores_of(q, c.kv_heads, c.dim, coded ? q->scalar_type() : c.k->scalar_type(), dev, args[6], args[8],
-                       args[7], nargs == 14 ? args[11] : Py_None, args[9], true, true, c.sequences,
+                       args[7], nargs == 14 ? args[11] : Py_None, args[9], coded ? 2 : 1, true, c.sequences,
                        c.width * c.page_size, s))
     Py_RETURN_NONE;
   void* stream = nullptr;
@@ -793,7 +793,7 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (keys > (1 << 24) || !optional_vector(args[6], documents ? documents : 1, at::kInt, dev, &prefix) ||
       (prefix && (!causal || args[4] != Py_None)) ||
       !scores_of(q, kv_heads, dim, k->scalar_type(), dev, args[9], args[7], args[4], nargs == 11 ? args[10] : Py_None,
-                 args[8], false, causal, documents, keys, s))
+                 args[8], 0, causal, documents, keys, s))
     Py_RETURN_NONE;
   void* stream = nullptr;
   if (!stream_of(dev, &stream)) return nullptr;

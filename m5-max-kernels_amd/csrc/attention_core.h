@@ -111,6 +111,8 @@ __device__ __forceinline__ float max_halves(float v) {
 
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4s* lds_v4s;
+typedef int v2i __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) v2i* lds_v2i;
 
 // 16 bytes a lane from a 64-bit address straight into LDS at lds_base + 16 lane.  Inline asm for the reason given at
 // gemm::dma16; it has no register outputs, and every reader waits for vmcnt and a barrier.
@@ -141,6 +143,15 @@ template <int D>
 __device__ __forceinline__ int swizzle(int row) {
   if constexpr (D == 64) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
   else return ((row & 3) << 2) | ((row >> 2) & 3);
+}
+
+// The same for a tile of codes, rows of D bytes: the 16 rows of a ds_read_b128 phase (K) fall on 16 bank groups, and so
+// do the 8 rows x 32 bytes of half a wave's transposed read (V), rows 0 .. 3 and 8 .. 11, or 4 .. 7 and 12 .. 15, whose
+// pairs of chunks therefore differ in a bit above the lowest.
+template <int D>
+__device__ __forceinline__ int code_swizzle(int row) {
+  if constexpr (D == 64) return (row >> 2) & 3;
+  else return (((row >> 3) & 1) << 2) | (((row >> 1) & 1) << 1) | ((row >> 2) & 1);
 }
 
 // Where keys and values lie.  PAGES16: pages of a multiple of 16 keys, so that the 16 rows of a tile that one wave
@@ -189,29 +200,42 @@ __device__ __forceinline__ int exponent_byte(const uint8_t* at) {
   }
 }
 
-// Two codes, bytes 2 HI and 2 HI + 1 of a word, times a power of two, as 16-bit values.
+// A block's scale, 2^(e - 127), as code_pair takes it.  E4M3: e in FP32's exponent field, which is all that its conversion
+// reads.  INT8: the number, which for e = 0 has no exponent field of its own; NaN for e = 255.
+template <int CODES>
+__device__ __forceinline__ float code_scale(int e) {
+  uint32_t bits = static_cast<uint32_t>(e) << 23;
+  if constexpr (CODES == INT8) bits = e == 0 ? 0x00400000u : e == 255 ? 0x7FC00000u : bits;
+  return __uint_as_float(bits);
+}
+
+// Two codes, bytes 2 HI and 2 HI + 1 of a word, times their scale, as 16-bit values.  Exact in BF16, which has more bits
+// than a code and FP32's range; rounded once to FP16, which only numbers below 2^-14 need.  E4M3: one conversion, whose
+// results are those of an FP32 product rounded to the type, for every code and exponent (compared on MI355X).
 template <int DT, int CODES, bool HI>
 __device__ __forceinline__ uint32_t code_pair(int w, float scale) {
-  if constexpr (CODES == E4M3) {
-    const auto f = __builtin_amdgcn_cvt_pk_f32_fp8(w, HI);
-    return pack2<DT>(f[0] * scale, f[1] * scale);
+  if constexpr (CODES == E4M3 && DT == M5K_BF16) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI));
+  } else if constexpr (CODES == E4M3) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, HI));
   } else {
     const int w0 = HI ? w << 8 : w << 24, w1 = HI ? w : w << 16;
     return pack2<DT>(static_cast<float>(w0 >> 24) * scale, static_cast<float>(w1 >> 24) * scale);
   }
 }
 
-// 16 codes times 2^(e - 127), in order, as 16-bit values.  Exact in BF16, which has more bits than a code and FP32's
-// range; rounded once to FP16, which only numbers below 2^-14 need.  e = 255: NaN.
+// 8 and 16 codes times their scale, in order, as 16-bit values.
 template <int DT, int CODES>
-__device__ __forceinline__ void expand16(v4i c, int e, v4i (&x)[2]) {
-  // 2^-127 has no exponent field of its own in FP32.
-  const float scale = __uint_as_float(e == 0 ? 0x00400000u : e == 255 ? 0x7FC00000u : static_cast<uint32_t>(e) << 23);
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    x[w >> 1][2 * (w & 1)] = static_cast<int>(code_pair<DT, CODES, false>(c[w], scale));
-    x[w >> 1][2 * (w & 1) + 1] = static_cast<int>(code_pair<DT, CODES, true>(c[w], scale));
-  }
+__device__ __forceinline__ v4i expand8(int w0, int w1, float scale) {
+  return v4i{static_cast<int>(code_pair<DT, CODES, false>(w0, scale)),
+             static_cast<int>(code_pair<DT, CODES, true>(w0, scale)),
+             static_cast<int>(code_pair<DT, CODES, false>(w1, scale)),
+             static_cast<int>(code_pair<DT, CODES, true>(w1, scale))};
+}
+template <int DT, int CODES>
+__device__ __forceinline__ void expand16(v4i c, float scale, v4i (&x)[2]) {
+  x[0] = expand8<DT, CODES>(c[0], c[1], scale);
+  x[1] = expand8<DT, CODES>(c[2], c[3], scale);
 }
 
 struct RowRange {
@@ -413,9 +437,11 @@ __device__ __forceinline__ RowRange range_of(const Args& a, const Place& p, int 
 // SINKS: rows see their span's first keys beside their window.  The workgroup's tiles are those of the first keys, then
 // those of the windows: `t` counts them, real(t) is where tile t lies.
 //
-// CODES: K and V are codes of 8 bits with an exponent byte a block of tokens.  A wave's codes go to LDS as they are, by
-// the loads above, and from there, times their scale, to the tile of 16-bit values that the products read: by the wave
-// that loaded them, so that no barrier stands between and each code is expanded once a workgroup.
+// CODES: K and V are codes of 8 bits with an exponent byte a block of tokens.  They go to LDS as they are.  With FEW the
+// products' fragments are made from them as they are read: two tiles of each operand then take less LDS than one of
+// 16 bits, and no code is read twice.  Otherwise they go, times their scale, to the tile of 16-bit values that the
+// products read: by the wave that loaded them, so that no barrier stands between and each code is expanded once a
+// workgroup, not once a wave.
 template <int DT, int D, int KEYS, bool MODS, bool FEW, bool SINKS, int CODES>
 __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   static_assert(CODES == NO_CODES || KEYS == PAGES16, "codes lie in pages of a multiple of 16");
@@ -429,14 +455,14 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   constexpr int QS = D / 16, OB = D / 32;
   constexpr int AHEAD = 1;  // steps of two products between a fragment's read and its use (2: no faster)
   constexpr int ROWS = FEW ? 32 : 32 * WAVES;
-  constexpr int STAGES = FEW && !(KEYS == PAGES && D == 64) ? 1 : 2;  // tiles of K, and of V, in LDS
-  constexpr uint32_t ROWB = D * 2, TILE = KT * ROWB, VTILE = STAGES * TILE;
+  constexpr bool DIRECT = CODES != NO_CODES && FEW;  // fragments from codes
+  constexpr int STAGES = FEW && !DIRECT && !(KEYS == PAGES && D == 64) ? 1 : 2;  // tiles of K, and of V, in LDS
+  constexpr uint32_t ROWB = DIRECT ? D : D * 2, TILE = KT * ROWB, VTILE = STAGES * TILE;
   // K stages, V stages.  FEW: those of each wave, later its sums, in rows of D + 4 floats (16 bytes a lane without bank
   // conflicts), and their maxima and totals.
-  // CODES: behind them a wave's codes of one tile of K and one of V.
-  constexpr uint32_t RAW = CODES ? LOADED * D : 0;
-  constexpr uint32_t HELD = 2 * VTILE + 2 * RAW;
-  constexpr uint32_t SUMS = (D + 4) * 4, JOIN = 32 * SUMS + 256, AREA = JOIN > HELD ? JOIN : HELD;
+  // CODES, not FEW: behind them a wave's codes of one tile of K and one of V.
+  constexpr uint32_t RAW = CODES && !FEW ? LOADED * D : 0;
+  constexpr uint32_t SUMS = (D + 4) * 4, JOIN = 32 * SUMS + 256, AREA = JOIN > 2 * VTILE ? JOIN : 2 * VTILE;
   __shared__ __attribute__((aligned(256))) uint8_t lds[FEW ? WAVES * AREA : 4 * TILE + 2 * WAVES * RAW];
   // Bounds of the waves' rows.  CODES: where the codes come later, since two workgroups' LDS fills the compute unit.
   __shared__ int bounds_own[FEW || CODES ? 1 : SINKS ? 5 * WAVES : 2 * WAVES];
@@ -534,7 +560,11 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   {
     const uint16_t* qp = a.q + int64_t{head} * a.q_head + int64_t{token} * a.q_token + 8 * half;
 #pragma unroll
-    for (int s = 0; s < QS; ++s) qf[s] = *reinterpret_cast<const v4i*>(qp + 16 * s);
+    for (int s = 0; s < QS; ++s) {
+      // DIRECT: the channel order of K's fragments, two from the 16 codes of one read.
+      const int channel = DIRECT ? 32 * (s >> 1) + 8 * half + 8 * (s & 1) : 16 * s;
+      qf[s] = *reinterpret_cast<const v4i*>(qp + channel);
+    }
   }
   const float scale2 = a.scale * LOG2E;
   const float unit = MODS ? 1.0f : scale2;  // what turns finished scores into base 2, launch_unit()
@@ -555,14 +585,16 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int r = KEYS == DENSE ? ld_row + i * RPI : lane / CH + i % (NI / GROUPS) * RPI;  // pages: of 16 rows
-      const int chunk = CODES ? ld_chunk * 16 : (ld_chunk ^ swizzle<D>(ld_row + i * RPI)) * 8;
+      const int chunk = DIRECT  ? (ld_chunk ^ code_swizzle<D>(ld_row + i * RPI)) * 16
+                        : CODES ? ld_chunk * 16
+                                : (ld_chunk ^ swizzle<D>(ld_row + i * RPI)) * 8;
       kofs[i] = static_cast<uint32_t>(r * static_cast<int>(a.k_row) + chunk) * sizeof(Elem);
       vofs[i] = static_cast<uint32_t>(r * static_cast<int>(a.v_row) + chunk) * sizeof(Elem);
     }
   }
   constexpr int NIDS = KEYS == PAGES ? NI : GROUPS;
   int ids[2][NIDS] = {};  // pages of the next tile's keys, and of the tile before it, whose values come next
-  int ek[GROUPS] = {}, ev[GROUPS] = {};  // CODES: exponents of the codes on their way
+  int ek[STAGES][GROUPS] = {}, ev[STAGES][GROUPS] = {};  // CODES: exponents of the codes on their way
   bool lacking = false;
 
   // Unconditional, at the last key where tile t has none: a load under a condition would be waited for at the
@@ -628,7 +660,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
 
   // CODES: exponents of the groups of 16 keys that this wave loads of tile t, 0 where there is no page.  FEW: as the
   // aligned word around each, by a scalar load (see table_entry); the word's other bytes share the byte's allocation.
-  const uint32_t raw_k = FEW ? lds0 + 2 * VTILE : lds0 + 4 * TILE + wave_s * 2 * RAW, raw_v = raw_k + RAW;
+  const uint32_t raw_k = lds0 + 4 * TILE + wave_s * 2 * RAW, raw_v = raw_k + RAW;
   auto load_exps = [&](int u, const int (&id)[NIDS], const uint8_t* base, int64_t page_stride, int (&to)[GROUPS])
                        __attribute__((always_inline)) {
     if constexpr (CODES) {
@@ -645,16 +677,16 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   };
   // This wave's codes at `raw`, times their scale, to its rows of the 16-bit tile at `dst`.
   auto expand = [&](uint32_t raw, const int (&exps)[GROUPS], uint32_t dst) __attribute__((always_inline)) {
-    if constexpr (CODES) {
+    if constexpr (CODES && !FEW) {
       constexpr int PER = NI / GROUPS;
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g) {
-        const int e = __builtin_amdgcn_readfirstlane(exps[g]);
+        const float scale = code_scale<CODES>(__builtin_amdgcn_readfirstlane(exps[g]));
 #pragma unroll
         for (int i = g * PER; i < (g + 1) * PER; ++i) {
           const v4i c = *reinterpret_cast<const __attribute__((address_space(3))) v4i*>(raw + i * 1024 + lane * 16);
           v4i x[2];
-          expand16<DT, CODES>(c, e, x);
+          expand16<DT, CODES>(c, scale, x);
           const int r = ld_row + i * RPI;
           const uint32_t at = dst + r * ROWB + (((2 * ld_chunk) ^ swizzle<D>(r)) << 4);
           *reinterpret_cast<__attribute__((address_space(3))) v4i*>(at) = x[0];
@@ -666,18 +698,27 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
 
   // Fragment addresses in stage 0 (the other stage and the rows further on are instruction offsets): chunk c of a row
   // is its chunk 0 XOR 16 c, rows being aligned to their size.
-  uint32_t kread[QS], vread[2][OB];
+  constexpr int KREADS = DIRECT ? QS / 2 : QS, VREADS = DIRECT ? 1 : 2;
+  uint32_t kread[KREADS], vread[VREADS][OB];
   const int g = lane >> 4, gi = lane & 15;
   const int vrow = 4 * half + (gi >> 2), vchunk = 2 * (g & 1) + ((gi & 3) >> 1);
+  const int ksw = DIRECT ? code_swizzle<D>(lane & 31) : swizzle<D>(lane & 31);
 #pragma unroll
-  for (int c = 0; c < QS; ++c)
-    kread[c] = (lds0 + (lane & 31) * ROWB + ((half ^ swizzle<D>(lane & 31)) << 4)) ^ (c << 5);
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
+  for (int c = 0; c < KREADS; ++c) kread[c] = (lds0 + (lane & 31) * ROWB + ((half ^ ksw) << 4)) ^ (c << 5);
+  if constexpr (DIRECT) {
+    // The 8 keys of a fragment in the accumulator's order, two lanes a key.
+    const int key = 8 * (gi >> 3) + 4 * half + ((gi >> 1) & 3);
 #pragma unroll
     for (int b = 0; b < OB; ++b)
-      vread[h][b] =
-          (lds0 + (8 * h + vrow) * ROWB + ((vchunk ^ swizzle<D>(8 * h + vrow)) << 4) + (gi & 1) * 8) ^ (b << 6);
+      vread[0][b] = (lds0 + key * ROWB + (((g & 1) ^ code_swizzle<D>(key)) << 4) + (gi & 1) * 8) ^ (b << 5);
+  } else {
+#pragma unroll
+    for (int h = 0; h < VREADS; ++h)
+#pragma unroll
+      for (int b = 0; b < OB; ++b)
+        vread[h][b] =
+            (lds0 + (8 * h + vrow) * ROWB + ((vchunk ^ swizzle<D>(8 * h + vrow)) << 4) + (gi & 1) * 8) ^ (b << 6);
+  }
 
   wait_all();
   v16f o[OB], s[2][NB];
@@ -693,11 +734,19 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     for (int b = 0; b < NB; ++b)
       f[b] = *reinterpret_cast<const __attribute__((address_space(3))) v4i*>(kread[c] + b * 32 * ROWB + st * TILE);
   };
-  // V^T fragment of k-step c and channel block b: keys 16 c + 8 h + 4 (lane >> 5) .. + 3 for h = 0, 1.
+  // V^T fragment of k-step c and channel block b: keys 16 c + 8 h + 4 (lane >> 5) .. + 3 for h = 0, 1.  DIRECT: its codes,
+  // which value_of makes a fragment of.
   auto value_frag = [&](int st, int c, int b) __attribute__((always_inline)) {
-    v4i f;
+    v4i f{};
+    if constexpr (DIRECT) {
+      const v2i x = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+          reinterpret_cast<lds_v2i>(vread[0][b] + 16 * c * ROWB + VTILE + st * TILE));
+      f[0] = x[0];
+      f[1] = x[1];
+      return f;
+    }
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < VREADS; ++h) {
       const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
           reinterpret_cast<lds_v4s>(vread[h][b] + 16 * c * ROWB + VTILE + st * TILE));
       const auto y = __builtin_bit_cast(m5k_u32x2, x);
@@ -705,6 +754,10 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
       f[2 * h + 1] = static_cast<int>(y[1]);
     }
     return f;
+  };
+  auto value_of = [&](v4i f, int st, int c) __attribute__((always_inline)) {
+    if constexpr (DIRECT) return expand8<DT, CODES>(f[0], f[1], code_scale<CODES>(ev[st][c]));
+    else return f;
   };
   constexpr std::false_type quick{};
   constexpr std::true_type careful{};
@@ -728,6 +781,26 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     }
   };
   auto product = [&](v16f (&y)[NB], int st, const v16f (&x)[NB], bool prob) __attribute__((always_inline)) {
+    if constexpr (DIRECT) {
+      // Rows 0 .. 15 and 16 .. 31 of the tile are two groups.
+      int e0 = ek[st][0], e1 = ek[st][GROUPS - 1];
+      __asm__("" : "+s"(e0), "+s"(e1));  // values, not two places to choose from: those would go to memory
+      const float scale = code_scale<CODES>((lane & 16) ? e1 : e0);
+      v4i code[2];
+      auto read = [&](int c) __attribute__((always_inline)) {
+        return *reinterpret_cast<const __attribute__((address_space(3))) v4i*>(kread[c] + st * TILE);
+      };
+      code[0] = read(0);
+#pragma unroll
+      for (int c = 0; c < KREADS; ++c) {
+        if (c + 1 < KREADS) code[(c + 1) & 1] = read(c + 1);
+        v4i f[2];
+        expand16<DT, CODES>(code[c & 1], scale, f);
+        y[0] = mfma32<DT>(f[0], qf[2 * c], c == 0 ? v16f{} : y[0]);
+        y[0] = mfma32<DT>(f[1], qf[2 * c + 1], y[0]);
+      }
+      return;
+    }
     v4i kf[AHEAD + 1][NB];
     float sum[2] = {};
 #pragma unroll
@@ -813,7 +886,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int b = 2 * i % OB + j;
-        o[b] = mfma32<DT>(vf[i % (AHEAD + 1)][j], pf[2 * i / OB], o[b]);
+        o[b] = mfma32<DT>(value_of(vf[i % (AHEAD + 1)][j], st, 2 * i / OB), pf[2 * i / OB], o[b]);
       }
 #pragma unroll
       for (int e = i * EL / STEPS; e < (i + 1) * EL / STEPS; e += 2) {
@@ -832,7 +905,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
 #pragma unroll
       for (int c = 0; c < 2 * NB; ++c) {
         v4i clean, mark, see;
-        split_nonfinite<DT>(value_frag(0, c, b), clean, mark);
+        split_nonfinite<DT>(value_of(value_frag(0, c, b), 0, c), clean, mark);
         const uint32_t one = pack2<DT>(1.0f, 1.0f);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
@@ -892,12 +965,12 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     gemm::stage_barrier();
     if constexpr (CODES) {
       // The codes of V of tile t + 1 and K of t + 2 are here: expand them, and load those of a tile further on.
-      if (t + 1 < t_end) expand(raw_v, ev, lds0 + (2 + ODD) * TILE);
+      if (t + 1 < t_end) expand(raw_v, ev[0], lds0 + (2 + ODD) * TILE);
       if (t + 2 < t_end) {
-        expand(raw_k, ek, lds0 + EVEN * TILE);
+        expand(raw_k, ek[0], lds0 + EVEN * TILE);
         __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        load_exps(t + 2, ids[1], vexp, a.ve_page, ev);
-        load_exps(t + 3, ids[0], kexp, a.ke_page, ek);
+        load_exps(t + 2, ids[1], vexp, a.ve_page, ev[0]);
+        load_exps(t + 3, ids[0], kexp, a.ke_page, ek[0]);
         load_rows(t + 2, ids[1], vbase, a.v_page, a.v_row, vofs, raw_v);
         if (t + 3 < t_end) load_rows(t + 3, ids[0], kbase, a.k_page, a.k_row, kofs, raw_k);
       }
@@ -931,18 +1004,11 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   auto own_tile = [&](int t, auto stage) __attribute__((always_inline)) {
     constexpr int ST = decltype(stage)::value;
     const bool more = t + WAVES < t_end;
-    if constexpr (CODES) {
-      gemm::wait_stage<NI>();  // K, behind which V was issued
-      expand(raw_k, ek, lds0);
-      __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      if (more) {
-        load_exps(t + WAVES, ids[0], kexp, a.ke_page, ek);
-        load_rows(t + WAVES, ids[0], kbase, a.k_page, a.k_row, kofs, raw_k);
-      }
-      product(s[0], 0, s[0], false);
-    } else if constexpr (STAGES == 2) {
+    if constexpr (STAGES == 2) {
       if (more) {
         __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last reads of that stage
+        load_exps(t + WAVES, ids[0], kexp, a.ke_page, ek[STAGES - 1 - ST]);
+        load_exps(t + WAVES, ids[0], vexp, a.ve_page, ev[STAGES - 1 - ST]);
         load_rows(t + WAVES, ids[0], kbase, a.k_page, a.k_row, kofs, lds0 + (1 - ST) * TILE);
         load_rows(t + WAVES, ids[0], vbase, a.v_page, a.v_row, vofs, lds0 + VTILE + (1 - ST) * TILE);
         load_ids(t + 2 * WAVES, ids[0]);
@@ -969,17 +1035,8 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
       if (more) gemm::wait_stage<NI>();
       else gemm::wait_stage<0>();
     }
-    if constexpr (CODES) {
-      expand(raw_v, ev, lds0 + VTILE);
-      __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      if (more) {
-        load_exps(t + WAVES, ids[0], vexp, a.ve_page, ev);
-        load_rows(t + WAVES, ids[0], vbase, a.v_page, a.v_row, vofs, raw_v);
-        load_ids(t + 2 * WAVES, ids[0]);
-      }
-    }
     accumulate(ST, s[0]);
-    if constexpr (STAGES == 1 && !CODES) {
+    if constexpr (STAGES == 1) {
       if (more) {
         __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         load_rows(t + WAVES, ids[0], vbase, a.v_page, a.v_row, vofs, lds0 + VTILE);
@@ -992,10 +1049,10 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     int t = t_begin + wave_s;
     if (t < t_end) {
       load_ids(t, ids[0]);
-      load_exps(t, ids[0], kexp, a.ke_page, ek);
-      load_exps(t, ids[0], vexp, a.ve_page, ev);
-      load_rows(t, ids[0], kbase, a.k_page, a.k_row, kofs, CODES ? raw_k : lds0);
-      load_rows(t, ids[0], vbase, a.v_page, a.v_row, vofs, CODES ? raw_v : lds0 + VTILE);
+      load_exps(t, ids[0], kexp, a.ke_page, ek[0]);
+      load_exps(t, ids[0], vexp, a.ve_page, ev[0]);
+      load_rows(t, ids[0], kbase, a.k_page, a.k_row, kofs, lds0);
+      load_rows(t, ids[0], vbase, a.v_page, a.v_row, vofs, lds0 + VTILE);
       load_ids(t + WAVES, ids[0]);
     }
     for (; t < t_end; t += STAGES * WAVES) {
@@ -1006,13 +1063,13 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     load_ids(t_begin, ids[1]);
     if constexpr (CODES) {
       load_ids(t_begin + 1, ids[0]);
-      load_exps(t_begin, ids[1], kexp, a.ke_page, ek);
-      load_exps(t_begin, ids[1], vexp, a.ve_page, ev);
+      load_exps(t_begin, ids[1], kexp, a.ke_page, ek[0]);
+      load_exps(t_begin, ids[1], vexp, a.ve_page, ev[0]);
       load_rows(t_begin, ids[1], kbase, a.k_page, a.k_row, kofs, raw_k);
       wait_all();
-      expand(raw_k, ek, lds0);
+      expand(raw_k, ek[0], lds0);
       __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      load_exps(t_begin + 1, ids[0], kexp, a.ke_page, ek);
+      load_exps(t_begin + 1, ids[0], kexp, a.ke_page, ek[0]);
       load_rows(t_begin, ids[1], vbase, a.v_page, a.v_row, vofs, raw_v);
       if (t_begin + 1 < t_end) load_rows(t_begin + 1, ids[0], kbase, a.k_page, a.k_row, kofs, raw_k);
       ids[1][0] = ids[0][0];
@@ -1067,14 +1124,14 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     for (int t = t_begin; t < t_end; ++t) {
       if (FEW && ((t - t_begin) & (WAVES - 1)) != wave_s) continue;
       load_ids(t, ids[0]);
-      load_exps(t, ids[0], kexp, a.ke_page, ek);
-      load_exps(t, ids[0], vexp, a.ve_page, ev);
-      load_rows(t, ids[0], kbase, a.k_page, a.k_row, kofs, CODES ? raw_k : lds0);
-      load_rows(t, ids[0], vbase, a.v_page, a.v_row, vofs, CODES ? raw_v : lds0 + VTILE);
+      load_exps(t, ids[0], kexp, a.ke_page, ek[0]);
+      load_exps(t, ids[0], vexp, a.ve_page, ev[0]);
+      load_rows(t, ids[0], kbase, a.k_page, a.k_row, kofs, CODES && !FEW ? raw_k : lds0);
+      load_rows(t, ids[0], vbase, a.v_page, a.v_row, vofs, CODES && !FEW ? raw_v : lds0 + VTILE);
       wait_all();
-      if constexpr (CODES) {
-        expand(raw_k, ek, lds0);
-        expand(raw_v, ev, lds0 + VTILE);
+      if constexpr (CODES && !FEW) {
+        expand(raw_k, ek[0], lds0);
+        expand(raw_v, ev[0], lds0 + VTILE);
         wait_all();
       }
       if constexpr (!FEW) gemm::stage_barrier();
@@ -1303,10 +1360,11 @@ struct Plan {
   bool few;
   int slots;
 };
-inline Plan plan(bool paged, int64_t tokens, int group, int kv_heads, int64_t sequences, int64_t keys, int cus) {
+enum Paged { UNPAGED = 0, PAGED = 1, CODED = 2 };
+inline Plan plan(int paged, int64_t tokens, int group, int kv_heads, int64_t sequences, int64_t keys, int cus) {
   const int64_t rows = tokens * group, own = paged ? sequences : 1;
   const int64_t tiles = (rows / (32 * WAVES) + own) * kv_heads, thin = (rows / 32 + own) * kv_heads;
-  const bool few = (rows <= 32 * own && own * kv_heads < 2 * cus) ||
+  const bool few = (rows <= 32 * own && (paged == CODED || own * kv_heads < 2 * cus)) ||
                    (tiles < cus && thin <= (keys < 512 ? 2 : 4) * cus && keys <= 4096);
   const int64_t r = few ? 32 : 32 * WAVES;
   return Plan{few, static_cast<int>(paged ? rows / r + sequences + 1 : (rows + r - 1) / r)};
@@ -1316,7 +1374,7 @@ inline Plan plan(bool paged, int64_t tokens, int group, int kv_heads, int64_t se
 // of the longest span; twice as many were slower (2048 tokens, 8 heads: 22 and 36 us).  Full workgroups of `few` to
 // one: their waves split the keys already, and the sums of 32 rows cost as much as their keys (2000 tokens, 4 query
 // heads on one key head, 250 workgroups: 19 us, 26 us in two splits).
-inline int plan_splits(bool paged, int64_t tokens, int group, int kv_heads, int64_t sequences, int64_t keys,
+inline int plan_splits(int paged, int64_t tokens, int group, int kv_heads, int64_t sequences, int64_t keys,
                        int cus) {
   const Plan p = plan(paged, tokens, group, kv_heads, sequences, keys, cus);
   // Slots that have rows: of a paged launch about half a tile a sequence on top of the whole ones.
@@ -1336,7 +1394,7 @@ int launch_join(const Args& a, int dtype, int head_dim, hipStream_t st);
 template <int DT, int D, int KEYS, bool SINKS, int CODES>
 int launch(Args& a, hipStream_t st) {
   const bool mods = a.softcap > 0.0f || a.slopes;
-  const Plan p = plan(KEYS != DENSE, a.tokens, a.group, a.kv_heads, a.sequences, a.reach, device_cus());
+  const Plan p = plan(KEYS == DENSE ? UNPAGED : CODES ? CODED : PAGED, a.tokens, a.group, a.kv_heads, a.sequences, a.reach, device_cus());
   a.slots = p.slots;
   a.cus = device_cus();
   a.spread = a.kv_heads % 8 != 0 && (KEYS != DENSE || a.causal || a.starts);

@@ -495,7 +495,7 @@ def paged_attention(q, k_cache, v_cache, page_table, query_starts, context_lengt
     q = _rows(q, "q")
     qs = _strides(q)
     pages, page_size = k_cache.shape[0], k_cache.shape[2]
-    splits, _ = _plan(1, tokens, heads, kv_heads, sequences, _reach(table_width * page_size, window, sinks, True),
+    splits, _ = _plan(2 if codes else 1, tokens, heads, kv_heads, sequences, _reach(table_width * page_size, window, sinks, True),
                       hip._cu_count_of(device.index))
     workspace, n = _workspace(splits, tokens, heads, width, device)
     name, mode, k_more, v_more = "m5k_paged_attention_sinks", (), (), ()
