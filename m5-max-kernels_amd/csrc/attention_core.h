@@ -185,21 +185,6 @@ __device__ __forceinline__ v4i rows_rsrc(const Elem* p, int rows, int64_t stride
 
 constexpr int NEVER = 0x3FFFFFFF;  // behind every key
 
-// An exponent byte, the same for the whole wave.  SCALAR: see table_entry.
-template <bool SCALAR>
-__device__ __forceinline__ int exponent_byte(const uint8_t* at) {
-  if constexpr (SCALAR) {
-    const uintptr_t p = reinterpret_cast<uintptr_t>(at);
-    const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(p));
-    const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(p >> 32));
-    const uintptr_t word = (static_cast<uintptr_t>(hi) << 32) | (lo & ~3u);
-    const uint32_t w = *reinterpret_cast<const __attribute__((address_space(4))) uint32_t*>(word);
-    return static_cast<int>((w >> (8 * (lo & 3u))) & 0xFFu);
-  } else {
-    return *at;
-  }
-}
-
 // A block's scale, 2^(e - 127), as code_pair takes it.  E4M3: e in FP32's exponent field, which is all that its conversion
 // reads.  INT8: the number, which for e = 0 has no exponent field of its own; NaN for e = 255.
 template <int CODES>
@@ -658,22 +643,42 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     }
   };
 
-  // CODES: exponents of the groups of 16 keys that this wave loads of tile t, 0 where there is no page.  FEW: as the
-  // aligned word around each, by a scalar load (see table_entry); the word's other bytes share the byte's allocation.
+  // CODES: where the exponent of a key's block lies, on a page `id` (or a 0, where that is none).
+  auto exponent_at = [&](int key, int id, const uint8_t* base, int64_t page_stride) __attribute__((always_inline)) {
+    const int slot = key - static_cast<int>(fast_div(key, a.page_magic, a.page_shift)) * a.page_size;
+    const bool has = key < p.span && static_cast<uint32_t>(id) < static_cast<uint32_t>(a.pages);
+    return has ? base + id * page_stride + fast_div(slot, a.block_magic, a.block_shift)
+               : reinterpret_cast<const uint8_t*>(kZeros);
+  };
+  // CODES, not FEW: exponents of the 16 keys that this wave loads of tile t.
   const uint32_t raw_k = lds0 + 4 * TILE + wave_s * 2 * RAW, raw_v = raw_k + RAW;
-  auto load_exps = [&](int u, const int (&id)[NIDS], const uint8_t* base, int64_t page_stride, int (&to)[GROUPS])
+  auto load_exps = [&](int t, const int (&id)[NIDS], const uint8_t* base, int64_t page_stride, int (&to)[GROUPS])
                        __attribute__((always_inline)) {
-    if constexpr (CODES) {
-#pragma unroll
-      for (int g = 0; g < GROUPS; ++g) {
-        const int key = real(u) * KT + first_row + 16 * g;
-        const int slot = key - static_cast<int>(fast_div(key, a.page_magic, a.page_shift)) * a.page_size;
-        const bool has = key < p.span && static_cast<uint32_t>(id[g]) < static_cast<uint32_t>(a.pages);
-        const uint8_t* at = has ? base + id[g] * page_stride + fast_div(slot, a.block_magic, a.block_shift)
-                                : reinterpret_cast<const uint8_t*>(kZeros);
-        to[g] = exponent_byte<FEW>(at);
-      }
+    if constexpr (CODES && !FEW) to[0] = *exponent_at(real(t) * KT + first_row, id[0], base, page_stride);
+  };
+  // DIRECT: pages and exponents of the 32 tiles that this wave takes from tile t on, a group of 16 keys a lane, by vector
+  // loads that it waits for once.  By scalar loads a tile, each would hold up the LDS reads issued behind it.
+  int held_id = 0, held_k = 0, held_v = 0, held_at = 0;
+  auto look_ahead = [&](int t) __attribute__((always_inline)) {
+    if constexpr (DIRECT) {
+      const int key = real(t + WAVES * (lane >> 1)) * KT + 16 * (lane & 1);
+      held_id = table[fast_div(min(key, p.span - 1), a.page_magic, a.page_shift)];
+      held_k = *exponent_at(key, held_id, kexp, a.ke_page);
+      held_v = *exponent_at(key, held_id, vexp, a.ve_page);
+      held_at = 0;
     }
+  };
+  auto take_ids = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int g = 0; g < NIDS; ++g) ids[0][g] = __builtin_amdgcn_readlane(held_id, 2 * held_at + g);
+  };
+  auto take_exps = [&](int (&k)[GROUPS], int (&v)[GROUPS]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+      k[g] = __builtin_amdgcn_readlane(held_k, 2 * held_at + g);
+      v[g] = __builtin_amdgcn_readlane(held_v, 2 * held_at + g);
+    }
+    ++held_at;
   };
   // This wave's codes at `raw`, times their scale, to its rows of the 16-bit tile at `dst`.
   auto expand = [&](uint32_t raw, const int (&exps)[GROUPS], uint32_t dst) __attribute__((always_inline)) {
@@ -1007,11 +1012,17 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     if constexpr (STAGES == 2) {
       if (more) {
         __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last reads of that stage
-        load_exps(t + WAVES, ids[0], kexp, a.ke_page, ek[STAGES - 1 - ST]);
-        load_exps(t + WAVES, ids[0], vexp, a.ve_page, ev[STAGES - 1 - ST]);
+        if constexpr (DIRECT) {
+          if (held_at == 32) {
+            look_ahead(t + WAVES);
+            __asm__ volatile("" : "+v"(held_id), "+v"(held_k), "+v"(held_v));  // waited for here, not in every round
+          }
+          take_ids();
+          take_exps(ek[1 - ST], ev[1 - ST]);
+        }
         load_rows(t + WAVES, ids[0], kbase, a.k_page, a.k_row, kofs, lds0 + (1 - ST) * TILE);
         load_rows(t + WAVES, ids[0], vbase, a.v_page, a.v_row, vofs, lds0 + VTILE + (1 - ST) * TILE);
-        load_ids(t + 2 * WAVES, ids[0]);
+        if constexpr (!DIRECT) load_ids(t + 2 * WAVES, ids[0]);
         gemm::wait_stage<2 * NI>();
       } else {
         gemm::wait_stage<0>();
@@ -1048,12 +1059,16 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   if constexpr (FEW) {
     int t = t_begin + wave_s;
     if (t < t_end) {
-      load_ids(t, ids[0]);
-      load_exps(t, ids[0], kexp, a.ke_page, ek[0]);
-      load_exps(t, ids[0], vexp, a.ve_page, ev[0]);
+      if constexpr (DIRECT) {
+        look_ahead(t);
+        take_ids();
+      } else {
+        load_ids(t, ids[0]);
+      }
       load_rows(t, ids[0], kbase, a.k_page, a.k_row, kofs, lds0);
       load_rows(t, ids[0], vbase, a.v_page, a.v_row, vofs, lds0 + VTILE);
-      load_ids(t + WAVES, ids[0]);
+      if constexpr (DIRECT) take_exps(ek[0], ev[0]);
+      else load_ids(t + WAVES, ids[0]);
     }
     for (; t < t_end; t += STAGES * WAVES) {
       own_tile(t, std::integral_constant<int, 0>{});
@@ -1123,9 +1138,15 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     start();
     for (int t = t_begin; t < t_end; ++t) {
       if (FEW && ((t - t_begin) & (WAVES - 1)) != wave_s) continue;
-      load_ids(t, ids[0]);
-      load_exps(t, ids[0], kexp, a.ke_page, ek[0]);
-      load_exps(t, ids[0], vexp, a.ve_page, ev[0]);
+      if constexpr (DIRECT) {
+        look_ahead(t);
+        take_ids();
+        take_exps(ek[0], ev[0]);
+      } else {
+        load_ids(t, ids[0]);
+        load_exps(t, ids[0], kexp, a.ke_page, ek[0]);
+        load_exps(t, ids[0], vexp, a.ve_page, ev[0]);
+      }
       load_rows(t, ids[0], kbase, a.k_page, a.k_row, kofs, CODES && !FEW ? raw_k : lds0);
       load_rows(t, ids[0], vbase, a.v_page, a.v_row, vofs, CODES && !FEW ? raw_v : lds0 + VTILE);
       wait_all();
