@@ -13,6 +13,7 @@
 // fewer bits cannot tell from the 64-bit number.  Sines and cosines stand in LDS for all heads of the walk.
 #include "attention_place.h"
 #include "m5k_common.h"
+#include "rope_turn.h"
 
 namespace m5k {
 namespace {
@@ -108,10 +109,6 @@ __device__ __forceinline__ double2 turn64(double a, double magnitude) {
   const double cosine = quarter & 1 ? s : c, sine = quarter & 1 ? c : s;
   return make_double2(quarter == 1 || quarter == 2 ? -cosine * magnitude : cosine * magnitude,
                       quarter >= 2 ? -sine * magnitude : sine * magnitude);
-}
-
-__device__ __forceinline__ float2 to_float2(double2 t) {
-  return make_float2(static_cast<float>(t.x), static_cast<float>(t.y));
 }
 
 // FP32 rounded to odd: cut off, with the last bit set where anything was.
@@ -251,31 +248,37 @@ __global__ __launch_bounds__(T) void append_codes(const AppendArgs a) {
         places[tid] = token >= s && token < e ? a.context[lo] - (e - token) : INT32_MIN;
       }
       __syncthreads();
-      for (int r = tid / PAIRS; r < ROWS && token0 + r < a.tokens && pair < a.pairs; r += TURNS)
-        turns32[r * PAIRS + turn_at<D>(pair)] = to_float2(turn64(places[r] * radians[pair], a.magnitude));
+      for (int r = tid / PAIRS; r < ROWS && token0 + r < a.tokens && pair < a.pairs; r += TURNS) {
+        float2& t = turns32[r * PAIRS + turn_at<D>(pair)];
+        turn_of(places[r], radians[pair], static_cast<float>(a.magnitude), t.x, t.y);
+      }
       __syncthreads();
 #pragma unroll
       for (int pass = 0; pass < PASSES; ++pass) {
         const int r = pass * RPP + row, token = token0 + r;
         if (token >= a.tokens) break;
         const bool known = places[r] != INT32_MIN;
-        for (int h0 = walk0; h0 < head1; h0 += Q_HEADS) {
+        const auto put = [&](int h, const float (&x)[8]) __attribute__((always_inline)) {
+          float y[8];
+          turned8<DT, D>(a.q, h * a.q_head + token * a.q_token, c0, turns32 + r * PAIRS, a.pairs, a.interleaved, x,
+                         [&](int i, float own, float other, float2 u, bool turns_it) {
+            const float z = turns_it ? own * u.x + other * u.y : own;
+            y[i] = known ? z : 0.0f;
+          });
+          store8<DT>(a.q_out, (int64_t{h} * a.tokens + token) * D + c0, y);
+        };
+        int h = walk0;
+        for (; h + Q_HEADS <= head1; h += Q_HEADS) {
           float x[Q_HEADS][8];
 #pragma unroll
-          for (int j = 0; j < Q_HEADS; ++j)
-            if (h0 + j < head1) load8<DT>(a.q, (h0 + j) * a.q_head + token * a.q_token + c0, x[j]);
+          for (int j = 0; j < Q_HEADS; ++j) load8<DT>(a.q, (h + j) * a.q_head + token * a.q_token + c0, x[j]);
 #pragma unroll
-          for (int j = 0; j < Q_HEADS; ++j) {
-            const int h = h0 + j;
-            if (h >= head1) break;
-            float y[8];
-            turned8<DT, D>(a.q, h * a.q_head + token * a.q_token, c0, turns32 + r * PAIRS, a.pairs, a.interleaved, x[j],
-                           [&](int i, float own, float other, float2 u, bool turns_it) {
-              const float z = turns_it ? own * u.x + other * u.y : own;
-              y[i] = known ? z : 0.0f;
-            });
-            store8<DT>(a.q_out, (int64_t{h} * a.tokens + token) * D + c0, y);
-          }
+          for (int j = 0; j < Q_HEADS; ++j) put(h + j, x[j]);
+        }
+        for (; h < head1; ++h) {
+          float x[8];
+          load8<DT>(a.q, h * a.q_head + token * a.q_token + c0, x);
+          put(h, x);
         }
       }
     }
