@@ -650,18 +650,14 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     return has ? base + id * page_stride + fast_div(slot, a.block_magic, a.block_shift)
                : reinterpret_cast<const uint8_t*>(kZeros);
   };
-  // CODES, not FEW: exponents of the 16 keys that this wave loads of tile t.
-  const uint32_t raw_k = lds0 + 4 * TILE + wave_s * 2 * RAW, raw_v = raw_k + RAW;
-  auto load_exps = [&](int t, const int (&id)[NIDS], const uint8_t* base, int64_t page_stride, int (&to)[GROUPS])
-                       __attribute__((always_inline)) {
-    if constexpr (CODES && !FEW) to[0] = *exponent_at(real(t) * KT + first_row, id[0], base, page_stride);
-  };
-  // DIRECT: pages and exponents of the 32 tiles that this wave takes from tile t on, a group of 16 keys a lane, by vector
-  // loads that it waits for once.  By scalar loads a tile, each would hold up the LDS reads issued behind it.
+  // Pages and exponents of the tiles that this wave loads from tile t on, a group of 16 keys a lane, by vector loads that
+  // it waits for once in 32 tiles (FEW) or 64.  Loads a tile would be waited for with the tiles in flight, or, as scalar
+  // loads, hold up the LDS reads behind them.
+  constexpr int HELD = 64 / GROUPS, APART = FEW ? WAVES : 1;
   int held_id = 0, held_k = 0, held_v = 0, held_at = 0;
   auto look_ahead = [&](int t) __attribute__((always_inline)) {
-    if constexpr (DIRECT) {
-      const int key = real(t + WAVES * (lane >> 1)) * KT + 16 * (lane & 1);
+    if constexpr (CODES) {
+      const int key = real(t + APART * (lane / GROUPS)) * KT + first_row + 16 * (lane % GROUPS);
       held_id = table[fast_div(min(key, p.span - 1), a.page_magic, a.page_shift)];
       held_k = *exponent_at(key, held_id, kexp, a.ke_page);
       held_v = *exponent_at(key, held_id, vexp, a.ve_page);
@@ -670,35 +666,45 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   };
   auto take_ids = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int g = 0; g < NIDS; ++g) ids[0][g] = __builtin_amdgcn_readlane(held_id, 2 * held_at + g);
+    for (int g = 0; g < NIDS; ++g) ids[0][g] = __builtin_amdgcn_readlane(held_id, GROUPS * held_at + g);
   };
   auto take_exps = [&](int (&k)[GROUPS], int (&v)[GROUPS]) __attribute__((always_inline)) {
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) {
-      k[g] = __builtin_amdgcn_readlane(held_k, 2 * held_at + g);
-      v[g] = __builtin_amdgcn_readlane(held_v, 2 * held_at + g);
+      k[g] = __builtin_amdgcn_readlane(held_k, GROUPS * held_at + g);
+      v[g] = __builtin_amdgcn_readlane(held_v, GROUPS * held_at + g);
     }
     ++held_at;
   };
-  // This wave's codes at `raw`, times their scale, to its rows of the 16-bit tile at `dst`.
-  auto expand = [&](uint32_t raw, const int (&exps)[GROUPS], uint32_t dst) __attribute__((always_inline)) {
+  // The next tile's, from tile t's lookup if the last one is used up.
+  auto take_next = [&](int t, int (&k)[GROUPS], int (&v)[GROUPS]) __attribute__((always_inline)) {
+    if (held_at == HELD) {
+      look_ahead(t);
+      __asm__ volatile("" : "+v"(held_id), "+v"(held_k), "+v"(held_v));  // waited for here, not in every round
+    }
+    take_ids();
+    take_exps(k, v);
+  };
+  const uint32_t raw_k = lds0 + 4 * TILE + wave_s * 2 * RAW, raw_v = raw_k + RAW;
+  // This wave's codes at `raw`, times their scale, to its rows of the 16-bit tile at `dst`: step `part` of PARTS, of four
+  // for each 16 codes of a lane.
+  constexpr int PARTS = 4 * NI;
+  v4i taken;
+  auto expand = [&](uint32_t raw, int exponent, uint32_t dst, int part) __attribute__((always_inline)) {
     if constexpr (CODES && !FEW) {
-      constexpr int PER = NI / GROUPS;
-#pragma unroll
-      for (int g = 0; g < GROUPS; ++g) {
-        const float scale = code_scale<CODES>(__builtin_amdgcn_readfirstlane(exps[g]));
-#pragma unroll
-        for (int i = g * PER; i < (g + 1) * PER; ++i) {
-          const v4i c = *reinterpret_cast<const __attribute__((address_space(3))) v4i*>(raw + i * 1024 + lane * 16);
-          v4i x[2];
-          expand16<DT, CODES>(c, scale, x);
-          const int r = ld_row + i * RPI;
-          const uint32_t at = dst + r * ROWB + (((2 * ld_chunk) ^ swizzle<D>(r)) << 4);
-          *reinterpret_cast<__attribute__((address_space(3))) v4i*>(at) = x[0];
-          *reinterpret_cast<__attribute__((address_space(3))) v4i*>(at ^ 16) = x[1];
-        }
+      const int i = part >> 2, r = ld_row + i * RPI;
+      const uint32_t at = dst + r * ROWB + (((2 * ld_chunk) ^ swizzle<D>(r)) << 4);
+      if ((part & 3) == 0) taken = *reinterpret_cast<const __attribute__((address_space(3))) v4i*>(raw + i * 1024 + lane * 16);
+      if (part & 2) {
+        const int h = part & 1;
+        *reinterpret_cast<__attribute__((address_space(3))) v4i*>(at ^ (h << 4)) =
+            expand8<DT, CODES>(taken[2 * h], taken[2 * h + 1], code_scale<CODES>(exponent));
       }
     }
+  };
+  auto expand_all = [&](uint32_t raw, int exponent, uint32_t dst) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) expand(raw, exponent, dst, i);
   };
 
   // Fragment addresses in stage 0 (the other stage and the rows further on are instruction offsets): chunk c of a row
@@ -785,7 +791,9 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
       if constexpr (decltype(with_care)::value) __builtin_amdgcn_sched_barrier(0);  // rare: few registers
     }
   };
-  auto product = [&](v16f (&y)[NB], int st, const v16f (&x)[NB], bool prob) __attribute__((always_inline)) {
+  // side(i): what else step i does.
+  auto nothing = [](int) {};
+  auto product = [&](v16f (&y)[NB], int st, const v16f (&x)[NB], bool prob, auto side) __attribute__((always_inline)) {
     if constexpr (DIRECT) {
       // Rows 0 .. 15 and 16 .. 31 of the tile are two groups.
       int e0 = ek[st][0], e1 = ek[st][GROUPS - 1];
@@ -816,6 +824,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
 #pragma unroll
       for (int b = 0; b < NB; ++b) y[b] = mfma32<DT>(kf[c % (AHEAD + 1)][b], qf[c], c == 0 ? v16f{} : y[b]);
       if (prob) probabilities(x, c * EL / QS, (c + 1) * EL / QS, sum, quick);
+      side(c);
       __builtin_amdgcn_sched_barrier(0);
     }
     if (prob) l += sum[0] + sum[1];
@@ -875,7 +884,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     }
   };
   // O += V^T P of a tile, V at stage `st`, in steps of two products as above; beside them the maximum of the scores x.
-  auto accumulate = [&](int st, const v16f (&x)[NB]) __attribute__((always_inline)) -> float {
+  auto accumulate = [&](int st, const v16f (&x)[NB], auto side) __attribute__((always_inline)) -> float {
     constexpr int STEPS = 2 * NB * OB / 2;
     v4i vf[AHEAD + 1][2];
     float t0 = x[0][0], t1 = x[0][1];
@@ -898,6 +907,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
         t0 = fmaxf(t0, x[e >> 4][e & 15]);
         t1 = fmaxf(t1, x[e >> 4][(e & 15) + 1]);
       }
+      side(i);
       __builtin_amdgcn_sched_barrier(0);
     }
     return fmaxf(t0, t1);
@@ -966,41 +976,76 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   // read.
   auto step = [&](int t, auto odd, v16f (&x)[NB], v16f (&next)[NB]) __attribute__((always_inline)) {
     constexpr int ODD = decltype(odd)::value, EVEN = 1 - ODD;
-    wait_all();
-    gemm::stage_barrier();
     if constexpr (CODES) {
-      // The codes of V of tile t + 1 and K of t + 2 are here: expand them, and load those of a tile further on.
-      if (t + 1 < t_end) expand(raw_v, ev[0], lds0 + (2 + ODD) * TILE);
-      if (t + 2 < t_end) {
-        expand(raw_k, ek[0], lds0 + EVEN * TILE);
-        __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        load_exps(t + 2, ids[1], vexp, a.ve_page, ev[0]);
-        load_exps(t + 3, ids[0], kexp, a.ke_page, ek[0]);
-        load_rows(t + 2, ids[1], vbase, a.v_page, a.v_row, vofs, raw_v);
-        if (t + 3 < t_end) load_rows(t + 3, ids[0], kbase, a.k_page, a.k_row, kofs, raw_k);
-      }
-    } else if (t + 1 < t_end) {
-      load_rows(t + 1, ids[1], vbase, a.v_page, a.v_row, vofs, lds0 + (2 + ODD) * TILE);
-      if (t + 2 < t_end) load_rows(t + 2, ids[0], kbase, a.k_page, a.k_row, kofs, lds0 + EVEN * TILE);
+      // The codes of V of tile t + 1 are here, those of K of t + 2 may be on their way: K's wait ends between the products.
+      if (t + 2 < t_end) gemm::wait_stage<NI>();
+      else gemm::wait_stage<0>();
+      __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    } else {
+      wait_all();
     }
+    gemm::stage_barrier();
+    if constexpr (!CODES) {
+      if (t + 1 < t_end) {
+        load_rows(t + 1, ids[1], vbase, a.v_page, a.v_row, vofs, lds0 + (2 + ODD) * TILE);
+        if (t + 2 < t_end) load_rows(t + 2, ids[0], kbase, a.k_page, a.k_row, kofs, lds0 + EVEN * TILE);
+      }
 #pragma unroll
-    for (int i = 0; i < NIDS; ++i) ids[1][i] = ids[0][i];
-    load_ids(t + (CODES ? 4 : 3), ids[0]);
+      for (int i = 0; i < NIDS; ++i) ids[1][i] = ids[0][i];
+      load_ids(t + 3, ids[0]);
+    }
+    // CODES: V of tile t + 1 is expanded beside the first product and K of t + 2 beside the second; then the next codes
+    // of each are loaded.
+    auto expand_v = [&](int i) __attribute__((always_inline)) {
+      if constexpr (CODES) expand(raw_v, ev[0][0], lds0 + (2 + ODD) * TILE, i);
+    };
+    auto expand_k = [&](int i) __attribute__((always_inline)) {
+      if constexpr (CODES) expand(raw_k, ek[0][0], lds0 + EVEN * TILE, i);
+    };
+    auto between = [&]() __attribute__((always_inline)) {
+      if constexpr (CODES) {
+        if (t + 2 < t_end) {
+          ev[0][0] = ev[1][0];
+          load_rows(t + 2, ids[0], vbase, a.v_page, a.v_row, vofs, raw_v);
+          gemm::wait_stage<NI>();
+        }
+      }
+    };
+    auto behind = [&]() __attribute__((always_inline)) {
+      if constexpr (CODES) {
+        if (t + 3 < t_end) {
+          take_next(t + 3, ek[0], ev[1]);
+          load_rows(t + 3, ids[0], kbase, a.k_page, a.k_row, kofs, raw_k);
+        }
+      }
+    };
     uint32_t none;
     const bool now = mine(t), then = mine(t + 1);  // the same for the whole wave
     if (now && then) {
-      product(next, ODD, x, true);
+      product(next, ODD, x, true, expand_v);
+      between();
       finish(next, t + 1, quick, none);
-      adopt(accumulate(EVEN, next), quick);
-    } else if (then) {
-      product(next, ODD, x, false);
+      adopt(accumulate(EVEN, next, expand_k), quick);
+      behind();
+      return;
+    }
+    if constexpr (CODES) {
+#pragma unroll
+      for (int i = 0; i < PARTS; ++i) expand_v(i);
+      between();
+#pragma unroll
+      for (int i = 0; i < PARTS; ++i) expand_k(i);
+      behind();
+    }
+    if (then) {
+      product(next, ODD, x, false, nothing);
       finish(next, t + 1, quick, none);
       adopt(maximum(next), quick);
     } else if (now) {
       float sum[2] = {};
       probabilities(x, 0, EL, sum, quick);
       l += sum[0] + sum[1];
-      accumulate(EVEN, x);
+      accumulate(EVEN, x, nothing);
     }
   };
   // FEW: this wave's tile t, from stage ST.  With two stages the next one (WAVES further on) is on its way to the other
@@ -1012,14 +1057,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     if constexpr (STAGES == 2) {
       if (more) {
         __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last reads of that stage
-        if constexpr (DIRECT) {
-          if (held_at == 32) {
-            look_ahead(t + WAVES);
-            __asm__ volatile("" : "+v"(held_id), "+v"(held_k), "+v"(held_v));  // waited for here, not in every round
-          }
-          take_ids();
-          take_exps(ek[1 - ST], ev[1 - ST]);
-        }
+        if constexpr (DIRECT) take_next(t + WAVES, ek[1 - ST], ev[1 - ST]);
         load_rows(t + WAVES, ids[0], kbase, a.k_page, a.k_row, kofs, lds0 + (1 - ST) * TILE);
         load_rows(t + WAVES, ids[0], vbase, a.v_page, a.v_row, vofs, lds0 + VTILE + (1 - ST) * TILE);
         if constexpr (!DIRECT) load_ids(t + 2 * WAVES, ids[0]);
@@ -1027,10 +1065,10 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
       } else {
         gemm::wait_stage<0>();
       }
-      product(s[0], ST, s[0], false);
+      product(s[0], ST, s[0], false, nothing);
     } else {
       gemm::wait_stage<NI>();  // K, behind which V was issued
-      product(s[0], ST, s[0], false);
+      product(s[0], ST, s[0], false, nothing);
       if (more) {
         __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         load_rows(t + WAVES, ids[0], kbase, a.k_page, a.k_row, kofs, lds0);
@@ -1046,7 +1084,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
       if (more) gemm::wait_stage<NI>();
       else gemm::wait_stage<0>();
     }
-    accumulate(ST, s[0]);
+    accumulate(ST, s[0], nothing);
     if constexpr (STAGES == 1) {
       if (more) {
         __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -1075,21 +1113,21 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
       if (STAGES == 2 && t + WAVES < t_end) own_tile(t + WAVES, std::integral_constant<int, STAGES - 1>{});
     }
   } else if (t_begin < t_end) {
-    load_ids(t_begin, ids[1]);
     if constexpr (CODES) {
-      load_ids(t_begin + 1, ids[0]);
-      load_exps(t_begin, ids[1], kexp, a.ke_page, ek[0]);
-      load_exps(t_begin, ids[1], vexp, a.ve_page, ev[0]);
-      load_rows(t_begin, ids[1], kbase, a.k_page, a.k_row, kofs, raw_k);
-      wait_all();
-      expand(raw_k, ek[0], lds0);
-      __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      load_exps(t_begin + 1, ids[0], kexp, a.ke_page, ek[0]);
-      load_rows(t_begin, ids[1], vbase, a.v_page, a.v_row, vofs, raw_v);
-      if (t_begin + 1 < t_end) load_rows(t_begin + 1, ids[0], kbase, a.k_page, a.k_row, kofs, raw_k);
-      ids[1][0] = ids[0][0];
-      load_ids(t_begin + 2, ids[0]);
+      look_ahead(t_begin);
+      take_ids();
+      load_rows(t_begin, ids[0], kbase, a.k_page, a.k_row, kofs, raw_k);
+      load_rows(t_begin, ids[0], vbase, a.v_page, a.v_row, vofs, raw_v);
+      take_exps(ek[0], ev[0]);
+      gemm::wait_stage<NI>();
+      expand_all(raw_k, ek[0][0], lds0);
+      if (t_begin + 1 < t_end) {
+        __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        take_next(t_begin + 1, ek[0], ev[1]);
+        load_rows(t_begin + 1, ids[0], kbase, a.k_page, a.k_row, kofs, raw_k);
+      }
     } else {
+      load_ids(t_begin, ids[1]);
       load_rows(t_begin, ids[1], kbase, a.k_page, a.k_row, kofs, lds0);
       load_ids(t_begin + 1, ids[0]);
     }
@@ -1138,27 +1176,25 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     start();
     for (int t = t_begin; t < t_end; ++t) {
       if (FEW && ((t - t_begin) & (WAVES - 1)) != wave_s) continue;
-      if constexpr (DIRECT) {
+      if constexpr (CODES) {
         look_ahead(t);
         take_ids();
         take_exps(ek[0], ev[0]);
       } else {
         load_ids(t, ids[0]);
-        load_exps(t, ids[0], kexp, a.ke_page, ek[0]);
-        load_exps(t, ids[0], vexp, a.ve_page, ev[0]);
       }
       load_rows(t, ids[0], kbase, a.k_page, a.k_row, kofs, CODES && !FEW ? raw_k : lds0);
       load_rows(t, ids[0], vbase, a.v_page, a.v_row, vofs, CODES && !FEW ? raw_v : lds0 + VTILE);
       wait_all();
       if constexpr (CODES && !FEW) {
-        expand(raw_k, ek[0], lds0);
-        expand(raw_v, ev[0], lds0 + VTILE);
+        expand_all(raw_k, ek[0][0], lds0);
+        expand_all(raw_v, ev[0][0], lds0 + VTILE);
         wait_all();
       }
       if constexpr (!FEW) gemm::stage_barrier();
       if (mine(t)) {
         uint32_t sees;
-        product(s[0], 0, s[1], false);
+        product(s[0], 0, s[1], false, nothing);
         finish(s[0], t, careful, sees);
         adopt(maximum(s[0]), careful);
         float sum[2] = {};
