@@ -93,10 +93,13 @@ __device__ __forceinline__ v16f mfma32(v4i a, v4i b, v16f c) {
                                                   __builtin_bit_cast(gemm::f16x8, b), c, 0, 0, 0);
 }
 
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+
+// Two values to the inputs' type, to the nearest, by one instruction.
 template <int DT>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   if constexpr (DT == M5K_BF16) return f32x2_to_bf16x2(lo, hi);
-  else return f32_to_f16_bits(lo) | (f32_to_f16_bits(hi) << 16);
+  else return __builtin_bit_cast(uint32_t, __builtin_convertvector((m5k_f32x2{lo, hi}), half2v));
 }
 
 // The other half-wave's value of the same row.
@@ -203,9 +206,17 @@ __device__ __forceinline__ uint32_t code_pair(int w, float scale) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI));
   } else if constexpr (CODES == E4M3) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, HI));
-  } else {
+  } else if constexpr (DT == M5K_BF16) {
     const int w0 = HI ? w << 8 : w << 24, w1 = HI ? w : w << 16;
     return pack2<DT>(static_cast<float>(w0 >> 24) * scale, static_cast<float>(w1 >> 24) * scale);
+  } else {
+    // 1024 + (code + 128) is an FP16 number with the code's bits in its mantissa; the product is FP32's, rounded once.
+    const uint32_t biased = static_cast<uint32_t>(w) ^ 0x80808080u;
+    const uint32_t bits = __builtin_amdgcn_perm(0x64646464u, biased, HI ? 0x07030702u : 0x07010700u);
+    const half2v c = __builtin_bit_cast(half2v, bits) - half2v{1152.0f16, 1152.0f16};
+    const half2v r = {static_cast<_Float16>(__builtin_fmaf(static_cast<float>(c[0]), scale, 0.0f)),
+                      static_cast<_Float16>(__builtin_fmaf(static_cast<float>(c[1]), scale, 0.0f))};
+    return __builtin_bit_cast(uint32_t, r);
   }
 }
 
@@ -523,6 +534,8 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     }
   }
   if constexpr (CODES && !FEW) __syncthreads();  // the bounds have been read
+  // Whether a row of this wave has first keys in the window's tiles.
+  const bool both = SINKS && __builtin_amdgcn_ballot_w64(rr.slo < rr.shi && with_window) != 0;
   // Tile t lies at real(t), and a window's tile T is tile t = T - ahead.
   const int window_tile = SINKS ? lo / KT : 0, ahead = window_tile - kept;
   auto real = [&](int t) __attribute__((always_inline)) {
@@ -863,24 +876,35 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
       }
     }
     if (careful || key0 < all_lo || key0 + KT > all_hi) {
-      const uint32_t width = static_cast<uint32_t>(max(rr.hi - rr.lo, 0));
-      const uint32_t first_keys = SINKS ? static_cast<uint32_t>(max(rr.shi - rr.slo, 0)) : 0;
       if constexpr (careful) sees_bits = 0;
+      // SINKS: a tile of first keys shows those, the others the window; one that holds both is compared with both.
+      const bool kept_here = SINKS && D == 64 && t < kept;
+      const int from = kept_here ? rr.slo : rr.lo;
+      const uint32_t width = static_cast<uint32_t>(max(kept_here ? rr.shi - rr.slo : rr.hi - rr.lo, 0));
+      const uint32_t first_keys = SINKS ? static_cast<uint32_t>(max(rr.shi - rr.slo, 0)) : 0;
+      auto compare = [&](auto with_both) __attribute__((always_inline)) {
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int key = kofs0 + 32 * b + 8 * (r >> 2) + (r & 3);
-          bool sees = static_cast<uint32_t>(key - rr.lo) < width;
-          if constexpr (SINKS) sees |= static_cast<uint32_t>(key - rr.slo) < first_keys;
-          if constexpr (KEYS != DENSE && careful) {
-            if (sees)
-              sees = static_cast<uint32_t>(table[fast_div(key, a.page_magic, a.page_shift)]) <
-                     static_cast<uint32_t>(a.pages);
+          for (int r = 0; r < 16; ++r) {
+            const int key = kofs0 + 32 * b + 8 * (r >> 2) + (r & 3);
+            bool sees = static_cast<uint32_t>(key - from) < width;
+            if constexpr (decltype(with_both)::value) sees |= static_cast<uint32_t>(key - rr.slo) < first_keys;
+            if constexpr (KEYS != DENSE && careful) {
+              if (sees)
+                sees = static_cast<uint32_t>(table[fast_div(key, a.page_magic, a.page_shift)]) <
+                       static_cast<uint32_t>(a.pages);
+            }
+            if constexpr (careful) sees_bits |= static_cast<uint32_t>(sees) << (16 * b + r);
+            x[b][r] = sees ? x[b][r] : -__builtin_inff();
           }
-          if constexpr (careful) sees_bits |= static_cast<uint32_t>(sees) << (16 * b + r);
-          x[b][r] = sees ? x[b][r] : -__builtin_inff();
-        }
+      };
+      if constexpr (SINKS) {
+        if (D == 128 || (!kept_here && both)) compare(std::true_type{});
+        else compare(std::false_type{});
+      } else {
+        compare(std::false_type{});
+      }
     }
   };
   // O += V^T P of a tile, V at stage `st`, in steps of two products as above; beside them the maximum of the scores x.
