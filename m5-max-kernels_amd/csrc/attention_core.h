@@ -267,6 +267,11 @@ __device__ __forceinline__ RowRange row_range(int s, int e, int p, int prefix, i
   return RowRange{lo, hi, p, slo, shi};
 }
 
+// Bits 0 .. n - 1 of a word.
+__device__ __forceinline__ uint32_t bits_below(int n) {
+  return n <= 0 ? 0u : 0xFFFFFFFFu >> (32 - min(n, 32));
+}
+
 // The last b in [0, n) with key(b) <= x, by binary search over a nondecreasing key; 0 if there is none.
 template <class Key>
 __device__ __forceinline__ int last_not_above(int n, int x, Key key) {
@@ -279,16 +284,21 @@ __device__ __forceinline__ int last_not_above(int n, int x, Key key) {
   return lo;
 }
 
+// Minimum and maximum over the wave: lane movement within the rows of 16, then four scalars.  (By five shuffles through
+// LDS each, the four or seven of a workgroup's beginning cost it half a microsecond.)
+template <int CTRL>
+__device__ __forceinline__ int moved(int v) {
+  return __builtin_amdgcn_update_dpp(v, v, CTRL, 0xF, 0xF, false);
+}
 __device__ __forceinline__ int wave_min_i(int v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v = min(v, __shfl_xor(v, o));
-  return __builtin_amdgcn_readfirstlane(v);
+  v = min(v, moved<0xB1>(v));   // quad_perm [1,0,3,2]
+  v = min(v, moved<0x4E>(v));   // quad_perm [2,3,0,1]
+  v = min(v, moved<0x141>(v));  // row_half_mirror
+  v = min(v, moved<0x140>(v));  // row_mirror
+  return min(min(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+             min(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
 }
-__device__ __forceinline__ int wave_max_i(int v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v = max(v, __shfl_xor(v, o));
-  return __builtin_amdgcn_readfirstlane(v);
-}
+__device__ __forceinline__ int wave_max_i(int v) { return -wave_min_i(-v); }
 
 // tanh in FP32 to a few units of its last place: the series below 1/4 (first term left out 9e-3 y^11), elsewhere
 // 1 - 2 / (e^(2y) + 1), whose absolute error is 1e-7.
@@ -474,6 +484,16 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   int token, head;
   const RowRange rr = range_of<KEYS, SINKS>(a, p, min(row, p.rows - 1), token, head);
 
+  v4i qf[QS];
+  {
+    const uint16_t* qp = a.q + int64_t{head} * a.q_head + int64_t{token} * a.q_token + 8 * half;
+#pragma unroll
+    for (int s = 0; s < QS; ++s) {
+      // DIRECT: the channel order of K's fragments, two from the 16 codes of one read.
+      const int channel = DIRECT ? 32 * (s >> 1) + 8 * half + 8 * (s & 1) : 16 * s;
+      qf[s] = *reinterpret_cast<const v4i*>(qp + channel);
+    }
+  }
   // Key ranges: of the wave (any row, every row), and of the workgroup.
   const bool idle = !FEW && row0 + 32 * wave >= p.rows;
   int any_lo = idle ? NEVER : wave_min_i(rr.lo);
@@ -534,8 +554,6 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     }
   }
   if constexpr (CODES && !FEW) __syncthreads();  // the bounds have been read
-  // Whether a row of this wave has first keys in the window's tiles.
-  const bool both = SINKS && __builtin_amdgcn_ballot_w64(rr.slo < rr.shi && with_window) != 0;
   // Tile t lies at real(t), and a window's tile T is tile t = T - ahead.
   const int window_tile = SINKS ? lo / KT : 0, ahead = window_tile - kept;
   auto real = [&](int t) __attribute__((always_inline)) {
@@ -554,16 +572,6 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     }
   }
 
-  v4i qf[QS];
-  {
-    const uint16_t* qp = a.q + int64_t{head} * a.q_head + int64_t{token} * a.q_token + 8 * half;
-#pragma unroll
-    for (int s = 0; s < QS; ++s) {
-      // DIRECT: the channel order of K's fragments, two from the 16 codes of one read.
-      const int channel = DIRECT ? 32 * (s >> 1) + 8 * half + 8 * (s & 1) : 16 * s;
-      qf[s] = *reinterpret_cast<const v4i*>(qp + channel);
-    }
-  }
   const float scale2 = a.scale * LOG2E;
   const float unit = MODS ? 1.0f : scale2;  // what turns finished scores into base 2, launch_unit()
   const float slope2 = MODS && a.slopes ? a.slopes[head] * LOG2E : 0.0f;
@@ -875,36 +883,39 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
         }
       }
     }
-    if (careful || key0 < all_lo || key0 + KT > all_hi) {
-      if constexpr (careful) sees_bits = 0;
-      // SINKS: a tile of first keys shows those, the others the window; one that holds both is compared with both.
-      const bool kept_here = SINKS && D == 64 && t < kept;
-      const int from = kept_here ? rr.slo : rr.lo;
-      const uint32_t width = static_cast<uint32_t>(max(kept_here ? rr.shi - rr.slo : rr.hi - rr.lo, 0));
-      const uint32_t first_keys = SINKS ? static_cast<uint32_t>(max(rr.shi - rr.slo, 0)) : 0;
-      auto compare = [&](auto with_both) __attribute__((always_inline)) {
+    if constexpr ((SINKS || CODES) && !careful) {
+      if (key0 >= all_lo && key0 + KT <= all_hi) return;
+      // The lane's keys of the tile as bits, and two instructions a score.
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
+      for (int b = 0; b < NB; ++b) {
+        const int at = kofs0 + 32 * b;
+        uint32_t seen = bits_below(rr.hi - at) & ~bits_below(rr.lo - at);
+        if constexpr (SINKS) seen |= bits_below(rr.shi - at) & ~bits_below(rr.slo - at);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int key = kofs0 + 32 * b + 8 * (r >> 2) + (r & 3);
-            bool sees = static_cast<uint32_t>(key - from) < width;
-            if constexpr (decltype(with_both)::value) sees |= static_cast<uint32_t>(key - rr.slo) < first_keys;
-            if constexpr (KEYS != DENSE && careful) {
-              if (sees)
-                sees = static_cast<uint32_t>(table[fast_div(key, a.page_magic, a.page_shift)]) <
-                       static_cast<uint32_t>(a.pages);
-            }
-            if constexpr (careful) sees_bits |= static_cast<uint32_t>(sees) << (16 * b + r);
-            x[b][r] = sees ? x[b][r] : -__builtin_inff();
-          }
-      };
-      if constexpr (SINKS) {
-        if (D == 128 || (!kept_here && both)) compare(std::true_type{});
-        else compare(std::false_type{});
-      } else {
-        compare(std::false_type{});
+        for (int r = 0; r < 16; ++r) {
+          const uint32_t keep = __builtin_amdgcn_sbfe(seen, 8 * (r >> 2) + (r & 3), 1);
+          x[b][r] = __uint_as_float((keep & __float_as_uint(x[b][r])) | (~keep & 0xFF800000u));
+        }
       }
+    } else if (careful || key0 < all_lo || key0 + KT > all_hi) {
+      const uint32_t width = static_cast<uint32_t>(max(rr.hi - rr.lo, 0));
+      const uint32_t first_keys = SINKS ? static_cast<uint32_t>(max(rr.shi - rr.slo, 0)) : 0;
+      if constexpr (careful) sees_bits = 0;
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = kofs0 + 32 * b + 8 * (r >> 2) + (r & 3);
+          bool sees = static_cast<uint32_t>(key - rr.lo) < width;
+          if constexpr (SINKS) sees |= static_cast<uint32_t>(key - rr.slo) < first_keys;
+          if constexpr (KEYS != DENSE && careful) {
+            if (sees)
+              sees = static_cast<uint32_t>(table[fast_div(key, a.page_magic, a.page_shift)]) <
+                     static_cast<uint32_t>(a.pages);
+          }
+          if constexpr (careful) sees_bits |= static_cast<uint32_t>(sees) << (16 * b + r);
+          x[b][r] = sees ? x[b][r] : -__builtin_inff();
+        }
     }
   };
   // O += V^T P of a tile, V at stage `st`, in steps of two products as above; beside them the maximum of the scores x.
