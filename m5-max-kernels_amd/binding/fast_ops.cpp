@@ -729,12 +729,16 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   Codes e{};
   const bool coded = nargs == 14 && (args[12] != Py_None || args[13] != Py_None);
   if (coded && !codes_of(args + 12, c, e)) Py_RETURN_NONE;
+  // m5k_attention_plan's name for the cache.
+  const int kind = !coded ? 1
+                          : (e.mode == M5K_QUANT_FP8 ? 2 : 4) + (c.dim == 128 ? 8 : 0) +
+                                (args[8] != Py_None || args[9] != Py_None ? 16 : 0);
   const at::Tensor* q = heads_of(args[0]);
   const c10::Device dev = c.k->device();
   if (!optional_vector(args[10], c.sequences, at::kInt, dev, &prefix) || (prefix && args[7] != Py_None) ||
       !rows16(*c.k) || !rows16(*c.v) ||
       !q || !scores_of(q, c.kv_heads, c.dim, coded ? q->scalar_type() : c.k->scalar_type(), dev, args[6], args[8],
-                       args[7], nargs == 14 ? args[11] : Py_None, args[9], coded ? 2 : 1, true, c.sequences,
+                       args[7], nargs == 14 ? args[11] : Py_None, args[9], kind, true, c.sequences,
                        c.width * c.page_size, s))
     Py_RETURN_NONE;
   void* stream = nullptr;

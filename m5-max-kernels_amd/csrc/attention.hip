@@ -95,7 +95,8 @@ int64_t reach(int64_t keys, int64_t window, int64_t sinks, bool causal) {
 extern "C" int m5k_attention_plan(int paged, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t sequences,
                                   int64_t keys, int cus, int* splits, int* few) {
   m5k::clear_error();
-  M5K_REQUIRE(paged >= 0 && paged <= 2, "attention_plan: paged must be 0, 1 or 2");
+  M5K_REQUIRE(paged == 0 || paged == 1 || (paged > 1 && paged < 32 && ((paged & 7) == 2 || (paged & 7) == 4)),
+              "attention_plan: bad paged");
   M5K_REQUIRE(splits && tokens > 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && sequences >= 0 && keys >= 0,
               "attention_plan: bad sizes");
   if (cus <= 0) cus = m5k::device_cus();

@@ -188,8 +188,8 @@ __device__ __forceinline__ v4i rows_rsrc(const Elem* p, int rows, int64_t stride
 
 constexpr int NEVER = 0x3FFFFFFF;  // behind every key
 
-// A block's scale, 2^(e - 127), as code_pair takes it.  E4M3: e in FP32's exponent field, which is all that its conversion
-// reads.  INT8: the number, which for e = 0 has no exponent field of its own; NaN for e = 255.
+// A block's scale, 2^(e - 127), as code_pair takes it.  E4M3: e in FP32's exponent field, which is all that its
+// conversion reads.  INT8: the number, which for e = 0 has no exponent field of its own; NaN for e = 255.
 template <int CODES>
 __device__ __forceinline__ float code_scale(int e) {
   uint32_t bits = static_cast<uint32_t>(e) << 23;
@@ -197,9 +197,9 @@ __device__ __forceinline__ float code_scale(int e) {
   return __uint_as_float(bits);
 }
 
-// Two codes, bytes 2 HI and 2 HI + 1 of a word, times their scale, as 16-bit values.  Exact in BF16, which has more bits
-// than a code and FP32's range; rounded once to FP16, which only numbers below 2^-14 need.  E4M3: one conversion, whose
-// results are those of an FP32 product rounded to the type, for every code and exponent (compared on MI355X).
+// Two codes, bytes 2 HI and 2 HI + 1 of a word, times their scale, as 16-bit values.  Exact in BF16, which has more
+// bits than a code and FP32's range; rounded once to FP16, which only numbers below 2^-14 need.  E4M3: one conversion,
+// whose results are those of an FP32 product rounded to the type, for every code and exponent (compared on MI355X).
 template <int DT, int CODES, bool HI>
 __device__ __forceinline__ uint32_t code_pair(int w, float scale) {
   if constexpr (CODES == E4M3 && DT == M5K_BF16) {
@@ -443,11 +443,12 @@ __device__ __forceinline__ RowRange range_of(const Args& a, const Place& p, int 
 // SINKS: rows see their span's first keys beside their window.  The workgroup's tiles are those of the first keys, then
 // those of the windows: `t` counts them, real(t) is where tile t lies.
 //
-// CODES: K and V are codes of 8 bits with an exponent byte a block of tokens.  They go to LDS as they are.  With FEW the
-// products' fragments are made from them as they are read: two tiles of each operand then take less LDS than one of
-// 16 bits, and no code is read twice.  Otherwise they go, times their scale, to the tile of 16-bit values that the
-// products read: by the wave that loaded them, so that no barrier stands between and each code is expanded once a
-// workgroup, not once a wave.
+// CODES: K and V are codes of 8 bits with an exponent byte a block of tokens.  They go to LDS as they are.  With FEW
+// the products' fragments are made from them as they are read: two tiles of each operand then take less LDS than one of
+// 16 bits, and no code is read twice (131073 keys, 8 key heads of 128, E4M3: by way of a 16-bit tile 105 us, so 64).
+// Otherwise they go, times their scale, to the tile of 16-bit values that the products read: by the wave that loaded
+// them, so that no barrier stands between and each code is expanded once a workgroup, not once a wave, in steps beside
+// the products (chunks of up to 1024 tokens over up to 8192 keys: ahead of them 246 us, so 207; 16-bit values 182).
 template <int DT, int D, int KEYS, bool MODS, bool FEW, bool SINKS, int CODES>
 __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   static_assert(CODES == NO_CODES || KEYS == PAGES16, "codes lie in pages of a multiple of 16");
@@ -671,9 +672,9 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     return has ? base + id * page_stride + fast_div(slot, a.block_magic, a.block_shift)
                : reinterpret_cast<const uint8_t*>(kZeros);
   };
-  // Pages and exponents of the tiles that this wave loads from tile t on, a group of 16 keys a lane, by vector loads that
-  // it waits for once in 32 tiles (FEW) or 64.  Loads a tile would be waited for with the tiles in flight, or, as scalar
-  // loads, hold up the LDS reads behind them.
+  // Pages and exponents of the tiles that this wave loads from tile t on, a group of 16 keys a lane, by vector loads
+  // that it waits for once in 32 tiles (FEW) or 64.  Loads a tile would be waited for with the tiles in flight, or, as
+  // scalar loads, hold up the LDS reads behind them (64 single tokens over 0 to 8190 keys, INT8: 130 us and 120).
   constexpr int HELD = 64 / GROUPS, APART = FEW ? WAVES : 1;
   int held_id = 0, held_k = 0, held_v = 0, held_at = 0;
   auto look_ahead = [&](int t) __attribute__((always_inline)) {
@@ -707,7 +708,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     take_exps(k, v);
   };
   const uint32_t raw_k = lds0 + 4 * TILE + wave_s * 2 * RAW, raw_v = raw_k + RAW;
-  // This wave's codes at `raw`, times their scale, to its rows of the 16-bit tile at `dst`: step `part` of PARTS, of four
+  // This wave's codes at `raw`, times their scale, to its rows of the 16-bit tile at `dst`: step `part` of PARTS, four
   // for each 16 codes of a lane.
   constexpr int PARTS = 4 * NI;
   v4i taken;
@@ -715,7 +716,8 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     if constexpr (CODES && !FEW) {
       const int i = part >> 2, r = ld_row + i * RPI;
       const uint32_t at = dst + r * ROWB + (((2 * ld_chunk) ^ swizzle<D>(r)) << 4);
-      if ((part & 3) == 0) taken = *reinterpret_cast<const __attribute__((address_space(3))) v4i*>(raw + i * 1024 + lane * 16);
+      if ((part & 3) == 0)
+        taken = *reinterpret_cast<const __attribute__((address_space(3))) v4i*>(raw + i * 1024 + lane * 16);
       if (part & 2) {
         const int h = part & 1;
         *reinterpret_cast<__attribute__((address_space(3))) v4i*>(at ^ (h << 4)) =
@@ -766,8 +768,8 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     for (int b = 0; b < NB; ++b)
       f[b] = *reinterpret_cast<const __attribute__((address_space(3))) v4i*>(kread[c] + b * 32 * ROWB + st * TILE);
   };
-  // V^T fragment of k-step c and channel block b: keys 16 c + 8 h + 4 (lane >> 5) .. + 3 for h = 0, 1.  DIRECT: its codes,
-  // which value_of makes a fragment of.
+  // V^T fragment of k-step c and channel block b: keys 16 c + 8 h + 4 (lane >> 5) .. + 3 for h = 0, 1.  DIRECT: its
+  // codes, which value_of makes a fragment of.
   auto value_frag = [&](int st, int c, int b) __attribute__((always_inline)) {
     v4i f{};
     if constexpr (DIRECT) {
@@ -1012,7 +1014,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   auto step = [&](int t, auto odd, v16f (&x)[NB], v16f (&next)[NB]) __attribute__((always_inline)) {
     constexpr int ODD = decltype(odd)::value, EVEN = 1 - ODD;
     if constexpr (CODES) {
-      // The codes of V of tile t + 1 are here, those of K of t + 2 may be on their way: K's wait ends between the products.
+      // The codes of V of tile t + 1 are here, those of K of t + 2 may be on their way until the second product.
       if (t + 2 < t_end) gemm::wait_stage<NI>();
       else gemm::wait_stage<0>();
       __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -1448,16 +1450,27 @@ __global__ __launch_bounds__(256) void attention_join(const Args a) {
 // evenly spread: 161, 170; at random: 228, 236 and 208, 201; spread over the logarithm: 146, 105; 65 of these: 148, 97.
 // Beyond the limit `few` is mostly the better one, by up to a third; tiles are where lengths are spread evenly, and
 // where few key heads just fill the chip.  The limit has not been moved to what these say.
+//
+// Codes.  `few` takes them without a detour, so it goes further, up to 64 rows on average whatever their number.  32 on
+// 8 heads, tiles and `few`, E4M3 / INT8: 64 sequences of 16 tokens over 2048 keys, heads of 128 109, 85 / 127, 106 us,
+// of 64 82, 53 / 88, 68; single tokens of 64 sequences, 56 heads on 8 of 128, 0 to 8190 keys, INT8 201 and 120.  INT8
+// and heads of 64 pay more for expanding a code in every workgroup of 32 rows: 8 sequences of 64 tokens over 4096 keys,
+// INT8, 71 and 82, heads of 64 47 and 53, but E4M3 with heads of 128 64 and 54.  With a cap or bias, heads of 128 in
+// tiles have more in registers than there is room for: cap, chunks of up to 1024 tokens over up to 8192 keys 431 and
+// 290 / 465 and 410, 8192 tokens 948 and 925 / 1008 and 1303.
 struct Plan {
   bool few;
   int slots;
 };
-enum Paged { UNPAGED = 0, PAGED = 1, CODED = 2 };
-inline Plan plan(int paged, int64_t tokens, int group, int kv_heads, int64_t sequences, int64_t keys, int cus) {
+enum Kind { UNPAGED = 0, PAGED = 1, E4M3_PAGES = 2, INT8_PAGES = 4, WIDE_HEADS = 8, SCORE_MODS = 16 };  // bits
+inline Plan plan(int kind, int64_t tokens, int group, int kv_heads, int64_t sequences, int64_t keys, int cus) {
+  const bool paged = kind != UNPAGED, codes = kind & (E4M3_PAGES | INT8_PAGES);
+  const bool spills = kind & SCORE_MODS && kind & WIDE_HEADS, cheap = kind & E4M3_PAGES && kind & WIDE_HEADS;
   const int64_t rows = tokens * group, own = paged ? sequences : 1;
   const int64_t tiles = (rows / (32 * WAVES) + own) * kv_heads, thin = (rows / 32 + own) * kv_heads;
-  const bool few = (rows <= 32 * own && (paged == CODED || own * kv_heads < 2 * cus)) ||
-                   (tiles < cus && thin <= (keys < 512 ? 2 : 4) * cus && keys <= 4096);
+  bool few = tiles < cus && thin <= (keys < 512 || (codes && !cheap) ? 2 : 4) * cus && keys <= 4096;
+  if (codes) few = few || rows <= 64 * own || (spills && (cheap || tiles <= 4 * cus));
+  else few = few || (rows <= 32 * own && own * kv_heads < 2 * cus);
   const int64_t r = few ? 32 : 32 * WAVES;
   return Plan{few, static_cast<int>(paged ? rows / r + sequences + 1 : (rows + r - 1) / r)};
 }
@@ -1466,9 +1479,10 @@ inline Plan plan(int paged, int64_t tokens, int group, int kv_heads, int64_t seq
 // of the longest span; twice as many were slower (2048 tokens, 8 heads: 22 and 36 us).  Full workgroups of `few` to
 // one: their waves split the keys already, and the sums of 32 rows cost as much as their keys (2000 tokens, 4 query
 // heads on one key head, 250 workgroups: 19 us, 26 us in two splits).
-inline int plan_splits(int paged, int64_t tokens, int group, int kv_heads, int64_t sequences, int64_t keys,
+inline int plan_splits(int kind, int64_t tokens, int group, int kv_heads, int64_t sequences, int64_t keys,
                        int cus) {
-  const Plan p = plan(paged, tokens, group, kv_heads, sequences, keys, cus);
+  const bool paged = kind != UNPAGED;
+  const Plan p = plan(kind, tokens, group, kv_heads, sequences, keys, cus);
   // Slots that have rows: of a paged launch about half a tile a sequence on top of the whole ones.
   const int64_t r = p.few ? 32 : 32 * WAVES, whole = tokens * group / r, own = tokens < sequences ? tokens : sequences;
   const int64_t tiles = !paged ? p.slots : whole + own / 2 > own ? whole + own / 2 : own;
@@ -1486,15 +1500,19 @@ int launch_join(const Args& a, int dtype, int head_dim, hipStream_t st);
 template <int DT, int D, int KEYS, bool SINKS, int CODES>
 int launch(Args& a, hipStream_t st) {
   const bool mods = a.softcap > 0.0f || a.slopes;
-  const Plan p = plan(KEYS == DENSE ? UNPAGED : CODES ? CODED : PAGED, a.tokens, a.group, a.kv_heads, a.sequences, a.reach, device_cus());
+  constexpr int KIND = KEYS == DENSE ? UNPAGED : !CODES ? PAGED : (CODES == E4M3 ? E4M3_PAGES : INT8_PAGES) |
+                                                                      (D == 128 ? WIDE_HEADS : 0);
+  const Plan p = plan(KIND | (CODES && mods ? SCORE_MODS : 0), a.tokens, a.group, a.kv_heads, a.sequences, a.reach,
+                      device_cus());
   a.slots = p.slots;
   a.cus = device_cus();
   a.spread = a.kv_heads % 8 != 0 && (KEYS != DENSE || a.causal || a.starts);
   const int64_t blocks = int64_t{a.slots} * a.kv_heads * a.splits;
   M5K_REQUIRE(blocks <= INT32_MAX, "attention: too many tiles for one launch");
+  constexpr bool ALWAYS_FEW = CODES == E4M3 && D == 128;  // with MODS
   auto kernel = p.few ? (mods ? attention_tile<DT, D, KEYS, true, true, SINKS, CODES>
                               : attention_tile<DT, D, KEYS, false, true, SINKS, CODES>)
-                      : (mods ? attention_tile<DT, D, KEYS, true, false, SINKS, CODES>
+                      : (mods ? attention_tile<DT, D, KEYS, true, ALWAYS_FEW, SINKS, CODES>
                               : attention_tile<DT, D, KEYS, false, false, SINKS, CODES>);
   launch_kernel(kernel, dim3(static_cast<uint32_t>(blocks)), dim3(THREADS), st, a);
   int rc = launch_status("attention");

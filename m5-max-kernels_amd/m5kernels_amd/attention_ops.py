@@ -391,6 +391,11 @@ def _plan(paged, tokens, heads, kv_heads, sequences, keys, cus):
     return n.value, bool(few.value)
 
 
+def _coded_plan(mode, width, modified):
+    """What m5k_attention_plan calls a cache of codes."""
+    return (2 if mode == _lib.QUANT_FP8 else 4) + 8 * (width == 128) + 16 * modified
+
+
 def _first_keys(sinks, window):
     if sinks is None:
         return 0
@@ -495,7 +500,8 @@ def paged_attention(q, k_cache, v_cache, page_table, query_starts, context_lengt
     q = _rows(q, "q")
     qs = _strides(q)
     pages, page_size = k_cache.shape[0], k_cache.shape[2]
-    splits, _ = _plan(2 if codes else 1, tokens, heads, kv_heads, sequences, _reach(table_width * page_size, window, sinks, True),
+    kind = _coded_plan(codes[0], width, softcap > 0 or slopes is not None) if codes else 1
+    splits, _ = _plan(kind, tokens, heads, kv_heads, sequences, _reach(table_width * page_size, window, sinks, True),
                       hip._cu_count_of(device.index))
     workspace, n = _workspace(splits, tokens, heads, width, device)
     name, mode, k_more, v_more = "m5k_paged_attention_sinks", (), (), ()

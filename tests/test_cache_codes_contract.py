@@ -115,8 +115,8 @@ def test_c_entries_check_before_launching():
     def attend(mode=0, block=16, slot=64, exps=p, sinks=0, window=0):
         row = (4096, 2048, slot)
         return lib.m5k_paged_attention_codes(
-            p, _lib.BF16, 5, 4, 64, 320, 64, mode, p, *row, exps, 4, 2, p, *row, p, 4, 2, block, 6, 32, 2, p, 4, 3, p, p,
-            ctypes.c_float(0.1), window, sinks, ctypes.c_float(0), None, None, p, 1, None, 0, None)
+            p, _lib.BF16, 5, 4, 64, 320, 64, mode, p, *row, exps, 4, 2, p, *row, p, 4, 2, block, 6, 32, 2, p, 4, 3, p,
+            p, ctypes.c_float(0.1), window, sinks, ctypes.c_float(0), None, None, p, 1, None, 0, None)
 
     for kw, word in ((dict(mode=7), b"codes"), (dict(block=8), b"block"), (dict(block=24), b"block"),
                      (dict(slot=32), b"apart"), (dict(slot=72), b"aligned"), (dict(exps=None), b"null"),
@@ -138,6 +138,7 @@ def test_c_entries_check_before_launching():
         return lib.m5k_paged_read(0, p, *rows, p, 4, 2, p, *rows, p, 4, 2, 16, 6, 32, 2, 64, p, 4, 3, p, p, tokens, out,
                                   p, dtype, None)
 
-    for kw, word in ((dict(dtype=9), b"dtype"), (dict(tokens=0), b"tokens"), (dict(out=ctypes.c_void_p(8)), b"aligned")):
+    for kw, word in ((dict(dtype=9), b"dtype"), (dict(tokens=0), b"tokens"),
+                     (dict(out=ctypes.c_void_p(8)), b"aligned")):
         assert read(**kw) == 1
         assert word in lib.m5k_last_error(), (kw, lib.m5k_last_error())

@@ -74,8 +74,9 @@ def test_chunks(d, page, block, dtype, mode, device):
            device)
 
 
-def _forms(tokens, heads, kv_heads, sequences, keys):
-    return module._plan(1, tokens, heads, kv_heads, sequences, keys, 256)
+def _forms(tokens, heads, kv_heads, sequences, keys, mode=U8, d=128, modified=False):
+    kind = module._coded_plan(_lib.QUANT_FP8 if mode == U8 else _lib.QUANT_INT8, d, modified)
+    return module._plan(kind, tokens, heads, kv_heads, sequences, keys, 256)
 
 
 @pytest.mark.parametrize("mode,dtype", [(U8, BF16), (I8, F16), (I8, BF16)])
@@ -83,7 +84,7 @@ def _forms(tokens, heads, kv_heads, sequences, keys):
 def test_tiles_of_128_rows(d, dtype, mode, device):
     """Rows enough for the form whose waves share key tiles, unsplit, with and without the rest of the options."""
     c = _case([700, 350, 1], [900, 350, 40], hq=128, hkv=64, d=d, mode=mode, dtype=dtype, page=32, block=32)
-    splits, few = _forms(1051, 128, 64, 3, c["table"].shape[1] * 32)
+    splits, few = _forms(1051, 128, 64, 3, c["table"].shape[1] * 32, mode, d)
     assert not few and splits == 1
     _check(c, device)
     _check(c, device, softcap=20.0, slopes=torch.exp2(-8 * torch.arange(1, 129).float() / 128))
@@ -94,7 +95,7 @@ def test_tiles_of_128_rows(d, dtype, mode, device):
 @pytest.mark.parametrize("d", [64, 128])
 def test_key_splits(new, context, d, mode, device):
     c = _case(new, context, d=d, mode=mode, page=64, block=64)
-    assert _forms(sum(new), 8, 2, len(new), c["table"].shape[1] * 64)[0] > 1
+    assert _forms(sum(new), 8, 2, len(new), c["table"].shape[1] * 64, mode, d)[0] > 1
     _check(c, device)
     _check(c, device, window=300)
 

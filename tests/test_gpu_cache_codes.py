@@ -82,8 +82,8 @@ def _same(got, want):
                                           (128, 64, 16), (128, 96, 32), (128, 48, 48), (128, 64, 64), (128, 256, 128)])
 def test_append(d, page, block, dtype, mode, device):
     """One token, none, chunks that begin and end inside blocks and on their borders, fresh sequences."""
-    case = Case([1, 0, 70, 33, 1, 16, 150, 1], [1, 40, 70, 100, 17, 48, 151, 16], d=d, page=page, block=block, mode=mode,
-                dtype=dtype)
+    case = Case([1, 0, 70, 33, 1, 16, 150, 1], [1, 40, 70, 100, 17, 48, 151, 16], d=d, page=page, block=block,
+                mode=mode, dtype=dtype)
     out, got = case.append(device)
     assert out is None
     _same(got, case.want())
