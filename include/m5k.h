@@ -455,9 +455,9 @@ int m5k_attention_sinks(const void* q, int dtype, int64_t tokens, int64_t heads,
 
 /* The plan of m5k_attention (paged 0, sequences = documents), m5k_paged_attention (paged 1,
  * keys = table_width * page_size) or m5k_paged_attention_codes (paged 2 for FP8 codes or 4 for INT8, plus 8 with
- * head_dim 128, plus 16 with a softcap or slopes) on `cus` compute units (host only; cus <= 0: those of the current device): the key
- * splits that pay, and whether the waves of a workgroup share 32 rows (few 1) or take 32 each (few 0; few may be
- * NULL). */
+ * head_dim 128, plus 16 with a softcap or slopes) on `cus` compute units (host only; cus <= 0: those of the current
+ * device): the key splits that pay, and whether the waves of a workgroup share 32 rows (few 1) or take 32 each (few 0;
+ * few may be NULL). */
 int m5k_attention_plan(int paged, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t sequences, int64_t keys,
                        int cus, int* splits, int* few);
 

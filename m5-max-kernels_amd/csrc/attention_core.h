@@ -665,12 +665,12 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     }
   };
 
-  // CODES: where the exponent of a key's block lies, on a page `id` (or a 0, where that is none).
-  auto exponent_at = [&](int key, int id, const uint8_t* base, int64_t page_stride) __attribute__((always_inline)) {
+  // CODES: the exponent of a key's block on page `id`, 0 where there is none.
+  auto exponent_of = [&](int key, int id, const uint8_t* base, int64_t page_stride) __attribute__((always_inline)) {
     const int slot = key - static_cast<int>(fast_div(key, a.page_magic, a.page_shift)) * a.page_size;
     const bool has = key < p.span && static_cast<uint32_t>(id) < static_cast<uint32_t>(a.pages);
-    return has ? base + id * page_stride + fast_div(slot, a.block_magic, a.block_shift)
-               : reinterpret_cast<const uint8_t*>(kZeros);
+    const int e = base[has ? id * page_stride + fast_div(slot, a.block_magic, a.block_shift) : 0];
+    return has ? e : 0;
   };
   // Pages and exponents of the tiles that this wave loads from tile t on, a group of 16 keys a lane, by vector loads
   // that it waits for once in 32 tiles (FEW) or 64.  Loads a tile would be waited for with the tiles in flight, or, as
@@ -681,8 +681,8 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     if constexpr (CODES) {
       const int key = real(t + APART * (lane / GROUPS)) * KT + first_row + 16 * (lane % GROUPS);
       held_id = table[fast_div(min(key, p.span - 1), a.page_magic, a.page_shift)];
-      held_k = *exponent_at(key, held_id, kexp, a.ke_page);
-      held_v = *exponent_at(key, held_id, vexp, a.ve_page);
+      held_k = exponent_of(key, held_id, kexp, a.ke_page);
+      held_v = exponent_of(key, held_id, vexp, a.ve_page);
       held_at = 0;
     }
   };

@@ -150,16 +150,16 @@ __device__ __forceinline__ int first_block_slot(const AppendArgs& a, int b) {
   return block_slots(attn::start_of(a.starts, b, a.tokens), a.block, b);
 }
 
-// Where a pair's cosine and sine stand in its row of LDS: those of a half-layout chunk 8 pairs apart from each other, so
-// that the lanes of a row read neighbours.
+// Where a pair's cosine and sine stand in its row of LDS: the first of each half-layout chunk side by side, then the
+// second and so on, so that the lanes of a row read neighbours.
 template <int D>
 __device__ __forceinline__ int turn_at(int pair) {
   return (pair & 7) * (D / 16) + (pair >> 3);
 }
 
 // Channels c0 .. c0 + 7 of a row, turned: `turns` holds the row's cosines and sines a pair.  put(i, own, other, turn,
-// turns) gets each channel, its partner, and what they are multiplied by.  D / 8 neighbouring lanes, all of them active,
-// have the row's chunks.
+// turns) gets each channel, its partner, and what they are multiplied by.  D / 8 neighbouring lanes, all of them
+// active, have the row's chunks.
 template <int DT, int D, class Turn, class F>
 __device__ __forceinline__ void turned8(const void* src, int64_t row, int c0, const Turn* turns, int pairs,
                                         bool interleaved, const float (&x)[8], F put) {
@@ -618,8 +618,8 @@ extern "C" int m5k_paged_read(int mode, const void* k_codes, int64_t kc_page, in
   a.pages = static_cast<int>(pages);
   a.page_size = static_cast<int>(page_size);
   a.block = static_cast<int>(block);
-  // 64: 32769 tokens of 8 heads 43.3 us, 19569 tokens of 33 sequences and 16 heads 22.7 us (with 16: 45.0 and 22.3; with
-  // 128: 42.4 and 26.2, the search of the sequence once a walk).
+  // 64: 32769 tokens of 8 heads 43.3 us, 19569 tokens of 33 sequences and 16 heads 22.7 us (with 16: 45.0 and 22.3;
+  // with 128: 42.4 and 26.2, the search of the sequence once a walk).
   a.walk = walk_of((tokens * (head_dim / 16) + THREADS - 1) / THREADS, 2 * a.kv_heads, THREADS, 64);
   a.groups = (a.kv_heads + a.walk - 1) / a.walk;
   const int dim = static_cast<int>(head_dim);

@@ -107,6 +107,26 @@ def test_reach():
     assert module._reach(70, 10, 4, True) == 70
 
 
+@pytest.mark.parametrize("kind", [-1, 3, 5, 6, 7, 8, 16, 24, 34])
+def test_plans_of_no_such_cache(kind):
+    n = ctypes.c_int()
+    lib = _lib.load()
+    assert lib.m5k_attention_plan(kind, 5, 8, 2, 3, 1000, 256, ctypes.byref(n), None) == 1
+    assert b"paged" in lib.m5k_last_error()
+
+
+def test_plans_by_what_the_cache_holds():
+    """(key splits, whether waves share rows): codes take few rows a sequence in that form whatever their number."""
+    few = lambda *a: module._plan(*a, 256)[1]  # noqa: E731
+    for mode, capped in ((_lib.QUANT_FP8, False), (_lib.QUANT_INT8, True)):
+        assert few(module._coded_plan(mode, 128, capped), 1024, 32, 8, 64, 2048)
+        assert few(module._coded_plan(mode, 64, capped), 300, 8, 8, 300, 8192)
+    assert few(module._coded_plan(_lib.QUANT_FP8, 128, True), 8192, 32, 8, 1, 8192)
+    assert not few(module._coded_plan(_lib.QUANT_FP8, 128, False), 8192, 32, 8, 1, 8192)
+    assert not few(module._coded_plan(_lib.QUANT_INT8, 128, True), 8192, 32, 8, 1, 8192)
+    assert not few(1, 300, 8, 8, 300, 8192)
+
+
 def test_c_entries_check_before_launching():
     lib = _lib.load()
     p = ctypes.c_void_p(256)  # never dereferenced

@@ -148,6 +148,108 @@ def test_lacking_pages_and_lost_blocks(new, d, device):
     del want
 
 
+@pytest.mark.parametrize("new", [[1], [200], [250]])
+def test_codes_that_are_not_numbers(new, device):
+    """E4M3's NaN in a key that the window hides, and behind the context; then where a row sees it."""
+    c = _case(new, [400], d=64, page=16, block=16)
+    want = _got(c, device, window=20)
+    first = int(c["table"][0, 10])  # positions 160 .. 175: seen by the first rows of the longest chunk alone
+    c["k"][first, :, 3], c["v"][first, :, 7, 5] = 0x7F, 0xFF
+    c["v"][int(c["table"][0, 25 - 1]), :, 15] = 0x7F  # position 399, seen by the last
+    c["v"][-1], c["k"][-1] = 0x7F, 0x7F
+    got = _got(c, device, window=20)
+    position = torch.arange(400 - new[0], 400)
+    hit = (position == 399) | ((position >= 163) & (position < 163 + 24))
+    assert torch.equal(got[~hit.to(device)], want[~hit.to(device)])
+    assert got[position == 399].isnan().all()
+    sees = (position >= 167) & (position < 183)
+    assert int(sees.sum()) == (16 if new[0] == 250 else 0)
+    assert got[sees].reshape(-1, 8, 64)[..., 5].isnan().all()
+
+
+def test_pages_behind_32_bits(device):
+    """Codes more than 2^32 bytes into the cache, pages in descending order."""
+    pages, hkv, page, d = 33000, 16, 64, 128
+    small = _case([40, 1], [300, 200], hq=16, hkv=hkv, d=d, page=page, block=64)
+    k = torch.zeros(pages, hkv, page, d, dtype=U8, device=device)
+    scales = torch.zeros(pages, hkv, 1, dtype=U8, device=device)
+    n = small["k"].shape[0]
+    at = torch.arange(pages - 1, pages - 1 - n, -1)
+    table = torch.where(small["table"] < 0, -1, pages - 1 - small["table"]).to(torch.int32).to(device)
+    k[at.to(device)], scales[at.to(device)] = small["k"].to(device), small["ks"].to(device)
+    got = m5.paged_attention(small["q"].to(device), k, k, table, small["starts"].to(device),
+                             small["context"].to(device), k_scales=scales, v_scales=scales)
+    assert ref.close(got, *_want({**small, "v": small["k"], "vs": small["ks"]})) <= 0
+
+
+@pytest.mark.parametrize("starts,context", [((0, 9, 4, 12), (20, 20, 20)), ((3, 3, 12, 12), (30, 2 ** 31 - 1, 5)),
+                                            ((0, -5, 2 ** 31 - 1, 6), (10, -7, 2 ** 31 - 1)),
+                                            ((0, 4, 8, 12), (-2 ** 31, 2 ** 30, 4))])
+@pytest.mark.parametrize("options", [{}, dict(window=7, sinks=3)])
+def test_any_starts_and_lengths(options, starts, context, device):
+    """What the device holds is not checked: the call stays inside its buffers, and its rows are finite."""
+    for kw in (dict(d=64), dict(d=128, mode=I8), dict(d=128, hq=256, hkv=128)):
+        c = _case([4, 4, 4], [20, 20, 20], page=16, block=16, **kw)
+        c["starts"], c["context"] = _ints(*starts), _ints(*context)
+        got = _got(c, device, **options)
+        assert got.shape == (12, c["q"].shape[0] * kw["d"])
+
+
+def test_a_serving_step_in_a_graph(device):
+    """Append and attention captured together and replayed for step after step, with the lengths on the device."""
+    c = _case([1, 1], [33, 90], d=128, page=32, block=32)
+    t = {n: x.to(device) for n, x in c.items()}
+    f, _ = m5.rope_frequencies(128, device=device)
+    k, v = (torch.zeros(2, 2, 128, dtype=BF16, device=device) for _ in range(2))
+
+    def step(s):
+        q = m5.paged_append(k, v, s["k"], s["v"], s["table"], s["starts"], s["context"], q=s["q"], frequencies=f,
+                            k_scales=s["ks"], v_scales=s["vs"])
+        return m5.paged_attention(q, s["k"], s["v"], s["table"], s["starts"], s["context"], k_scales=s["ks"],
+                                  v_scales=s["vs"], window=40, sinks=4)
+
+    eager = {n: x.clone() if n in ("k", "v", "ks", "vs") else x for n, x in t.items()}
+    step(t)
+    for n in ("k", "v", "ks", "vs"):
+        t[n].copy_(eager[n])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(t)
+    for n in ("k", "v", "ks", "vs"):
+        t[n].copy_(eager[n])
+    g = torch.Generator().manual_seed(1)
+    for i in range(5):
+        k.copy_(torch.randn(2, 2, 128, generator=g).mul(2.0 ** i))
+        v.copy_(torch.randn(2, 2, 128, generator=g))
+        t["q"].copy_(torch.randn(8, 2, 128, generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step(eager)
+        assert torch.equal(out, want)
+        assert all(torch.equal(t[n], eager[n]) for n in ("k", "v", "ks", "vs"))
+        t["context"] += 1
+
+
+def test_two_streams_at_once(device):
+    """Two calls in key splits under way together: each has a workspace of its own."""
+    sides = [{n: x.to(device) for n, x in _case([1], [9000], d=128, page=64, block=64, seed=s).items()} for s in (0, 5)]
+
+    def call(c):
+        return m5.paged_attention(c["q"], c["k"], c["v"], c["table"], c["starts"], c["context"], k_scales=c["ks"],
+                                  v_scales=c["vs"])
+
+    want = [call(c) for c in sides]
+    streams = [torch.cuda.Stream() for _ in sides]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for c, stream in zip(sides, streams):
+            with torch.cuda.stream(stream):
+                got.append(call(c))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_window_behind_a_lost_block(device):
     """A NaN block that the window has left behind is not seen."""
     c = _case([1], [400], d=128, page=16, block=16)
