@@ -80,7 +80,7 @@ int common(Args& a, const void* q, int dtype, int64_t tokens, int64_t heads, int
   a.splits = splits;
   a.part_o = workspace;
   a.part_ml = workspace ? workspace + splits * tokens * heads * head_dim : nullptr;
-  m5k::attn::magic_of(static_cast<uint32_t>(a.group), a.group_magic, a.group_shift);
+  m5k::magic_of(static_cast<uint32_t>(a.group), a.group_magic, a.group_shift);
   return M5K_OK;
 }
 
@@ -189,7 +189,7 @@ int paged(Args& a, const void* k_cache, int64_t k_page, int64_t k_head, int64_t 
   a.keys = static_cast<int>(table_width * page_size);
   a.reach = reach(a.keys, a.window, a.sinks, true);
   a.causal = 1;
-  m5k::attn::magic_of(static_cast<uint32_t>(page_size), a.page_magic, a.page_shift);
+  m5k::magic_of(static_cast<uint32_t>(page_size), a.page_magic, a.page_shift);
   return M5K_OK;
 }
 
@@ -263,7 +263,7 @@ extern "C" int m5k_paged_attention_codes(
   a.ke_head = ke_head;
   a.ve_page = ve_page;
   a.ve_head = ve_head;
-  m5k::attn::magic_of(static_cast<uint32_t>(block), a.block_magic, a.block_shift);
+  m5k::magic_of(static_cast<uint32_t>(block), a.block_magic, a.block_shift);
   using namespace m5k::attn;
   const auto run = mode == M5K_QUANT_FP8
                        ? (sinks ? launch_typed<PAGES16, true, E4M3> : launch_typed<PAGES16, false, E4M3>)

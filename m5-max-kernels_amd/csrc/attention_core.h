@@ -43,6 +43,7 @@
 #pragma once
 
 #include "attention_place.h"
+#include "fast_div.h"
 #include "gemm_core.h"
 #include "m5k_common.h"
 
@@ -76,12 +77,6 @@ struct Args {
   int64_t ke_page, ke_head, ve_page, ve_head;
   uint32_t block_magic, block_shift;
 };
-
-// n / d of 0 <= n < 2^31 by one multiplication: magic = ceil(2^(31 + shift) / d), shift = ceil(log2 d).  The excess
-// magic * d - 2^(31 + shift) is below d <= 2^shift, so n times it stays below 2^(31 + shift) and the quotient is exact.
-__device__ __forceinline__ uint32_t fast_div(uint32_t n, uint32_t magic, uint32_t shift) {
-  return __umulhi(2 * n, magic) >> shift;
-}
 
 template <int DT>
 __device__ __forceinline__ v16f mfma32(v4i a, v4i b, v16f c) {
@@ -1537,12 +1532,6 @@ int launch_typed(Args& a, int dtype, int head_dim, hipStream_t st);
   }                                                                                                     \
   }                                                                                                     \
   }
-
-inline void magic_of(uint32_t d, uint32_t& magic, uint32_t& shift) {
-  shift = 0;
-  while ((uint64_t{1} << shift) < d) ++shift;
-  magic = static_cast<uint32_t>(((uint64_t{1} << (31 + shift)) + d - 1) / d);
-}
 
 }  // namespace attn
 }  // namespace m5k

@@ -12,6 +12,7 @@
 // border, would be another one than the formula's.  The result enters FP32 rounded to odd, which a second rounding to
 // fewer bits cannot tell from the 64-bit number.  Sines and cosines stand in LDS for all heads of the walk.
 #include "attention_place.h"
+#include "fast_div.h"
 #include "m5k_common.h"
 #include "rope_turn.h"
 
@@ -128,6 +129,19 @@ struct Operand {
   int64_t src_head, src_token, page, head, slot, exp_page, exp_head;
 };
 
+// A number that the device divides by.
+struct Divisor {
+  uint32_t magic, shift;
+  int value;
+};
+Divisor divisor(int value) {
+  Divisor d;
+  d.value = value;
+  magic_of(static_cast<uint32_t>(value), d.magic, d.shift);
+  return d;
+}
+__device__ __forceinline__ int over(int n, const Divisor& d) { return static_cast<int>(fast_div(n, d.magic, d.shift)); }
+
 struct AppendArgs {
   Operand op[2];  // K, V
   const void* q;
@@ -136,18 +150,20 @@ struct AppendArgs {
   const int32_t *table, *starts, *context;
   const double* frequencies;
   int64_t table_width;
-  int tokens, kv_heads, heads, pairs, interleaved, sequences, pages, page_size, block, walk, groups, slots;
+  int tokens, kv_heads, heads, pairs, interleaved, sequences, pages, walk, slots;
+  Divisor block, page_size, groups, q_groups;
   double magnitude;
 };
 
 // First block slot of a sequence.  Its n tokens touch no more than min(n, floor(n / block) + 2) blocks, wherever the
 // first one falls, and both terms of the minimum here grow by at least that much from a sequence to the next.
-__host__ __device__ __forceinline__ int block_slots(int tokens, int block, int sequences) {
-  const int blocks = tokens / block + 2 * sequences;
+__host__ __device__ __forceinline__ int block_slots(int tokens, int whole_blocks, int sequences) {
+  const int blocks = whole_blocks + 2 * sequences;
   return tokens < blocks ? tokens : blocks;
 }
 __device__ __forceinline__ int first_block_slot(const AppendArgs& a, int b) {
-  return block_slots(attn::start_of(a.starts, b, a.tokens), a.block, b);
+  const int start = attn::start_of(a.starts, b, a.tokens);
+  return block_slots(start, over(start, a.block), b);
 }
 
 // Where a pair's cosine and sine stand in its row of LDS: the first of each half-layout chunk side by side, then the
@@ -222,9 +238,9 @@ __global__ __launch_bounds__(T) void append_codes(const AppendArgs a) {
   __shared__ int places[TURNED ? ROWS : 1];
   const int tid = threadIdx.x, c0 = tid % CH * 8, row = tid / CH;
   // Workgroups of K, then V, then Q; of each, the heads' groups of a slot side by side.
-  const int kv = a.slots * a.groups, id = blockIdx.x, role = id < kv ? 0 : id < 2 * kv ? 1 : 2;
-  const int q_groups = (a.heads + a.walk - 1) / a.walk, groups = role == 2 ? q_groups : a.groups;
-  const int slot = (id - role * kv) / groups, walk0 = (id - role * kv - slot * groups) * a.walk;
+  const int kv = a.slots * a.groups.value, id = blockIdx.x, role = id < kv ? 0 : id < 2 * kv ? 1 : 2;
+  const Divisor& groups = role == 2 ? a.q_groups : a.groups;
+  const int slot = over(id - role * kv, groups), walk0 = (id - role * kv - slot * groups.value) * a.walk;
   const int head1 = min(walk0 + a.walk, role == 2 ? a.heads : a.kv_heads);
   const bool turn = TURNED && role != 1;
   const int pair = tid % PAIRS;
@@ -296,26 +312,32 @@ __global__ __launch_bounds__(T) void append_codes(const AppendArgs a) {
   if (n == 0 || context <= 0) return;
   const int start = attn::start_of(a.starts, b, a.tokens), p_new = context - n;  // position of the first new token
   const int p0 = max(p_new, 0), tile = slot - first_block_slot(a, b);
-  const int base = (p0 / a.block + tile) * a.block;  // position of the block's first token
-  if (tile < 0 || base < 0 || base >= context || base / a.page_size >= a.table_width) return;
-  const int page = a.table[b * a.table_width + base / a.page_size];
+  // The position of the block's first token; below 0 where it passes 31 bits, which unsigned products may.
+  const uint32_t block = static_cast<uint32_t>(a.block.value);
+  const int base = static_cast<int>(static_cast<uint32_t>(over(p0, a.block) + tile) * block);
+  if (tile < 0 || base < 0 || base >= context) return;
+  const int page_at = over(base, a.page_size);
+  if (page_at >= a.table_width) return;
+  const int page = a.table[b * a.table_width + page_at];
   if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.pages)) return;
-  const int slot0 = base % a.page_size;
+  const int slot0 = base - page_at * a.page_size.value;
   const bool has_old = base < p_new;
+  uint8_t* const exps = op.exps + page * op.exp_page + over(slot0, a.block);
   float x[PASSES][8], next[PASSES][8];  // of this head and the next
   auto load = [&](int h, float (&to)[PASSES][8]) __attribute__((always_inline)) {
 #pragma unroll
     for (int pass = 0; pass < PASSES; ++pass) {
       const int r = pass * RPP + row, p = base + r;
-      if (r < a.block && p >= p0 && p < context)
+      if (r < a.block.value && p >= p0 && p < context)
         load8<DT>(op.src, h * op.src_head + (start + (p - p_new)) * op.src_token + c0, to[pass]);
     }
   };
   load(walk0, x);
+  int before = has_old ? exps[walk0 * op.exp_head] : 0;
   if constexpr (TURNED) {
     if (turn) {
       __syncthreads();
-      for (int r = tid / PAIRS; r < a.block && pair < a.pairs; r += TURNS) {
+      for (int r = tid / PAIRS; r < a.block.value && pair < a.pairs; r += TURNS) {
         const int p = base + r;
         if (p >= p0 && p < context) turns[r * PAIRS + turn_at<D>(pair)] = turn64(p * radians[pair], a.magnitude);
       }
@@ -323,15 +345,17 @@ __global__ __launch_bounds__(T) void append_codes(const AppendArgs a) {
     }
   }
   for (int h = walk0; h < head1; ++h) {
-    uint8_t* exp = op.exps + page * op.exp_page + h * op.exp_head + slot0 / a.block;
     uint8_t* codes = op.codes + page * op.page + h * op.head + slot0 * op.slot + c0;
-    const int before = has_old ? *exp : 0;
     float top = 0.0f;
-    if (h + 1 < head1) load(h + 1, next);
+    int next_before = 0;
+    if (h + 1 < head1) {
+      load(h + 1, next);
+      if (has_old) next_before = exps[(h + 1) * op.exp_head];
+    }
 #pragma unroll
     for (int pass = 0; pass < PASSES; ++pass) {
       const int r = pass * RPP + row, p = base + r;
-      if (r >= a.block || p < p0 || p >= context) continue;
+      if (r >= a.block.value || p < p0 || p >= context) continue;
       if constexpr (TURNED) {
         if (turn) {
           float y[8];
@@ -358,7 +382,7 @@ __global__ __launch_bounds__(T) void append_codes(const AppendArgs a) {
 #pragma unroll
     for (int pass = 0; pass < PASSES; ++pass) {
       const int r = pass * RPP + row, p = base + r;
-      if (r >= a.block || p >= context) continue;
+      if (r >= a.block.value || p >= context) continue;
       uint2* to = reinterpret_cast<uint2*>(codes + r * op.slot);
       float y[8];
       if (p >= p0) {
@@ -375,7 +399,8 @@ __global__ __launch_bounds__(T) void append_codes(const AppendArgs a) {
       }
       *to = encode8<MODE>(y);
     }
-    if (tid == 0) *exp = static_cast<uint8_t>(after);
+    if (tid == 0) exps[h * op.exp_head] = static_cast<uint8_t>(after);
+    before = next_before;
 #pragma unroll
     for (int pass = 0; pass < PASSES; ++pass)
 #pragma unroll
@@ -391,7 +416,8 @@ struct ReadArgs {
   void* out[2];
   const int32_t *table, *starts, *context;
   int64_t table_width;
-  int tokens, kv_heads, sequences, pages, page_size, block, walk, groups;
+  int tokens, kv_heads, sequences, pages, walk, groups;
+  Divisor page_size, block;
 };
 
 // A thread has 16 channels of one token and walks over heads: 16 bytes in, 16 values out.  Memory bound.
@@ -412,18 +438,19 @@ __global__ __launch_bounds__(THREADS) void read_codes(const ReadArgs a) {
   const int s = a.starts[lo], e = a.starts[lo + 1];
   bool known = token >= s && token < e;
   const int position = known ? a.context[lo] - (e - token) : -1;
-  const int page_at = position / a.page_size;
-  known = known && position >= 0 && page_at < a.table_width;
+  known = known && position >= 0;
+  const int page_at = known ? over(position, a.page_size) : 0;
+  known = known && page_at < a.table_width;
   const int page = known ? a.table[lo * a.table_width + page_at] : -1;
   known = known && static_cast<uint32_t>(page) < static_cast<uint32_t>(a.pages);
-  const int at = position - page_at * a.page_size;
+  const int at = position - page_at * a.page_size.value, block = known ? over(at, a.block) : 0;
   for (int h = head0; h < head1; ++h) {
     uint4 w = make_uint4(0, 0, 0, 0);
     float scale = 0.0f;
     if (known) {
       w = *reinterpret_cast<const uint4*>(a.codes[which] + page * a.page[which] + h * a.head[which] +
                                           at * a.slot[which] + c0);
-      scale = scale_of(a.exps[which][page * a.exp_page[which] + h * a.exp_head[which] + at / a.block]);
+      scale = scale_of(a.exps[which][page * a.exp_page[which] + h * a.exp_head[which] + block]);
     }
     float x[2][8];
     const uint32_t words[4] = {w.x, w.y, w.z, w.w};
@@ -451,13 +478,15 @@ int walk_of(int64_t workgroups, int heads, int threads, int waves) {
 template <int DT, int D, int MODE, int T, int PASSES, bool TURNED>
 int append_threads(AppendArgs& a, hipStream_t st) {
   constexpr int ROWS = PASSES * T / (D / 8);  // of q a workgroup
-  a.slots = block_slots(a.tokens, a.block, a.sequences);
+  const int block = a.block.value;
+  a.slots = block_slots(a.tokens, a.tokens / block, a.sequences);
   // 16: sines and cosines are made once a walk (4096 tokens turned, 32 heads of q, 8 of k and v of 128, blocks of 64,
   // read back: 36 us; with 8 and 32 waves 36 and 50 us; single tokens have too few rows to walk).
-  a.walk = walk_of(a.tokens / a.block, 2 * a.kv_heads + a.heads, T, 16);
-  a.groups = (a.kv_heads + a.walk - 1) / a.walk;
+  a.walk = walk_of(a.tokens / block, 2 * a.kv_heads + a.heads, T, 16);
+  a.groups = divisor((a.kv_heads + a.walk - 1) / a.walk);
+  a.q_groups = divisor(a.heads ? (a.heads + a.walk - 1) / a.walk : 1);
   const int q_slots = a.heads ? (a.tokens + ROWS - 1) / ROWS : 0;
-  const int64_t blocks = int64_t{2} * a.slots * a.groups + int64_t{q_slots} * ((a.heads + a.walk - 1) / a.walk);
+  const int64_t blocks = int64_t{2} * a.slots * a.groups.value + int64_t{q_slots} * a.q_groups.value;
   M5K_REQUIRE(blocks <= INT32_MAX, "paged_append: too many rows for one launch");
   launch_kernel(append_codes<DT, D, MODE, T, PASSES, TURNED>, dim3(static_cast<uint32_t>(blocks)), dim3(T), st, a);
   return launch_status("paged_append");
@@ -465,7 +494,7 @@ int append_threads(AppendArgs& a, hipStream_t st) {
 
 template <int DT, int D, int MODE>
 int append_block(AppendArgs& a, hipStream_t st) {
-  const int threads = a.block * (D / 8);
+  const int threads = a.block.value * (D / 8);
   if (a.pairs) {
     if (threads <= 256) return append_threads<DT, D, MODE, 256, 1, true>(a, st);
     if (threads <= 512) return append_threads<DT, D, MODE, 512, 1, true>(a, st);
@@ -568,8 +597,8 @@ extern "C" int m5k_paged_append_codes(
   a.interleaved = interleaved != 0;
   a.sequences = static_cast<int>(sequences);
   a.pages = static_cast<int>(pages);
-  a.page_size = static_cast<int>(page_size);
-  a.block = static_cast<int>(block);
+  a.page_size = divisor(static_cast<int>(page_size));
+  a.block = divisor(static_cast<int>(block));
   a.magnitude = magnitude;
   const int dim = static_cast<int>(head_dim);
   if (dtype == M5K_BF16) return append_typed<M5K_BF16>(a, mode, dim, as_stream(stream));
@@ -616,8 +645,8 @@ extern "C" int m5k_paged_read(int mode, const void* k_codes, int64_t kc_page, in
   a.kv_heads = static_cast<int>(kv_heads);
   a.sequences = static_cast<int>(sequences);
   a.pages = static_cast<int>(pages);
-  a.page_size = static_cast<int>(page_size);
-  a.block = static_cast<int>(block);
+  a.page_size = divisor(static_cast<int>(page_size));
+  a.block = divisor(static_cast<int>(block));
   // 64: 32769 tokens of 8 heads 43.3 us, 19569 tokens of 33 sequences and 16 heads 22.7 us (with 16: 45.0 and 22.3;
   // with 128: 42.4 and 26.2, the search of the sequence once a walk).
   a.walk = walk_of((tokens * (head_dim / 16) + THREADS - 1) / THREADS, 2 * a.kv_heads, THREADS, 64);
