@@ -22,6 +22,7 @@ namespace {
 constexpr int THREADS = 256;
 constexpr int BLOCK_MAX = 128;  // tokens of a block
 constexpr int Q_HEADS = 4;      // heads of q whose rows are under way at once
+constexpr int READ_HEADS = 4;   // heads of a read
 
 // ---- codes ----------------------------------------------------------------------------------------
 
@@ -420,12 +421,16 @@ struct ReadArgs {
   Divisor page_size, block;
 };
 
-// A thread has 16 channels of one token and walks over heads: 16 bytes in, 16 values out.  Memory bound.
+// A thread has 8 channels of one token and walks over heads, READ_HEADS of them under way at once: 8 bytes in, 8 values
+// out, neighbours side by side.  Memory bound: 32769 tokens of 8 heads of 128, E4M3 to BF16, 36 us, 5.6 TB/s; 19569
+// tokens of 33 sequences, 16 heads of 64, INT8 to FP16, 24.5 us, 4.9 TB/s.  (16 channels, two stores that leave every
+// other 16 bytes to each other, one head at a time: 48 and 31 us; 8 channels, one head at a time 37.6 and 29.2, two
+// 37.1 and 28.0, eight 36.4 and 24.1.)
 template <int DT, int D, int MODE>
 __global__ __launch_bounds__(THREADS) void read_codes(const ReadArgs a) {
-  constexpr int CH = D / 16;
+  constexpr int CH = D / 8;
   const int64_t unit = int64_t{blockIdx.x} * THREADS + threadIdx.x;
-  const int token = static_cast<int>(unit / CH), c0 = static_cast<int>(unit % CH) * 16;
+  const int token = static_cast<int>(unit / CH), c0 = static_cast<int>(unit % CH) * 8;
   if (token >= a.tokens) return;
   const int which = blockIdx.y >= a.groups, head0 = (blockIdx.y - which * a.groups) * a.walk;
   const int head1 = min(head0 + a.walk, a.kv_heads);
@@ -444,26 +449,30 @@ __global__ __launch_bounds__(THREADS) void read_codes(const ReadArgs a) {
   const int page = known ? a.table[lo * a.table_width + page_at] : -1;
   known = known && static_cast<uint32_t>(page) < static_cast<uint32_t>(a.pages);
   const int at = position - page_at * a.page_size.value, block = known ? over(at, a.block) : 0;
-  for (int h = head0; h < head1; ++h) {
-    uint4 w = make_uint4(0, 0, 0, 0);
-    float scale = 0.0f;
+  const uint8_t* const codes = a.codes[which] + page * a.page[which] + at * a.slot[which] + c0;
+  const uint8_t* const exps = a.exps[which] + page * a.exp_page[which] + block;
+  for (int h0 = head0; h0 < head1; h0 += READ_HEADS) {
+    uint2 w[READ_HEADS] = {};
+    int exponent[READ_HEADS] = {};
     if (known) {
-      w = *reinterpret_cast<const uint4*>(a.codes[which] + page * a.page[which] + h * a.head[which] +
-                                          at * a.slot[which] + c0);
-      scale = scale_of(a.exps[which][page * a.exp_page[which] + h * a.exp_head[which] + block]);
-    }
-    float x[2][8];
-    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float v[4];
-      decode4<MODE>(words[i], v);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[i >> 1][4 * (i & 1) + j] = v[j] * scale;
+      for (int i = 0; i < READ_HEADS; ++i) {
+        const int h = min(h0 + i, head1 - 1);
+        w[i] = *reinterpret_cast<const uint2*>(codes + h * a.head[which]);
+        exponent[i] = exps[h * a.exp_head[which]];
+      }
     }
-    const int64_t to = (int64_t{h} * a.tokens + token) * D + c0;
-    store8<DT>(a.out[which], to, x[0]);
-    store8<DT>(a.out[which], to + 8, x[1]);
+#pragma unroll
+    for (int i = 0; i < READ_HEADS; ++i) {
+      if (h0 + i >= head1) break;
+      const float scale = scale_of(exponent[i]);
+      float lo4[4], hi4[4], x[8];
+      decode4<MODE>(w[i].x, lo4);
+      decode4<MODE>(w[i].y, hi4);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = (j < 4 ? lo4[j & 3] : hi4[j & 3]) * scale;
+      store8<DT>(a.out[which], (int64_t{h0 + i} * a.tokens + token) * D + c0, x);
+    }
   }
 }
 
@@ -518,7 +527,7 @@ int append_typed(AppendArgs& a, int mode, int head_dim, hipStream_t st) {
 
 template <int DT>
 int read_typed(const ReadArgs& a, int mode, int head_dim, hipStream_t st) {
-  const int64_t blocks = (int64_t{a.tokens} * (head_dim / 16) + THREADS - 1) / THREADS;
+  const int64_t blocks = (int64_t{a.tokens} * (head_dim / 8) + THREADS - 1) / THREADS;
   const dim3 grid(static_cast<uint32_t>(blocks), static_cast<uint32_t>(2 * a.groups));
   auto kernel = mode == M5K_QUANT_FP8
                     ? (head_dim == 64 ? read_codes<DT, 64, M5K_QUANT_FP8> : read_codes<DT, 128, M5K_QUANT_FP8>)
@@ -647,9 +656,8 @@ extern "C" int m5k_paged_read(int mode, const void* k_codes, int64_t kc_page, in
   a.pages = static_cast<int>(pages);
   a.page_size = divisor(static_cast<int>(page_size));
   a.block = divisor(static_cast<int>(block));
-  // 64: 32769 tokens of 8 heads 43.3 us, 19569 tokens of 33 sequences and 16 heads 22.7 us (with 16: 45.0 and 22.3;
-  // with 128: 42.4 and 26.2, the search of the sequence once a walk).
-  a.walk = walk_of((tokens * (head_dim / 16) + THREADS - 1) / THREADS, 2 * a.kv_heads, THREADS, 64);
+  // 16: the second of the reads above with 64 26.3 us, with 128 34.5; the first the same from 8 to 128.
+  a.walk = walk_of((tokens * (head_dim / 8) + THREADS - 1) / THREADS, 2 * a.kv_heads, THREADS, 16);
   a.groups = (a.kv_heads + a.walk - 1) / a.walk;
   const int dim = static_cast<int>(head_dim);
   if (dtype == M5K_BF16) return read_typed<M5K_BF16>(a, mode, dim, as_stream(stream));
