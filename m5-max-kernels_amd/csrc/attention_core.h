@@ -97,6 +97,14 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   else return __builtin_bit_cast(uint32_t, __builtin_convertvector((m5k_f32x2{lo, hi}), half2v));
 }
 
+// Two finished values to the inputs' type: in FP16 by a conversion each, which the compiler makes one instruction, and
+// one rounding, with the division of the sum before it.
+template <int DT>
+__device__ __forceinline__ uint32_t out2(float lo, float hi) {
+  if constexpr (DT == M5K_BF16) return f32x2_to_bf16x2(lo, hi);
+  else return f32_to_f16_bits(lo) | (f32_to_f16_bits(hi) << 16);
+}
+
 // The other half-wave's value of the same row.
 __device__ __forceinline__ float other_half(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -1313,7 +1321,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
       uint32_t v[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        v[i] = total == 0.0f ? pack2<DT>(none, none) : pack2<DT>(acc[e + 2 * i] * inv, acc[e + 2 * i + 1] * inv);
+        v[i] = total == 0.0f ? out2<DT>(none, none) : out2<DT>(acc[e + 2 * i] * inv, acc[e + 2 * i + 1] * inv);
       *reinterpret_cast<uint4*>(op + e) = make_uint4(v[0], v[1], v[2], v[3]);
     }
     return;
@@ -1335,15 +1343,15 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
     return;
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l, none = m < M_FLOOR ? __builtin_nanf("") : 0.0f;
-  const uint32_t nones = pack2<DT>(none, none);
+  const uint32_t nones = out2<DT>(none, none);
   uint16_t* op = a.out + (int64_t{token} * a.heads + head) * D + 4 * half;
 #pragma unroll
   for (int b = 0; b < OB; ++b)
 #pragma unroll
     for (int r = 0; r < 16; r += 4) {
       const uint2 w = l == 0.0f ? make_uint2(nones, nones)
-                                : make_uint2(pack2<DT>(o[b][r] * inv, o[b][r + 1] * inv),
-                                             pack2<DT>(o[b][r + 2] * inv, o[b][r + 3] * inv));
+                                : make_uint2(out2<DT>(o[b][r] * inv, o[b][r + 1] * inv),
+                                             out2<DT>(o[b][r + 2] * inv, o[b][r + 3] * inv));
       *reinterpret_cast<uint2*>(op + 32 * b + 2 * r) = w;
     }
 }
@@ -1427,8 +1435,8 @@ __global__ __launch_bounds__(256) void attention_join(const Args a) {
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = total == 0.0f ? none : acc[e] * inv;
   uint16_t* dst = a.out + at * D + lane * E;
-  if constexpr (E == 2) *reinterpret_cast<uint32_t*>(dst) = pack2<DT>(acc[0], acc[1]);
-  else *dst = static_cast<uint16_t>(pack2<DT>(acc[0], 0.0f) & 0xFFFFu);
+  if constexpr (E == 2) *reinterpret_cast<uint32_t*>(dst) = out2<DT>(acc[0], acc[1]);
+  else *dst = static_cast<uint16_t>(out2<DT>(acc[0], 0.0f) & 0xFFFFu);
 }
 
 // How a call is launched.  `few`: sequences of no more than 32 packed rows on average that are fewer, with their key
