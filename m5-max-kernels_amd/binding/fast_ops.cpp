@@ -12,7 +12,8 @@
 // the HIP launch takes about 3 each.  The projections' staged form, two launches, takes
 // 18 to 20 us through Python and 8 to 10 us here; the fused one 10 to 13 and 5 to 6 us.  Calls of the
 // attention step back to back, each with its kernel: rope of one token 9.5 and 4.7 us, paged_append of 64
-// tokens 18 and 5.6, attention of 128 tokens 14.4 and 6.6, which is its kernel.
+// tokens 18 and 5.6, attention of 128 tokens 14.4 and 6.6, which is its kernel.  Over a cache in 8 bits:
+// paged_attention of one token 4.8 us of host time, paged_append and paged_read of 64 tokens 9.6 together.
 #include <Python.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/Dtype.h>

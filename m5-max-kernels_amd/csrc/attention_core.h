@@ -1,5 +1,5 @@
 // Attention for gfx950: out = softmax(scores(Q K^T) + mask) V with one pass over the keys, K and V dense or in
-// the pages of a cache.
+// the pages of a cache, in 16 bits or as codes of 8 bits.
 //
 // Rows.  The query heads that share a key head are packed: packed row r of a sequence is token r / G, query head
 // kvh * G + r % G (G = heads / kv_heads), so one K/V tile serves all of them and a single token still fills G rows.
@@ -7,7 +7,9 @@
 //
 // Masks.  Every mask of these operators (causal, window, document, prefix, length) leaves a row one interval
 // [lo, hi) of keys.  Key tiles outside the union of a wave's intervals are skipped, tiles inside all of them need
-// no comparison, the others compare the key index.
+// no comparison, the others compare the key index.  A window that keeps a sequence's first keys (SINKS) leaves a row
+// two intervals: tiles of the first keys are taken ahead of those of the windows, by the same loop, and where either
+// ends inside a tile the lane's keys are bits of a word.
 //
 // Products.  v_mfma_f32_32x32x16 on S^T = K Q^T and O^T = V^T P^T.  With S transposed a lane holds scores of one
 // query (lane & 31) only: 16 of the 32 keys of a block, the other 16 in lane ^ 32, so that a row's maximum is a
@@ -36,10 +38,18 @@
 // of 128: 2.51 to 2.64 ms by the card, 1.1 PFLOP/s, matrix cores busy 64% of the cycles, no LDS bank conflicts).
 // Single tokens: the cache's bytes (131073 keys, 8 key heads of 128: 94 to 100 us and 5 us of joining, 5.5 TB/s).
 // Heads of 64: the exponentials.
+// Codes: bytes again where tokens are single (131073 keys, E4M3: 54 us, 5.0 TB/s, and 5 of joining); 64 tokens over 0
+// to 6400 keys take 118 us in INT8 and 104 in E4M3, 3.4 and 3.8 TB/s, the longest sequences alone at the end (0.8 waves
+// a SIMD on average).  Chunks as in 16 bits, with the expansion beside the products (of up to 1024 tokens over up to
+// 8192 keys 207 us, so 182; 0.9 waves a SIMD, and one alone takes 3800 cycles a tile where two take 2600 each).
+// First keys: 9914 causal tokens, 56 heads of 128, window 1024, 4 first keys: 363 to 373 us, 0.85 PFLOP/s over the 1090
+// keys a row that are multiplied, of which 975 count; without first keys 343.  8192 tokens in 7 documents, 32 on 8
+// heads of 64, FP16, window 256, 64 first keys: 54 to 60 us, VALU work, 19 of its instructions a product.
 //
 // Registers.  Tiles of 128 rows with heads of 128 use 241 to 256, all there are for two waves a SIMD.  With a cap or a
 // bias 8 to 10 of them go to memory and come back inside the loop, 34 by pages of no multiple of 16 (chunks of up to
 // 1024 tokens over up to 8192 keys, bias: 232 us in pages of 64, 536 in pages of 24; without the bias 182 and 251).
+// Codes: 7 to 22, with cap or bias 40 to 54, where the form of few rows is mostly taken instead (none spilled there).
 #pragma once
 
 #include "attention_place.h"

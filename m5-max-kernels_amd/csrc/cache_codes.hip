@@ -11,6 +11,10 @@
 // the old codes are rounded again under it.  Keys are turned in 64 bits: in 32, about one code in 10^6, next to a
 // border, would be another one than the formula's.  The result enters FP32 rounded to odd, which a second rounding to
 // fewer bits cannot tell from the 64-bit number.  Sines and cosines stand in LDS for all heads of the walk.
+//
+// What bounds it.  Single tokens: a chain of dependent loads (sequence, length, page, exponent) and the angles in 64
+// bits: 64 tokens, 8 key heads and 56 query heads of 128 take 7.4 us, 5.9 without the queries, 4.7 without turning.
+// Chunks: 4096 tokens, 32 heads of 64, FP16 to INT8, 15 us, 3.3 TB/s, two waves a SIMD.
 #include "attention_place.h"
 #include "fast_div.h"
 #include "m5k_common.h"
