@@ -1484,8 +1484,8 @@ inline Plan plan(int kind, int64_t tokens, int group, int kv_heads, int64_t sequ
   bool few = tiles < cus && thin <= (keys < 512 || (codes && !cheap) ? 2 : 4) * cus && keys <= 4096;
   if (codes) few = few || rows <= 64 * own || (spills && (cheap || tiles <= 4 * cus));
   else few = few || (rows <= 32 * own && own * kv_heads < 2 * cus);
-  const int64_t r = few ? 32 : 32 * WAVES;
-  return Plan{few, static_cast<int>(paged ? rows / r + sequences + 1 : (rows + r - 1) / r)};
+  const int r = few ? 32 : 32 * WAVES;
+  return Plan{few, static_cast<int>(paged ? slots_before(tokens, sequences + 1, group, r) : (rows + r - 1) / r)};
 }
 
 // Key splits: as many as bring the workgroups to two a compute unit, what it holds at once, each over at least 256 keys

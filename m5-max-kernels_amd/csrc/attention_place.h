@@ -2,8 +2,10 @@
 // tokens, apart from the kernels so that a host compiler takes it too.
 //
 // The packed rows (token * G + head of its group) of a sequence are cut into tiles of R.  Sequence b owns the slots
-// from (starts[b] * G / R) + b on: at least as many as it has tiles, and the first of them is known without the lengths
-// of the sequences before it.  The tokens behind the last sequence are sequence number `sequences`, which sees nothing.
+// from min(starts[b] * ceil(G / R), starts[b] * G / R + b) on: both grow by its tiles at least, so that it owns as
+// many, and the first of them is known without the lengths of the sequences before it.  The first term leaves single
+// tokens no slot without rows (see slots_before).  The tokens behind the last sequence are sequence number
+// `sequences`, which sees nothing.
 //
 // Starts lie on the device and nothing checks them.  In any order and of any value they are taken as cut to [0,
 // tokens]; a slot then finds some sequence, perhaps one that does not own it, and has rows only if its tile is one of
@@ -34,8 +36,17 @@ M5K_PLACE int tokens_of(const int32_t* starts, int b, int sequences, int tokens)
   return n < 0 ? 0 : n;
 }
 
+// Slots of `sequences` sequences that have `tokens` tokens together.  Workgroups go to parts of the chip in turn, and
+// wait for their part even while another has room: empty slots in between, of no regular distance, let some parts have
+// more work than others.  (64 single tokens over 4096 keys each, 8 key heads, E4M3, groups of 8 and of 7 query heads,
+// by the second term alone: 110 and 132 us.)
+M5K_PLACE int64_t slots_before(int64_t tokens, int64_t sequences, int group, int rows_per_tile) {
+  const int64_t each = tokens * ((group + rows_per_tile - 1) / rows_per_tile);
+  const int64_t packed = tokens * group / rows_per_tile + sequences;
+  return each < packed ? each : packed;
+}
 M5K_PLACE int first_slot(const int32_t* starts, int b, int tokens, int group, int rows_per_tile) {
-  return static_cast<int>(int64_t{start_of(starts, b, tokens)} * group / rows_per_tile) + b;
+  return static_cast<int>(slots_before(start_of(starts, b, tokens), b, group, rows_per_tile));
 }
 
 // The last b of [0, n) whose first slot does not lie behind a slot, 64 probes at a time: count(lo, left, apart) says
