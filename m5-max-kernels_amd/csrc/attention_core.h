@@ -38,10 +38,11 @@
 // of 128: 2.51 to 2.64 ms by the card, 1.1 PFLOP/s, matrix cores busy 64% of the cycles, no LDS bank conflicts).
 // Single tokens: the cache's bytes (131073 keys, 8 key heads of 128: 94 to 100 us and 5 us of joining, 5.5 TB/s).
 // Heads of 64: the exponentials.
-// Codes: bytes again where tokens are single (131073 keys, E4M3: 54 us, 5.0 TB/s, and 5 of joining); 64 tokens over 0
-// to 6400 keys take 118 us in INT8 and 104 in E4M3, 3.4 and 3.8 TB/s, the longest sequences alone at the end (0.8 waves
-// a SIMD on average).  Chunks as in 16 bits, with the expansion beside the products (of up to 1024 tokens over up to
-// 8192 keys 207 us, so 182; 0.9 waves a SIMD, and one alone takes 3800 cycles a tile where two take 2600 each).
+// Codes: bytes again where tokens are single (131073 keys, E4M3: 54 us, 5.0 TB/s, and 5 of joining; 64 over 4000 keys
+// each 103 us, 5.1 TB/s); 64 over 0 to 6400 keys take 102 to 109 us in INT8 and 94 in E4M3, 3.8 and 4.2 TB/s, the
+// longest sequences alone at the end.  Chunks as in 16 bits, with the expansion beside the products (of up to 1024
+// tokens over up to 8192 keys 207 us, so 182; 0.9 waves a SIMD, and one alone takes 3800 cycles a tile where two take
+// 2600 each).
 // First keys: 9914 causal tokens, 56 heads of 128, window 1024, 4 first keys: 363 to 373 us, 0.85 PFLOP/s over the 1090
 // keys a row that are multiplied, of which 975 count; without first keys 343.  8192 tokens in 7 documents, 32 on 8
 // heads of 64, FP16, window 256, 64 first keys: 54 to 60 us, VALU work, 19 of its instructions a product.
@@ -1456,17 +1457,17 @@ __global__ __launch_bounds__(256) void attention_join(const Args a) {
 // with `few`: 128 tokens, 56 heads of 128: 8.7 and 6.5 us; 300 tokens: 12.8 and 15.8; 1024 tokens, 16 heads: 33.8 and
 // 18.0; 1999 tokens, 4 key heads of 64, prefix and cap: 43.8 and 32.2; 9914 tokens, one head: 71 and 98.
 //
-// The first limit is no crossing of the forms.  Single tokens of 8 key heads of 128, with tiles and with `few`, over
-// 300 / 1000 / 4000 keys each: 32 sequences 14, 13 / 29, 28 / 98, 98 us; 63: 20, 17 / 45, 42 / 177, 176; 64: 20, 18 /
-// 46, 44 / 182, 180; 65: 26, 21 / 63, 50 / 248, 209; 128: 34, 31 / 99, 95 / 355, 352; 256: 68, 62 / 191, 184.  Two key
-// heads, 256 sequences: 20, 21 / 46, 48 / 183, 205; 400: 30, 27 / 82, 82 / 289, 304.  64 of unequal lengths up to 8190,
-// evenly spread: 161, 170; at random: 228, 236 and 208, 201; spread over the logarithm: 146, 105; 65 of these: 148, 97.
-// Beyond the limit `few` is mostly the better one, by up to a third; tiles are where lengths are spread evenly, and
-// where few key heads just fill the chip.  The limit has not been moved to what these say.
+// The first limit is no crossing of the forms.  Single tokens, 56 query heads on 8 key heads of 128, with tiles and
+// with `few`, over 300 / 1000 / 4000 keys each: 32 sequences 13, 12 / 29, 28 / 104, 104 us; 63: 19, 18 / 54, 53 / 189,
+// 188; 64: 19, 19 / 58, 57 / 192, 191; 65: 25, 23 / 73, 62; 128: 37, 36 / 104, 101; 256: 75, 70 / 200, 195.  Two key
+// heads, 256 sequences: 19, 19 / 55, 54 / 193, 192; 400: 31, 29 / 88, 88 / 308, 319.  64 of unequal lengths up to 8190,
+// in steps: 240, 229; at random: 248, 251; spread over the logarithm: 158, 107; 65 of these: 154, 98.  Beyond the limit
+// `few` is mostly the better one, by up to a third.  The limit stays: the forms add up in another order, and calls
+// keep the bits of their results.
 //
 // Codes.  `few` takes them without a detour, so it goes further, up to 64 rows on average whatever their number.  32 on
 // 8 heads, tiles and `few`, E4M3 / INT8: 64 sequences of 16 tokens over 2048 keys, heads of 128 109, 85 / 127, 106 us,
-// of 64 82, 53 / 88, 68; single tokens of 64 sequences, 56 heads on 8 of 128, 0 to 8190 keys, INT8 201 and 120.  INT8
+// of 64 82, 53 / 88, 68; single tokens of 64 sequences, 56 heads on 8 of 128, 0 to 6400 keys, INT8 173 and 104.  INT8
 // and heads of 64 pay more for expanding a code in every workgroup of 32 rows: 8 sequences of 64 tokens over 4096 keys,
 // INT8, 71 and 82, heads of 64 47 and 53, but E4M3 with heads of 128 64 and 54.  With a cap or bias, heads of 128 in
 // tiles have more in registers than there is room for: cap, chunks of up to 1024 tokens over up to 8192 keys 431 and
