@@ -557,6 +557,18 @@ int m5k_paged_append_codes(
     int64_t q_token, void* q_out, const double* frequencies, int64_t pairs, int interleaved, float magnitude,
     void* stream);
 
+/* The same with a magnitude that FP32 need not have: keys are turned with it as it is, q with the FP32 number next to
+ * it. */
+int m5k_paged_append_codes64(
+    const void* k, int64_t k_head, int64_t k_token, const void* v, int64_t v_head, int64_t v_token, int dtype,
+    int64_t tokens, int64_t kv_heads, int64_t head_dim, int mode, void* k_codes, int64_t kc_page, int64_t kc_head,
+    int64_t kc_slot, uint8_t* k_exponents, int64_t ke_page, int64_t ke_head, void* v_codes, int64_t vc_page,
+    int64_t vc_head, int64_t vc_slot, uint8_t* v_exponents, int64_t ve_page, int64_t ve_head, int64_t block,
+    int64_t pages, int64_t page_size, const int32_t* page_table, int64_t table_width, int64_t sequences,
+    const int32_t* query_starts, const int32_t* context_lengths, const void* q, int64_t heads, int64_t q_head,
+    int64_t q_token, void* q_out, const double* frequencies, int64_t pairs, int interleaved, double magnitude,
+    void* stream);
+
 /*
  * Read a cache in 8 bits back: k, v [kv_heads, tokens, head_dim] (F32, F16 or BF16, contiguous, 16-byte aligned) are
  * the values of the last n of each sequence's context_lengths[b] keys, n = query_starts[b + 1] - query_starts[b]: what

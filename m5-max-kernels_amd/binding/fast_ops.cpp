@@ -590,6 +590,7 @@ PyObject* paged_append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (!k || !v || layout < 0 || !paged_of(args + 2, c) || !current(k->device()) || args[10] == Py_None ||
       !positive(args[10], 1.0f, magnitude))
     Py_RETURN_NONE;
+  const double magnitude64 = PyFloat_AS_DOUBLE(args[10]);
   const c10::Device dev = k->device();
   const int64_t tokens = k->size(1);
   if (v->sizes() != k->sizes() || v->scalar_type() != k->scalar_type() || v->device() != dev ||
@@ -620,14 +621,14 @@ PyObject* paged_append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   int rc;
   if (coded) {
     Py_BEGIN_ALLOW_THREADS
-    rc = m5k_paged_append_codes(kp, stride(*k, 0), stride(*k, 1), vp, stride(*v, 0), stride(*v, 1), code, tokens,
-                                c.kv_heads, c.dim, e.mode, kc, stride(*c.k, 0), stride(*c.k, 1), stride(*c.k, 2), e.ke,
-                                stride(*e.k, 0), stride(*e.k, 1), vc, stride(*c.v, 0), stride(*c.v, 1),
-                                stride(*c.v, 2), e.ve, stride(*e.v, 0), stride(*e.v, 1), e.block, c.pages, c.page_size,
-                                c.table, c.width, c.sequences, c.starts, c.context, qp, heads, q ? stride(*q, 0) : 0,
-                                q ? stride(*q, 1) : 0, yp, fp, pairs, layout, magnitude, stream);
+    rc = m5k_paged_append_codes64(
+        kp, stride(*k, 0), stride(*k, 1), vp, stride(*v, 0), stride(*v, 1), code, tokens, c.kv_heads, c.dim, e.mode, kc,
+        stride(*c.k, 0), stride(*c.k, 1), stride(*c.k, 2), e.ke, stride(*e.k, 0), stride(*e.k, 1), vc, stride(*c.v, 0),
+        stride(*c.v, 1), stride(*c.v, 2), e.ve, stride(*e.v, 0), stride(*e.v, 1), e.block, c.pages, c.page_size,
+        c.table, c.width, c.sequences, c.starts, c.context, qp, heads, q ? stride(*q, 0) : 0, q ? stride(*q, 1) : 0, yp,
+        fp, pairs, layout, magnitude64, stream);
     Py_END_ALLOW_THREADS
-    if (rc) return failed("m5k_paged_append_codes", rc);
+    if (rc) return failed("m5k_paged_append_codes64", rc);
     if (!q) Py_RETURN_TRUE;
     return THPVariable_Wrap(std::move(y));
   }

@@ -563,14 +563,14 @@ int check_cache(const char* what, int mode, int64_t head_dim, const void* k, con
 }  // namespace
 }  // namespace m5k
 
-extern "C" int m5k_paged_append_codes(
+extern "C" int m5k_paged_append_codes64(
     const void* k, int64_t k_head, int64_t k_token, const void* v, int64_t v_head, int64_t v_token, int dtype,
     int64_t tokens, int64_t kv_heads, int64_t head_dim, int mode, void* k_codes, int64_t kc_page, int64_t kc_head,
     int64_t kc_slot, uint8_t* k_exponents, int64_t ke_page, int64_t ke_head, void* v_codes, int64_t vc_page,
     int64_t vc_head, int64_t vc_slot, uint8_t* v_exponents, int64_t ve_page, int64_t ve_head, int64_t block,
     int64_t pages, int64_t page_size, const int32_t* page_table, int64_t table_width, int64_t sequences,
     const int32_t* query_starts, const int32_t* context_lengths, const void* q, int64_t heads, int64_t q_head,
-    int64_t q_token, void* q_out, const double* frequencies, int64_t pairs, int interleaved, float magnitude,
+    int64_t q_token, void* q_out, const double* frequencies, int64_t pairs, int interleaved, double magnitude,
     void* stream) {
   using namespace m5k;
   clear_error();
@@ -617,6 +617,22 @@ extern "C" int m5k_paged_append_codes(
   if (dtype == M5K_BF16) return append_typed<M5K_BF16>(a, mode, dim, as_stream(stream));
   if (dtype == M5K_F16) return append_typed<M5K_F16>(a, mode, dim, as_stream(stream));
   return append_typed<M5K_F32>(a, mode, dim, as_stream(stream));
+}
+
+extern "C" int m5k_paged_append_codes(
+    const void* k, int64_t k_head, int64_t k_token, const void* v, int64_t v_head, int64_t v_token, int dtype,
+    int64_t tokens, int64_t kv_heads, int64_t head_dim, int mode, void* k_codes, int64_t kc_page, int64_t kc_head,
+    int64_t kc_slot, uint8_t* k_exponents, int64_t ke_page, int64_t ke_head, void* v_codes, int64_t vc_page,
+    int64_t vc_head, int64_t vc_slot, uint8_t* v_exponents, int64_t ve_page, int64_t ve_head, int64_t block,
+    int64_t pages, int64_t page_size, const int32_t* page_table, int64_t table_width, int64_t sequences,
+    const int32_t* query_starts, const int32_t* context_lengths, const void* q, int64_t heads, int64_t q_head,
+    int64_t q_token, void* q_out, const double* frequencies, int64_t pairs, int interleaved, float magnitude,
+    void* stream) {
+  return m5k_paged_append_codes64(k, k_head, k_token, v, v_head, v_token, dtype, tokens, kv_heads, head_dim, mode,
+                                  k_codes, kc_page, kc_head, kc_slot, k_exponents, ke_page, ke_head, v_codes, vc_page,
+                                  vc_head, vc_slot, v_exponents, ve_page, ve_head, block, pages, page_size, page_table,
+                                  table_width, sequences, query_starts, context_lengths, q, heads, q_head, q_token,
+                                  q_out, frequencies, pairs, interleaved, magnitude, stream);
 }
 
 extern "C" int m5k_paged_read(int mode, const void* k_codes, int64_t kc_page, int64_t kc_head, int64_t kc_slot,

@@ -43,6 +43,7 @@ _p = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 _rows3 = [_p, _i64, _i64, _i64]  # a cache: base and three strides
 
 # name -> argtypes (restype is int status unless noted)
@@ -106,6 +107,10 @@ SIGNATURES = {
     "m5k_paged_append_codes": [
         _p, _i64, _i64, _p, _i64, _i64, _i32, _i64, _i64, _i64, _i32, *_rows3, _p, _i64, _i64, *_rows3, _p, _i64, _i64,
         _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _i64, _i64, _i64, _p, _p, _i64, _i32, _f32, _p,
+    ],
+    "m5k_paged_append_codes64": [
+        _p, _i64, _i64, _p, _i64, _i64, _i32, _i64, _i64, _i64, _i32, *_rows3, _p, _i64, _i64, *_rows3, _p, _i64, _i64,
+        _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _i64, _i64, _i64, _p, _p, _i64, _i32, _f64, _p,
     ],
     "m5k_paged_read": [
         _i32, *_rows3, _p, _i64, _i64, *_rows3, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p, _p,

@@ -320,7 +320,7 @@ def paged_append(k, v, k_cache, v_cache, page_table, query_starts, context_lengt
         mode, block, ke, ve = codes
         with _on(device):
             _lib.call(
-                "m5k_paged_append_codes", _lib.ptr(k), kr[0], kr[1], _lib.ptr(v), vr[0], vr[1], _lib.dtype_code(k),
+                "m5k_paged_append_codes64", _lib.ptr(k), kr[0], kr[1], _lib.ptr(v), vr[0], vr[1], _lib.dtype_code(k),
                 tokens, kv_heads, width, mode, _lib.ptr(k_cache), ks[0], ks[1], ks[2], _lib.ptr(k_scales), ke[0], ke[1],
                 _lib.ptr(v_cache), vs[0], vs[1], vs[2], _lib.ptr(v_scales), ve[0], ve[1], block, k_cache.shape[0],
                 k_cache.shape[2], _lib.ptr(page_table), page_table.shape[1], page_table.shape[0],
