@@ -117,11 +117,11 @@ __device__ __forceinline__ double2 turn64(double a, double magnitude) {
                       quarter >= 2 ? -sine * magnitude : sine * magnitude);
 }
 
-// FP32 rounded to odd: cut off, with the last bit set where anything was.
+// FP32 rounded to odd: cut off, with the last bit set where anything was.  Infinity beyond FP32's range.
 __device__ __forceinline__ float round_to_odd(double v) {
   const float f = static_cast<float>(v);
   const double back = f;
-  if (!(fabs(v) < __builtin_inf()) || back == v) return f;
+  if (!(fabs(back) < __builtin_inf()) || back == v) return f;
   const uint32_t u = __float_as_uint(f);
   return __uint_as_float((u - (fabs(back) > fabs(v) ? 1u : 0u)) | 1u);
 }

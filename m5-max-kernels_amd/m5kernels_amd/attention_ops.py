@@ -271,8 +271,8 @@ def paged_append(k, v, k_cache, v_cache, page_table, query_starts, context_lengt
     holds older tokens (positions below context_lengths[b] - n), the scale that it has, if that is larger; a code is
     x / 2^e to the nearest, ties to even.  Where the scale grows, the older tokens' codes are rounded again under it.
     Slots behind the context stay as they are.  A block that gets an infinity or NaN reads as NaN until it is written
-    from its first slot on.  Keys are turned in 64 bits, and their codes rounded from that.  Where two sequences of a
-    call write into one block, its codes are unspecified."""
+    from its first slot on.  Keys are turned in 64 bits, and their codes rounded from that; one turned beyond FP32's
+    range counts as an infinity.  Where two sequences of a call write into one block, its codes are unspecified."""
     fast = hip._fast
     if fast is not None:
         done = fast.paged_append(k, v, k_cache, v_cache, page_table, query_starts, context_lengths, q, frequencies,
