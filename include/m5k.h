@@ -544,7 +544,8 @@ int m5k_paged_append(const void* k, int64_t k_head, int64_t k_token, const void*
  * the exponent that it has; a code is x / 2^e to the nearest, ties to even, and where the exponent grows the older
  * codes are rounded again under it.  Slots behind the context stay as they are.  A block that gets an infinity or NaN
  * takes exponent 255.
- * Keys are turned in 64 bits, and infinities beyond FP32's range; q, in 32, as m5k_rope's.  head_dim 64 or 128; rows of k, v and q 16-byte aligned.
+ * Keys are turned in 64 bits, and infinities beyond FP32's range; q, in 32, as m5k_rope's.  head_dim 64 or 128; rows of
+ * k, v and q 16-byte aligned.
  * Two tokens that name the same place, or two sequences that name the same block, leave unspecified codes there.
  */
 int m5k_paged_append_codes(

@@ -657,7 +657,8 @@ PyObject* paged_read(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const int64_t tokens = PyLong_AsLongLongAndOverflow(args[5], &overflow);
   const at::ScalarType st = reinterpret_cast<THPDtype*>(args[8])->scalar_type;
   const int code = dtype_code(st);
-  if (overflow || tokens <= 0 || tokens > (1 << 28) || code < 0) Py_RETURN_NONE;
+  if (overflow || tokens <= 0 || tokens > (1 << 28) || tokens * c.dim > (int64_t{1} << 35) - 2048 || code < 0)
+    Py_RETURN_NONE;
   const c10::Device dev = c.k->device();
   void* stream = nullptr;
   if (!stream_of(dev, &stream)) return nullptr;

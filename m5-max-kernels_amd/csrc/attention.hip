@@ -18,7 +18,7 @@ template <> int launch_typed<PAGES16, true, INT8>(Args&, int, int, hipStream_t);
 template <int DT, int D>
 static int launch_join_of(const Args& a, hipStream_t st) {
   const int64_t rows = int64_t{a.tokens} * a.heads;
-  if (a.splits > 8)
+  if (a.splits > JOINED_TOGETHER)
     launch_kernel(attention_join<DT, D, 4>, dim3(static_cast<uint32_t>(rows)), dim3(256), st, a);
   else
     launch_kernel(attention_join<DT, D, 1>, dim3(static_cast<uint32_t>((rows + 3) / 4)), dim3(256), st, a);

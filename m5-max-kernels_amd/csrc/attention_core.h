@@ -1508,7 +1508,12 @@ inline int plan_splits(int kind, int64_t tokens, int group, int kv_heads, int64_
   return static_cast<int>(n < 1 ? 1 : n > 64 ? 64 : n);
 }
 
-// The second launch of a call in key splits (attention.hip).
+// The second launch of a call in key splits (attention.hip): a row a workgroup where there are many splits, else four.
+constexpr int JOINED_TOGETHER = 8;
+inline bool join_fits(const Args& a) {
+  const int64_t rows = int64_t{a.tokens} * a.heads;
+  return fits_launch(a.splits > JOINED_TOGETHER ? rows : (rows + 3) / 4, 256);
+}
 int launch_join(const Args& a, int dtype, int head_dim, hipStream_t st);
 
 template <int DT, int D, int KEYS, bool SINKS, int CODES>
@@ -1522,7 +1527,8 @@ int launch(Args& a, hipStream_t st) {
   a.cus = device_cus();
   a.spread = a.kv_heads % 8 != 0 && (KEYS != DENSE || a.causal || a.starts);
   const int64_t blocks = int64_t{a.slots} * a.kv_heads * a.splits;
-  M5K_REQUIRE(blocks <= INT32_MAX, "attention: too many tiles for one launch");
+  M5K_REQUIRE(fits_launch(blocks, THREADS), "attention: too many tiles for one launch");
+  M5K_REQUIRE(a.splits == 1 || join_fits(a), "attention: too many rows for one launch of their join");
   constexpr bool ALWAYS_FEW = CODES == E4M3 && D == 128;  // with MODS
   auto kernel = p.few ? (mods ? attention_tile<DT, D, KEYS, true, true, SINKS, CODES>
                               : attention_tile<DT, D, KEYS, false, true, SINKS, CODES>)

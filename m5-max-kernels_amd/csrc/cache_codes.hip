@@ -500,7 +500,7 @@ int append_threads(AppendArgs& a, hipStream_t st) {
   a.q_groups = divisor(a.heads ? (a.heads + a.walk - 1) / a.walk : 1);
   const int q_slots = a.heads ? (a.tokens + ROWS - 1) / ROWS : 0;
   const int64_t blocks = int64_t{2} * a.slots * a.groups.value + int64_t{q_slots} * a.q_groups.value;
-  M5K_REQUIRE(blocks <= INT32_MAX, "paged_append: too many rows for one launch");
+  M5K_REQUIRE(fits_launch(blocks, T), "paged_append: too many rows for one launch");
   launch_kernel(append_codes<DT, D, MODE, T, PASSES, TURNED>, dim3(static_cast<uint32_t>(blocks)), dim3(T), st, a);
   return launch_status("paged_append");
 }
@@ -532,6 +532,7 @@ int append_typed(AppendArgs& a, int mode, int head_dim, hipStream_t st) {
 template <int DT>
 int read_typed(const ReadArgs& a, int mode, int head_dim, hipStream_t st) {
   const int64_t blocks = (int64_t{a.tokens} * (head_dim / 8) + THREADS - 1) / THREADS;
+  M5K_REQUIRE(fits_launch(blocks, THREADS), "paged_read: too many tokens for one launch");
   const dim3 grid(static_cast<uint32_t>(blocks), static_cast<uint32_t>(2 * a.groups));
   auto kernel = mode == M5K_QUANT_FP8
                     ? (head_dim == 64 ? read_codes<DT, 64, M5K_QUANT_FP8> : read_codes<DT, 128, M5K_QUANT_FP8>)

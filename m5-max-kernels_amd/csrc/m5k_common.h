@@ -27,6 +27,9 @@ int device_cus();
 
 inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
 
+// Whether the threads of a launch along an axis are counted by 32 bits, as a launch counts them.
+inline bool fits_launch(int64_t workgroups, int64_t threads) { return workgroups <= int64_t{UINT32_MAX} / threads; }
+
 template <typename... KArgs, typename... Args>
 inline void launch_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block, hipStream_t st, Args&&... args) {
   kernel<<<grid, block, 0, st>>>(static_cast<KArgs>(args)...);

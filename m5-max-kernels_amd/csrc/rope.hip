@@ -166,7 +166,7 @@ int launch(Args& a, bool vector, bool interleaved, hipStream_t st) {
   int blocks = 0;
   for (Part& p : a.part) blocks += p.blocks = (p.heads + a.walk - 1) / a.walk;
   const int64_t gx = (units + 255) / 256;
-  M5K_REQUIRE(gx <= INT32_MAX && blocks <= 65535, "rope: too many rows for one launch");
+  M5K_REQUIRE(fits_launch(gx, 256) && blocks <= 65535, "rope: too many rows for one launch");
   const dim3 grid(static_cast<uint32_t>(gx), static_cast<uint32_t>(blocks));
   const bool whole = a.pairs % 8 == 0;
   // With one channel a thread the partner's place is found by itself in either layout.

@@ -37,6 +37,7 @@ _FLOAT_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 _CODE_MODES = {torch.uint8: _lib.QUANT_FP8, torch.int8: _lib.QUANT_INT8}
 HEAD_DIMS = (64, 128)
 BLOCK_MAX = 128
+_READ_MAX = (1 << 35) - 2048  # values a head of a read, 8 a thread in workgroups of 256, below 2^32 threads
 _WINDOW_MAX = (1 << 30) - 1
 _F32_LEAST = 2.0 ** -126
 _RATIO_MAX = 1e37  # scale / softcap: what a score is multiplied by before the cap's tanh, finite with its log2(e)
@@ -365,8 +366,8 @@ def paged_read(k_cache, v_cache, page_table, query_starts, context_lengths, toke
         raise ValueError("dtype must be bfloat16, float16 or float32")
     if not _lib.is_int(tokens) or tokens < 0:
         raise ValueError("tokens must be a nonnegative integer")
-    if tokens > 1 << 28:
-        raise NotImplementedError("paged_read supports up to 2^28 tokens")
+    if tokens > 1 << 28 or tokens * width > _READ_MAX:
+        raise NotImplementedError("paged_read supports up to 2^28 tokens, and 2^35 - 2048 values a head")
     page_table, query_starts, context_lengths = _paged(k_cache, v_cache, page_table, query_starts, context_lengths)
     device = _device(k_cache, (v_cache, "v_cache"), (k_scales, "k_scales"), (v_scales, "v_scales"),
                      (page_table, "page_table"), (query_starts, "query_starts"), (context_lengths, "context_lengths"))
