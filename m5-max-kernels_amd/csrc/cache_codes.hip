@@ -16,6 +16,7 @@
 // bits: 64 tokens, 8 key heads and 56 query heads of 128 take 7.4 us, 5.9 without the queries, 4.7 without turning.
 // Chunks: 4096 tokens, 32 heads of 64, FP16 to INT8, 15 us, 3.3 TB/s, two waves a SIMD.
 #include "attention_place.h"
+#include "cache_walk.h"
 #include "fast_div.h"
 #include "m5k_common.h"
 #include "rope_turn.h"
@@ -482,20 +483,12 @@ __global__ __launch_bounds__(THREADS) void read_codes(const ReadArgs a) {
 
 // ---- launches -------------------------------------------------------------------------------------
 
-// Heads that a workgroup walks over: as many as leave each compute unit `waves` waves' work.
-int walk_of(int64_t workgroups, int heads, int threads, int waves) {
-  const int64_t w = workgroups * heads * (threads / 64) / (int64_t{256} * waves);
-  return static_cast<int>(w < 1 ? 1 : w > 8 ? 8 : w);
-}
-
 template <int DT, int D, int MODE, int T, int PASSES, bool TURNED>
 int append_threads(AppendArgs& a, hipStream_t st) {
   constexpr int ROWS = PASSES * T / (D / 8);  // of q a workgroup
   const int block = a.block.value;
   a.slots = block_slots(a.tokens, a.tokens / block, a.sequences);
-  // 16: sines and cosines are made once a walk (4096 tokens turned, 32 heads of q, 8 of k and v of 128, blocks of 64,
-  // read back: 36 us; with 8 and 32 waves 36 and 50 us; single tokens have too few rows to walk).
-  a.walk = walk_of(a.tokens / block, 2 * a.kv_heads + a.heads, T, 16);
+  a.walk = append_walk(a.tokens, block, a.kv_heads, a.heads, T);
   a.groups = divisor((a.kv_heads + a.walk - 1) / a.walk);
   a.q_groups = divisor(a.heads ? (a.heads + a.walk - 1) / a.walk : 1);
   const int q_slots = a.heads ? (a.tokens + ROWS - 1) / ROWS : 0;
@@ -677,8 +670,8 @@ extern "C" int m5k_paged_read(int mode, const void* k_codes, int64_t kc_page, in
   a.pages = static_cast<int>(pages);
   a.page_size = divisor(static_cast<int>(page_size));
   a.block = divisor(static_cast<int>(block));
-  // 16: the second of the reads above with 64 26.3 us, with 128 34.5; the first the same from 8 to 128.
-  a.walk = walk_of((tokens * (head_dim / 8) + THREADS - 1) / THREADS, 2 * a.kv_heads, THREADS, 16);
+  static_assert(THREADS == 256, "read_walk counts with it");
+  a.walk = read_walk(tokens, static_cast<int>(head_dim), a.kv_heads);
   a.groups = (a.kv_heads + a.walk - 1) / a.walk;
   const int dim = static_cast<int>(head_dim);
   if (dtype == M5K_BF16) return read_typed<M5K_BF16>(a, mode, dim, as_stream(stream));
