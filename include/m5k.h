@@ -70,7 +70,9 @@ extern "C" {
 /* Message for the last failure on this thread ("" if none). */
 const char* m5k_last_error(void);
 
-/* ABI version (major*100 + minor). */
+/* ABI version (major*100 + minor).  Entries are added under the same number; what an argument was documented to mean
+ * stays.  m5k_attention_plan once took any `paged` other than 0 for a paged call: it takes 1 for it now, as it was
+ * documented, gives 2 and 4 (plus 8, 16) their own meaning, and refuses the rest. */
 #define M5K_ABI_VERSION 100
 int m5k_abi_version(void);
 
@@ -496,7 +498,7 @@ int m5k_paged_attention_sinks(const void* q, int dtype, int64_t tokens, int64_t 
  * page_size) and head stands for code * 2^(exponent - 127); under exponent 255 every code is NaN.
  *
  * m5k_paged_attention_codes: m5k_paged_attention_sinks over such a cache, whose values are taken in q's dtype (exact in
- * BF16 down to its subnormals; in FP16 rounded, to an infinity above its range).  Rows of codes are 16-byte aligned,
+ * BF16 down to its subnormals; in FP16 rounded; infinities above either's range).  Rows of codes are 16-byte aligned,
  * head_dim to 2^23 bytes apart.
  */
 int m5k_paged_attention_codes(

@@ -39,13 +39,16 @@
 // Single tokens: the cache's bytes (131073 keys, 8 key heads of 128: 94 to 100 us and 5 us of joining, 5.5 TB/s).
 // Heads of 64: the exponentials.
 // Codes: bytes again where tokens are single (131073 keys, E4M3: 54 us, 5.0 TB/s, and 5 of joining; 64 over 4000 keys
-// each 103 us, 5.1 TB/s); 64 over 0 to 6400 keys take 102 to 109 us in INT8 and 94 in E4M3, 3.8 and 4.2 TB/s, the
-// longest sequences alone at the end.  Chunks as in 16 bits, with the expansion beside the products (of up to 1024
-// tokens over up to 8192 keys 207 us, so 182; 0.9 waves a SIMD, and one alone takes 3800 cycles a tile where two take
-// 2600 each).
+// each 103 us, 5.1 TB/s); 64 over 0 to 6122 keys, in three bands, take 102 to 109 us in INT8 and 91 to 94 in E4M3, 3.8
+// and 4.3 TB/s, the longest sequences alone at the end; 64 with lengths spread over the logarithm from 32 to 8191 71 to
+// 97 us in E4M3 and 98 to 135 in INT8, where their bytes take 32 to 58.  Chunks as in 16 bits, with the expansion
+// beside the products (of up to 1024 tokens over up to 8192 keys 207 us, so 182; 0.9 waves a SIMD, and one alone takes
+// 3800 cycles a tile where two take 2600 each).
 // First keys: 9914 causal tokens, 56 heads of 128, window 1024, 4 first keys: 363 to 373 us, 0.85 PFLOP/s over the 1090
-// keys a row that are multiplied, of which 975 count; without first keys 343.  8192 tokens in 7 documents, 32 on 8
-// heads of 64, FP16, window 256, 64 first keys: 54 to 60 us, VALU work, 19 of its instructions a product.
+// keys a row that are multiplied, of which 975 count; without first keys 343.  19 tiles a workgroup leave its beginning
+// and end more to hide than the 155 of a call without a window.  8192 tokens in 7 documents, 32 on 8 heads of 64, FP16,
+// window 256, 64 first keys: 54 to 60 us, 7 tiles a workgroup; nothing is full there (VALU 46% of the cycles, matrix
+// cores 16%, 1.5 waves a SIMD, which wait for 29%).
 //
 // Registers.  Tiles of 128 rows with heads of 128 use 241 to 256, all there are for two waves a SIMD.  With a cap or a
 // bias 8 to 10 of them go to memory and come back inside the loop, 34 by pages of no multiple of 16 (chunks of up to
@@ -688,7 +691,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_tile(const Args a) {
   };
   // Pages and exponents of the tiles that this wave loads from tile t on, a group of 16 keys a lane, by vector loads
   // that it waits for once in 32 tiles (FEW) or 64.  Loads a tile would be waited for with the tiles in flight, or, as
-  // scalar loads, hold up the LDS reads behind them (64 single tokens over 0 to 8190 keys, INT8: 130 us and 120).
+  // scalar loads, hold up the LDS reads behind them (64 single tokens over 0 to 6122 keys, INT8: 130 us and 120).
   constexpr int HELD = 64 / GROUPS, APART = FEW ? WAVES : 1;
   int held_id = 0, held_k = 0, held_v = 0, held_at = 0;
   auto look_ahead = [&](int t) __attribute__((always_inline)) {
@@ -1460,14 +1463,14 @@ __global__ __launch_bounds__(256) void attention_join(const Args a) {
 // The first limit is no crossing of the forms.  Single tokens, 56 query heads on 8 key heads of 128, with tiles and
 // with `few`, over 300 / 1000 / 4000 keys each: 32 sequences 13, 12 / 29, 28 / 104, 104 us; 63: 19, 18 / 54, 53 / 189,
 // 188; 64: 19, 19 / 58, 57 / 192, 191; 65: 25, 23 / 73, 62; 128: 37, 36 / 104, 101; 256: 75, 70 / 200, 195.  Two key
-// heads, 256 sequences: 19, 19 / 55, 54 / 193, 192; 400: 31, 29 / 88, 88 / 308, 319.  64 of unequal lengths up to 8190,
-// in steps: 240, 229; at random: 248, 251; spread over the logarithm: 158, 107; 65 of these: 154, 98.  Beyond the limit
-// `few` is mostly the better one, by up to a third.  The limit stays: the forms add up in another order, and calls
-// keep the bits of their results.
+// heads, 256 sequences: 19, 19 / 55, 54 / 193, 192; 400: 31, 29 / 88, 88 / 308, 319.  64 of unequal lengths up to
+// 8190, in steps: 240, 229; at random: 248, 251; spread over the logarithm: 158, 107; 65 of these: 154, 98 (one draw
+// each: see slots_before for how far draws differ).  Beyond the limit `few` is mostly the better one, by up to a
+// third.  The limit stays: the forms add up in another order, and calls keep the bits of their results.
 //
 // Codes.  `few` takes them without a detour, so it goes further, up to 64 rows on average whatever their number.  32 on
 // 8 heads, tiles and `few`, E4M3 / INT8: 64 sequences of 16 tokens over 2048 keys, heads of 128 109, 85 / 127, 106 us,
-// of 64 82, 53 / 88, 68; single tokens of 64 sequences, 56 heads on 8 of 128, 0 to 6400 keys, INT8 173 and 104.  INT8
+// of 64 82, 53 / 88, 68; single tokens of 64 sequences, 56 heads on 8 of 128, 0 to 6122 keys, INT8 173 and 104.  INT8
 // and heads of 64 pay more for expanding a code in every workgroup of 32 rows: 8 sequences of 64 tokens over 4096 keys,
 // INT8, 71 and 82, heads of 64 47 and 53, but E4M3 with heads of 128 64 and 54.  With a cap or bias, heads of 128 in
 // tiles have more in registers than there is room for: cap, chunks of up to 1024 tokens over up to 8192 keys 431 and

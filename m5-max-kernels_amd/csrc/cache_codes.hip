@@ -13,8 +13,10 @@
 // fewer bits cannot tell from the 64-bit number.  Sines and cosines stand in LDS for all heads of the walk.
 //
 // What bounds it.  Single tokens: a chain of dependent loads (sequence, length, page, exponent) and the angles in 64
-// bits: 64 tokens, 8 key heads and 56 query heads of 128 take 7.4 us, 5.9 without the queries, 4.7 without turning.
-// Chunks: 4096 tokens, 32 heads of 64, FP16 to INT8, 15 us, 3.3 TB/s, two waves a SIMD.
+// bits: 64 tokens, 8 key heads and 56 query heads of 128 take 7.4 us by graph replay (7.9 in a kernel trace), 5.9
+// without the queries, 4.7 without turning.  Chunks: 4096 tokens, 32 heads of 64, FP16 to INT8, 15.7 us in a kernel
+// trace (14.8 the least), 3.2 TB/s of 4.9: a barrier a head, with one head's loads ahead of it, and two waves a SIMD,
+// which wait for 65% of their cycles.
 #include "attention_place.h"
 #include "cache_walk.h"
 #include "fast_div.h"

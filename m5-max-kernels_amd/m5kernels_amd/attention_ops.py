@@ -345,9 +345,10 @@ def paged_read(k_cache, v_cache, page_table, query_starts, context_lengths, toke
 
     Arguments are paged_append's: of sequence b the last n = query_starts[b + 1] - query_starts[b] of its
     context_lengths[b] keys, so that the call with paged_append's arguments gives what that call stored.  `tokens` is
-    how many rows come back: query_starts[-1], or more where the host does not know it (rows behind it are 0).  Rows
-    that paged_append would not store are 0 too.  Values are exact in float32 and bfloat16 down to their subnormals; in
-    float16 they are rounded, to an infinity above its range."""
+    how many rows come back: query_starts[-1], or more where the host does not know it (rows behind it are 0), 2^28 at
+    most and fewer than 2^28 - 15 of 128 channels.  Rows that paged_append would not store are 0 too.  Values are exact
+    in float32 and bfloat16 down to their subnormals and rounded in float16; above a type's range they are
+    infinities."""
     fast = hip._fast
     if fast is not None:
         done = fast.paged_read(k_cache, v_cache, page_table, query_starts, context_lengths, tokens, k_scales, v_scales,
